@@ -29,6 +29,8 @@
 #ifndef NENGO_HIP_H
 #define NENGO_HIP_H
 
+#include "nengo_hip_selective.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -854,6 +856,24 @@ int nhip_rtc_destroy(void *program);
 int nhip_rtc_launch_direct(void *stream, void *function, int n, const int *t_starts,
                            const float *T, const int *x_starts, const float *X,
                            const int *y_starts, float *Y);
+
+/* ---- blocks that filter selectively ------------------------------------------
+ * The arguments are described in nengo_hip_selective.h.  Sizes: width 1 ... 8; states 1 ...
+ * 256; any others from 1 (tokens, sequences and requests from 0).  The `*_workspace` functions give
+ * the bytes of workspace that a call with these arguments needs (a smaller one is refused
+ * with NHIP_E_TOOBIG); its contents need not be kept between calls. */
+int nhip_causal_conv(void *stream, const nhip_conv_args *args);
+int nhip_causal_conv_grad(void *stream, const nhip_conv_args *args);
+int nhip_causal_conv_grad_workspace(const nhip_conv_args *args, long long *bytes_out);
+int nhip_causal_conv_step(void *stream, const nhip_conv_step_args *args);
+int nhip_selective_scan(void *stream, const nhip_scan_args *args);
+int nhip_selective_scan_workspace(const nhip_scan_args *args, long long *bytes_out);
+int nhip_selective_scan_grad(void *stream, const nhip_scan_args *args);
+int nhip_selective_scan_grad_workspace(const nhip_scan_args *args, long long *bytes_out);
+int nhip_selective_step(void *stream, const nhip_scan_step_args *args);
+int nhip_block_norm(void *stream, const nhip_norm_args *args);
+int nhip_block_norm_grad(void *stream, const nhip_norm_args *args);
+int nhip_block_norm_grad_workspace(const nhip_norm_args *args, long long *bytes_out);
 
 /* ---- executor ----------------------------------------------------------
  * replaces the Python launch loop of `Plans.enqueue_n_times` (plan.py:137-149):

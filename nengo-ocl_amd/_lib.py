@@ -100,6 +100,18 @@ SIGNATURES = {
     "nhip_sequence": [P, P, c_int, c_int],
     "nhip_sequence_chains": [P, P, P, P, c_int],
     "nhip_gemv_tile_carry": [P, P, P, c_int, c_int],
+    "nhip_causal_conv": [P, P],
+    "nhip_causal_conv_grad": [P, P],
+    "nhip_causal_conv_grad_workspace": [P, P],
+    "nhip_causal_conv_step": [P, P],
+    "nhip_selective_scan": [P, P],
+    "nhip_selective_scan_workspace": [P, P],
+    "nhip_selective_scan_grad": [P, P],
+    "nhip_selective_scan_grad_workspace": [P, P],
+    "nhip_selective_step": [P, P],
+    "nhip_block_norm": [P, P],
+    "nhip_block_norm_grad": [P, P],
+    "nhip_block_norm_grad_workspace": [P, P],
     "nhip_capture_begin": [P],
     "nhip_capture_end": [P, ctypes.POINTER(c_void_p)],
     "nhip_graph_upload": [P, P],

@@ -1,0 +1,365 @@
+// The short causal convolution along a sequence, channel by channel (a filter with `width`
+// taps per channel in front of a selective scan), its gradient and its step for single tokens.
+//
+//     u[t, d] = bias[d] + sum_k weight[d, k] x[t - width + 1 + k, d],   y = u  or  u sigmoid(u)
+//
+// The operators move memory: 2 width + 6 operations per element of 2 or 4 bytes.  A lane
+// takes 16 bytes of neighbouring channels and goes along a strip of tokens with the window in
+// registers, so that each input is read once (and width - 1 rows again where strips meet, from
+// the caches).
+#include <type_traits>
+
+#include "selective_common.h"
+
+namespace {
+
+constexpr int kStrip = 16;           // tokens that a wave goes along
+constexpr int kChunk = 4 * kStrip;   // tokens of a work-group: four waves
+constexpr int kMaxWidth = 8;
+
+// lane's channels: c0 ... c0 + V - 1
+template <class T, int V>
+__device__ __forceinline__ int first_channel() {
+    return (blockIdx.y * NHIP_WAVE + (threadIdx.x & (NHIP_WAVE - 1))) * V;
+}
+
+// Input of token t of the sequence: of `initial` in front of its first token, zero beyond both
+// ends.
+template <class T, int V, int K>
+__device__ __forceinline__ void load_token(const nhip_conv_args& a, const SelSeq& s, int t, int c0,
+                                           float (&v)[V]) {
+    if (t >= 0 && t < s.n) {
+        sel_load<T, V>(sel_row<T>(a.x, a.tokens, s, t) + c0, v);
+    } else if (t < 0 && a.initial && t >= 1 - K) {
+        sel_load<T, V>(static_cast<const T*>(a.initial) +
+                           ((long long)s.seq * (K - 1) + (K - 1 + t)) * a.channels + c0, v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = 0.0f;
+    }
+}
+
+template <int V, int K>
+__device__ __forceinline__ void load_taps(const nhip_conv_args& a, int c0, float (&w)[K][V],
+                                          float (&b)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        b[i] = a.bias ? a.bias[c0 + i] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k][i] = a.weight[(long long)(c0 + i) * K + k];
+    }
+}
+
+template <class T, int V, int K>
+__global__ __launch_bounds__(NHIP_WG) void conv_kernel(nhip_conv_args a) {
+    const SelSeq s = sel_seq_of_chunk(a.tokens, blockIdx.x, kChunk);
+    if (s.seq < 0) return;
+    const int c0 = first_channel<T, V>();
+    if (c0 >= a.channels) return;
+    const int t0 = s.chunk * kChunk + (threadIdx.x / NHIP_WAVE) * kStrip;
+    float w[K][V], b[V];
+    load_taps<V, K>(a, c0, w, b);
+    const int t1 = min(t0 + kStrip, s.n);
+    if (t0 < t1) {
+        float x[K][V];  // the window: x[k] is token t - K + 1 + k
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) load_token<T, V, K>(a, s, t0 - K + 1 + k, c0, x[k]);
+        T* out = static_cast<T*>(a.y) + (s.row0 + t0) * a.channels + c0;
+        const T* in = sel_row<T>(a.x, a.tokens, s, t0) + c0;
+#pragma unroll 8
+        for (int t = t0; t < t1; ++t) {
+            sel_load<T, V>(in, x[K - 1]);
+            float u[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                u[i] = b[i];
+#pragma unroll
+                for (int k = 0; k < K; ++k) u[i] = fmaf(w[k][i], x[k][i], u[i]);
+                if (a.silu) u[i] *= sel_sigmoid(u[i]);
+            }
+            sel_store<T, V>(out, u);
+#pragma unroll
+            for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                for (int i = 0; i < V; ++i) x[k][i] = x[k + 1][i];
+            in += a.x.token;
+            out += a.channels;
+        }
+    }
+    // the last chunk's first wave hands on the end of the sequence
+    if (a.final && K > 1 && threadIdx.x < NHIP_WAVE && s.chunk == sel_chunks(s.n, kChunk) - 1) {
+#pragma unroll
+        for (int j = 0; j < K - 1; ++j) {
+            float v[V];
+            load_token<T, V, K>(a, s, s.n + j - (K - 1), c0, v);
+            sel_store<T, V>(static_cast<T*>(a.final) + ((long long)s.seq * (K - 1) + j) * a.channels + c0, v);
+        }
+    }
+}
+
+// dx[t] = sum_k weight[k] g[t + K - 1 - k], g = dy f'(u).  A strip goes on over the K - 1 tokens
+// behind it, whose g its last tokens need; g is zero outside the sequence.  The sums for the
+// taps go to a row of the workspace per chunk, [K + 1][channels], and are added up by a second
+// launch in the order of the chunks: the same result on every call.
+template <class T, int V, int K>
+__global__ __launch_bounds__(NHIP_WG) void conv_grad_kernel(nhip_conv_args a, float* parts) {
+    __shared__ float sums[4][NHIP_WAVE * V];
+    const int chunk = blockIdx.x;
+    const SelSeq s = sel_seq_of_chunk(a.tokens, chunk, kChunk);
+    const int c0 = first_channel<T, V>();
+    const bool here = s.seq >= 0 && c0 < a.channels;
+    const int wave = threadIdx.x / NHIP_WAVE, lane = threadIdx.x & (NHIP_WAVE - 1);
+    float dw[K + 1][V];
+#pragma unroll
+    for (int k = 0; k <= K; ++k)
+#pragma unroll
+        for (int i = 0; i < V; ++i) dw[k][i] = 0.0f;
+    if (here) {
+        const int t0 = s.chunk * kChunk + wave * kStrip;
+        const int t1 = min(t0 + kStrip, s.n);
+        // the sequence's first strip also forms what goes to `initial`: rows of t < 0
+        const int from = s.chunk == 0 && wave == 0 && a.dinitial ? 1 - K : t0;
+        if (from < t1 || from < 0) {
+            float w[K][V], b[V], x[K][V], g[K][V];  // x[k], g[k]: token t - K + 1 + k
+            load_taps<V, K>(a, c0, w, b);
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                if (k < K - 1) load_token<T, V, K>(a, s, t0 - K + 1 + k, c0, x[k]);
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[k][i] = 0.0f;
+            }
+#pragma unroll 4
+            for (int t = t0; t < max(t1, t0) + K - 1; ++t) {
+                load_token<T, V, K>(a, s, t, c0, x[K - 1]);
+                const bool in = t < s.n;
+                if (in) sel_load<T, V>(sel_row<T>(a.dy, a.tokens, s, t) + c0, g[K - 1]);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    float u = b[i];
+#pragma unroll
+                    for (int k = 0; k < K; ++k) u = fmaf(w[k][i], x[k][i], u);
+                    float d = in ? g[K - 1][i] : 0.0f;
+                    if (a.silu && in) {
+                        const float sg = sel_sigmoid(u);
+                        d *= sg * fmaf(u, 1.0f - sg, 1.0f);
+                    }
+                    g[K - 1][i] = d;
+                    if (t < t1) {
+#pragma unroll
+                        for (int k = 0; k < K; ++k) dw[k][i] = fmaf(d, x[k][i], dw[k][i]);
+                        dw[K][i] += d;
+                    }
+                }
+                const int td = t - (K - 1);  // the token whose gradient is complete
+                if (td >= from) {
+                    float dx[V];
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        dx[i] = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < K; ++k) dx[i] = fmaf(w[k][i], g[K - 1 - k][i], dx[i]);
+                    }
+                    const int j = td + (K - 1) - s.n;  // its place among the last K - 1 inputs
+                    if (a.dfinal && j >= 0) {
+                        float more[V];
+                        sel_load<T, V>(static_cast<const T*>(a.dfinal) +
+                                           ((long long)s.seq * (K - 1) + j) * a.channels + c0, more);
+#pragma unroll
+                        for (int i = 0; i < V; ++i) dx[i] += more[i];
+                    }
+                    T* out = td >= 0 ? static_cast<T*>(a.dx) + (s.row0 + td) * a.channels + c0
+                                     : static_cast<T*>(a.dinitial) +
+                                           ((long long)s.seq * (K - 1) + (K - 1 + td)) * a.channels + c0;
+                    sel_store<T, V>(out, dx);
+                }
+#pragma unroll
+                for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        x[k][i] = x[k + 1][i];
+                        g[k][i] = g[k + 1][i];
+                    }
+            }
+        }
+    }
+    for (int k = 0; k <= K; ++k) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            float v = dw[0][i];
+#pragma unroll
+            for (int q = 1; q <= K; ++q) v = k == q ? dw[q][i] : v;
+            sums[wave][lane * V + i] = v;
+        }
+        __syncthreads();
+        for (int c = threadIdx.x; c < NHIP_WAVE * V; c += NHIP_WG) {
+            const int d = blockIdx.y * NHIP_WAVE * V + c;
+            if (d < a.channels)
+                parts[((long long)chunk * (K + 1) + k) * a.channels + d] =
+                    (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+        }
+        __syncthreads();
+    }
+}
+
+template <class T, int V, int K>
+__global__ __launch_bounds__(NHIP_WG) void conv_step_kernel(nhip_conv_step_args a) {
+    const int per = (a.channels + V - 1) / V;
+    const long long i0 = (long long)blockIdx.x * NHIP_WG + threadIdx.x;
+    if (i0 >= (long long)a.n * per) return;
+    const int r = (int)(i0 / per), c0 = (int)(i0 % per) * V;
+    const int slot = a.slots ? a.slots[r] : r;
+    float u[V];
+    if (slot >= 0 && slot < a.n_slots) {
+        T* state = static_cast<T*>(a.state) + slot * a.state_stride + c0;
+        float x[K][V];
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) sel_load<T, V>(state + (long long)k * a.channels, x[k]);
+        sel_load<T, V>(static_cast<const T*>(a.x) + r * a.x_stride + c0, x[K - 1]);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            u[i] = a.bias ? a.bias[c0 + i] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < K; ++k)
+                u[i] = fmaf(a.weight[(long long)(c0 + i) * K + k], x[k][i], u[i]);
+            if (a.silu) u[i] *= sel_sigmoid(u[i]);
+        }
+#pragma unroll
+        for (int k = 0; k < K - 1; ++k) sel_store<T, V>(state + (long long)k * a.channels, x[k + 1]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) u[i] = 0.0f;
+    }
+    sel_store<T, V>(static_cast<T*>(a.y) + (long long)r * a.channels + c0, u);
+}
+
+template <class F> bool with_width(int width, F&& f) {
+    switch (width) {
+        case 1: f(std::integral_constant<int, 1>()); return true;
+        case 2: f(std::integral_constant<int, 2>()); return true;
+        case 3: f(std::integral_constant<int, 3>()); return true;
+        case 4: f(std::integral_constant<int, 4>()); return true;
+        case 5: f(std::integral_constant<int, 5>()); return true;
+        case 6: f(std::integral_constant<int, 6>()); return true;
+        case 7: f(std::integral_constant<int, 7>()); return true;
+        case 8: f(std::integral_constant<int, 8>()); return true;
+    }
+    return false;
+}
+
+// A lane reads 16 bytes of neighbouring channels where every row begins at a multiple of 16 bytes,
+// otherwise one channel.
+bool wide(int type, int channels, std::initializer_list<const void*> pointers,
+          std::initializer_list<long long> strides) {
+    const int v = 16 / sel_size(type);
+    if (channels % v) return false;
+    for (const void* p : pointers)
+        if (!sel_aligned(p, 16)) return false;
+    for (long long s : strides)
+        if (s % v) return false;
+    return true;
+}
+
+int check(const nhip_conv_args* a) {
+    if (!a || !a->weight || a->channels <= 0 || a->width < 1 || a->width > kMaxWidth) return NHIP_E_BADARG;
+    if (a->type < NHIP_F32 || a->type > NHIP_F16 || !sel_tokens_ok(a->tokens)) return NHIP_E_BADARG;
+    if (a->tokens.n_tokens && !a->x.p) return NHIP_E_BADARG;
+    if (sel_max_chunks(a->tokens, kChunk) > 0x7fffffffLL || a->channels > SEL_MAX_GRID_Y * NHIP_WAVE)
+        return NHIP_E_BADARG;
+    return 0;
+}
+
+bool grid(const nhip_conv_args& a, int v, dim3* g) {
+    const long long chunks = sel_max_chunks(a.tokens, kChunk);
+    *g = dim3((unsigned)chunks, (unsigned)((a.channels + NHIP_WAVE * v - 1) / (NHIP_WAVE * v)));
+    return chunks > 0;
+}
+
+}  // namespace
+
+extern "C" int nhip_causal_conv(void* stream, const nhip_conv_args* args) {
+    if (int e = check(args)) return e;
+    const nhip_conv_args& a = *args;
+    if (a.tokens.n_tokens && !a.y) return NHIP_E_BADARG;
+    int rc = NHIP_E_BADARG;
+    sel_with_type(a.type, [&](auto t) {
+        using T = decltype(t);
+        with_width(a.width, [&](auto k) {
+            constexpr int K = decltype(k)::value, V = 16 / sizeof(T);
+            dim3 g;
+            hipStream_t st = static_cast<hipStream_t>(stream);
+            if (wide(a.type, a.channels, {a.x.p, a.initial, a.y, a.final}, {a.x.seq, a.x.token})) {
+                if (grid(a, V, &g)) NHIP_LAUNCH((conv_kernel<T, V, K>), g, dim3(NHIP_WG), 0, st, a);
+            } else {
+                if (grid(a, 1, &g)) NHIP_LAUNCH((conv_kernel<T, 1, K>), g, dim3(NHIP_WG), 0, st, a);
+            }
+            rc = (int)hipGetLastError();
+        });
+    });
+    return rc;
+}
+
+extern "C" int nhip_causal_conv_grad_workspace(const nhip_conv_args* args, long long* bytes_out) {
+    if (int e = check(args)) return e;
+    if (!bytes_out) return NHIP_E_BADARG;
+    *bytes_out = sel_max_chunks(args->tokens, kChunk) * (args->width + 1) * args->channels * 4;
+    return 0;
+}
+
+extern "C" int nhip_causal_conv_grad(void* stream, const nhip_conv_args* args) {
+    long long need = 0;
+    if (int e = nhip_causal_conv_grad_workspace(args, &need)) return e;
+    const nhip_conv_args& a = *args;
+    if (a.tokens.n_tokens && (!a.dy.p || !a.dx)) return NHIP_E_BADARG;
+    if (!a.dweight || !a.dbias) return NHIP_E_BADARG;
+    if (need > a.workspace_bytes) return NHIP_E_TOOBIG;
+    if (need && !a.workspace) return NHIP_E_BADARG;
+    int rc = NHIP_E_BADARG;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    float* parts = static_cast<float*>(a.workspace);
+    sel_with_type(a.type, [&](auto t) {
+        using T = decltype(t);
+        with_width(a.width, [&](auto k) {
+            constexpr int K = decltype(k)::value, V = 16 / sizeof(T);
+            dim3 g;
+            if (wide(a.type, a.channels, {a.x.p, a.dy.p, a.initial, a.dfinal, a.dx, a.dinitial},
+                     {a.x.seq, a.x.token, a.dy.seq, a.dy.token})) {
+                if (grid(a, V, &g))
+                    NHIP_LAUNCH_FIRST((conv_grad_kernel<T, V, K>), g, dim3(NHIP_WG), 0, st, a, parts);
+            } else {
+                if (grid(a, 1, &g))
+                    NHIP_LAUNCH_FIRST((conv_grad_kernel<T, 1, K>), g, dim3(NHIP_WG), 0, st, a, parts);
+            }
+            rc = (int)hipGetLastError();
+        });
+    });
+    if (rc) return rc;
+    const int rows = (int)sel_max_chunks(a.tokens, kChunk);
+    const long long taps = (long long)a.width * a.channels, n = taps + a.channels;
+    // columns of a row of `parts`: tap k of channel d at k * channels + d; dweight is [channels, width]
+    return sel_reduce(st, SelReduce{parts, n, rows, taps, n, a.dweight, a.channels, a.width, a.dbias, nullptr});
+}
+
+extern "C" int nhip_causal_conv_step(void* stream, const nhip_conv_step_args* args) {
+    if (!args || !args->weight || args->channels <= 0 || args->width < 1 || args->width > kMaxWidth ||
+        args->n < 0 || args->n_slots < 0)
+        return NHIP_E_BADARG;
+    const nhip_conv_step_args& a = *args;
+    if (a.type < NHIP_F32 || a.type > NHIP_F16) return NHIP_E_BADARG;
+    if (a.n == 0) return 0;
+    if (!a.x || !a.y || (!a.state && a.width > 1)) return NHIP_E_BADARG;
+    int rc = NHIP_E_BADARG;
+    sel_with_type(a.type, [&](auto t) {
+        using T = decltype(t);
+        with_width(a.width, [&](auto k) {
+            constexpr int K = decltype(k)::value, V = 16 / sizeof(T);
+            hipStream_t st = static_cast<hipStream_t>(stream);
+            const bool w = wide(a.type, a.channels, {a.x, a.state, a.y}, {a.x_stride, a.state_stride});
+            const long long lanes = (long long)a.n * (w ? a.channels / V : a.channels);
+            const dim3 g((unsigned)((lanes + NHIP_WG - 1) / NHIP_WG));
+            if (w) NHIP_LAUNCH((conv_step_kernel<T, V, K>), g, dim3(NHIP_WG), 0, st, a);
+            else NHIP_LAUNCH((conv_step_kernel<T, 1, K>), g, dim3(NHIP_WG), 0, st, a);
+            rc = (int)hipGetLastError();
+        });
+    });
+    return rc;
+}

@@ -1,0 +1,433 @@
+// The gradient of the selective scan.
+//
+// Two walks over the chunks leave the state S that enters each chunk and the gradient G of the state
+// that leaves it; then every chunk stands for itself.  With L_ij = e^{c_i - c_j} for j <= i (else
+// 0), sums over the heads of a group for B and C, and X_ij = dy_i . x_j, K_ij = C_i . B_j:
+//     dx_j = step_j (sum_i K_ij L_ij dy_i + e^{c_Q - c_j} G B_j) + D dy_j
+//     dB_j = step_j (sum_i X_ij L_ij C_i  + e^{c_Q - c_j} G^T x_j)
+//     dC_i = sum_j X_ij L_ij step_j B_j   + e^{c_i} S^T dy_i
+// and the gradient of a_t = step_t A, through every decay that spans token t:
+//     da_t = sum_{i >= t > j} K_ij X_ij L_ij step_j + sum_{i >= t} q_i + sum_{j < t} r_j step_j + e^{c_Q} <G, S>
+//     q_i = e^{c_i} C_i . S^T dy_i,     r_j = e^{c_Q - c_j} B_j . G^T x_j
+//     dstep_t = A da_t + sum_{i >= t} K_it X_it L_it + r_t
+// None of these is a difference of sums over the sequence, so their errors do not grow with its length.
+// The first sum of da_t is formed from the strict row and column sums of one and the same matrix, in
+// which the terms with both tokens behind t cancel term by term.
+#include <type_traits>
+
+#include "selective_scan.h"
+
+namespace {
+
+struct GradPlan {
+    int vec, n_tiles;
+    int heads_per_group;   // heads that a work-group goes through
+    int blocks;            // work-groups for the heads of one group
+    long long n_chunks;
+    const float *S, *G;    // [chunk][head][dim][states]
+    float* parts;          // [chunk][3][head]: dA, dD, ddt_bias
+    float* shared;         // blocks > 1: [block][dB, dC][token][group][states]
+};
+
+template <class Tc, int NP> struct GradLds {
+    static constexpr int Q = sel_chunk_of(NP);
+    alignas(16) Tc x[Q * sel_stride<Tc>(64)];
+    alignas(16) Tc dy[Q * sel_stride<Tc>(64)];
+    alignas(16) Tc B[Q * sel_stride<Tc>(NP)];
+    alignas(16) Tc C[Q * sel_stride<Tc>(NP)];
+    alignas(16) Tc xl[Q * sel_stride<Tc>(Q)];  // [j][i]: X_ij L_ij step_j
+    alignas(16) Tc kl[Q * sel_stride<Tc>(Q)];  // [j][i]: K_ij L_ij step_j
+    SelSteps<Q> steps;
+    // sums of a head, by tile of the other index or by wave
+    float row[Q / 16][Q], col[Q / 16][Q], diag[Q], dot[Q], q[4][Q], r[4][Q], z[4];
+};
+
+// Eight elements of a state across its rows: k over 32 rows from p0, column n
+__device__ __forceinline__ void state_cols(const float* s, int p0, int n, int dim, int states, int g, float (&v)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int p = p0 + 16 * (e >> 2) + 4 * g + (e & 3);
+        v[e] = p < dim && n < states ? s[(long long)p * states + n] : 0.0f;
+    }
+}
+
+template <class T, class Tc, int NP>
+__global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPlan plan) {
+    using Lds = GradLds<Tc, NP>;
+    constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
+    constexpr int kTiles = QT * (QT + 1) / 2, kMyTiles = (kTiles + 3) / 4, kMyNT = (NT + 3) / 4;
+    constexpr int SX = sel_stride<Tc>(64), SN = sel_stride<Tc>(NP), SW = sel_stride<Tc>(Q);
+    constexpr int kSplits = SelSplit<Tc>::n;
+    extern __shared__ __align__(16) char lds_bytes[];
+    Lds& s = *reinterpret_cast<Lds*>(lds_bytes);
+
+    const int id = nhip_xcd_remap(blockIdx.x, gridDim.x);
+    const int block = id % plan.blocks, group = (id / plan.blocks) % a.n_groups;
+    const int chunk = id / (plan.blocks * a.n_groups);
+    const int per_group = a.n_heads / a.n_groups;
+    const int head0 = group * per_group + block * plan.heads_per_group;
+    const int head1 = min(head0 + plan.heads_per_group, (group + 1) * per_group);
+    const SelSeq seq = sel_seq_of_chunk(a.tokens, chunk, Q);
+    const int t0 = seq.chunk * Q, n = seq.seq < 0 ? 0 : min(Q, seq.n - t0);
+    float* const parts = plan.parts + (long long)chunk * 3 * a.n_heads;
+    if (n <= 0) {  // no such chunk, or an empty sequence's
+        for (int h = head0 + threadIdx.x; h < head1; h += NHIP_WG)
+            parts[h] = parts[a.n_heads + h] = parts[2 * a.n_heads + h] = 0.0f;
+        return;
+    }
+    const int tid = threadIdx.x, wave = tid / NHIP_WAVE, lane = tid & 63, l = tid & 15, g = lane >> 4;
+    const long long head_state = (long long)a.dim * a.states;
+    const bool vec_state = plan.vec & kSelVecState;
+
+    sel_stage<T, Tc, Q, NP>(s.B, sel_row<T>(a.B, a.tokens, seq, t0) + group * a.B.head, a.B.token, n, a.states,
+                            plan.vec & kSelVecB);
+    sel_stage<T, Tc, Q, NP>(s.C, sel_row<T>(a.C, a.tokens, seq, t0) + group * a.C.head, a.C.token, n, a.states,
+                            plan.vec & kSelVecC);
+    for (int q = tid; q < Q * SW; q += NHIP_WG) s.xl[q] = s.kl[q] = (Tc)0.0f;  // (i < j for good)
+    __syncthreads();
+
+    int tile_i[kMyTiles], tile_j[kMyTiles];  // this wave's tiles of the lower triangle
+    sel_f4 K[kMyTiles];                      // column j = 16 tile_j + l, rows i = 16 tile_i + 4 g + r
+#pragma unroll
+    for (int m = 0; m < kMyTiles; ++m) {
+        const int t = wave + 4 * m;
+        int it = 0;
+        while ((it + 1) * (it + 2) / 2 <= t) ++it;
+        tile_i[m] = t < kTiles ? it : -1;
+        tile_j[m] = t - it * (it + 1) / 2;
+        K[m] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (t < kTiles)
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks)
+                sel_mma(K[m], sel_rows(s.C + (16 * it + l) * SN + 32 * ks, g),
+                        sel_rows(s.B + (16 * tile_j[m] + l) * SN + 32 * ks, g));
+    }
+
+    sel_f4 dB[kMyNT][QT], dC[kMyNT][QT];  // states 16 (wave + 4 m) + 4 g + r of token 16 t + l
+#pragma unroll
+    for (int m = 0; m < kMyNT; ++m)
+#pragma unroll
+        for (int t = 0; t < QT; ++t) dB[m][t] = dC[m][t] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+
+    for (int head = head0; head < head1; ++head) {
+        const float D = a.D ? a.D[head] : 0.0f;
+        const float* const S = plan.S + ((long long)chunk * a.n_heads + head) * head_state;
+        const float* const G = plan.G + ((long long)chunk * a.n_heads + head) * head_state;
+        for (int tile = 0; tile < plan.n_tiles; ++tile) {
+            const int p_tile = tile * 64, cols = min(64, a.dim - p_tile);
+            __syncthreads();  // the tile before has been read
+            sel_stage<T, Tc, Q, 64>(s.x, sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n,
+                                    cols, plan.vec & kSelVecX);
+            sel_stage<T, Tc, Q, 64>(s.dy, sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token,
+                                    n, cols, plan.vec & kSelVecDy);
+            if (tile == 0) {
+                if (wave == 0) sel_steps<Q>(s.steps, a, seq, t0, head);
+                for (int q = tid; q < QT * Q; q += NHIP_WG) s.row[q / Q][q % Q] = s.col[q / Q][q % Q] = 0.0f;
+                for (int q = tid; q < 4 * Q; q += NHIP_WG) s.q[q / Q][q % Q] = s.r[q / Q][q % Q] = 0.0f;
+                if (tid < Q) s.diag[tid] = s.dot[tid] = 0.0f;
+                if (tid < 4) s.z[tid] = 0.0f;
+            }
+            __syncthreads();
+
+#pragma unroll
+            for (int m = 0; m < kMyTiles; ++m) {
+                if (tile_i[m] < 0) continue;
+                const int it = tile_i[m], jt = tile_j[m], j = 16 * jt + l, i0 = 16 * it + 4 * g;
+                sel_f4 X = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+                    sel_mma(X, sel_rows(s.dy + (16 * it + l) * SX + 32 * ks, g), sel_rows(s.x + j * SX + 32 * ks, g));
+                const float step = s.steps.step[j];
+                float kl[4], xl[4], below = 0.0f;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = i0 + r;
+                    const float L = i >= j ? sel_decay(s.steps, j, i) : 0.0f;
+                    const float ml = i >= j ? K[m][r] * X[r] * L : 0.0f;
+                    kl[r] = i >= j ? K[m][r] * L * step : 0.0f;
+                    xl[r] = i >= j ? X[r] * L * step : 0.0f;
+                    if (i == j) {
+                        s.diag[j] += ml;
+                        s.dot[j] += X[r];
+                    }
+                    const float strict = i > j ? ml : 0.0f;
+                    below += strict;
+                    float across = strict * step;  // over the 16 columns of the tile
+#pragma unroll
+                    for (int d = 1; d < 16; d *= 2) across += __shfl_xor(across, d);
+                    if (l == 0) s.row[jt][i] += across;
+                }
+                below += __shfl_xor(below, 16);
+                below += __shfl_xor(below, 32);
+                if (g == 0) s.col[it][j] += below;
+                sel_store<Tc, 4>(s.kl + j * SW + i0, kl);
+                sel_store<Tc, 4>(s.xl + j * SW + i0, xl);
+            }
+            __syncthreads();
+
+            // dx: 16 of the dimension to a wave
+            if (16 * wave < cols) {
+                const int p = p_tile + 16 * wave + l;
+                SelFrag<Tc> gf[NK];
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const int c = 32 * ks + 16 * h + 4 * g;
+                        sel_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+                        if (p < a.dim) v = sel_state_load(G + (long long)p * a.states, c, a.states, vec_state);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) gf[ks].set(4 * h + r, v[r]);
+                    }
+                SelFrag<Tc> df[QK];
+#pragma unroll
+                for (int ks = 0; ks < QK; ++ks) df[ks] = sel_cols(s.dy + 32 * ks * SX + 16 * wave, SX, l, g);
+#pragma unroll
+                for (int jt = 0; jt < QT; ++jt) {
+                    const int j = 16 * jt + l;
+                    sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int ks = 0; ks < NK; ++ks) sel_mma(acc, gf[ks], sel_rows(s.B + j * SN + 32 * ks, g));
+                    acc *= sel_decay(s.steps, j, Q - 1) * s.steps.step[j];
+#pragma unroll
+                    for (int ks = jt / 2; ks < QK; ++ks) sel_mma(acc, df[ks], sel_rows(s.kl + j * SW + 32 * ks, g));
+                    if (j < n) {
+                        const int c = 16 * wave + 4 * g;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[r] = fmaf(D, (float)s.dy[j * SX + c + r], acc[r]);
+                        T* row = static_cast<T*>(a.dx) + ((seq.row0 + t0 + j) * a.n_heads + head) * a.dim + p_tile;
+                        sel_store4(row, c, cols, plan.vec & kSelVecY, acc);
+                    }
+                }
+            }
+
+            // dB, dC: every fourth tile of the states to a wave
+            float z = 0.0f, qs[QT], rs[QT];
+#pragma unroll
+            for (int t = 0; t < QT; ++t) qs[t] = rs[t] = 0.0f;
+#pragma unroll
+            for (int m = 0; m < kMyNT; ++m) {
+                const int nt = wave + 4 * m;
+                if (nt >= NT) continue;
+                float Sv[2][8], Gv[2][8];
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    state_cols(S, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Sv[ks]);
+                    state_cols(G, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Gv[ks]);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) z = fmaf(Sv[ks][e], Gv[ks][e], z);
+                }
+                SelFrag<Tc> f[2][kSplits];
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Sv[ks], f[ks]);
+#pragma unroll
+                for (int it = 0; it < QT; ++it) {
+                    const int i = 16 * it + l;
+                    sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks) {
+                        const SelFrag<Tc> d = sel_rows(s.dy + i * SX + 32 * ks, g);
+#pragma unroll
+                        for (int q = 0; q < kSplits; ++q) sel_mma(acc, f[ks][q], d);
+                    }
+                    acc *= sel_decay_from_start(s.steps, i);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        qs[it] = fmaf(acc[r], (float)s.C[i * SN + 16 * nt + 4 * g + r], qs[it]);
+                    dC[m][it] += acc;
+#pragma unroll
+                    for (int ks = 0; ks <= it / 2; ++ks)
+                        sel_mma(dC[m][it], sel_cols(s.B + 32 * ks * SN + 16 * nt, SN, l, g),
+                                sel_cols(s.xl + 32 * ks * SW + 16 * it, SW, l, g));
+                }
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Gv[ks], f[ks]);
+#pragma unroll
+                for (int jt = 0; jt < QT; ++jt) {
+                    const int j = 16 * jt + l;
+                    sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int ks = 0; ks < 2; ++ks) {
+                        const SelFrag<Tc> d = sel_rows(s.x + j * SX + 32 * ks, g);
+#pragma unroll
+                        for (int q = 0; q < kSplits; ++q) sel_mma(acc, f[ks][q], d);
+                    }
+                    acc *= sel_decay(s.steps, j, Q - 1);
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        rs[jt] = fmaf(acc[r], (float)s.B[j * SN + 16 * nt + 4 * g + r], rs[jt]);
+                    dB[m][jt] += acc * s.steps.step[j];
+#pragma unroll
+                    for (int ks = jt / 2; ks < QK; ++ks)
+                        sel_mma(dB[m][jt], sel_cols(s.C + 32 * ks * SN + 16 * nt, SN, l, g),
+                                sel_rows(s.xl + j * SW + 32 * ks, g));
+                }
+            }
+            z = sel_wave_sum(z);
+            if (lane == 0) s.z[wave] += z;
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+                qs[t] += __shfl_xor(qs[t], 16);
+                qs[t] += __shfl_xor(qs[t], 32);
+                rs[t] += __shfl_xor(rs[t], 16);
+                rs[t] += __shfl_xor(rs[t], 32);
+                if (g == 0) {
+                    s.q[wave][16 * t + l] += qs[t];
+                    s.r[wave][16 * t + l] += rs[t];
+                }
+            }
+        }
+        __syncthreads();
+        if (wave == 0) {
+            float step = 0.0f, own = 0.0f, r = 0.0f, dot = 0.0f;
+            double behind = 0.0, passed = 0.0;  // what counts for this token and those in front of it / behind it
+            const bool live = lane < Q && lane < n;
+            if (live) {
+                step = s.steps.step[lane];
+                r = (s.r[0][lane] + s.r[1][lane]) + (s.r[2][lane] + s.r[3][lane]);
+                float row = 0.0f, col = 0.0f;
+#pragma unroll
+                for (int t = 0; t < QT; ++t) {
+                    row += s.row[t][lane];
+                    col += s.col[t][lane];
+                }
+                const float q = (s.q[0][lane] + s.q[1][lane]) + (s.q[2][lane] + s.q[3][lane]);
+                behind = (double)row + (double)q - (double)col * (double)step;
+                passed = (double)r * (double)step;
+                own = col + s.diag[lane] + r;
+                dot = s.dot[lane];
+            }
+            const double sum = sel_prefix(behind, lane), before = sel_prefix(passed, lane) - passed;
+            const double all = __shfl(sum, NHIP_WAVE - 1);
+            const float z = ((s.z[0] + s.z[1]) + (s.z[2] + s.z[3])) * sel_decay_from_start(s.steps, Q - 1);
+            float da = 0.0f, draw = 0.0f;
+            if (live) {
+                da = (float)((all - sum + behind) + before + (double)z);
+                draw = fmaf(a.A[head], da, own);
+                if (a.softplus) draw *= 1.0f / (1.0f + expf(-s.steps.raw[lane]));
+                sel_set_element(a.ddt, a.dt_type, (seq.row0 + t0 + lane) * a.n_heads + head, draw);
+            }
+            const float dA = sel_wave_sum(da * step), dD = sel_wave_sum(dot), dbias = sel_wave_sum(draw);
+            if (lane == 0) {
+                parts[head] = dA;
+                parts[a.n_heads + head] = dD;
+                parts[2 * a.n_heads + head] = dbias;
+            }
+        }
+    }
+
+    const long long row = (long long)a.n_groups * a.states;
+#pragma unroll
+    for (int m = 0; m < kMyNT; ++m) {
+        const int c = 16 * (wave + 4 * m) + 4 * g;
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+            const int i = 16 * t + l;
+            if (i >= n || c >= a.states) continue;
+            const long long at = (seq.row0 + t0 + i) * row + (long long)group * a.states;
+            if (plan.blocks == 1) {
+                sel_store4(static_cast<T*>(a.dB) + at, c, a.states, vec_state, dB[m][t]);
+                sel_store4(static_cast<T*>(a.dC) + at, c, a.states, vec_state, dC[m][t]);
+            } else {
+                float* out = plan.shared + (long long)block * 2 * a.tokens.n_tokens * row;
+                sel_state_store(out + at, c, a.states, vec_state, dB[m][t]);
+                sel_state_store(out + a.tokens.n_tokens * row + at, c, a.states, vec_state, dC[m][t]);
+            }
+        }
+    }
+}
+
+// dB and dC from the blocks of heads, in their order
+template <class T>
+__global__ __launch_bounds__(NHIP_WG) void add_blocks_kernel(const float* shared, int blocks, long long n, T* dB, T* dC) {
+    const long long i = (long long)blockIdx.x * NHIP_WG + threadIdx.x;
+    if (i >= 2 * n) return;
+    float sum = 0.0f;
+#pragma unroll 8
+    for (int b = 0; b < blocks; ++b) sum += shared[(long long)b * 2 * n + i];
+    if (i < n) dB[i] = (T)sum;
+    else dC[i - n] = (T)sum;
+}
+
+struct Layout {
+    long long n_chunks, states, parts, shared;  // floats
+    int heads_per_group, blocks;
+};
+
+Layout layout(const nhip_scan_args& a) {
+    Layout m;
+    m.n_chunks = sel_max_chunks(a.tokens, sel_chunk_tokens(a.states));
+    m.states = m.n_chunks * a.n_heads * a.dim * a.states;
+    m.parts = m.n_chunks * 3 * a.n_heads;
+    // Heads share a work-group, and with it B, C and the sums for their gradients, as long as there are
+    // work-groups for every compute unit twice over.
+    const int per_group = a.n_heads / a.n_groups;
+    long long blocks = m.n_chunks * a.n_groups > 0 ? (512 + m.n_chunks * a.n_groups - 1) / (m.n_chunks * a.n_groups) : 1;
+    if (blocks > per_group) blocks = per_group;
+    m.heads_per_group = (int)((per_group + blocks - 1) / blocks);
+    m.blocks = (per_group + m.heads_per_group - 1) / m.heads_per_group;
+    m.shared = m.blocks > 1 ? (long long)m.blocks * 2 * a.tokens.n_tokens * a.n_groups * a.states : 0;
+    return m;
+}
+
+long long round4(long long floats) { return (floats + 3) & ~3LL; }
+
+}  // namespace
+
+extern "C" int nhip_selective_scan_grad_workspace(const nhip_scan_args* args, long long* bytes_out) {
+    if (int e = sel_scan_check(args)) return e;
+    if (!bytes_out) return NHIP_E_BADARG;
+    const Layout m = layout(*args);
+    *bytes_out = 4 * (2 * round4(m.states) + round4(m.parts) + round4(m.shared));
+    return 0;
+}
+
+extern "C" int nhip_selective_scan_grad(void* stream, const nhip_scan_args* args) {
+    long long need = 0;
+    if (int e = nhip_selective_scan_grad_workspace(args, &need)) return e;
+    const nhip_scan_args& a = *args;
+    if (!a.dA || !a.dD || !a.ddt_bias) return NHIP_E_BADARG;
+    if (a.tokens.n_tokens && (!a.dy.p || !a.dx || !a.ddt || !a.dB || !a.dC)) return NHIP_E_BADARG;
+    if (need > a.workspace_bytes) return NHIP_E_TOOBIG;
+    if (need && (!a.workspace || !sel_aligned(a.workspace, 16))) return NHIP_E_BADARG;
+    const Layout m = layout(a);
+    const long long groups = m.n_chunks * a.n_groups * m.blocks;
+    if (groups > 0x7fffffffLL) return NHIP_E_BADARG;
+    hipStream_t st = static_cast<hipStream_t>(stream);
+    float* S = static_cast<float*>(a.workspace);
+    float* G = S + round4(m.states);
+    float* parts = G + round4(m.states);
+    float* shared = parts + round4(m.parts);
+    const SelWalkPlan w = sel_walk_plan(a, S);
+    if (int e = sel_walk<kSelStates>(st, a, w)) return e;
+    if (int e = sel_walk<kSelStatesBack>(st, a, sel_walk_plan(a, G))) return e;
+    int rc = 0;
+    if (groups) {
+        const GradPlan plan{w.vec, w.n_tiles, m.heads_per_group, m.blocks, m.n_chunks, S, G, parts, shared};
+        sel_with_type(a.type, [&](auto t) {
+            using T = decltype(t);
+            using Tc = typename SelCompute<T>::type;
+            sel_with_states(a.states, [&](auto np) {
+                constexpr int NP = decltype(np)::value;
+                constexpr size_t lds = sizeof(GradLds<Tc, NP>);
+                auto kernel = grad_kernel<T, Tc, NP>;
+                rc = sel_allow_lds(kernel, lds);
+                if (rc) return;
+                hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(NHIP_WG), lds, st, a, plan);
+                rc = (int)hipGetLastError();
+            });
+            if (!rc && m.blocks > 1) {
+                const long long n = a.tokens.n_tokens * a.n_groups * a.states;
+                if (n) {
+                    hipLaunchKernelGGL(add_blocks_kernel<T>, dim3((unsigned)((2 * n + NHIP_WG - 1) / NHIP_WG)),
+                                       dim3(NHIP_WG), 0, st, shared, m.blocks, n, static_cast<T*>(a.dB),
+                                       static_cast<T*>(a.dC));
+                    rc = (int)hipGetLastError();
+                }
+            }
+        });
+    }
+    if (rc) return rc;
+    const long long h = a.n_heads;
+    return sel_reduce(st, SelReduce{parts, 3 * h, (int)m.n_chunks, h, 2 * h, a.dA, h, 1, a.dD, a.ddt_bias});
+}

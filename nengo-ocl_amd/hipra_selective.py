@@ -1,0 +1,543 @@
+"""Operators of blocks that filter selectively: short causal convolution, selective scan, gated norm.
+
+A synapse of the simulator is a linear filter whose matrices are constant
+(`hipra_nonlinearities.plan_linearfilter`).  A selective scan is one whose step, input and
+output matrices come from the signal itself; with the short convolution in front of it and
+the gated norm around it, it makes a block that is trained on sequences and then answers
+token by token.  No counterpart in the reference.
+
+=====================  ===========================  ====================================
+immediate              bound to its arrays          C entry
+=====================  ===========================  ====================================
+causal_conv            plan_causal_conv             nhip_causal_conv
+causal_conv_grad       plan_causal_conv_grad        nhip_causal_conv_grad
+causal_conv_step       plan_causal_conv_step        nhip_causal_conv_step
+selective_scan         plan_selective_scan          nhip_selective_scan
+selective_scan_grad    plan_selective_scan_grad     nhip_selective_scan_grad
+selective_step         plan_selective_step          nhip_selective_step
+block_norm             plan_block_norm              nhip_block_norm
+block_norm_grad        plan_block_norm_grad         nhip_block_norm_grad
+=====================  ===========================  ====================================
+
+A ``plan_*`` function checks its arguments and returns a `Plan` bound to them, with the
+arrays that it writes as attributes; such plans go into a `Plans` list (a decoding step is
+recorded once and replayed).  The function without the prefix makes the plan and enqueues
+it once, in order with torch's current stream whatever stream the queue has.
+
+Arrays are torch tensors or `DeviceArray`, on the queue's device: float32, bfloat16 or
+float16 (parameters and states: float32).  Sequences lie side by side, ``[S, L, ...]``, or,
+with ``starts`` (int32, S + 1 offsets on the device, the layout of a ragged array's
+``starts``), back to back, ``[T, ...]``; sequences may be empty.  Rows may have any
+strides, the last axis has stride one.  ValueError and TypeError say what does not fit.
+"""
+
+import collections
+import ctypes
+
+from . import _lib
+from .hipraggedarray import DeviceArray, _torch
+from .plan import Plan
+
+c_int, c_ll, c_float, c_p = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, ctypes.c_void_p
+
+MAX_WIDTH = 8     # taps of the convolution
+MAX_STATES = 256  # states per row of a head
+
+ConvGradients = collections.namedtuple("ConvGradients", "x weight bias initial")
+ScanGradients = collections.namedtuple("ScanGradients", "x dt A B C D dt_bias initial")
+NormGradients = collections.namedtuple("NormGradients", "x weight gate residual scale")
+
+
+# ------------------------------------------------------- structs of nengo_hip_selective.h
+class _Rows(ctypes.Structure):
+    _fields_ = [("p", c_p), ("seq", c_ll), ("token", c_ll), ("head", c_ll)]
+
+
+class _Tokens(ctypes.Structure):
+    _fields_ = [("starts", c_p), ("n_tokens", c_ll), ("n_seqs", c_int), ("length", c_int)]
+
+
+class _ConvArgs(ctypes.Structure):
+    _fields_ = [("tokens", _Tokens), ("type", c_int), ("channels", c_int), ("width", c_int), ("silu", c_int),
+                ("x", _Rows), ("dy", _Rows), ("weight", c_p), ("bias", c_p), ("initial", c_p), ("y", c_p),
+                ("final", c_p), ("dfinal", c_p), ("dx", c_p), ("dinitial", c_p), ("dweight", c_p), ("dbias", c_p),
+                ("workspace", c_p), ("workspace_bytes", c_ll)]
+
+
+class _ConvStepArgs(ctypes.Structure):
+    _fields_ = [("type", c_int), ("channels", c_int), ("width", c_int), ("silu", c_int), ("n", c_int),
+                ("n_slots", c_int), ("slots", c_p), ("x", c_p), ("x_stride", c_ll), ("state_stride", c_ll),
+                ("weight", c_p), ("bias", c_p), ("state", c_p), ("y", c_p)]
+
+
+class _ScanArgs(ctypes.Structure):
+    _fields_ = [("tokens", _Tokens), ("type", c_int), ("dt_type", c_int), ("softplus", c_int), ("n_heads", c_int),
+                ("dim", c_int), ("n_groups", c_int), ("states", c_int), ("x", _Rows), ("dt", _Rows), ("B", _Rows),
+                ("C", _Rows), ("dy", _Rows), ("A", c_p), ("D", c_p), ("dt_bias", c_p), ("initial", c_p),
+                ("dfinal", c_p), ("y", c_p), ("final", c_p), ("dx", c_p), ("ddt", c_p), ("dB", c_p), ("dC", c_p),
+                ("dA", c_p), ("dD", c_p), ("ddt_bias", c_p), ("dinitial", c_p), ("workspace", c_p),
+                ("workspace_bytes", c_ll)]
+
+
+class _ScanStepArgs(ctypes.Structure):
+    _fields_ = [("type", c_int), ("dt_type", c_int), ("softplus", c_int), ("n_heads", c_int), ("dim", c_int),
+                ("n_groups", c_int), ("states", c_int), ("n", c_int), ("n_slots", c_int), ("slots", c_p),
+                ("x", _Rows), ("dt", _Rows), ("B", _Rows), ("C", _Rows), ("A", c_p), ("D", c_p), ("dt_bias", c_p),
+                ("state", c_p), ("state_stride", c_ll), ("y", c_p)]
+
+
+class _NormArgs(ctypes.Structure):
+    _fields_ = [("type", c_int), ("channels", c_int), ("groups", c_int), ("after", c_int), ("rows", c_ll),
+                ("eps", c_float), ("x", c_p), ("gate", c_p), ("residual", c_p), ("x_stride", c_ll),
+                ("gate_stride", c_ll), ("residual_stride", c_ll), ("weight", c_p), ("scale", c_p), ("out", c_p),
+                ("v_out", c_p), ("dout", c_p), ("dv", c_p), ("dout_stride", c_ll), ("dv_stride", c_ll), ("dx", c_p),
+                ("dgate", c_p), ("dresidual", c_p), ("dweight", c_p), ("dscale", c_p), ("workspace", c_p),
+                ("workspace_bytes", c_ll)]
+
+
+# ------------------------------------------------------------------------ argument checks
+_codes = {}
+
+
+def _type_code(name, t):
+    if not _codes:
+        torch = _torch()
+        _codes.update({torch.float32: 0, torch.bfloat16: 1, torch.float16: 2})
+    code = _codes.get(t.dtype)
+    if code is None:
+        raise TypeError("%s is %s: float32, bfloat16 or float16 are known" % (name, t.dtype))
+    return code
+
+
+def _array(queue, name, t, shape, dtype, contiguous=False):
+    """The tensor behind an argument, after its checks: its shape, type, device and the stride of its last axis."""
+    if isinstance(t, DeviceArray):
+        t = t.tensor
+    if dtype is not None and t.dtype != dtype:
+        raise TypeError("%s is %s, not %s" % (name, t.dtype, dtype))
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
+    if t.device != queue.device:
+        raise ValueError("%s is on %s, the queue on %s" % (name, t.device, queue.device))
+    if contiguous:
+        if not t.is_contiguous():
+            raise ValueError("%s has to be contiguous" % name)
+    elif t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
+        raise ValueError("%s has stride %d along its last axis, not 1" % (name, t.stride(-1)))
+    return t
+
+
+def _parameter(queue, name, t, shape):
+    return None if t is None else _array(queue, name, t, shape, _torch().float32, contiguous=True)
+
+
+def _output(queue, name, t, shape, dtype):
+    """An array to write: the caller's, or a new one."""
+    if t is None:
+        return _torch().empty(shape, dtype=dtype, device=queue.device)
+    return _array(queue, name, t, shape, dtype, contiguous=True)
+
+
+def _ptr(t):
+    return None if t is None else t.data_ptr() or None
+
+
+def _plain(t):
+    return t.tensor if isinstance(t, DeviceArray) else t
+
+
+def _tokens(queue, x, starts, axes):
+    """(struct, leading sizes of row arrays, sequences, the tensor of starts) of `x` with `axes` axes behind the tokens."""
+    lead = x.dim() - axes
+    if starts is None:
+        if lead != 2:
+            raise ValueError("x has %d axes: [S, L, ...] needs %d, back-to-back sequences need `starts`"
+                             % (x.dim(), 2 + axes))
+        s, n = x.shape[0], x.shape[1]
+        if s * n > 0x7fffffff:
+            raise ValueError("%d tokens: at most 2**31 - 1 in a call" % (s * n))
+        return _Tokens(None, s * n, s, n), (s, n), s, None
+    if lead != 1:
+        raise ValueError("x has %d axes: with `starts` it has %d, [T, ...]" % (x.dim(), 1 + axes))
+    starts = _plain(starts)
+    if starts.dim() != 1 or starts.shape[0] < 1:
+        raise ValueError("starts has shape %s: S + 1 offsets are wanted" % (tuple(starts.shape),))
+    starts = _array(queue, "starts", starts, starts.shape, _torch().int32, contiguous=True)
+    t, s = x.shape[0], starts.shape[0] - 1
+    if t > 0x7fffffff:
+        raise ValueError("%d tokens: at most 2**31 - 1 in a call" % t)
+    return _Tokens(starts.data_ptr(), t, s, 0), (t,), s, starts
+
+
+def _rows(t, lead, heads=False):
+    """How the rows of `t` lie: [S, L, (heads,) ...] or [T, (heads,) ...]."""
+    st = t.stride()
+    if lead == 2:
+        return _Rows(_ptr(t), st[0], st[1], st[2] if heads else 0)
+    return _Rows(_ptr(t), 0, st[0], st[1] if heads else 0)
+
+
+def _activation(name):
+    if name not in (None, "silu"):
+        raise ValueError("activation is %r: None and 'silu' are known" % (name,))
+    return int(name == "silu")
+
+
+def _slots(queue, slots, n, n_slots):
+    if slots is None:
+        if n > n_slots:
+            raise ValueError("%d requests for a state with %d slots" % (n, n_slots))
+        return None
+    return _array(queue, "slots", slots, (n,), _torch().int32, contiguous=True)
+
+
+def _workspace(queue, args, entry):
+    need = c_ll()
+    _lib.check(entry(ctypes.byref(args), ctypes.byref(need)), "workspace")
+    if not need.value:
+        return None
+    space = _torch().empty(need.value, dtype=_torch().uint8, device=queue.device)
+    args.workspace, args.workspace_bytes = space.data_ptr(), need.value
+    return space
+
+
+def _plan(queue, entry, args, keep, name, tag, **results):
+    plan = Plan(queue, entry, (ctypes.byref(args),), gsize=(64,), full_args=(args,) + tuple(keep), name=name, tag=tag)
+    for key, value in results.items():
+        setattr(plan, key, value)
+    return plan
+
+
+def _enqueue(queue, plan):
+    """Enqueue once, in order with torch's current stream: the plan's arrays were made there, and are used there next."""
+    current = _torch().cuda.current_stream(queue.device)
+    if current.cuda_stream == queue.stream.cuda_stream:
+        plan.enqueue()
+        return plan
+    queue.stream.wait_stream(current)
+    plan.enqueue()
+    current.wait_stream(queue.stream)
+    return plan
+
+
+# ----------------------------------------------------------------- short causal convolution
+def _conv(queue, x, weight, bias, activation, initial, starts):
+    x, weight = _plain(x), _plain(weight)
+    code = _type_code("x", x)
+    if weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_WIDTH:
+        raise ValueError("weight has shape %s: [channels, width] with a width of 1 to %d is wanted"
+                         % (tuple(weight.shape), MAX_WIDTH))
+    d, k = weight.shape
+    tokens, lead, s, starts = _tokens(queue, x, starts, 1)
+    x = _array(queue, "x", x, lead + (d,), None)
+    weight, bias = _parameter(queue, "weight", weight, (d, k)), _parameter(queue, "bias", bias, (d,))
+    if initial is not None:
+        initial = _array(queue, "initial", initial, (s, k - 1, d), x.dtype, contiguous=True)
+    if d < 1:
+        raise ValueError("x has no channels")
+    args = _ConvArgs(tokens=tokens, type=code, channels=d, width=k, silu=_activation(activation),
+                     x=_rows(x, len(lead)), weight=_ptr(weight), bias=_ptr(bias), initial=_ptr(initial))
+    return args, x, lead, (s, k - 1, d), [x, weight, bias, initial, starts]
+
+
+def plan_causal_conv(queue, x, weight, bias=None, activation=None, initial=None, starts=None, y=None, final=None,
+                     tag=None):
+    """``y[t] = f(bias + sum_k weight[:, k] * x[t - width + 1 + k])``, channel by channel; f is the
+    identity or (``activation="silu"``) v sigmoid(v).  In front of a sequence's first token lies
+    `initial` ``[S, width - 1, channels]``, or zeros.  ``plan.y``, and ``plan.final``: the last
+    width - 1 inputs of each sequence, what `causal_conv_step` goes on with."""
+    args, x, lead, ends, keep = _conv(queue, x, weight, bias, activation, initial, starts)
+    y = _output(queue, "y", y, x.shape, x.dtype)
+    final = _output(queue, "final", final, ends, x.dtype)
+    args.y, args.final = _ptr(y), _ptr(final)
+    return _plan(queue, queue.lib.nhip_causal_conv, args, keep + [y, final], "hip_causal_conv", tag, y=y, final=final)
+
+
+def causal_conv(queue, x, weight, bias=None, activation=None, initial=None, starts=None):
+    """(y, final): see `plan_causal_conv`."""
+    plan = _enqueue(queue, plan_causal_conv(queue, x, weight, bias, activation, initial, starts))
+    return plan.y, plan.final
+
+
+def plan_causal_conv_grad(queue, dy, x, weight, bias=None, activation=None, initial=None, starts=None, dfinal=None,
+                          tag=None):
+    """The gradient of `plan_causal_conv`, from `dy` and (where it went on) `dfinal`; ``plan.gradients``."""
+    torch = _torch()
+    args, x, lead, ends, keep = _conv(queue, x, weight, bias, activation, initial, starts)
+    dy = _array(queue, "dy", dy, x.shape, x.dtype)
+    if dfinal is not None:
+        dfinal = _array(queue, "dfinal", dfinal, ends, x.dtype, contiguous=True)
+    d, k = args.channels, args.width
+    dx, dweight = _output(queue, "dx", None, x.shape, x.dtype), _output(queue, "dweight", None, (d, k), torch.float32)
+    dbias = _output(queue, "dbias", None, (d,), torch.float32)
+    dinitial = None if initial is None else _output(queue, "dinitial", None, ends, x.dtype)
+    args.dy, args.dfinal = _rows(dy, len(lead)), _ptr(dfinal)
+    args.dx, args.dinitial, args.dweight, args.dbias = _ptr(dx), _ptr(dinitial), _ptr(dweight), _ptr(dbias)
+    space = _workspace(queue, args, queue.lib.nhip_causal_conv_grad_workspace)
+    got = ConvGradients(dx, dweight, None if bias is None else dbias, dinitial)
+    return _plan(queue, queue.lib.nhip_causal_conv_grad, args, keep + [dy, dfinal, dbias, space, got],
+                 "hip_causal_conv_grad", tag, gradients=got)
+
+
+def causal_conv_grad(queue, dy, x, weight, bias=None, activation=None, initial=None, starts=None, dfinal=None):
+    """`ConvGradients` (x, weight, bias, initial): see `plan_causal_conv_grad`."""
+    return _enqueue(queue, plan_causal_conv_grad(queue, dy, x, weight, bias, activation, initial, starts,
+                                                 dfinal)).gradients
+
+
+def plan_causal_conv_step(queue, state, x, weight, bias=None, activation=None, slots=None, y=None, tag=None):
+    """One token each of n requests, `x` ``[n, channels]``: `state` ``[slots, width - 1, channels]`` holds
+    the inputs before it, oldest first, and moves on by one.  Request r has the slot ``slots[r]`` (int32;
+    each at most once), or r; one outside the state gets zeros.  ``plan.y``."""
+    state, x, weight = _plain(state), _plain(x), _plain(weight)
+    code = _type_code("x", x)
+    if weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_WIDTH:
+        raise ValueError("weight has shape %s: [channels, width] with a width of 1 to %d is wanted"
+                         % (tuple(weight.shape), MAX_WIDTH))
+    if state.dim() != 3 or x.dim() != 2:
+        raise ValueError("state and x have %d and %d axes, not 3 and 2" % (state.dim(), x.dim()))
+    (d, k), n, n_slots = weight.shape, x.shape[0], state.shape[0]
+    x = _array(queue, "x", x, (n, d), None)
+    state = _array(queue, "state", state, (n_slots, k - 1, d), x.dtype)
+    if k > 2 and state.stride(1) != d:
+        raise ValueError("a slot of the state has to be contiguous")
+    weight, bias = _parameter(queue, "weight", weight, (d, k)), _parameter(queue, "bias", bias, (d,))
+    slots = _slots(queue, slots, n, n_slots)
+    y = _output(queue, "y", y, (n, d), x.dtype)
+    if d < 1:
+        raise ValueError("x has no channels")
+    args = _ConvStepArgs(type=code, channels=d, width=k, silu=_activation(activation), n=n, n_slots=n_slots,
+                         slots=_ptr(slots), x=_ptr(x), x_stride=x.stride(0), state_stride=state.stride(0),
+                         weight=_ptr(weight), bias=_ptr(bias), state=_ptr(state), y=_ptr(y))
+    return _plan(queue, queue.lib.nhip_causal_conv_step, args, (state, x, weight, bias, slots, y),
+                 "hip_causal_conv_step", tag, y=y)
+
+
+def causal_conv_step(queue, state, x, weight, bias=None, activation=None, slots=None):
+    """y: see `plan_causal_conv_step`."""
+    return _enqueue(queue, plan_causal_conv_step(queue, state, x, weight, bias, activation, slots)).y
+
+
+# ------------------------------------------------------------------------- selective scan
+def _scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts):
+    x, B = _plain(x), _plain(B)
+    code = _type_code("x", x)
+    tokens, lead, s, starts = _tokens(queue, x, starts, 2)
+    h, p = x.shape[-2:]
+    if B.dim() != len(lead) + 2:
+        raise ValueError("B has %d axes, x has %d" % (B.dim(), x.dim()))
+    g, n = B.shape[-2:]
+    if h < 1 or p < 1 or g < 1 or h % g:
+        raise ValueError("%d heads of %d in %d groups: every group has the same heads" % (h, p, g))
+    if not 1 <= n <= MAX_STATES:
+        raise ValueError("%d states: 1 to %d are known" % (n, MAX_STATES))
+    x = _array(queue, "x", x, lead + (h, p), None)
+    B, C = _array(queue, "B", B, lead + (g, n), x.dtype), _array(queue, "C", C, lead + (g, n), x.dtype)
+    dt = _plain(dt)
+    dt_code = _type_code("dt", dt)
+    if tuple(dt.shape) != lead + (h,) or dt.device != queue.device:
+        raise ValueError("dt has shape %s on %s, not %s on %s" % (tuple(dt.shape), dt.device, lead + (h,), queue.device))
+    if A is None:
+        raise TypeError("A is None")
+    A, D, dt_bias = (_parameter(queue, k, v, (h,)) for k, v in (("A", A), ("D", D), ("dt_bias", dt_bias)))
+    initial = _parameter(queue, "initial", initial, (s, h, p, n))
+    args = _ScanArgs(tokens=tokens, type=code, dt_type=dt_code, softplus=int(bool(softplus)), n_heads=h, dim=p,
+                     n_groups=g, states=n, x=_rows(x, len(lead), True), dt=_rows(dt, len(lead), True),
+                     B=_rows(B, len(lead), True), C=_rows(C, len(lead), True), A=_ptr(A), D=_ptr(D),
+                     dt_bias=_ptr(dt_bias), initial=_ptr(initial))
+    return args, x, dt, B, lead, (s, h, p, n), [x, dt, A, B, C, D, dt_bias, initial, starts]
+
+
+def plan_selective_scan(queue, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None, starts=None, y=None,
+                        final=None, tag=None):
+    """The scan of `x` ``[..., heads, dim]``: with ``step = f(dt + dt_bias)`` (f: identity or softplus),
+
+        S[t] = exp(step A) S[t - 1] + step x[t] (outer) B[t],     y[t] = S[t] C[t] + D x[t]
+
+    per head, S of ``dim x states`` in float32.  `dt` ``[..., heads]``; `B`, `C` ``[..., groups, states]``,
+    each for heads / groups heads; `A` (rates, below zero for a filter that forgets), `D`, `dt_bias`
+    ``[heads]``.  `initial` ``[S, heads, dim, states]`` enters, or zeros.  ``plan.y``, ``plan.final``."""
+    torch = _torch()
+    args, x, _, _, _, ends, keep = _scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts)
+    y = _output(queue, "y", y, x.shape, x.dtype)
+    final = _output(queue, "final", final, ends, torch.float32)
+    args.y, args.final = _ptr(y), _ptr(final)
+    space = _workspace(queue, args, queue.lib.nhip_selective_scan_workspace)
+    return _plan(queue, queue.lib.nhip_selective_scan, args, keep + [y, final, space], "hip_selective_scan", tag, y=y,
+                 final=final)
+
+
+def selective_scan(queue, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None, starts=None):
+    """(y, final): see `plan_selective_scan`."""
+    plan = _enqueue(queue, plan_selective_scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts))
+    return plan.y, plan.final
+
+
+def plan_selective_scan_grad(queue, dy, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None,
+                             starts=None, dfinal=None, tag=None):
+    """The gradient of `plan_selective_scan`, from `dy` and (where the state went on) `dfinal`; it needs
+    nothing that the forward pass computed.  ``plan.gradients``: those of A, D and dt_bias are float32."""
+    torch = _torch()
+    args, x, dt, B, lead, ends, keep = _scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts)
+    dy = _array(queue, "dy", dy, x.shape, x.dtype)
+    dfinal = _parameter(queue, "dfinal", dfinal, ends)
+    h = args.n_heads
+    dx, ddt = (_output(queue, "", None, v.shape, v.dtype) for v in (x, dt))
+    dB, dC = (_output(queue, "", None, B.shape, B.dtype) for _ in range(2))
+    dA, dD, dbias = (_output(queue, "", None, (h,), torch.float32) for _ in range(3))
+    dinitial = None if initial is None else _output(queue, "", None, ends, torch.float32)
+    args.dy, args.dfinal = _rows(dy, len(lead), True), _ptr(dfinal)
+    args.dx, args.ddt, args.dB, args.dC = _ptr(dx), _ptr(ddt), _ptr(dB), _ptr(dC)
+    args.dA, args.dD, args.ddt_bias, args.dinitial = _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dinitial)
+    space = _workspace(queue, args, queue.lib.nhip_selective_scan_grad_workspace)
+    got = ScanGradients(dx, ddt, dA, dB, dC, None if D is None else dD, None if dt_bias is None else dbias, dinitial)
+    return _plan(queue, queue.lib.nhip_selective_scan_grad, args, keep + [dy, dfinal, dD, dbias, space, got],
+                 "hip_selective_scan_grad", tag, gradients=got)
+
+
+def selective_scan_grad(queue, dy, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None, starts=None,
+                        dfinal=None):
+    """`ScanGradients` (x, dt, A, B, C, D, dt_bias, initial): see `plan_selective_scan_grad`."""
+    return _enqueue(queue, plan_selective_scan_grad(queue, dy, x, dt, A, B, C, D, dt_bias, softplus, initial, starts,
+                                                    dfinal)).gradients
+
+
+def plan_selective_step(queue, state, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, slots=None, y=None,
+                        tag=None):
+    """One token each of n requests: `x` ``[n, heads, dim]``, `dt` ``[n, heads]``, `B`, `C`
+    ``[n, groups, states]``; `state` ``[slots, heads, dim, states]`` (float32) is moved on by a token.  Slots
+    as for `plan_causal_conv_step`.  ``plan.y``."""
+    torch = _torch()
+    state, x, B, dt = _plain(state), _plain(x), _plain(B), _plain(dt)
+    code, dt_code = _type_code("x", x), _type_code("dt", dt)
+    if x.dim() != 3 or B.dim() != 3 or state.dim() != 4:
+        raise ValueError("x, B and state have %d, %d and %d axes, not 3, 3 and 4" % (x.dim(), B.dim(), state.dim()))
+    n, h, p = x.shape
+    g, k = B.shape[1:]
+    if h < 1 or p < 1 or g < 1 or h % g:
+        raise ValueError("%d heads of %d in %d groups: every group has the same heads" % (h, p, g))
+    if not 1 <= k <= MAX_STATES:
+        raise ValueError("%d states: 1 to %d are known" % (k, MAX_STATES))
+    n_slots = state.shape[0]
+    x = _array(queue, "x", x, (n, h, p), None)
+    B, C = _array(queue, "B", B, (n, g, k), x.dtype), _array(queue, "C", C, (n, g, k), x.dtype)
+    if tuple(dt.shape) != (n, h) or dt.device != queue.device:
+        raise ValueError("dt has shape %s on %s, not %s on %s" % (tuple(dt.shape), dt.device, (n, h), queue.device))
+    if A is None:
+        raise TypeError("A is None")
+    A, D, dt_bias = (_parameter(queue, name, v, (h,)) for name, v in (("A", A), ("D", D), ("dt_bias", dt_bias)))
+    state = _array(queue, "state", state, (n_slots, h, p, k), torch.float32)
+    if n_slots and not state[0].is_contiguous():
+        raise ValueError("a slot of the state has to be contiguous")
+    slots = _slots(queue, slots, n, n_slots)
+    y = _output(queue, "y", y, (n, h, p), x.dtype)
+    args = _ScanStepArgs(type=code, dt_type=dt_code, softplus=int(bool(softplus)), n_heads=h, dim=p, n_groups=g,
+                         states=k, n=n, n_slots=n_slots, slots=_ptr(slots), x=_rows(x, 1, True), dt=_rows(dt, 1, True),
+                         B=_rows(B, 1, True), C=_rows(C, 1, True), A=_ptr(A), D=_ptr(D), dt_bias=_ptr(dt_bias),
+                         state=_ptr(state), state_stride=state.stride(0), y=_ptr(y))
+    return _plan(queue, queue.lib.nhip_selective_step, args, (state, x, dt, A, B, C, D, dt_bias, slots, y),
+                 "hip_selective_step", tag, y=y)
+
+
+def selective_step(queue, state, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, slots=None):
+    """y: see `plan_selective_step`."""
+    return _enqueue(queue, plan_selective_step(queue, state, x, dt, A, B, C, D, dt_bias, softplus, slots)).y
+
+
+# ----------------------------------------------------------------------------- gated norm
+def _flat(queue, name, t, like):
+    """(tensor, row stride) of an array [..., channels] whose leading axes make rows of one stride."""
+    t = _array(queue, name, t, like.shape, like.dtype)
+    if t.dim() == 2:
+        return t, t.stride(0)
+    try:
+        rows = t.view(-1, t.shape[-1])
+    except RuntimeError:
+        raise ValueError("the rows of %s do not lie at one distance" % name)
+    return rows, rows.stride(0)
+
+
+def _norm(queue, x, weight, gate, residual, scale, groups, eps, after):
+    x = _plain(x)
+    code = _type_code("x", x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError("x has shape %s: [..., channels] is wanted" % (tuple(x.shape),))
+    d, groups = x.shape[-1], int(groups)
+    if groups < 1 or d % groups:
+        raise ValueError("%d channels in %d groups: every group has as many" % (d, groups))
+    if scale is not None and residual is None:
+        raise ValueError("scale goes with a residual")
+    if not eps >= 0.0:
+        raise ValueError("eps is %r" % (eps,))
+    weight, scale = _parameter(queue, "weight", weight, (d,)), _parameter(queue, "scale", scale, (d,))
+    if weight is None:
+        raise TypeError("weight is None")
+    args = _NormArgs(type=code, channels=d, groups=groups, after=int(bool(after)), rows=x.numel() // d,
+                     eps=float(eps), weight=_ptr(weight), scale=_ptr(scale))
+    keep = [weight, scale]
+    for name, t in (("x", x), ("gate", gate), ("residual", residual)):
+        if t is not None:
+            t, stride = _flat(queue, name, t, x)
+            setattr(args, name, _ptr(t))
+            setattr(args, name + "_stride", stride)
+            keep.append(t)
+    return args, x, residual is not None and not after, keep
+
+
+def plan_block_norm(queue, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False, out=None,
+                    v=None, tag=None):
+    """The norm of ``u = x`` or ``x * gate * sigmoid(gate)``, in front of a block or (`after`) behind it:
+
+        before:  v = residual + scale * u,   out = v / sqrt(mean(v**2) + eps) * weight
+        after:   out = residual + scale * (u / sqrt(mean(u**2) + eps) * weight)
+
+    with means over each of `groups` equal parts of the last axis.  `residual` (like x) and `scale`
+    (``[channels]``, ones) are optional.  ``plan.out``, and ``plan.v`` where there is a residual in front."""
+    args, x, before, keep = _norm(queue, x, weight, gate, residual, scale, groups, eps, after)
+    out = _output(queue, "out", out, x.shape, x.dtype)
+    if v is not None and not before:
+        raise ValueError("v is written with a residual in front of a block only")
+    v = _output(queue, "v", v, x.shape, x.dtype) if before else None
+    args.out, args.v_out = _ptr(out), _ptr(v)
+    return _plan(queue, queue.lib.nhip_block_norm, args, keep + [out, v], "hip_block_norm", tag, out=out, v=v)
+
+
+def block_norm(queue, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False):
+    """(out, v or None): see `plan_block_norm`."""
+    plan = _enqueue(queue, plan_block_norm(queue, x, weight, gate, residual, scale, groups, eps, after))
+    return plan.out, plan.v
+
+
+def plan_block_norm_grad(queue, dout, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False,
+                         dv=None, tag=None):
+    """The gradient of `plan_block_norm`, from `dout` and (with a residual in front) `dv`;
+    ``plan.gradients``: those of weight and scale are float32."""
+    torch = _torch()
+    args, x, before, keep = _norm(queue, x, weight, gate, residual, scale, groups, eps, after)
+    d = args.channels
+    plain_dout = dout = _plain(dout)
+    dout, args.dout_stride = _flat(queue, "dout", dout, x)
+    args.dout = _ptr(dout)
+    if dv is not None:
+        if not before:
+            raise ValueError("dv goes with a residual in front of a block")
+        dv, args.dv_stride = _flat(queue, "dv", dv, x)
+        args.dv = _ptr(dv)
+    dx = _output(queue, "", None, x.shape, x.dtype)
+    dgate = None if gate is None else _output(queue, "", None, x.shape, x.dtype)
+    dresidual = _output(queue, "", None, x.shape, x.dtype) if before else None
+    dweight, dscale = (_output(queue, "", None, (d,), torch.float32) for _ in range(2))
+    args.dx, args.dgate, args.dresidual = _ptr(dx), _ptr(dgate), _ptr(dresidual)
+    args.dweight, args.dscale = _ptr(dweight), _ptr(dscale)
+    space = _workspace(queue, args, queue.lib.nhip_block_norm_grad_workspace)
+    got = NormGradients(dx, dweight, dgate, None if residual is None else dresidual if before else plain_dout,
+                        None if scale is None else dscale)
+    return _plan(queue, queue.lib.nhip_block_norm_grad, args, keep + [dout, dv, dscale, space, got],
+                 "hip_block_norm_grad", tag, gradients=got)
+
+
+def block_norm_grad(queue, dout, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False,
+                    dv=None):
+    """`NormGradients` (x, weight, gate, residual, scale): see `plan_block_norm_grad`."""
+    return _enqueue(queue, plan_block_norm_grad(queue, dout, x, weight, gate, residual, scale, groups, eps, after,
+                                                dv)).gradients
