@@ -320,8 +320,9 @@ bool wide(const nhip_norm_args& a) {
 
 int check(const nhip_norm_args* a) {
     if (!a || a->channels <= 0 || a->groups <= 0 || a->channels % a->groups || a->rows < 0) return NHIP_E_BADARG;
-    if (a->type < NHIP_F32 || a->type > NHIP_F16 || !a->weight || (a->scale && !a->residual)) return NHIP_E_BADARG;
-    if (a->rows && (!a->x)) return NHIP_E_BADARG;
+    if (a->type < NHIP_F32 || a->type > NHIP_F16 || !a->weight) return NHIP_E_BADARG;
+    // (arrays without elements may be null)
+    if (a->rows && (!a->x || (a->scale && !a->residual))) return NHIP_E_BADARG;
     if (a->rows * a->groups > 0x7fffffffLL || a->groups > SEL_MAX_GRID_Y) return NHIP_E_BADARG;
     return 0;
 }

@@ -177,6 +177,17 @@ __device__ __forceinline__ float sel_wave_sum(float v) {
     return v;
 }
 
+// Over the 16 lanes of a quarter of the wave, by rotations within it
+template <int N> __device__ __forceinline__ float sel_rotated(float v) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), 0x120 + N, 0xf, 0xf, false));
+}
+__device__ __forceinline__ float sel_row_sum(float v) {
+    v += sel_rotated<8>(v);
+    v += sel_rotated<4>(v);
+    v += sel_rotated<2>(v);
+    return v + sel_rotated<1>(v);
+}
+
 // Column sums of parts[rows][n], always in the same order: 16 waves take a share of the rows each.
 // The columns go to up to three results: those below `split` to out[(c % width) * stride + c / width]
 // (a transposition where the rows hold another order than the result), those below `split2` to out2,

@@ -42,6 +42,20 @@ __device__ __forceinline__ void sel_mma(sel_f4& acc, const SelFrag<float>& a, co
     for (int e = 0; e < 8; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(a.v[e], b.v[e], acc, 0, 0, 0);
 }
 
+// Waits until the products before it are done and leaves their sums in vector registers.  A result that
+// is read behind a branch needs this: the wait states between a matrix instruction and what
+// reads its registers are the program's to keep, and this compiler counts them within a block
+// (roc-7.2.0: a branch right behind the instruction led to reads one wait state after it, which
+// returned the last of the four registers' old value).
+__device__ __forceinline__ void sel_settle(sel_f4& a) { asm volatile("s_nop 15" : "+v"(a)); }
+__device__ __forceinline__ void sel_settle(sel_f4& a, sel_f4& b) { asm volatile("s_nop 15" : "+v"(a), "+v"(b)); }
+template <int N> __device__ __forceinline__ void sel_settle(sel_f4 (&a)[N]) {
+    if constexpr (N == 1) sel_settle(a[0]);
+#pragma unroll
+    for (int i = 0; i + 1 < N; i += 2) sel_settle(a[i], a[i + 1]);
+    if constexpr (N > 1 && N % 2 == 1) sel_settle(a[N - 1]);
+}
+
 // Fragment of a matrix in LDS whose rows run along k: `row` is this lane's row, at the first k.
 __device__ __forceinline__ SelFrag<__bf16> sel_rows(const __bf16* row, int g) {
     const sel_b4 lo = *reinterpret_cast<const sel_b4*>(row + 4 * g);
@@ -94,95 +108,132 @@ __device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<Tc> (&f)[
     }
 }
 
-// Row length in LDS: `n` elements (a multiple of 8) and 16 bytes, so that the rows of a tile begin
-// in different banks and at multiples of 16 bytes.
+// Row length in LDS of `n` elements (a multiple of 32).  Reads of rows (sel_rows) meet no bank twice with
+// 16 bytes more than the elements, reads across 16-bit rows (sel_cols) with 32.
 template <class Tc> __host__ __device__ constexpr int sel_stride(int n) { return n + 16 / (int)sizeof(Tc); }
+template <class Tc> __host__ __device__ constexpr int sel_stride_cols(int n) {
+    return n + (sizeof(Tc) == 2 ? 16 : 4);
+}
 
-// Rows of inputs into LDS, zero beyond their ends: ROWS x COLS from `src` (row stride `stride`), of which
-// n_rows x n_cols are there.  vec: rows begin at multiples of 16 bytes.
-template <class T, class Tc, int ROWS, int COLS>
-__device__ __forceinline__ void sel_stage(Tc* dst, const T* src, long long stride, int n_rows, int n_cols,
-                                          bool vec) {
-    constexpr int V = 16 / (int)sizeof(T), kPer = COLS / V, kRow = sel_stride<Tc>(COLS);
-#pragma unroll 4
-    for (int q = threadIdx.x; q < ROWS * kPer; q += NHIP_WG) {
-        const int r = q / kPer, c = (q % kPer) * V;
-        SelPack<Tc, V> v;
-        if (vec && r < n_rows && c + V <= n_cols) {
-            const SelPack<T, V> in = *reinterpret_cast<const SelPack<T, V>*>(src + r * stride + c);
+// Rows of inputs on their way into LDS through registers, so that the next chunk's are fetched while
+// one is worked on: ROWS x COLS elements, zero beyond the n_rows x n_cols that are there.  vec: rows
+// begin at multiples of 16 bytes.
+template <class T, class Tc, int ROWS, int COLS> struct SelStage {
+    static constexpr int V = 16 / (int)sizeof(T), kRow = COLS / V, kPacks = ROWS * kRow / NHIP_WG;
+    static_assert(ROWS * kRow % NHIP_WG == 0, "every thread holds as many packs");
+    SelPack<T, V> held[kPacks];
+
+    __device__ __forceinline__ void load(const T* src, long long stride, int n_rows, int n_cols, bool vec) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) v.v[i] = (Tc)in.v[i];
-        } else {
+        for (int q = 0; q < kPacks; ++q) {
+            const int at = threadIdx.x + q * NHIP_WG, r = at / kRow, c = (at % kRow) * V;
+            const T* p = src + r * stride + c;
 #pragma unroll
-            for (int i = 0; i < V; ++i)
-                v.v[i] = r < n_rows && c + i < n_cols ? (Tc)src[r * stride + c + i] : (Tc)0.0f;
-        }
-        // (packs of 16 bytes: rows in LDS begin at multiples of 16)
-        Tc* out = dst + r * kRow + c;
-        if constexpr (sizeof(Tc) * V == 16) {
-            *reinterpret_cast<SelPack<Tc, V>*>(out) = v;
-        } else {
+            for (int i = 0; i < V; ++i) held[q].v[i] = (T)0.0f;
+            if (r < n_rows) {
+                if (vec && c + V <= n_cols) {
+                    held[q] = *reinterpret_cast<const SelPack<T, V>*>(p);
+                } else {
 #pragma unroll
-            for (int i = 0; i < V; i += 4)
-                *reinterpret_cast<sel_f4*>(out + i) = sel_f4{v.v[i], v.v[i + 1], v.v[i + 2], v.v[i + 3]};
+                    for (int i = 0; i < V; ++i)
+                        if (c + i < n_cols) held[q].v[i] = p[i];
+                }
+            }
         }
     }
-}
+    template <int STRIDE> __device__ __forceinline__ void store(Tc* dst) const {
+#pragma unroll
+        for (int q = 0; q < kPacks; ++q) {
+            const int at = threadIdx.x + q * NHIP_WG, r = at / kRow, c = (at % kRow) * V;
+            Tc* out = dst + r * STRIDE + c;
+            if constexpr (sizeof(Tc) == sizeof(T)) {
+                *reinterpret_cast<SelPack<Tc, V>*>(out) = *reinterpret_cast<const SelPack<Tc, V>*>(&held[q]);
+            } else {
+#pragma unroll
+                for (int i = 0; i < V; i += 4)
+                    *reinterpret_cast<sel_f4*>(out + i) = sel_f4{(float)held[q].v[i], (float)held[q].v[i + 1],
+                                                                 (float)held[q].v[i + 2], (float)held[q].v[i + 3]};
+            }
+        }
+    }
+};
 
 // ------------------------------------------------------------------------- steps of a chunk
 // With step_t = f(dt_t + bias) and c_t = sum of step A over the tokens up to t of the chunk, in
 // units of log 2: what decays from token j to token i is 2^(c_i - c_j).  c is summed in 64 bits
-// and kept as a whole part and a rest, whose differences are exact to 2^-24: a large step
-// (c of thousands) costs the tokens behind it nothing.
+// and kept as a whole part, whose differences are exact, and a rest of at most 1/2: a large step
+// (c of thousands) costs the tokens behind it nothing, and no argument of an exponential is
+// rounded to less than 2^-24.
 template <int Q> struct SelSteps {
     alignas(16) float step[Q];
-    alignas(16) float whole[Q], rest[Q];
+    alignas(16) int whole[Q];
+    alignas(16) float rest[Q];
     alignas(16) float raw[Q];
+    alignas(16) float from_start[Q];  // 2^c_t
+    alignas(16) float to_end[Q];      // 2^(c_Q - c_t)
 };
 
 constexpr double kSelLog2e = 1.4426950408889634;
 
-__device__ __forceinline__ double sel_prefix(double v, int lane) {
-#pragma unroll
-    for (int d = 1; d < NHIP_WAVE; d *= 2) {
-        const double other = __shfl_up(v, d);
-        if (lane >= d) v += other;
-    }
+template <int CTRL, int ROWS> __device__ __forceinline__ double sel_dpp(double v) {
+    const long long b = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_update_dpp(0, (int)b, CTRL, ROWS, 0xf, false);
+    const int hi = __builtin_amdgcn_update_dpp(0, (int)(b >> 32), CTRL, ROWS, 0xf, false);
+    return __longlong_as_double(((long long)hi << 32) | (unsigned)lo);
+}
+
+// Sum over the lanes up to this one: lanes 1, 2, 4, 8 back within each row of 16, then the last lane
+// of the row or rows before.
+__device__ __forceinline__ double sel_prefix(double v) {
+    v += sel_dpp<0x111, 0xf>(v);
+    v += sel_dpp<0x112, 0xf>(v);
+    v += sel_dpp<0x114, 0xf>(v);
+    v += sel_dpp<0x118, 0xf>(v);
+    v += sel_dpp<0x142, 0xa>(v);
+    v += sel_dpp<0x143, 0xc>(v);
     return v;
 }
 
-// One wave; lane t: token t0 + t of the sequence.  Beyond its end step is zero and c goes on as it is.
+__device__ __forceinline__ float sel_exp2(int whole, float rest) {
+    return __builtin_ldexpf(__builtin_amdgcn_exp2f(rest), whole);
+}
+
+// What lane t of a wave reads of token t0 + t of the sequence; zero beyond its end
 template <int Q>
-__device__ __forceinline__ void sel_steps(SelSteps<Q>& s, const nhip_scan_args& a, const SelSeq& seq,
-                                          int t0, int head) {
+__device__ __forceinline__ float sel_dt(const nhip_scan_args& a, const SelSeq& seq, int t0, int head) {
+    const int lane = threadIdx.x & (NHIP_WAVE - 1);
+    if (lane >= Q || t0 < 0 || t0 + lane >= seq.n) return 0.0f;
+    const long long at = a.tokens.starts ? (seq.row0 + t0 + lane) * a.dt.token
+                                         : seq.seq * a.dt.seq + (t0 + lane) * a.dt.token;
+    return sel_element(a.dt.p, a.dt_type, at + head * a.dt.head);
+}
+
+// One wave; lane t: token t of the chunk, n of which there are, with dt as read.  Beyond them step is
+// zero and c goes on as it is.
+template <int Q>
+__device__ __forceinline__ void sel_steps(SelSteps<Q>& s, float dt, int n, float A, float bias, bool softplus) {
     const int lane = threadIdx.x & (NHIP_WAVE - 1);
     float step = 0.0f, raw = 0.0f;
     double c = 0.0;
-    if (lane < Q && t0 + lane < seq.n) {
-        const long long at = a.tokens.starts ? (seq.row0 + t0 + lane) * a.dt.token
-                                             : seq.seq * a.dt.seq + (t0 + lane) * a.dt.token;
-        raw = sel_element(a.dt.p, a.dt_type, at + head * a.dt.head) + (a.dt_bias ? a.dt_bias[head] : 0.0f);
-        step = a.softplus ? sel_softplus(raw) : raw;
-        c = (double)step * (double)a.A[head] * kSelLog2e;
+    if (lane < Q && lane < n) {
+        raw = dt + bias;
+        step = softplus ? sel_softplus(raw) : raw;
+        c = (double)step * (double)A * kSelLog2e;
         // 2^-2000 is zero in 32 bits, as everything below it
         c = c < -2000.0 ? -2000.0 : (c > 2000.0 ? 2000.0 : c);
     }
-    c = sel_prefix(c, lane);
+    c = sel_prefix(c);
+    const double whole = rint(c);
+    const int w = whole == whole ? (int)whole : 0;  // (what is no number is so in the rest)
+    const float rest = (float)(c - whole);
+    const int w_end = __builtin_amdgcn_readlane(w, Q - 1);
+    const float rest_end = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(rest), Q - 1));
     if (lane < Q) {
-        const double whole = rint(c);
         s.step[lane] = step;
         s.raw[lane] = raw;
-        s.whole[lane] = (float)whole;
-        s.rest[lane] = (float)(c - whole);
+        s.whole[lane] = w;
+        s.rest[lane] = rest;
+        s.from_start[lane] = sel_exp2(w, rest);
+        s.to_end[lane] = sel_exp2(w_end - w, rest_end - rest);
     }
-}
-
-__device__ __forceinline__ float sel_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
-
-template <int Q>
-__device__ __forceinline__ float sel_decay(const SelSteps<Q>& s, int from, int to) {
-    return sel_exp2((s.whole[to] - s.whole[from]) + (s.rest[to] - s.rest[from]));
-}
-template <int Q> __device__ __forceinline__ float sel_decay_from_start(const SelSteps<Q>& s, int to) {
-    return sel_exp2(s.whole[to] + s.rest[to]);
 }

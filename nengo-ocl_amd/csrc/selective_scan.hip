@@ -57,7 +57,7 @@ __global__ __launch_bounds__(NHIP_WG) void step_kernel(nhip_scan_step_args a, in
 extern "C" int nhip_selective_scan_workspace(const nhip_scan_args* args, long long* bytes_out) {
     if (int e = sel_scan_check(args)) return e;
     if (!bytes_out) return NHIP_E_BADARG;
-    *bytes_out = 0;
+    *bytes_out = 4 * sel_walk_space(*args, sel_walk_plan(*args, 1, nullptr));
     return 0;
 }
 
@@ -65,7 +65,12 @@ extern "C" int nhip_selective_scan(void* stream, const nhip_scan_args* args) {
     if (int e = sel_scan_check(args)) return e;
     const nhip_scan_args& a = *args;
     if (a.tokens.n_tokens && !a.y) return NHIP_E_BADARG;
-    return sel_walk<kSelOutputs>(static_cast<hipStream_t>(stream), a, sel_walk_plan(a, nullptr));
+    SelWalkPlan plan = sel_walk_plan(a, 1, nullptr);
+    const long long need = 4 * sel_walk_space(a, plan);
+    if (need > a.workspace_bytes) return NHIP_E_TOOBIG;
+    if (need && (!a.workspace || !sel_aligned(a.workspace, 16))) return NHIP_E_BADARG;
+    sel_walk_place(a, plan, static_cast<float*>(a.workspace));
+    return sel_walk<kSelOutputs>(static_cast<hipStream_t>(stream), a, plan, true);
 }
 
 extern "C" int nhip_selective_step(void* stream, const nhip_scan_step_args* args) {

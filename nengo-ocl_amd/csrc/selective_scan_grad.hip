@@ -10,9 +10,8 @@
 //     da_t = sum_{i >= t > j} K_ij X_ij L_ij step_j + sum_{i >= t} q_i + sum_{j < t} r_j step_j + e^{c_Q} <G, S>
 //     q_i = e^{c_i} C_i . S^T dy_i,     r_j = e^{c_Q - c_j} B_j . G^T x_j
 //     dstep_t = A da_t + sum_{i >= t} K_it X_it L_it + r_t
-// None of these is a difference of sums over the sequence, so their errors do not grow with its length.
-// The first sum of da_t is formed from the strict row and column sums of one and the same matrix, in
-// which the terms with both tokens behind t cancel term by term.
+// No sum of these is the difference of larger ones: the errors of da, which add up in dA over all the
+// tokens, stay those of its own terms.
 #include <type_traits>
 
 #include "selective_scan.h"
@@ -31,6 +30,7 @@ struct GradPlan {
 
 template <class Tc, int NP> struct GradLds {
     static constexpr int Q = sel_chunk_of(NP);
+    static constexpr int SX = sel_stride<Tc>(64), SN = sel_stride<Tc>(NP), SW = sel_stride<Tc>(Q);
     alignas(16) Tc x[Q * sel_stride<Tc>(64)];
     alignas(16) Tc dy[Q * sel_stride<Tc>(64)];
     alignas(16) Tc B[Q * sel_stride<Tc>(NP)];
@@ -38,8 +38,9 @@ template <class Tc, int NP> struct GradLds {
     alignas(16) Tc xl[Q * sel_stride<Tc>(Q)];  // [j][i]: X_ij L_ij step_j
     alignas(16) Tc kl[Q * sel_stride<Tc>(Q)];  // [j][i]: K_ij L_ij step_j
     SelSteps<Q> steps;
-    // sums of a head, by tile of the other index or by wave
-    float row[Q / 16][Q], col[Q / 16][Q], diag[Q], dot[Q], q[4][Q], r[4][Q], z[4];
+    // Sums of a head.  over[jt][t]: of K X L step over i >= t in t's own tile of 16 and j < t in tile jt;
+    // col[it][j]: of K X L over the i > j of tile it;  q, r, z: by wave
+    float over[Q / 16][Q], col[Q / 16][Q], diag[Q], dot[Q], q[4][Q], r[4][Q], z[4];
 };
 
 // Eight elements of a state across its rows: k over 32 rows from p0, column n
@@ -56,7 +57,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
     using Lds = GradLds<Tc, NP>;
     constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
     constexpr int kTiles = QT * (QT + 1) / 2, kMyTiles = (kTiles + 3) / 4, kMyNT = (NT + 3) / 4;
-    constexpr int SX = sel_stride<Tc>(64), SN = sel_stride<Tc>(NP), SW = sel_stride<Tc>(Q);
+    constexpr int SX = Lds::SX, SN = Lds::SN, SW = Lds::SW;
     constexpr int kSplits = SelSplit<Tc>::n;
     extern __shared__ __align__(16) char lds_bytes[];
     Lds& s = *reinterpret_cast<Lds*>(lds_bytes);
@@ -79,10 +80,13 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
     const long long head_state = (long long)a.dim * a.states;
     const bool vec_state = plan.vec & kSelVecState;
 
-    sel_stage<T, Tc, Q, NP>(s.B, sel_row<T>(a.B, a.tokens, seq, t0) + group * a.B.head, a.B.token, n, a.states,
-                            plan.vec & kSelVecB);
-    sel_stage<T, Tc, Q, NP>(s.C, sel_row<T>(a.C, a.tokens, seq, t0) + group * a.C.head, a.C.token, n, a.states,
-                            plan.vec & kSelVecC);
+    {
+        SelStage<T, Tc, Q, NP> stage;
+        stage.load(sel_row<T>(a.B, a.tokens, seq, t0) + group * a.B.head, a.B.token, n, a.states, plan.vec & kSelVecB);
+        stage.template store<SN>(s.B);
+        stage.load(sel_row<T>(a.C, a.tokens, seq, t0) + group * a.C.head, a.C.token, n, a.states, plan.vec & kSelVecC);
+        stage.template store<SN>(s.C);
+    }
     for (int q = tid; q < Q * SW; q += NHIP_WG) s.xl[q] = s.kl[q] = (Tc)0.0f;  // (i < j for good)
     __syncthreads();
 
@@ -101,6 +105,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
             for (int ks = 0; ks < NK; ++ks)
                 sel_mma(K[m], sel_rows(s.C + (16 * it + l) * SN + 32 * ks, g),
                         sel_rows(s.B + (16 * tile_j[m] + l) * SN + 32 * ks, g));
+        sel_settle(K[m]);
     }
 
     sel_f4 dB[kMyNT][QT], dC[kMyNT][QT];  // states 16 (wave + 4 m) + 4 g + r of token 16 t + l
@@ -115,14 +120,19 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
         const float* const G = plan.G + ((long long)chunk * a.n_heads + head) * head_state;
         for (int tile = 0; tile < plan.n_tiles; ++tile) {
             const int p_tile = tile * 64, cols = min(64, a.dim - p_tile);
+            SelStage<T, Tc, Q, 64> stage_x, stage_dy;
+            stage_x.load(sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n, cols,
+                         plan.vec & kSelVecX);
+            stage_dy.load(sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token, n, cols,
+                          plan.vec & kSelVecDy);
             __syncthreads();  // the tile before has been read
-            sel_stage<T, Tc, Q, 64>(s.x, sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n,
-                                    cols, plan.vec & kSelVecX);
-            sel_stage<T, Tc, Q, 64>(s.dy, sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token,
-                                    n, cols, plan.vec & kSelVecDy);
+            stage_x.template store<SX>(s.x);
+            stage_dy.template store<SX>(s.dy);
             if (tile == 0) {
-                if (wave == 0) sel_steps<Q>(s.steps, a, seq, t0, head);
-                for (int q = tid; q < QT * Q; q += NHIP_WG) s.row[q / Q][q % Q] = s.col[q / Q][q % Q] = 0.0f;
+                if (wave == 0)
+                    sel_steps<Q>(s.steps, sel_dt<Q>(a, seq, t0, head), n, a.A[head], a.dt_bias ? a.dt_bias[head] : 0.0f,
+                                 a.softplus);
+                for (int q = tid; q < QT * Q; q += NHIP_WG) s.over[q / Q][q % Q] = s.col[q / Q][q % Q] = 0.0f;
                 for (int q = tid; q < 4 * Q; q += NHIP_WG) s.q[q / Q][q % Q] = s.r[q / Q][q % Q] = 0.0f;
                 if (tid < Q) s.diag[tid] = s.dot[tid] = 0.0f;
                 if (tid < 4) s.z[tid] = 0.0f;
@@ -137,29 +147,37 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks)
                     sel_mma(X, sel_rows(s.dy + (16 * it + l) * SX + 32 * ks, g), sel_rows(s.x + j * SX + 32 * ks, g));
+                sel_settle(X);
                 const float step = s.steps.step[j];
-                float kl[4], xl[4], below = 0.0f;
+                float kl[4], xl[4], ml[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = i0 + r;
-                    const float L = i >= j ? sel_decay(s.steps, j, i) : 0.0f;
-                    const float ml = i >= j ? K[m][r] * X[r] * L : 0.0f;
+                    const float L = sel_exp2(s.steps.whole[i] - s.steps.whole[j], s.steps.rest[i] - s.steps.rest[j]);
+                    const float all = i >= j ? K[m][r] * X[r] * L : 0.0f;
                     kl[r] = i >= j ? K[m][r] * L * step : 0.0f;
                     xl[r] = i >= j ? X[r] * L * step : 0.0f;
                     if (i == j) {
-                        s.diag[j] += ml;
+                        s.diag[j] += all;
                         s.dot[j] += X[r];
                     }
-                    const float strict = i > j ? ml : 0.0f;
-                    below += strict;
-                    float across = strict * step;  // over the 16 columns of the tile
-#pragma unroll
-                    for (int d = 1; d < 16; d *= 2) across += __shfl_xor(across, d);
-                    if (l == 0) s.row[jt][i] += across;
+                    ml[r] = i > j ? all : 0.0f;
                 }
-                below += __shfl_xor(below, 16);
-                below += __shfl_xor(below, 32);
-                if (g == 0) s.col[it][j] += below;
+                // sums over the rows from each on: this lane's four, and those of the quarters behind
+#pragma unroll
+                for (int r = 2; r >= 0; --r) ml[r] += ml[r + 1];
+                float tail = ml[0], other = __shfl_down(tail, 16);
+                tail += g < 3 ? other : 0.0f;
+                other = __shfl_down(tail, 32);
+                tail += g < 2 ? other : 0.0f;
+                if (g == 0) s.col[it][j] += tail;
+                other = __shfl_down(tail, 16);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int i = i0 + r;
+                    const float over = sel_row_sum(i > j ? (ml[r] + (g < 3 ? other : 0.0f)) * step : 0.0f);
+                    if (l == 0) s.over[jt][i] += over;
+                }
                 sel_store<Tc, 4>(s.kl + j * SW + i0, kl);
                 sel_store<Tc, 4>(s.xl + j * SW + i0, xl);
             }
@@ -188,9 +206,10 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
                     sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int ks = 0; ks < NK; ++ks) sel_mma(acc, gf[ks], sel_rows(s.B + j * SN + 32 * ks, g));
-                    acc *= sel_decay(s.steps, j, Q - 1) * s.steps.step[j];
+                    acc *= s.steps.to_end[j] * s.steps.step[j];
 #pragma unroll
                     for (int ks = jt / 2; ks < QK; ++ks) sel_mma(acc, df[ks], sel_rows(s.kl + j * SW + 32 * ks, g));
+                    sel_settle(acc);
                     if (j < n) {
                         const int c = 16 * wave + 4 * g;
 #pragma unroll
@@ -230,7 +249,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
 #pragma unroll
                         for (int q = 0; q < kSplits; ++q) sel_mma(acc, f[ks][q], d);
                     }
-                    acc *= sel_decay_from_start(s.steps, i);
+                    acc *= s.steps.from_start[i];
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         qs[it] = fmaf(acc[r], (float)s.C[i * SN + 16 * nt + 4 * g + r], qs[it]);
@@ -240,6 +259,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
                         sel_mma(dC[m][it], sel_cols(s.B + 32 * ks * SN + 16 * nt, SN, l, g),
                                 sel_cols(s.xl + 32 * ks * SW + 16 * it, SW, l, g));
                 }
+                sel_settle(dC[m]);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Gv[ks], f[ks]);
 #pragma unroll
@@ -252,7 +272,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
 #pragma unroll
                         for (int q = 0; q < kSplits; ++q) sel_mma(acc, f[ks][q], d);
                     }
-                    acc *= sel_decay(s.steps, j, Q - 1);
+                    acc *= s.steps.to_end[j];
 #pragma unroll
                     for (int r = 0; r < 4; ++r)
                         rs[jt] = fmaf(acc[r], (float)s.B[j * SN + 16 * nt + 4 * g + r], rs[jt]);
@@ -262,6 +282,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
                         sel_mma(dB[m][jt], sel_cols(s.C + 32 * ks * SN + 16 * nt, SN, l, g),
                                 sel_rows(s.xl + j * SW + 32 * ks, g));
                 }
+                sel_settle(dB[m]);
             }
             z = sel_wave_sum(z);
             if (lane == 0) s.z[wave] += z;
@@ -280,29 +301,34 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
         __syncthreads();
         if (wave == 0) {
             float step = 0.0f, own = 0.0f, r = 0.0f, dot = 0.0f;
-            double behind = 0.0, passed = 0.0;  // what counts for this token and those in front of it / behind it
+            double behind = 0.0, passed = 0.0;  // what counts for the tokens up to this one / behind it
+            double across = 0.0;                // the first sum of da
             const bool live = lane < Q && lane < n;
             if (live) {
                 step = s.steps.step[lane];
                 r = (s.r[0][lane] + s.r[1][lane]) + (s.r[2][lane] + s.r[3][lane]);
-                float row = 0.0f, col = 0.0f;
+                behind = (double)((s.q[0][lane] + s.q[1][lane]) + (s.q[2][lane] + s.q[3][lane]));
+                passed = (double)r * (double)step;
+                own = s.diag[lane] + r;
+                dot = s.dot[lane];
 #pragma unroll
                 for (int t = 0; t < QT; ++t) {
-                    row += s.row[t][lane];
-                    col += s.col[t][lane];
+                    across += (double)s.over[t][lane];
+                    own += s.col[t][lane];
                 }
-                const float q = (s.q[0][lane] + s.q[1][lane]) + (s.q[2][lane] + s.q[3][lane]);
-                behind = (double)row + (double)q - (double)col * (double)step;
-                passed = (double)r * (double)step;
-                own = col + s.diag[lane] + r;
-                dot = s.dot[lane];
             }
-            const double sum = sel_prefix(behind, lane), before = sel_prefix(passed, lane) - passed;
+#pragma unroll
+            for (int t = 1; t < QT; ++t) {  // rows of the tiles behind this token's, columns in front of it
+                const double v = live ? (double)s.col[t][lane] * (double)step : 0.0;
+                const double in_front = sel_prefix(v) - v;
+                across += lane < 16 * t ? in_front : 0.0;
+            }
+            const double sum = sel_prefix(behind), before = sel_prefix(passed) - passed;
             const double all = __shfl(sum, NHIP_WAVE - 1);
-            const float z = ((s.z[0] + s.z[1]) + (s.z[2] + s.z[3])) * sel_decay_from_start(s.steps, Q - 1);
+            const float z = ((s.z[0] + s.z[1]) + (s.z[2] + s.z[3])) * s.steps.from_start[Q - 1];
             float da = 0.0f, draw = 0.0f;
             if (live) {
-                da = (float)((all - sum + behind) + before + (double)z);
+                da = (float)(across + (all - sum + behind) + before + (double)z);
                 draw = fmaf(a.A[head], da, own);
                 if (a.softplus) draw *= 1.0f / (1.0f + expf(-s.steps.raw[lane]));
                 sel_set_element(a.ddt, a.dt_type, (seq.row0 + t0 + lane) * a.n_heads + head, draw);
@@ -350,13 +376,16 @@ __global__ __launch_bounds__(NHIP_WG) void add_blocks_kernel(const float* shared
 }
 
 struct Layout {
-    long long n_chunks, states, parts, shared;  // floats
+    SelWalkPlan walk;
+    long long n_chunks, states, walk_space, parts, shared;  // floats
     int heads_per_group, blocks;
 };
 
 Layout layout(const nhip_scan_args& a) {
     Layout m;
-    m.n_chunks = sel_max_chunks(a.tokens, sel_chunk_tokens(a.states));
+    m.walk = sel_walk_plan(a, 2, nullptr);
+    m.walk_space = sel_walk_space(a, m.walk);
+    m.n_chunks = m.walk.n_chunks;
     m.states = m.n_chunks * a.n_heads * a.dim * a.states;
     m.parts = m.n_chunks * 3 * a.n_heads;
     // Heads share a work-group, and with it B, C and the sums for their gradients, as long as there are
@@ -370,15 +399,13 @@ Layout layout(const nhip_scan_args& a) {
     return m;
 }
 
-long long round4(long long floats) { return (floats + 3) & ~3LL; }
-
 }  // namespace
 
 extern "C" int nhip_selective_scan_grad_workspace(const nhip_scan_args* args, long long* bytes_out) {
     if (int e = sel_scan_check(args)) return e;
     if (!bytes_out) return NHIP_E_BADARG;
     const Layout m = layout(*args);
-    *bytes_out = 4 * (2 * round4(m.states) + round4(m.parts) + round4(m.shared));
+    *bytes_out = 4 * (sel_round4(2 * m.states) + m.walk_space + sel_round4(m.parts) + m.shared);
     return 0;
 }
 
@@ -390,20 +417,20 @@ extern "C" int nhip_selective_scan_grad(void* stream, const nhip_scan_args* args
     if (a.tokens.n_tokens && (!a.dy.p || !a.dx || !a.ddt || !a.dB || !a.dC)) return NHIP_E_BADARG;
     if (need > a.workspace_bytes) return NHIP_E_TOOBIG;
     if (need && (!a.workspace || !sel_aligned(a.workspace, 16))) return NHIP_E_BADARG;
-    const Layout m = layout(a);
+    Layout m = layout(a);
     const long long groups = m.n_chunks * a.n_groups * m.blocks;
     if (groups > 0x7fffffffLL) return NHIP_E_BADARG;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    float* S = static_cast<float*>(a.workspace);
-    float* G = S + round4(m.states);
-    float* parts = G + round4(m.states);
-    float* shared = parts + round4(m.parts);
-    const SelWalkPlan w = sel_walk_plan(a, S);
-    if (int e = sel_walk<kSelStates>(st, a, w)) return e;
-    if (int e = sel_walk<kSelStatesBack>(st, a, sel_walk_plan(a, G))) return e;
+    m.walk.states = static_cast<float*>(a.workspace);
+    float* space = m.walk.states + sel_round4(2 * m.states);
+    sel_walk_place(a, m.walk, space);
+    float* parts = space + m.walk_space;
+    float* shared = parts + sel_round4(m.parts);
+    if (int e = sel_walk<kSelStates>(st, a, m.walk, false)) return e;
     int rc = 0;
     if (groups) {
-        const GradPlan plan{w.vec, w.n_tiles, m.heads_per_group, m.blocks, m.n_chunks, S, G, parts, shared};
+        const GradPlan plan{m.walk.vec, m.walk.n_tiles, m.heads_per_group, m.blocks, m.n_chunks,
+                            m.walk.states, m.walk.states + m.states, parts, shared};
         sel_with_type(a.type, [&](auto t) {
             using T = decltype(t);
             using Tc = typename SelCompute<T>::type;
