@@ -64,9 +64,19 @@ __device__ __forceinline__ float sel_sigmoid(float v) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896341f));
 }
 
-// max(v, 0) + log(1 + exp(-|v|)): no overflow, and no loss for large negative v
+// exp(v): 2^v' with the whole part of v' = v log2(e) set aside, so that its rounding costs nothing
+__device__ __forceinline__ float sel_exp(float v) {
+    const float whole = rintf(v * 1.44269504088896341f);
+    const float rest = fmaf(v, 1.925963033500e-8f, fmaf(v, 1.44269502162933349609f, -whole));  // log2(e) in two parts
+    return __builtin_ldexpf(__builtin_amdgcn_exp2f(rest), (int)fmaxf(fminf(whole, 300.0f), -300.0f));
+}
+
+// max(v, 0) + log(1 + exp(-|v|)), without loss for large negative v: with u = exp(-|v|) and w = 1 + u as
+// rounded, log(1 + u) = log(w) u / (w - 1) to first order in the rounding (Kahan).
 __device__ __forceinline__ float sel_softplus(float v) {
-    return fmaxf(v, 0.0f) + log1pf(expf(-fabsf(v)));
+    const float u = sel_exp(-fabsf(v)), w = 1.0f + u, d = w - 1.0f;
+    const float log_w = __builtin_amdgcn_logf(w) * 0.693147180559945309f;
+    return fmaxf(v, 0.0f) + (d > 0.0f ? log_w * (u * __builtin_amdgcn_rcpf(d)) : u);
 }
 
 // ---------------------------------------------------------------------- chunks of sequences

@@ -47,14 +47,12 @@ __device__ __forceinline__ void sel_mma(sel_f4& acc, const SelFrag<float>& a, co
 // reads its registers are the program's to keep, and this compiler counts them within a block
 // (roc-7.2.0: a branch right behind the instruction led to reads one wait state after it, which
 // returned the last of the four registers' old value).
-__device__ __forceinline__ void sel_settle(sel_f4& a) { asm volatile("s_nop 15" : "+v"(a)); }
-__device__ __forceinline__ void sel_settle(sel_f4& a, sel_f4& b) { asm volatile("s_nop 15" : "+v"(a), "+v"(b)); }
 template <int N> __device__ __forceinline__ void sel_settle(sel_f4 (&a)[N]) {
-    if constexpr (N == 1) sel_settle(a[0]);
 #pragma unroll
-    for (int i = 0; i + 1 < N; i += 2) sel_settle(a[i], a[i + 1]);
-    if constexpr (N > 1 && N % 2 == 1) sel_settle(a[N - 1]);
+    for (int i = 0; i < N - 1; ++i) asm volatile("" : "+v"(a[i]));
+    asm volatile("s_nop 15" : "+v"(a[N - 1]));
 }
+__device__ __forceinline__ void sel_settle(sel_f4& a) { asm volatile("s_nop 15" : "+v"(a)); }
 
 // Fragment of a matrix in LDS whose rows run along k: `row` is this lane's row, at the first k.
 __device__ __forceinline__ SelFrag<__bf16> sel_rows(const __bf16* row, int g) {
@@ -93,8 +91,7 @@ __device__ __forceinline__ SelFrag<float> sel_cols(const float* at, int stride, 
     return f;
 }
 
-// Eight float32 values as fragments that add up to them.  What is no number or infinite is so in
-// the first alone.
+// Eight float32 values as fragments that add up to them
 template <class Tc>
 __device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<Tc> (&f)[SelSplit<Tc>::n]) {
 #pragma unroll
@@ -103,9 +100,36 @@ __device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<Tc> (&f)[
 #pragma unroll
         for (int s = 0; s < SelSplit<Tc>::n; ++s) {
             f[s].set(e, rest);
-            if (s + 1 < SelSplit<Tc>::n) rest = fabsf(x[e]) < 3.0e38f ? rest - f[s].get(e) : 0.0f;
+            rest -= f[s].get(e);
         }
     }
+}
+
+// Whether all eight are finite, and what is left with zeros in the place of those that are not; ones in their place
+__device__ __forceinline__ bool sel_finite(const SelFrag<__bf16>& f) {
+    typedef unsigned short us8 __attribute__((ext_vector_type(8)));
+    typedef unsigned short us4 __attribute__((ext_vector_type(4)));
+    typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+    const us8 m = __builtin_bit_cast(us8, f.v) & (unsigned short)0x7fff;
+    const us4 a = __builtin_elementwise_max(m.lo, m.hi);
+    const us2 b = __builtin_elementwise_max(a.lo, a.hi);
+    return b.x < 0x7f80 && b.y < 0x7f80;
+}
+__device__ __forceinline__ bool sel_finite(const SelFrag<float>& f) {
+    float m = fabsf(f.v[0]) * 0.0f;
+#pragma unroll
+    for (int e = 1; e < 8; ++e) m = fmaf(f.v[e], 0.0f, m);
+    return m == 0.0f;
+}
+template <class Tc> __device__ __forceinline__ SelFrag<Tc> sel_take_unfinite(SelFrag<Tc>& f) {
+    SelFrag<Tc> ones;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const bool ok = fabsf(f.get(e)) < INFINITY;
+        ones.set(e, ok ? 0.0f : 1.0f);
+        if (!ok) f.set(e, 0.0f);
+    }
+    return ones;
 }
 
 // Row length in LDS of `n` elements (a multiple of 32).  Reads of rows (sel_rows) meet no bank twice with
@@ -116,45 +140,66 @@ template <class Tc> __host__ __device__ constexpr int sel_stride_cols(int n) {
 }
 
 // Rows of inputs on their way into LDS through registers, so that the next chunk's are fetched while
-// one is worked on: ROWS x COLS elements, zero beyond the n_rows x n_cols that are there.  vec: rows
-// begin at multiples of 16 bytes.
-template <class T, class Tc, int ROWS, int COLS> struct SelStage {
+// one is worked on: ROWS x COLS elements, zero beyond the n_rows x n_cols (one at least) that are
+// there.  VEC: rows begin at multiples of 16 bytes, hold whole packs and lie within 2^31 bytes.  The
+// loads are unconditional, from places cut to those that exist, and what is too much is left out when
+// it is stored; and VEC is a template's: a load under any condition, uniform or not, is waited for where
+// its branch ends, and the packs of a chunk came one after the other (9,000 cycles, not 3,000).
+template <class T, class Tc, int ROWS, int COLS, bool VEC> struct SelStage {
     static constexpr int V = 16 / (int)sizeof(T), kRow = COLS / V, kPacks = ROWS * kRow / NHIP_WG;
-    static_assert(ROWS * kRow % NHIP_WG == 0, "every thread holds as many packs");
+    static constexpr int kRowStep = NHIP_WG / kRow;  // rows between a thread's packs
+    static_assert(ROWS * kRow % NHIP_WG == 0 && NHIP_WG % kRow == 0, "every thread holds as many packs, in one column");
     SelPack<T, V> held[kPacks];
 
-    __device__ __forceinline__ void load(const T* src, long long stride, int n_rows, int n_cols, bool vec) {
+    // (formed anew each time: kept over a loop, the places take the registers of what is worked on)
+    static __device__ __forceinline__ int thread() {
+        int tid = threadIdx.x;
+        asm volatile("" : "+v"(tid));
+        return tid;
+    }
+
+    __device__ __forceinline__ void load(const T* src, long long stride, int n_rows, int n_cols) {
+        const int tid = thread(), row = tid / kRow, col = (tid % kRow) * V;
+        if constexpr (VEC) {
+            const unsigned st = (unsigned)stride, last = (unsigned)(n_rows - 1) * st;
+            const unsigned r0 = row * st, c = (unsigned)min(col, n_cols - V);
 #pragma unroll
-        for (int q = 0; q < kPacks; ++q) {
-            const int at = threadIdx.x + q * NHIP_WG, r = at / kRow, c = (at % kRow) * V;
-            const T* p = src + r * stride + c;
+            for (int q = 0; q < kPacks; ++q) {
+                const unsigned at = min(r0 + (unsigned)(q * kRowStep) * st, last) + c;
+                held[q] = *reinterpret_cast<const SelPack<T, V>*>(reinterpret_cast<const char*>(src) + at * (unsigned)sizeof(T));
+            }
+        } else {
 #pragma unroll
-            for (int i = 0; i < V; ++i) held[q].v[i] = (T)0.0f;
-            if (r < n_rows) {
-                if (vec && c + V <= n_cols) {
-                    held[q] = *reinterpret_cast<const SelPack<T, V>*>(p);
-                } else {
+            for (int q = 0; q < kPacks; ++q) {
+                const T* p = src + min(row + q * kRowStep, n_rows - 1) * stride;
 #pragma unroll
-                    for (int i = 0; i < V; ++i)
-                        if (c + i < n_cols) held[q].v[i] = p[i];
-                }
+                for (int i = 0; i < V; ++i) held[q].v[i] = p[min(col + i, n_cols - 1)];
             }
         }
     }
-    template <int STRIDE> __device__ __forceinline__ void store(Tc* dst) const {
+    template <int STRIDE, bool WHOLE> __device__ __forceinline__ void put(Tc* dst, int n_rows, int n_cols) const {
+        const int tid = thread(), row = tid / kRow, col = (tid % kRow) * V;
 #pragma unroll
         for (int q = 0; q < kPacks; ++q) {
-            const int at = threadIdx.x + q * NHIP_WG, r = at / kRow, c = (at % kRow) * V;
-            Tc* out = dst + r * STRIDE + c;
-            if constexpr (sizeof(Tc) == sizeof(T)) {
-                *reinterpret_cast<SelPack<Tc, V>*>(out) = *reinterpret_cast<const SelPack<Tc, V>*>(&held[q]);
+            const int r = row + q * kRowStep;
+            Tc* out = dst + r * STRIDE + col;
+            const int there = r < n_rows ? n_cols - col : 0;
+            SelPack<Tc, V> v;
+#pragma unroll
+            for (int i = 0; i < V; ++i) v.v[i] = WHOLE || (VEC ? 0 : i) < there ? (Tc)held[q].v[i] : (Tc)0.0f;
+            if constexpr (sizeof(Tc) * V == 16) {
+                *reinterpret_cast<SelPack<Tc, V>*>(out) = v;
             } else {
 #pragma unroll
                 for (int i = 0; i < V; i += 4)
-                    *reinterpret_cast<sel_f4*>(out + i) = sel_f4{(float)held[q].v[i], (float)held[q].v[i + 1],
-                                                                 (float)held[q].v[i + 2], (float)held[q].v[i + 3]};
+                    *reinterpret_cast<sel_f4*>(out + i) = sel_f4{(float)v.v[i], (float)v.v[i + 1], (float)v.v[i + 2],
+                                                                 (float)v.v[i + 3]};
             }
         }
+    }
+    template <int STRIDE> __device__ __forceinline__ void store(Tc* dst, int n_rows, int n_cols) const {
+        if (n_rows == ROWS && n_cols == COLS) put<STRIDE, true>(dst, n_rows, n_cols);
+        else put<STRIDE, false>(dst, n_rows, n_cols);
     }
 };
 
@@ -171,6 +216,7 @@ template <int Q> struct SelSteps {
     alignas(16) float raw[Q];
     alignas(16) float from_start[Q];  // 2^c_t
     alignas(16) float to_end[Q];      // 2^(c_Q - c_t)
+    alignas(16) float to_end_step[Q];
 };
 
 constexpr double kSelLog2e = 1.4426950408889634;
@@ -201,18 +247,23 @@ __device__ __forceinline__ float sel_exp2(int whole, float rest) {
 // What lane t of a wave reads of token t0 + t of the sequence; zero beyond its end
 template <int Q>
 __device__ __forceinline__ float sel_dt(const nhip_scan_args& a, const SelSeq& seq, int t0, int head) {
-    const int lane = threadIdx.x & (NHIP_WAVE - 1);
-    if (lane >= Q || t0 < 0 || t0 + lane >= seq.n) return 0.0f;
-    const long long at = a.tokens.starts ? (seq.row0 + t0 + lane) * a.dt.token
-                                         : seq.seq * a.dt.seq + (t0 + lane) * a.dt.token;
-    return sel_element(a.dt.p, a.dt_type, at + head * a.dt.head);
+    int lane = threadIdx.x & (NHIP_WAVE - 1);
+    asm volatile("" : "+v"(lane));  // (the address is formed anew each time: kept, it takes two registers)
+    if (lane >= Q || t0 + lane >= seq.n) return 0.0f;
+    const long long first = (a.tokens.starts ? (seq.row0 + t0) * a.dt.token : seq.seq * a.dt.seq + t0 * a.dt.token) +
+                            head * a.dt.head;
+    const long long at = first + lane * a.dt.token;
+    if (a.dt_type == NHIP_F32) return static_cast<const float*>(a.dt.p)[at];
+    const unsigned short bits = static_cast<const unsigned short*>(a.dt.p)[at];
+    return a.dt_type == NHIP_BF16 ? (float)__builtin_bit_cast(__bf16, bits) : (float)__builtin_bit_cast(_Float16, bits);
 }
 
 // One wave; lane t: token t of the chunk, n of which there are, with dt as read.  Beyond them step is
 // zero and c goes on as it is.
 template <int Q>
 __device__ __forceinline__ void sel_steps(SelSteps<Q>& s, float dt, int n, float A, float bias, bool softplus) {
-    const int lane = threadIdx.x & (NHIP_WAVE - 1);
+    int lane = threadIdx.x & (NHIP_WAVE - 1);
+    asm volatile("" : "+v"(lane));
     float step = 0.0f, raw = 0.0f;
     double c = 0.0;
     if (lane < Q && lane < n) {
@@ -234,6 +285,8 @@ __device__ __forceinline__ void sel_steps(SelSteps<Q>& s, float dt, int n, float
         s.whole[lane] = w;
         s.rest[lane] = rest;
         s.from_start[lane] = sel_exp2(w, rest);
-        s.to_end[lane] = sel_exp2(w_end - w, rest_end - rest);
+        const float to_end = sel_exp2(w_end - w, rest_end - rest);
+        s.to_end[lane] = to_end;
+        s.to_end_step[lane] = to_end * step;
     }
 }

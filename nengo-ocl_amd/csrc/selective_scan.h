@@ -19,12 +19,13 @@ enum SelWalk {
     kSelEnds = 2,     // only what a segment adds to the state by its end, and how much it keeps of it
 };
 
-// Sequences are cut into segments of `chunks` chunks, each a work-group's walk for 64 of a head's
-// dimension.  A first launch (kSelEnds) leaves every segment's own contribution, the second begins
+// Sequences are cut into segments of `chunks` chunks.  A work-group walks over one for two units of its heads'
+// group, a unit being 64 of a head's dimension.  A first launch (kSelEnds) leaves every segment's own contribution, the second begins
 // each with the sum over those before it.
 struct SelWalkPlan {
-    int n_tiles;            // of 64 of the head's dimension
-    int vec;                // which operands lie at multiples of 16 bytes: bits below
+    int n_tiles;            // units of a head
+    int pairs;              // of units in a group
+    bool vec;               // everything can be read and written 16 bytes at a time
     int chunks;             // per segment
     int directions;         // 2: both halves
     long long n_segments, n_chunks;
@@ -32,7 +33,6 @@ struct SelWalkPlan {
     float* ends;            // [direction][segment][head][dim][states], NULL: no sequence has two segments
     float* keeps;           // [direction][segment][head]: what a segment keeps of the state it begins with
 };
-enum { kSelVecX = 1, kSelVecB = 2, kSelVecC = 4, kSelVecY = 8, kSelVecState = 16, kSelVecDy = 32 };
 
 // Tokens of a chunk: 64, or 32 where 256 states would not fit the LDS otherwise.
 constexpr int sel_chunk_of(int np) { return np > 128 ? 32 : 64; }
@@ -49,121 +49,130 @@ template <class F> static inline bool sel_with_states(int n, F&& f) {
 }
 static inline int sel_chunk_tokens(int n) { return sel_chunk_of(n > 128 ? 256 : 128); }
 
-// Four neighbouring states of a row in memory
-__device__ __forceinline__ sel_f4 sel_state_load(const float* p, int n, int states, bool vec) {
-    if (vec && n + 4 <= states) return *reinterpret_cast<const sel_f4*>(p + n);
-    sel_f4 v;
+// Four neighbouring elements of a row of `cols`; VEC: rows hold whole fours, at multiples of 16 bytes (states) or
+// of their size (outputs)
+template <bool VEC>
+__device__ __forceinline__ sel_f4 sel_state_load(const float* p, int n, int states) {
+    sel_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if constexpr (VEC) {
+        if (n < states) v = *reinterpret_cast<const sel_f4*>(p + n);
+    } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r) v[r] = n + r < states ? p[n + r] : 0.0f;
+        for (int r = 0; r < 4; ++r)
+            if (n + r < states) v[r] = p[n + r];
+    }
     return v;
 }
-__device__ __forceinline__ void sel_state_store(float* p, int n, int states, bool vec, const sel_f4& v) {
-    if (vec && n + 4 <= states) {
-        *reinterpret_cast<sel_f4*>(p + n) = v;
-        return;
-    }
+template <bool VEC>
+__device__ __forceinline__ void sel_state_store(float* p, int n, int states, const sel_f4& v) {
+    if constexpr (VEC) {
+        if (n < states) *reinterpret_cast<sel_f4*>(p + n) = v;
+    } else {
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (n + r < states) p[n + r] = v[r];
+        for (int r = 0; r < 4; ++r)
+            if (n + r < states) p[n + r] = v[r];
+    }
+}
+template <bool VEC, class T>
+__device__ __forceinline__ void sel_store4(T* p, int c, int cols, const sel_f4& v) {
+    if constexpr (VEC) {
+        if (c < cols) sel_store<T, 4>(p + c, {v[0], v[1], v[2], v[3]});
+    } else {
+#pragma unroll
+        for (int r = 0; r < 4; ++r)
+            if (c + r < cols) p[c + r] = (T)v[r];
+    }
 }
 
-// Four neighbouring elements of a row of an output
-template <class T>
-__device__ __forceinline__ void sel_store4(T* p, int c, int cols, bool vec, const sel_f4& v) {
-    if (vec && c + 4 <= cols) {
-        sel_store<T, 4>(p + c, {v[0], v[1], v[2], v[3]});
-        return;
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (c + r < cols) p[c + r] = (T)v[r];
-}
+// The scheduler moves nothing across: left to itself it reads all operands of a chunk from the LDS at
+// once, and spills.
+__device__ __forceinline__ void sel_phase() { __builtin_amdgcn_sched_barrier(0); }
 
 template <class Tc, int NP, bool OUTPUTS> struct SelWalkLds {
     static constexpr int Q = sel_chunk_of(NP);
     static constexpr int SX = sel_stride_cols<Tc>(64), SB = sel_stride_cols<Tc>(NP), SC = sel_stride<Tc>(NP),
                          SW = sel_stride<Tc>(Q);
-    alignas(16) Tc x[Q * SX];
+    alignas(16) Tc x[2][Q * SX];
     alignas(16) Tc B[Q * SB];
     alignas(16) Tc C[OUTPUTS ? Q * SC : 8];
-    alignas(16) Tc weights[OUTPUTS ? Q * SW : 8];  // [i][j]: (C_i . B_j) e^{c_i - c_j} step_j
-    SelSteps<Q> steps[2];                          // of this chunk and the next
+    alignas(16) Tc weights[OUTPUTS ? 2 : 1][OUTPUTS ? Q * SW : 8];  // [i][j]: (C_i . B_j) e^{c_i - c_j} step_j
+    SelSteps<Q> steps[2][2];                                        // [unit][chunk % 2]
 };
 
-// Adds what elements of x that are no finite numbers contribute to rows that read them, one by one: in
-// the products they would reach the tokens in front of them too, as zero times infinity.
-template <class Tc, int Q, int SX, int SW>
-__device__ void sel_add_unfinite(sel_f4& acc, const Tc* x, const Tc* weights, int c, int i) {
-    for (int j = 0; j <= i; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float v = (float)x[j * SX + c + r];
-            if (!(fabsf(v) < INFINITY)) acc[r] = fmaf((float)weights[i * SW + j], v, acc[r]);
-        }
-}
-
-// One work-group walks over the chunks of a segment for 64 of a head's dimension, 16 to a wave, whose
-// part of the state stays in registers: lane l of a wave holds row p = l % 16 of it, the states
-// 16 t + 4 (l / 16) + r in register r of tile t -- the order of a fragment over the states, so that
-// the state is an operand of the next chunk's products as it is.  The inputs of the next chunk are
-// fetched, and its steps formed, while one is worked on.
-template <class T, class Tc, int NP, int WALK>
-__global__ __launch_bounds__(NHIP_WG) void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
+// One work-group walks over the chunks of a segment for two units, two waves to each, a wave to 32 of the
+// dimension, whose part of the state stays in registers: lane l holds rows p = 16 h + l % 16 of it, the
+// states 16 t + 4 (l / 16) + r in register r of tile t -- the order of a fragment over the states, so that
+// the state is an operand of the next chunk's products as it is.  Two units share B, C and their
+// products, and 32 rows share what a wave reads of them: with one unit and 16 rows the LDS, which all
+// operands but the state come from, was busy for as long as a chunk took.  The inputs of the next chunk
+// are fetched while one is worked on, the steps of two chunks formed at once, by a wave each.  A
+// work-group of the bfloat16 kernel with 128 states takes half of a compute unit's LDS and registers.
+template <class T, class Tc, int NP, int WALK, bool VEC>
+__global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1)
+void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
     constexpr bool kOut = WALK == kSelOutputs;
     using Lds = SelWalkLds<Tc, NP, kOut>;
     constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
     constexpr int SX = Lds::SX, SB = Lds::SB, SC = Lds::SC, SW = Lds::SW;
-    constexpr int kTiles = QT * (QT + 1) / 2, kMyTiles = (kTiles + 3) / 4;
     constexpr int kSplits = SelSplit<Tc>::n;
     extern __shared__ __align__(16) char lds_bytes[];
     Lds& s = *reinterpret_cast<Lds*>(lds_bytes);
 
     // neighbouring heads read the same B and C: they go to one die, whose L2 holds them
     const int groups = gridDim.x / plan.directions;
-    const int back = blockIdx.x >= groups;
+    const int back = kOut ? 0 : blockIdx.x >= groups;
     const int id = nhip_xcd_remap(blockIdx.x - back * groups, groups);
-    const int tile = id % plan.n_tiles, head = (id / plan.n_tiles) % a.n_heads;
-    const int segment = id / (plan.n_tiles * a.n_heads);
+    const int pair = id % plan.pairs, group = (id / plan.pairs) % a.n_groups;
+    const int segment = id / (plan.pairs * a.n_groups);
     const SelSeq seq = sel_seq_of_chunk(a.tokens, segment, Q * plan.chunks);
     if (seq.seq < 0) return;
     const int n_segments = sel_chunks(seq.n, Q * plan.chunks);
     // (nobody begins with what the last one, or going back the first, adds)
     if (WALK == kSelEnds && seq.chunk == (back ? 0 : n_segments - 1)) return;
-    const int group = head / (a.n_heads / a.n_groups);
-    const int wave = threadIdx.x / NHIP_WAVE, l = threadIdx.x & 15, g = (threadIdx.x & 63) >> 4;
-    const int p_tile = tile * 64, p = p_tile + wave * 16 + l;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NHIP_WAVE);
+    const int lane_l = threadIdx.x & 15, lane_g = (threadIdx.x & 63) >> 4;
+    // the units; a second one that is not there is the first again, and writes nothing
+    const int per_group = a.n_heads / a.n_groups, units = per_group * plan.n_tiles;
+    auto head_of = [&](int unit) { return group * per_group + min(2 * pair + unit, units - 1) / plan.n_tiles; };
+    auto tile_of = [&](int unit) { return 64 * (min(2 * pair + unit, units - 1) % plan.n_tiles); };
+    const int mine = wave >> 1, head = head_of(mine), p_tile = tile_of(mine);
+    const int p_wave = 32 * (wave & 1);  // within the unit
+    const bool writes = 2 * pair + mine < units;
     const int cols = min(64, a.dim - p_tile);
-    const bool vec_state = plan.vec & kSelVecState;
-    const long long head_state = (long long)a.dim * a.states;
-    const long long my_state = head * head_state + (long long)p * a.states, all_states = a.n_heads * head_state;
+    const long long head_state = (long long)a.dim * a.states, all_states = a.n_heads * head_state;
+    const long long my_state = head * head_state + (long long)(p_tile + p_wave + lane_l) * a.states;
+    const long long next_rows = 16LL * a.states;
+    const bool there[2] = {p_wave + lane_l < cols, p_wave + 16 + lane_l < cols};
     float* const ends = plan.ends ? plan.ends + back * plan.n_segments * all_states : nullptr;
 
-    sel_f4 state[NT];
+    sel_f4 state[2][NT];
 #pragma unroll
-    for (int t = 0; t < NT; ++t) state[t] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (WALK != kSelEnds && p < a.dim) {
-        const float* from = back ? a.dfinal : a.initial;
-        if (from)
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                state[t] = sel_state_load(from + seq.seq * all_states + my_state, 16 * t + 4 * g, a.states, vec_state);
-        // the segments walked before this one, in their order
-        const int first = segment - seq.chunk, before = back ? n_segments - 1 - seq.chunk : seq.chunk;
-        for (int k = 0; k < before; ++k) {
-            const int other = first + (back ? n_segments - 1 - k : k);
-            const float keeps = plan.keeps[(back * plan.n_segments + other) * a.n_heads + head];
-            const float* end = ends + other * all_states + my_state;
+        for (int t = 0; t < NT; ++t) state[h][t] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (WALK != kSelEnds && there[h]) {
+            const float* from = back ? a.dfinal : a.initial;
+            if (from)
 #pragma unroll
-            for (int t = 0; t < NT; ++t)
-                state[t] = state[t] * keeps + sel_state_load(end, 16 * t + 4 * g, a.states, vec_state);
+                for (int t = 0; t < NT; ++t)
+                    state[h][t] = sel_state_load<VEC>(from + seq.seq * all_states + my_state + h * next_rows, 16 * t + 4 * lane_g, a.states);
+            // the segments walked before this one, in their order
+            const int first = segment - seq.chunk, before = back ? n_segments - 1 - seq.chunk : seq.chunk;
+            for (int k = 0; k < before; ++k) {
+                const int other = first + (back ? n_segments - 1 - k : k);
+                const float keeps = plan.keeps[(back * plan.n_segments + other) * a.n_heads + head];
+                const float* end = ends + other * all_states + my_state + h * next_rows;
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    state[h][t] = state[h][t] * keeps + sel_state_load<VEC>(end, 16 * t + 4 * lane_g, a.states);
+            }
         }
     }
-    if constexpr (kOut)
-        for (int q = threadIdx.x; q < Q * SW; q += NHIP_WG) s.weights[q] = (Tc)0.0f;  // (above the diagonal for good)
+    if constexpr (kOut)  // (above the diagonal for good)
+        for (int q = threadIdx.x; q < Q * SW; q += NHIP_WG) s.weights[0][q] = s.weights[1][q] = (Tc)0.0f;
 
     const nhip_rows& x = back ? a.dy : a.x;
     const nhip_rows& B = back ? a.C : a.B;
-    const bool vec_x = plan.vec & (back ? kSelVecDy : kSelVecX), vec_B = plan.vec & (back ? kSelVecC : kSelVecB);
     const float D = kOut && a.D ? a.D[head] : 0.0f, A = a.A[head], bias = a.dt_bias ? a.dt_bias[head] : 0.0f;
     // chunks of the sequence that this segment holds, and the token at which walk number k of them begins
     const int chunk0 = seq.chunk * plan.chunks;
@@ -171,169 +180,285 @@ __global__ __launch_bounds__(NHIP_WG) void sel_walk_kernel(nhip_scan_args a, Sel
     auto token = [&](int k) { return (chunk0 + (back ? n_chunks - 1 - k : k)) * Q; };
     const int first_chunk = WALK == kSelStates ? sel_seq(a.tokens, seq.seq, Q).chunk : 0;
 
-    SelStage<T, Tc, Q, 64> stage_x;
-    SelStage<T, Tc, Q, NP> stage_B, stage_C;
-    auto fetch = [&](int k) {
-        const int t0 = token(k), n = min(Q, seq.n - t0);
-        stage_x.load(sel_row<T>(x, a.tokens, seq, t0) + head * x.head + p_tile, x.token, n, cols, vec_x);
-        stage_B.load(sel_row<T>(B, a.tokens, seq, t0) + group * B.head, B.token, n, a.states, vec_B);
-        if constexpr (kOut)
-            stage_C.load(sel_row<T>(a.C, a.tokens, seq, t0) + group * a.C.head, a.C.token, n, a.states,
-                         plan.vec & kSelVecC);
+    SelStage<T, Tc, Q, 64, VEC> stage_x[2];
+    SelStage<T, Tc, Q, NP, VEC> stage_B, stage_C;
+    // where the next chunk's rows begin
+    const int way = back ? -Q : Q, t_first = token(0);
+    const T* x_at = sel_row<T>(x, a.tokens, seq, t_first);
+    const T* B_at = sel_row<T>(B, a.tokens, seq, t_first) + group * B.head;
+    const T* C_at = kOut ? sel_row<T>(a.C, a.tokens, seq, t_first) + group * a.C.head : nullptr;
+    const long long x_way = way * x.token, B_way = way * B.token, C_way = kOut ? way * a.C.token : 0;
+    const long long unit_at[2] = {head_of(0) * x.head + tile_of(0), head_of(1) * x.head + tile_of(1)};
+    const int unit_cols[2] = {min(64, a.dim - tile_of(0)), min(64, a.dim - tile_of(1))};
+    auto fetch = [&](int n) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) stage_x[u].load(x_at + unit_at[u], x.token, n, unit_cols[u]);
+        stage_B.load(B_at, B.token, n, a.states);
+        if constexpr (kOut) stage_C.load(C_at, a.C.token, n, a.states);
     };
-    // the last wave, which has the fewest tiles, forms the steps
-    constexpr int kStepWave = 3;
     float dt = 0.0f, keeps = 1.0f;
+    const int ahead = wave & 1;  // which of two chunks this wave forms the steps of
     if (n_chunks > 0) {
-        fetch(0);
-        if (wave == kStepWave) {
-            dt = sel_dt<Q>(a, seq, token(0), head);
-            sel_steps<Q>(s.steps[0], dt, seq.n - token(0), A, bias, a.softplus);
-            dt = n_chunks > 1 ? sel_dt<Q>(a, seq, token(1), head) : 0.0f;
-        }
+        fetch(min(Q, seq.n - t_first));
+        if (ahead < n_chunks) dt = sel_dt<Q>(a, seq, token(ahead), head);
     }
     for (int k = 0; k < n_chunks; ++k) {
         const int t0 = token(k), n = min(Q, seq.n - t0);
         __syncthreads();
-        stage_x.template store<SX>(s.x);
-        stage_B.template store<SB>(s.B);
-        if constexpr (kOut) stage_C.template store<SC>(s.C);
-        __syncthreads();
-        if (k + 1 < n_chunks) fetch(k + 1);
-        const SelSteps<Q>& steps = s.steps[k & 1];
-
-        SelFrag<Tc> xf[QK];  // row p of x transposed, over the tokens
-        float odd = 0.0f;
 #pragma unroll
-        for (int ks = 0; ks < QK; ++ks) {
-            xf[ks] = sel_cols(s.x + 32 * ks * SX + 16 * wave, SX, l, g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) odd = fmaf(xf[ks].get(e), 0.0f, odd);
+        for (int u = 0; u < 2; ++u) stage_x[u].template store<SX>(s.x[u], n, unit_cols[u]);
+        stage_B.template store<SB>(s.B, n, a.states);
+        if constexpr (kOut) stage_C.template store<SC>(s.C, n, a.states);
+        if ((k & 1) == 0) {
+            if (k + ahead < n_chunks)
+                sel_steps<Q>(s.steps[mine][ahead], dt, seq.n - token(k + ahead), A, bias, a.softplus);
+            dt = k + 2 + ahead < n_chunks ? sel_dt<Q>(a, seq, token(k + 2 + ahead), head) : 0.0f;
         }
-        const bool unfinite = kOut && __any(odd != 0.0f);
-        if (unfinite)
+        __syncthreads();
+        // (unconditional, as the loads are: the last chunk is fetched twice)
+        const bool more = k + 1 < n_chunks;
+        x_at += more ? x_way : 0;
+        B_at += more ? B_way : 0;
+        if constexpr (kOut) C_at += more ? C_way : 0;
+        fetch(min(Q, seq.n - (more ? t0 + way : t0)));
+        const SelSteps<Q>& steps = s.steps[mine][k & 1];
+        const Tc* const xs = s.x[mine];
+        // (addresses are formed anew in each chunk: kept, they take the registers of the state)
+        int l = lane_l, g = lane_g;
+        asm volatile("" : "+v"(l), "+v"(g));
+
+        SelFrag<Tc> xf[2][QK];  // rows p of x transposed, over the tokens
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int ks = 0; ks < QK; ++ks) xf[h][ks] = sel_cols(xs + 32 * ks * SX + p_wave + 16 * h, SX, l, g);
+        // elements of x that are no finite numbers would reach, as zero times infinity, the tokens in front of them
+        // too: they are left out of the products, and what reads them is made no number
+        bool finite = true;
+        auto odd = [&](int h, int ks) {  // (from LDS again: kept, they take registers though there are none)
+            SelFrag<Tc> f = sel_cols(xs + 32 * ks * SX + p_wave + 16 * h, SX, l, g);
+            return sel_take_unfinite(f);
+        };
+        if constexpr (kOut) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int ks = 0; ks < QK; ++ks) finite = sel_finite(xf[h][ks]) && finite;
+            finite = __all(finite);
+        }
+        if (!finite)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int ks = 0; ks < QK; ++ks) (void)sel_take_unfinite(xf[h][ks]);
+
+        if constexpr (kOut) {
+            // Weights: tiles of the lower triangle of C . B, for both units.  A wave's tiles are in rows
+            // (3: 0, 1, 2), (2: 0, 1, 2), (1: 0, 1; 3: 3), (0: 0): the first two share the rows of C.
+            constexpr int kMine = QT == 4 ? 3 : 1;
+            const int row_a = QT == 4 ? 3 - wave : (wave > 0), row_b = QT == 4 && wave == 2 ? 3 : row_a;
+            auto col_of = [&](int m) { return QT == 4 ? (wave == 3 ? 0 : wave == 2 && m == 2 ? 3 : m) : (wave > 1); };
+            sel_f4 acc[kMine];
+#pragma unroll
+            for (int m = 0; m < kMine; ++m) acc[m] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) {
+                sel_phase();
+                const SelFrag<Tc> c = sel_rows(s.C + (16 * row_a + l) * SC + 32 * ks, g);
+#pragma unroll
+                for (int m = 0; m < kMine; ++m)
+                    sel_mma(acc[m], sel_rows(s.B + (16 * col_of(m) + l) * SB + 32 * ks, g),
+                            m < 2 ? c : sel_rows(s.C + (16 * row_b + l) * SC + 32 * ks, g));
+            }
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                sel_phase();
+                const SelSteps<Q>& st = s.steps[u][k & 1];
+#pragma unroll
+                for (int m = 0; m < kMine; ++m) {
+                    const int i = 16 * (m < 2 ? row_a : row_b) + l, j0 = 16 * col_of(m) + 4 * g;
+                    const int whole = st.whole[i];
+                    const float rest = st.rest[i];
+                    float v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float decay = sel_exp2(whole - st.whole[j0 + r], rest - st.rest[j0 + r]);
+                        const float w = acc[m][r] * (decay * st.step[j0 + r]);
+                        v[r] = j0 + r <= i ? w : 0.0f;
+                    }
+                    sel_store<Tc, 4>(s.weights[u] + i * SW + j0, v);
+                }
+            }
+            __syncthreads();
+
+            sel_f4 out[2][QT];
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+#pragma unroll
+                for (int it = 0; it < QT; ++it) out[h][it] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) {
+                sel_phase();
+                SelFrag<Tc> sf[2];  // the state that enters, over the states
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) sf[h].set(e, state[h][2 * ks + (e >> 2)][e & 3]);
+#pragma unroll
+                for (int it = 0; it < QT; ++it) {
+                    const SelFrag<Tc> c = sel_rows(s.C + (16 * it + l) * SC + 32 * ks, g);
+                    sel_mma(out[0][it], sf[0], c);
+                    sel_mma(out[1][it], sf[1], c);
+                }
+            }
+            sel_phase();
+#pragma unroll
+            for (int it = 0; it < QT; ++it) {
+                const float e = steps.from_start[16 * it + l];
+                out[0][it] *= e;
+                out[1][it] *= e;
+            }
 #pragma unroll
             for (int ks = 0; ks < QK; ++ks)
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (!(fabsf(xf[ks].get(e)) < INFINITY)) xf[ks].set(e, 0.0f);
-
-        if constexpr (kOut) {
-#pragma unroll
-            for (int m = 0; m < kMyTiles; ++m) {
-                const int t = wave + 4 * m;
-                if (t >= kTiles) break;
-                const int it = t >= 6 ? 3 : t >= 3 ? 2 : t >= 1 ? 1 : 0, jt = t - it * (it + 1) / 2;
-                const int i = 16 * it + l, j0 = 16 * jt + 4 * g;
-                sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-                for (int ks = 0; ks < NK; ++ks)
-                    sel_mma(acc, sel_rows(s.B + (16 * jt + l) * SB + 32 * ks, g), sel_rows(s.C + i * SC + 32 * ks, g));
-                sel_settle(acc);
-                const int whole = steps.whole[i];
-                const float rest = steps.rest[i];
-                float v[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float decay = sel_exp2(whole - steps.whole[j0 + r], rest - steps.rest[j0 + r]);
-                    v[r] = j0 + r <= i ? acc[r] * (decay * steps.step[j0 + r]) : 0.0f;
+                for (int it = 2 * ks; it < QT; ++it) {
+                    const SelFrag<Tc> w = sel_rows(s.weights[mine] + (16 * it + l) * SW + 32 * ks, g);
+                    sel_mma(out[0][it], xf[0][ks], w);
+                    sel_mma(out[1][it], xf[1][ks], w);
                 }
-                sel_store<Tc, 4>(s.weights + i * SW + j0, v);
-            }
-        }
-        if (wave == kStepWave && k + 1 < n_chunks) {
-            sel_steps<Q>(s.steps[(k + 1) & 1], dt, seq.n - token(k + 1), A, bias, a.softplus);
-            dt = k + 2 < n_chunks ? sel_dt<Q>(a, seq, token(k + 2), head) : 0.0f;
-        }
-        if constexpr (kOut) {
-            __syncthreads();
-            SelFrag<Tc> sf[NK];  // the state that enters, over the states
+            sel_settle(out[0]);
+            sel_settle(out[1]);
+            if (!finite)
 #pragma unroll
-            for (int ks = 0; ks < NK; ++ks)
+                for (int h = 0; h < 2; ++h) {
+                    sel_f4 count[QT];  // how many of them each token reads
 #pragma unroll
-                for (int e = 0; e < 8; ++e) sf[ks].set(e, state[2 * ks + (e >> 2)][e & 3]);
+                    for (int it = 0; it < QT; ++it) count[it] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int ks = 0; ks < QK; ++ks) {
+                        const SelFrag<Tc> ones = odd(h, ks);
+#pragma unroll
+                        for (int it = 2 * ks; it < QT; ++it) {
+                            SelFrag<Tc> up_to;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                up_to.set(e, 32 * ks + 16 * (e >> 2) + 4 * g + (e & 3) <= 16 * it + l ? 1.0f : 0.0f);
+                            sel_mma(count[it], ones, up_to);
+                        }
+                    }
+                    sel_settle(count);
+#pragma unroll
+                    for (int it = 0; it < QT; ++it)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) out[h][it][r] = count[it][r] > 0.0f ? NAN : out[h][it][r];
+                }
+            sel_phase();
+            T* const y = static_cast<T*>(a.y) + ((seq.row0 + t0) * a.n_heads + head) * a.dim + p_tile;
+            const unsigned row = (unsigned)(a.n_heads * a.dim);
 #pragma unroll
             for (int it = 0; it < QT; ++it) {
-                const int i = 16 * it + l, c = 16 * wave + 4 * g;
-                sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                const int i = 16 * it + l;
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks) sel_mma(acc, sf[ks], sel_rows(s.C + i * SC + 32 * ks, g));
-                acc *= steps.from_start[i];
-#pragma unroll
-                for (int ks = 0; ks <= it / 2; ++ks) sel_mma(acc, xf[ks], sel_rows(s.weights + i * SW + 32 * ks, g));
-                sel_settle(acc);
-                if (unfinite) sel_add_unfinite<Tc, Q, SX, SW>(acc, s.x, s.weights, c, i);
-                if (i < n && 16 * wave < cols) {
+                for (int h = 0; h < 2; ++h) {
+                    const int c = p_wave + 16 * h + 4 * g;
                     float own[4];
-                    sel_load<Tc, 4>(s.x + i * SX + c, own);
+                    sel_load<Tc, 4>(xs + i * SX + c, own);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[r] = fmaf(D, own[r], acc[r]);
-                    T* row = static_cast<T*>(a.y) + ((seq.row0 + t0 + i) * a.n_heads + head) * a.dim + p_tile;
-                    sel_store4(row, c, cols, plan.vec & kSelVecY, acc);
+                    for (int r = 0; r < 4; ++r) out[h][it][r] = fmaf(D, own[r], out[h][it][r]);
+                    if (i < n && writes) sel_store4<VEC>(y + (unsigned)i * row, c, cols, out[h][it]);
                 }
             }
         }
         if (WALK == kSelStates) {
             const long long chunk = first_chunk + t0 / Q;
-            if (p < a.dim && chunk < plan.n_chunks) {
+            if (writes && chunk < plan.n_chunks) {
                 float* out = plan.states + (back * plan.n_chunks + chunk) * all_states + my_state;
 #pragma unroll
-                for (int t = 0; t < NT; ++t) sel_state_store(out, 16 * t + 4 * g, a.states, vec_state, state[t]);
+                for (int h = 0; h < 2; ++h)
+                    if (there[h])
+#pragma unroll
+                        for (int t = 0; t < NT; ++t)
+                            sel_state_store<VEC>(out + h * next_rows, 16 * t + 4 * g, a.states, state[h][t]);
             }
         }
 
+        const float* const weight = back ? steps.from_start : steps.to_end_step;
         const float all = steps.from_start[Q - 1];
         keeps *= all;
 #pragma unroll
-        for (int t = 0; t < NT; ++t) state[t] *= all;
+        for (int h = 0; h < 2; ++h) {
+            float keep = all;
+            if (!finite) {  // (lane l of each quarter of the wave holds other tokens of row p)
+                float bad = 0.0f;
+#pragma unroll
+                for (int ks = 0; ks < QK; ++ks) {
+                    const SelFrag<Tc> ones = odd(h, ks);
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) bad += ones.get(e);
+                }
+                bad += __shfl_xor(bad, 16);
+                bad += __shfl_xor(bad, 32);
+                keep = bad > 0.0f ? NAN : all;
+            }
+#pragma unroll
+            for (int t = 0; t < NT; ++t) state[h][t] *= keep;
+        }
 #pragma unroll
         for (int ks = 0; ks < QK; ++ks) {
-            float v[8];
+            sel_phase();
+            SelFrag<Tc> split[2][kSplits];
+            float w[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int j = 32 * ks + 16 * (e >> 2) + 4 * g + (e & 3);
-                v[e] = xf[ks].get(e) * (back ? steps.from_start[j] : steps.to_end[j] * steps.step[j]);
+            for (int e = 0; e < 8; ++e) w[e] = weight[32 * ks + 16 * (e >> 2) + 4 * g + (e & 3)];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = xf[h][ks].get(e) * w[e];
+                sel_split<Tc>(v, split[h]);
             }
-            SelFrag<Tc> split[kSplits];
-            sel_split<Tc>(v, split);
+            constexpr int kSide = 2;  // tiles side by side
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const SelFrag<Tc> bf = sel_cols(s.B + 32 * ks * SB + 16 * t, SB, l, g);
+            for (int t0 = 0; t0 < NT; t0 += kSide) {
+                if (t0 % 4 == 0) sel_phase();
+                SelFrag<Tc> bf[kSide];
 #pragma unroll
-                for (int q = 0; q < kSplits; ++q) sel_mma(state[t], bf, split[q]);
+                for (int t = 0; t < kSide; ++t) bf[t] = sel_cols(s.B + 32 * ks * SB + 16 * (t0 + t), SB, l, g);
+#pragma unroll
+                for (int q = 0; q < kSplits; ++q)
+#pragma unroll
+                    for (int t = 0; t < kSide; ++t)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) sel_mma(state[h][t0 + t], bf[t], split[h][q]);
             }
         }
-        sel_settle(state);
-        if (unfinite)
-            for (int j = 0; j < n; ++j) {
-                const float v = (float)s.x[j * SX + 16 * wave + l];
-                if (!(fabsf(v) < INFINITY))
-#pragma unroll
-                    for (int t = 0; t < NT; ++t)
-#pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            state[t][r] = fmaf(v * (steps.to_end[j] * steps.step[j]),
-                                               (float)s.B[j * SB + 16 * t + 4 * g + r], state[t][r]);
-            }
     }
+    sel_settle(state[0]);
+    sel_settle(state[1]);
     float* end = nullptr;
     if (WALK == kSelEnds) {
         end = ends + segment * all_states + my_state;
-        if (tile == 0 && threadIdx.x == 0)
+        if (writes && p_tile == 0 && (threadIdx.x & 127) == 0)
             plan.keeps[(back * plan.n_segments + segment) * a.n_heads + head] = keeps;
     } else if (seq.chunk == (back ? 0 : n_segments - 1)) {
         end = kOut ? a.final : back ? a.dinitial : nullptr;
         if (end) end += seq.seq * all_states + my_state;
     }
-    if (end && p < a.dim)
+    if (end && writes)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) sel_state_store(end, 16 * t + 4 * g, a.states, vec_state, state[t]);
+        for (int h = 0; h < 2; ++h)
+            if (there[h])
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    sel_state_store<VEC>(end + h * next_rows, 16 * t + 4 * lane_g, a.states, state[h][t]);
 }
 
 // ------------------------------------------------------------------------------- host side
-static inline bool sel_rows_aligned(const nhip_rows& r, int type) {
+// Whether rows can be read 16 bytes at a time, with offsets of 32 bits within a chunk
+static inline bool sel_rows_wide(const nhip_rows& r, int type, int cols) {
     const int v = 16 / sel_size(type);
-    return sel_aligned(r.p, 16) && r.seq % v == 0 && r.token % v == 0 && r.head % v == 0;
+    return sel_aligned(r.p, 16) && cols % v == 0 && r.seq % v == 0 && r.token % v == 0 && r.head % v == 0 &&
+           r.token < (1 << 23);
 }
 
 static inline int sel_scan_check(const nhip_scan_args* a) {
@@ -344,6 +469,8 @@ static inline int sel_scan_check(const nhip_scan_args* a) {
     // (work-groups: at most one per chunk, head and tile of the dimension in each direction)
     const long long most = 0x7fffffffLL, chunks = sel_max_chunks(a->tokens, 32), tiles = (a->dim + 63) / 64;
     if (chunks > most || chunks * a->n_heads > most || 2 * chunks * a->n_heads * tiles > most) return NHIP_E_BADARG;
+    // (offsets of 32 bits within a chunk)
+    if ((long long)a->n_heads * a->dim >= (1 << 24)) return NHIP_E_BADARG;
     return 0;
 }
 
@@ -359,7 +486,8 @@ static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions,
     p.directions = directions;
     p.states = states;
     p.n_chunks = sel_max_chunks(a.tokens, q);
-    const long long walks = (long long)directions * a.n_heads * p.n_tiles;
+    p.pairs = (a.n_heads / a.n_groups * p.n_tiles + 1) / 2;
+    const long long walks = (long long)directions * a.n_groups * p.pairs;
     const long long longest = a.tokens.starts ? (a.tokens.n_tokens + q - 1) / q : sel_chunks(a.tokens.length, q);
     const long long total = a.tokens.starts ? longest : longest * a.tokens.n_seqs;
     long long wanted = (512 + walks - 1) / walks;  // segments
@@ -371,15 +499,11 @@ static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions,
     p.n_segments = sel_max_chunks(a.tokens, q * p.chunks);
     p.ends = cut ? reinterpret_cast<float*>(16) : nullptr;  // (its place is the caller's to fill in)
     p.keeps = nullptr;
-    p.vec = 0;
-    if (sel_rows_aligned(a.x, a.type)) p.vec |= kSelVecX;
-    if (sel_rows_aligned(a.B, a.type)) p.vec |= kSelVecB;
-    if (sel_rows_aligned(a.C, a.type)) p.vec |= kSelVecC;
-    if (sel_rows_aligned(a.dy, a.type)) p.vec |= kSelVecDy;
-    if (a.dim % 4 == 0 && sel_aligned(a.y, 16) && sel_aligned(a.dx, 16)) p.vec |= kSelVecY;
-    if (a.states % 4 == 0 && sel_aligned(a.initial, 16) && sel_aligned(a.final, 16) && sel_aligned(a.dfinal, 16) &&
-        sel_aligned(a.dinitial, 16) && sel_aligned(a.dB, 16) && sel_aligned(a.dC, 16))
-        p.vec |= kSelVecState;
+    p.vec = sel_rows_wide(a.x, a.type, a.dim) && sel_rows_wide(a.B, a.type, a.states) &&
+            sel_rows_wide(a.C, a.type, a.states) && (!a.dy.p || sel_rows_wide(a.dy, a.type, a.dim));
+    for (const void* q : {(const void*)a.y, (const void*)a.dx, (const void*)a.dB, (const void*)a.dC, (const void*)a.initial,
+                          (const void*)a.final, (const void*)a.dfinal, (const void*)a.dinitial})
+        p.vec = p.vec && sel_aligned(q, 16);
     return p;
 }
 
@@ -409,7 +533,7 @@ template <> struct SelCompute<__bf16> { using type = __bf16; };
 
 template <int WALK> static inline int sel_walk_launch(hipStream_t stream, const nhip_scan_args& a, const SelWalkPlan& plan,
                                                       bool first, bool last) {
-    const unsigned grid = (unsigned)(plan.directions * plan.n_segments * a.n_heads * plan.n_tiles);
+    const unsigned grid = (unsigned)(plan.directions * plan.n_segments * a.n_groups * plan.pairs);
     int rc = NHIP_E_BADARG;
     sel_with_type(a.type, [&](auto t) {
         using T = decltype(t);
@@ -417,7 +541,7 @@ template <int WALK> static inline int sel_walk_launch(hipStream_t stream, const 
         sel_with_states(a.states, [&](auto np) {
             constexpr int NP = decltype(np)::value;
             constexpr size_t lds = sizeof(SelWalkLds<Tc, NP, WALK == kSelOutputs>);
-            auto kernel = sel_walk_kernel<T, Tc, NP, WALK>;
+            auto kernel = plan.vec ? sel_walk_kernel<T, Tc, NP, WALK, true> : sel_walk_kernel<T, Tc, NP, WALK, false>;
             rc = sel_allow_lds(kernel, lds);
             if (rc) return;
             if (first && last) NHIP_LAUNCH(kernel, dim3(grid), dim3(NHIP_WG), lds, stream, a, plan);

@@ -19,7 +19,7 @@
 namespace {
 
 struct GradPlan {
-    int vec, n_tiles;
+    int n_tiles;
     int heads_per_group;   // heads that a work-group goes through
     int blocks;            // work-groups for the heads of one group
     long long n_chunks;
@@ -52,7 +52,7 @@ __device__ __forceinline__ void state_cols(const float* s, int p0, int n, int di
     }
 }
 
-template <class T, class Tc, int NP>
+template <class T, class Tc, int NP, bool VEC>
 __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPlan plan) {
     using Lds = GradLds<Tc, NP>;
     constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
@@ -78,14 +78,13 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
     }
     const int tid = threadIdx.x, wave = tid / NHIP_WAVE, lane = tid & 63, l = tid & 15, g = lane >> 4;
     const long long head_state = (long long)a.dim * a.states;
-    const bool vec_state = plan.vec & kSelVecState;
 
     {
-        SelStage<T, Tc, Q, NP> stage;
-        stage.load(sel_row<T>(a.B, a.tokens, seq, t0) + group * a.B.head, a.B.token, n, a.states, plan.vec & kSelVecB);
-        stage.template store<SN>(s.B);
-        stage.load(sel_row<T>(a.C, a.tokens, seq, t0) + group * a.C.head, a.C.token, n, a.states, plan.vec & kSelVecC);
-        stage.template store<SN>(s.C);
+        SelStage<T, Tc, Q, NP, VEC> stage_B, stage_C;
+        stage_B.load(sel_row<T>(a.B, a.tokens, seq, t0) + group * a.B.head, a.B.token, n, a.states);
+        stage_C.load(sel_row<T>(a.C, a.tokens, seq, t0) + group * a.C.head, a.C.token, n, a.states);
+        stage_B.template store<SN>(s.B, n, a.states);
+        stage_C.template store<SN>(s.C, n, a.states);
     }
     for (int q = tid; q < Q * SW; q += NHIP_WG) s.xl[q] = s.kl[q] = (Tc)0.0f;  // (i < j for good)
     __syncthreads();
@@ -120,14 +119,12 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
         const float* const G = plan.G + ((long long)chunk * a.n_heads + head) * head_state;
         for (int tile = 0; tile < plan.n_tiles; ++tile) {
             const int p_tile = tile * 64, cols = min(64, a.dim - p_tile);
-            SelStage<T, Tc, Q, 64> stage_x, stage_dy;
-            stage_x.load(sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n, cols,
-                         plan.vec & kSelVecX);
-            stage_dy.load(sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token, n, cols,
-                          plan.vec & kSelVecDy);
+            SelStage<T, Tc, Q, 64, VEC> stage_x, stage_dy;
+            stage_x.load(sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n, cols);
+            stage_dy.load(sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token, n, cols);
             __syncthreads();  // the tile before has been read
-            stage_x.template store<SX>(s.x);
-            stage_dy.template store<SX>(s.dy);
+            stage_x.template store<SX>(s.x, n, cols);
+            stage_dy.template store<SX>(s.dy, n, cols);
             if (tile == 0) {
                 if (wave == 0)
                     sel_steps<Q>(s.steps, sel_dt<Q>(a, seq, t0, head), n, a.A[head], a.dt_bias ? a.dt_bias[head] : 0.0f,
@@ -193,7 +190,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
                     for (int h = 0; h < 2; ++h) {
                         const int c = 32 * ks + 16 * h + 4 * g;
                         sel_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if (p < a.dim) v = sel_state_load(G + (long long)p * a.states, c, a.states, vec_state);
+                        if (p < a.dim) v = sel_state_load<VEC>(G + (long long)p * a.states, c, a.states);
 #pragma unroll
                         for (int r = 0; r < 4; ++r) gf[ks].set(4 * h + r, v[r]);
                     }
@@ -206,7 +203,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
                     sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                     for (int ks = 0; ks < NK; ++ks) sel_mma(acc, gf[ks], sel_rows(s.B + j * SN + 32 * ks, g));
-                    acc *= s.steps.to_end[j] * s.steps.step[j];
+                    acc *= s.steps.to_end_step[j];
 #pragma unroll
                     for (int ks = jt / 2; ks < QK; ++ks) sel_mma(acc, df[ks], sel_rows(s.kl + j * SW + 32 * ks, g));
                     sel_settle(acc);
@@ -215,7 +212,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
 #pragma unroll
                         for (int r = 0; r < 4; ++r) acc[r] = fmaf(D, (float)s.dy[j * SX + c + r], acc[r]);
                         T* row = static_cast<T*>(a.dx) + ((seq.row0 + t0 + j) * a.n_heads + head) * a.dim + p_tile;
-                        sel_store4(row, c, cols, plan.vec & kSelVecY, acc);
+                        sel_store4<VEC>(row, c, cols, acc);
                     }
                 }
             }
@@ -352,12 +349,12 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
             if (i >= n || c >= a.states) continue;
             const long long at = (seq.row0 + t0 + i) * row + (long long)group * a.states;
             if (plan.blocks == 1) {
-                sel_store4(static_cast<T*>(a.dB) + at, c, a.states, vec_state, dB[m][t]);
-                sel_store4(static_cast<T*>(a.dC) + at, c, a.states, vec_state, dC[m][t]);
+                sel_store4<VEC>(static_cast<T*>(a.dB) + at, c, a.states, dB[m][t]);
+                sel_store4<VEC>(static_cast<T*>(a.dC) + at, c, a.states, dC[m][t]);
             } else {
                 float* out = plan.shared + (long long)block * 2 * a.tokens.n_tokens * row;
-                sel_state_store(out + at, c, a.states, vec_state, dB[m][t]);
-                sel_state_store(out + a.tokens.n_tokens * row + at, c, a.states, vec_state, dC[m][t]);
+                sel_state_store<VEC>(out + at, c, a.states, dB[m][t]);
+                sel_state_store<VEC>(out + a.tokens.n_tokens * row + at, c, a.states, dC[m][t]);
             }
         }
     }
@@ -429,7 +426,7 @@ extern "C" int nhip_selective_scan_grad(void* stream, const nhip_scan_args* args
     if (int e = sel_walk<kSelStates>(st, a, m.walk, false)) return e;
     int rc = 0;
     if (groups) {
-        const GradPlan plan{m.walk.vec, m.walk.n_tiles, m.heads_per_group, m.blocks, m.n_chunks,
+        const GradPlan plan{m.walk.n_tiles, m.heads_per_group, m.blocks, m.n_chunks,
                             m.walk.states, m.walk.states + m.states, parts, shared};
         sel_with_type(a.type, [&](auto t) {
             using T = decltype(t);
@@ -437,7 +434,7 @@ extern "C" int nhip_selective_scan_grad(void* stream, const nhip_scan_args* args
             sel_with_states(a.states, [&](auto np) {
                 constexpr int NP = decltype(np)::value;
                 constexpr size_t lds = sizeof(GradLds<Tc, NP>);
-                auto kernel = grad_kernel<T, Tc, NP>;
+                auto kernel = m.walk.vec ? grad_kernel<T, Tc, NP, true> : grad_kernel<T, Tc, NP, false>;
                 rc = sel_allow_lds(kernel, lds);
                 if (rc) return;
                 hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(NHIP_WG), lds, st, a, plan);
