@@ -136,14 +136,16 @@ __device__ __forceinline__ SelSeq sel_seq_of_chunk(const nhip_tokens& t, int c, 
             const int other = __shfl_up(sum, d);
             if (lane >= d) sum += other;
         }
-        const int total = __shfl(sum, NHIP_WAVE - 1);
+        const int total = __builtin_amdgcn_readlane(sum, NHIP_WAVE - 1);
         if (c < before + total) {
             const unsigned long long past = __ballot(before + sum > c);
             const int at = __ffsll((long long)past) - 1;
-            r.seq = s0 + at;
-            r.n = __shfl(n, at);
-            r.chunk = c - (before + __shfl(sum, at) - __shfl(mine, at));
-            r.row0 = sel_bound(t, r.seq);
+            // (in scalar registers: they are the same in all lanes, which the compiler cannot see)
+            const int lane_of = __builtin_amdgcn_readfirstlane(at);
+            r.seq = s0 + lane_of;
+            r.n = __builtin_amdgcn_readlane(n, lane_of);
+            r.chunk = c - (before + __builtin_amdgcn_readlane(sum - mine, lane_of));
+            r.row0 = __builtin_amdgcn_readfirstlane(sel_bound(t, r.seq));
             return r;
         }
         before += total;
@@ -167,8 +169,8 @@ __device__ __forceinline__ SelSeq sel_seq(const nhip_tokens& t, int s, int q) {
 #pragma unroll
     for (int d = 1; d < NHIP_WAVE; d *= 2) sum += __shfl_xor(sum, d);
     r.chunk = __builtin_amdgcn_readfirstlane(sum);
-    r.n = sel_length(t, s);
-    r.row0 = sel_bound(t, s);
+    r.n = __builtin_amdgcn_readfirstlane(sel_length(t, s));
+    r.row0 = __builtin_amdgcn_readfirstlane(sel_bound(t, s));
     return r;
 }
 

@@ -20,8 +20,8 @@ enum SelWalk {
 };
 
 // Sequences are cut into segments of `chunks` chunks.  A work-group walks over one for two units of its heads'
-// group, a unit being 64 of a head's dimension.  A first launch (kSelEnds) leaves every segment's own contribution, the second begins
-// each with the sum over those before it.
+// group, a unit being 64 of a head's dimension.  A first launch (kSelEnds) leaves what every segment adds on its
+// own, a second turns that into the states that the segments begin with, for the walk itself.
 struct SelWalkPlan {
     int n_tiles;            // units of a head
     int pairs;              // of units in a group
@@ -151,21 +151,13 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
 #pragma unroll
         for (int t = 0; t < NT; ++t) state[h][t] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
         if (WALK != kSelEnds && there[h]) {
-            const float* from = back ? a.dfinal : a.initial;
+            const float* from = plan.ends ? ends + segment * all_states
+                                : back    ? (a.dfinal ? a.dfinal + seq.seq * all_states : nullptr)
+                                          : (a.initial ? a.initial + seq.seq * all_states : nullptr);
             if (from)
 #pragma unroll
                 for (int t = 0; t < NT; ++t)
-                    state[h][t] = sel_state_load<VEC>(from + seq.seq * all_states + my_state + h * next_rows, 16 * t + 4 * lane_g, a.states);
-            // the segments walked before this one, in their order
-            const int first = segment - seq.chunk, before = back ? n_segments - 1 - seq.chunk : seq.chunk;
-            for (int k = 0; k < before; ++k) {
-                const int other = first + (back ? n_segments - 1 - k : k);
-                const float keeps = plan.keeps[(back * plan.n_segments + other) * a.n_heads + head];
-                const float* end = ends + other * all_states + my_state + h * next_rows;
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    state[h][t] = state[h][t] * keeps + sel_state_load<VEC>(end, 16 * t + 4 * lane_g, a.states);
-            }
+                    state[h][t] = sel_state_load<VEC>(from + my_state + h * next_rows, 16 * t + 4 * lane_g, a.states);
         }
     }
     if constexpr (kOut)  // (above the diagonal for good)
@@ -453,6 +445,43 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
                     sel_state_store<VEC>(end + h * next_rows, 16 * t + 4 * lane_g, a.states, state[h][t]);
 }
 
+// From what each segment of a sequence adds to the state to the state that it begins with, in place: a lane takes
+// V elements of a head's state through the segments.
+template <int V>
+static __global__ __launch_bounds__(NHIP_WG) void sel_begin_kernel(nhip_scan_args a, SelWalkPlan plan, int q) {
+    const int head_state = a.dim * a.states, blocks = (head_state + NHIP_WG * V - 1) / (NHIP_WG * V);
+    const int block = blockIdx.x % blocks, head = (blockIdx.x / blocks) % a.n_heads;
+    const int which = blockIdx.x / (blocks * a.n_heads), s = which % a.tokens.n_seqs, back = which / a.tokens.n_seqs;
+    const SelSeq seq = sel_seq(a.tokens, s, q * plan.chunks);
+    const int at = (block * NHIP_WG + threadIdx.x) * V, n = sel_chunks(seq.n, q * plan.chunks);
+    if (at >= head_state) return;
+    const long long all_states = (long long)a.n_heads * head_state, mine = (long long)head * head_state + at;
+    float state[V];
+    const float* from = back ? a.dfinal : a.initial;
+#pragma unroll
+    for (int i = 0; i < V; ++i) state[i] = from ? from[s * all_states + mine + i] : 0.0f;
+    float* const ends = plan.ends + (back * plan.n_segments + seq.chunk) * all_states + mine;
+    const float* const keeps = plan.keeps + (back * plan.n_segments + seq.chunk) * a.n_heads + head;
+    constexpr int kAhead = 8;
+    for (int k0 = 0; k0 < n; k0 += kAhead) {
+        float adds[kAhead][V], keep[kAhead];
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {  // (the last one's was not formed: nobody begins with it)
+            const int w = min(k0 + k, n - 1), segment = back ? n - 1 - w : w;
+            sel_load<float, V>(ends + segment * all_states, adds[k]);
+            keep[k] = keeps[(long long)segment * a.n_heads];
+        }
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+            if (k0 + k >= n) break;
+            const int segment = back ? n - 1 - k0 - k : k0 + k;
+            sel_store<float, V>(ends + segment * all_states, state);
+#pragma unroll
+            for (int i = 0; i < V; ++i) state[i] = fmaf(state[i], keep[k], adds[k][i]);
+        }
+    }
+}
+
 // ------------------------------------------------------------------------------- host side
 // Whether rows can be read 16 bytes at a time, with offsets of 32 bits within a chunk
 static inline bool sel_rows_wide(const nhip_rows& r, int type, int cols) {
@@ -469,6 +498,7 @@ static inline int sel_scan_check(const nhip_scan_args* a) {
     // (work-groups: at most one per chunk, head and tile of the dimension in each direction)
     const long long most = 0x7fffffffLL, chunks = sel_max_chunks(a->tokens, 32), tiles = (a->dim + 63) / 64;
     if (chunks > most || chunks * a->n_heads > most || 2 * chunks * a->n_heads * tiles > most) return NHIP_E_BADARG;
+    if (a->tokens.n_seqs * tiles * 64 * a->states / 256 * a->n_heads * 2 > most) return NHIP_E_BADARG;
     // (offsets of 32 bits within a chunk)
     if ((long long)a->n_heads * a->dim >= (1 << 24)) return NHIP_E_BADARG;
     return 0;
@@ -558,7 +588,14 @@ template <int WALK> static inline int sel_walk_launch(hipStream_t stream, const 
 // follows in this entry point.
 template <int WALK> static inline int sel_walk(hipStream_t stream, const nhip_scan_args& a, const SelWalkPlan& plan, bool last) {
     if (plan.n_segments == 0) return 0;
-    if (plan.ends)
+    if (plan.ends) {
         if (int e = sel_walk_launch<kSelEnds>(stream, a, plan, true, false)) return e;
+        const int v = plan.vec ? 4 : 1, per = NHIP_WG * v, q = sel_chunk_tokens(a.states);
+        const long long blocks = ((long long)a.dim * a.states + per - 1) / per;
+        const dim3 grid((unsigned)(blocks * a.n_heads * a.tokens.n_seqs * plan.directions));
+        if (plan.vec) hipLaunchKernelGGL(sel_begin_kernel<4>, grid, dim3(NHIP_WG), 0, stream, a, plan, q);
+        else hipLaunchKernelGGL(sel_begin_kernel<1>, grid, dim3(NHIP_WG), 0, stream, a, plan, q);
+        NHIP_LAUNCH_CHECK();
+    }
     return sel_walk_launch<WALK>(stream, a, plan, !plan.ends, last);
 }
