@@ -43,17 +43,37 @@ template <class Tc, int NP> struct GradLds {
     float over[Q / 16][Q], col[Q / 16][Q], diag[Q], dot[Q], q[4][Q], r[4][Q], z[4];
 };
 
-// Eight elements of a state across its rows: k over 32 rows from p0, column n
+// Eight elements of a state across its rows: k over 32 rows from p0, column n.  Loads are unconditional (one
+// under a condition is waited for where its branch ends), from places cut to those that exist: what is too
+// much meets zeros of the other operand.
 __device__ __forceinline__ void state_cols(const float* s, int p0, int n, int dim, int states, int g, float (&v)[8]) {
+    const unsigned c = (unsigned)min(n, states - 1);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const int p = p0 + 16 * (e >> 2) + 4 * g + (e & 3);
-        v[e] = p < dim && n < states ? s[(long long)p * states + n] : 0.0f;
+        const int p = min(p0 + 16 * (e >> 2) + 4 * g + (e & 3), dim - 1);
+        v[e] = s[(unsigned)p * (unsigned)states + c];
+    }
+}
+// Eight elements of row p, as a fragment over the states from n0
+template <class Tc, bool VEC>
+__device__ __forceinline__ void state_row(const float* s, int p, int n0, int dim, int states, int g, float (&v)[8]) {
+    const float* row = s + (unsigned)min(p, dim - 1) * (unsigned)states;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const int n = n0 + 16 * h + 4 * g;
+        if constexpr (VEC) {
+            const sel_f4 four = *reinterpret_cast<const sel_f4*>(row + min(n, states - 4));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[4 * h + r] = four[r];
+        } else {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) v[4 * h + r] = row[min(n + r, states - 1)];
+        }
     }
 }
 
 template <class T, class Tc, int NP, bool VEC>
-__global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPlan plan) {
+__global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(nhip_scan_args a, GradPlan plan) {
     using Lds = GradLds<Tc, NP>;
     constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
     constexpr int kTiles = QT * (QT + 1) / 2, kMyTiles = (kTiles + 3) / 4, kMyNT = (NT + 3) / 4;
@@ -76,7 +96,8 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
             parts[h] = parts[a.n_heads + h] = parts[2 * a.n_heads + h] = 0.0f;
         return;
     }
-    const int tid = threadIdx.x, wave = tid / NHIP_WAVE, lane = tid & 63, l = tid & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, lane_l = tid & 15, lane_g = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid / NHIP_WAVE);
     const long long head_state = (long long)a.dim * a.states;
 
     {
@@ -102,8 +123,8 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
         if (t < kTiles)
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks)
-                sel_mma(K[m], sel_rows(s.C + (16 * it + l) * SN + 32 * ks, g),
-                        sel_rows(s.B + (16 * tile_j[m] + l) * SN + 32 * ks, g));
+                sel_mma(K[m], sel_rows(s.C + (16 * it + lane_l) * SN + 32 * ks, lane_g),
+                        sel_rows(s.B + (16 * tile_j[m] + lane_l) * SN + 32 * ks, lane_g));
         sel_settle(K[m]);
     }
 
@@ -122,6 +143,18 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
             SelStage<T, Tc, Q, 64, VEC> stage_x, stage_dy;
             stage_x.load(sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n, cols);
             stage_dy.load(sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token, n, cols);
+            // (addresses are formed anew in each tile: kept, they take the registers of the sums)
+            int l = lane_l, g = lane_g;
+            asm volatile("" : "+v"(l), "+v"(g));
+            float Sv[kMyNT][2][8], Gv[kMyNT][2][8];  // columns 16 (wave + 4 m) + l of both states
+#pragma unroll
+            for (int m = 0; m < kMyNT; ++m)
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks) {
+                    const int nt = min(wave + 4 * m, NT - 1);
+                    state_cols(S, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Sv[m][ks]);
+                    state_cols(G, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Gv[m][ks]);
+                }
             __syncthreads();  // the tile before has been read
             stage_x.template store<SX>(s.x, n, cols);
             stage_dy.template store<SX>(s.dy, n, cols);
@@ -135,10 +168,15 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
                 if (tid < 4) s.z[tid] = 0.0f;
             }
             __syncthreads();
+            float Gr[NK][8];  // row p of G
+            const int p = p_tile + 16 * wave + l;
+#pragma unroll
+            for (int ks = 0; ks < NK; ++ks) state_row<Tc, VEC>(G, p, 32 * ks, a.dim, a.states, g, Gr[ks]);
 
 #pragma unroll
             for (int m = 0; m < kMyTiles; ++m) {
                 if (tile_i[m] < 0) continue;
+                sel_phase();
                 const int it = tile_i[m], jt = tile_j[m], j = 16 * jt + l, i0 = 16 * it + 4 * g;
                 sel_f4 X = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -154,7 +192,7 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
                     const float all = i >= j ? K[m][r] * X[r] * L : 0.0f;
                     kl[r] = i >= j ? K[m][r] * L * step : 0.0f;
                     xl[r] = i >= j ? X[r] * L * step : 0.0f;
-                    if (i == j) {
+                    if (it == jt && i == j) {
                         s.diag[j] += all;
                         s.dot[j] += X[r];
                     }
@@ -182,23 +220,17 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
 
             // dx: 16 of the dimension to a wave
             if (16 * wave < cols) {
-                const int p = p_tile + 16 * wave + l;
                 SelFrag<Tc> gf[NK];
 #pragma unroll
                 for (int ks = 0; ks < NK; ++ks)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int c = 32 * ks + 16 * h + 4 * g;
-                        sel_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
-                        if (p < a.dim) v = sel_state_load<VEC>(G + (long long)p * a.states, c, a.states);
-#pragma unroll
-                        for (int r = 0; r < 4; ++r) gf[ks].set(4 * h + r, v[r]);
-                    }
+                    for (int e = 0; e < 8; ++e) gf[ks].set(e, Gr[ks][e]);
                 SelFrag<Tc> df[QK];
 #pragma unroll
                 for (int ks = 0; ks < QK; ++ks) df[ks] = sel_cols(s.dy + 32 * ks * SX + 16 * wave, SX, l, g);
 #pragma unroll
                 for (int jt = 0; jt < QT; ++jt) {
+                    sel_phase();
                     const int j = 16 * jt + l;
                     sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -225,19 +257,21 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
             for (int m = 0; m < kMyNT; ++m) {
                 const int nt = wave + 4 * m;
                 if (nt >= NT) continue;
-                float Sv[2][8], Gv[2][8];
+                sel_phase();
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) {
-                    state_cols(S, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Sv[ks]);
-                    state_cols(G, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Gv[ks]);
+                for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) z = fmaf(Sv[ks][e], Gv[ks][e], z);
-                }
+                    for (int e = 0; e < 8; ++e) {
+                        const int row = p_tile + 32 * ks + 16 * (e >> 2) + 4 * g + (e & 3);
+                        const float both = Sv[m][ks][e] * Gv[m][ks][e];
+                        z += row < a.dim && 16 * nt + l < a.states ? both : 0.0f;
+                    }
                 SelFrag<Tc> f[2][kSplits];
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Sv[ks], f[ks]);
+                for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Sv[m][ks], f[ks]);
 #pragma unroll
                 for (int it = 0; it < QT; ++it) {
+                    sel_phase();
                     const int i = 16 * it + l;
                     sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -258,9 +292,10 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
                 }
                 sel_settle(dC[m]);
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Gv[ks], f[ks]);
+                for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Gv[m][ks], f[ks]);
 #pragma unroll
                 for (int jt = 0; jt < QT; ++jt) {
+                    sel_phase();
                     const int j = 16 * jt + l;
                     sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
@@ -342,10 +377,10 @@ __global__ __launch_bounds__(NHIP_WG) void grad_kernel(nhip_scan_args a, GradPla
     const long long row = (long long)a.n_groups * a.states;
 #pragma unroll
     for (int m = 0; m < kMyNT; ++m) {
-        const int c = 16 * (wave + 4 * m) + 4 * g;
+        const int c = 16 * (wave + 4 * m) + 4 * lane_g;
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
-            const int i = 16 * t + l;
+            const int i = 16 * t + lane_l;
             if (i >= n || c >= a.states) continue;
             const long long at = (seq.row0 + t0 + i) * row + (long long)group * a.states;
             if (plan.blocks == 1) {
