@@ -61,29 +61,33 @@ __global__ __launch_bounds__(NHIP_WG) void conv_kernel(nhip_conv_args a) {
     load_taps<V, K>(a, c0, w, b);
     const int t1 = min(t0 + kStrip, s.n);
     if (t0 < t1) {
+        // All tokens of the strip are under way before the first is used.  (The loads are unconditional, the last
+        // token again where the strip ends early: one under a condition is waited for where its branch ends.)
+        SelPack<T, V> in[kStrip];
+        const T* const from = sel_row<T>(a.x, a.tokens, s, t0) + c0;
+#pragma unroll
+        for (int k = 0; k < kStrip; ++k)
+            in[k] = *reinterpret_cast<const SelPack<T, V>*>(from + min(k, t1 - 1 - t0) * a.x.token);
         float x[K][V];  // the window: x[k] is token t - K + 1 + k
 #pragma unroll
         for (int k = 0; k < K - 1; ++k) load_token<T, V, K>(a, s, t0 - K + 1 + k, c0, x[k]);
-        T* out = static_cast<T*>(a.y) + (s.row0 + t0) * a.channels + c0;
-        const T* in = sel_row<T>(a.x, a.tokens, s, t0) + c0;
-#pragma unroll 8
-        for (int t = t0; t < t1; ++t) {
-            sel_load<T, V>(in, x[K - 1]);
+        T* const out = static_cast<T*>(a.y) + (s.row0 + t0) * a.channels + c0;
+#pragma unroll
+        for (int q = 0; q < kStrip; ++q) {
             float u[V];
 #pragma unroll
             for (int i = 0; i < V; ++i) {
+                x[K - 1][i] = (float)in[q].v[i];
                 u[i] = b[i];
 #pragma unroll
                 for (int k = 0; k < K; ++k) u[i] = fmaf(w[k][i], x[k][i], u[i]);
                 if (a.silu) u[i] *= sel_sigmoid(u[i]);
             }
-            sel_store<T, V>(out, u);
+            if (q < t1 - t0) sel_store<T, V>(out + (long long)q * a.channels, u);
 #pragma unroll
             for (int k = 0; k < K - 1; ++k)
 #pragma unroll
                 for (int i = 0; i < V; ++i) x[k][i] = x[k + 1][i];
-            in += a.x.token;
-            out += a.channels;
         }
     }
     // the last chunk's first wave hands on the end of the sequence

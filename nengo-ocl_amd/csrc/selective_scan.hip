@@ -7,48 +7,71 @@ namespace {
 
 // One token: S <- e^{step A} S + step x (x) B, y = S C + D x.  The state is read and written, 8 bytes
 // per element for 5 operations: memory bound.  Lanes of a wave share the rows of a head's state: LPR
-// (a power of two) to a row, V neighbouring states at a time.
-template <class T, int V>
-__global__ __launch_bounds__(NHIP_WG) void step_kernel(nhip_scan_step_args a, int lpr, int rows_per_group) {
-    const int blocks = (a.dim + rows_per_group - 1) / rows_per_group;
+// (a power of two) to a row, V neighbouring states NS times over; each takes ROWS rows, whose loads are all
+// under way before the first is used, and B and C stay in registers for all of them.
+template <class T, int V, int NS, int ROWS>
+__global__ __launch_bounds__(NHIP_WG) void step_kernel(nhip_scan_step_args a, int lpr) {
+    const int side_by_side = NHIP_WG / lpr, per_group = side_by_side * ROWS;
+    const int blocks = (a.dim + per_group - 1) / per_group;
     const int block = blockIdx.x % blocks;
     const int head = (blockIdx.x / blocks) % a.n_heads;
     const int r = blockIdx.x / (blocks * a.n_heads);
     const int slot = a.slots ? a.slots[r] : r;
     const int group = head / (a.n_heads / a.n_groups);
-    const int c = threadIdx.x % lpr, side_by_side = NHIP_WG / lpr;
-    const bool live = slot >= 0 && slot < a.n_slots;
+    const int c = threadIdx.x % lpr, p0 = block * per_group + threadIdx.x / lpr;
     T* const y = static_cast<T*>(a.y) + ((long long)r * a.n_heads + head) * a.dim;
+    if (slot < 0 || slot >= a.n_slots) {
+        for (int q = 0; q < ROWS; ++q) {
+            const int p = p0 + q * side_by_side;
+            if (c == 0 && p < a.dim) y[p] = (T)0.0f;
+        }
+        return;
+    }
+    float* const state = a.state + slot * a.state_stride + (long long)head * a.dim * a.states;
+    float v[ROWS][NS][V];
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) {
+        const float* row = state + (unsigned)min(p0 + q * side_by_side, a.dim - 1) * (unsigned)a.states;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) sel_load<float, V>(row + min((c + s * lpr) * V, a.states - V), v[q][s]);
+    }
     const T* const x = static_cast<const T*>(a.x.p) + r * a.x.token + head * a.x.head;
     const T* const B = static_cast<const T*>(a.B.p) + r * a.B.token + group * a.B.head;
     const T* const C = static_cast<const T*>(a.C.p) + r * a.C.token + group * a.C.head;
+    float b[NS][V], k[NS][V], in[ROWS];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int n = (c + s * lpr) * V + i;
+            b[s][i] = (float)B[min(n, a.states - 1)];
+            k[s][i] = n < a.states ? (float)C[min(n, a.states - 1)] : 0.0f;
+        }
+#pragma unroll
+    for (int q = 0; q < ROWS; ++q) in[q] = (float)x[min(p0 + q * side_by_side, a.dim - 1)];
     const float raw = sel_element(a.dt.p, a.dt_type, r * a.dt.token + head * a.dt.head) +
                       (a.dt_bias ? a.dt_bias[head] : 0.0f);
     const float step = a.softplus ? sel_softplus(raw) : raw;
-    const float decay = expf(step * a.A[head]);
+    const float decay = sel_exp(step * a.A[head]);
     const float D = a.D ? a.D[head] : 0.0f;
-    const int p1 = min(a.dim, (block + 1) * rows_per_group);
-    for (int p0 = block * rows_per_group; p0 < p1; p0 += side_by_side) {
-        const int p = p0 + threadIdx.x / lpr;
-        float sum = 0.0f;
-        if (p < p1 && live) {
-            const float in = step * (float)x[p];
-            float* const row = a.state + slot * a.state_stride + ((long long)head * a.dim + p) * a.states;
-            for (int n = c * V; n < a.states; n += lpr * V) {
-                float v[V], b[V], k[V];
-                sel_load<float, V>(row + n, v);
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    b[i] = (float)B[n + i];
-                    k[i] = (float)C[n + i];
-                    v[i] = fmaf(decay, v[i], in * b[i]);
-                    sum = fmaf(v[i], k[i], sum);
-                }
-                sel_store<float, V>(row + n, v);
+    for (int q = 0; q < ROWS; ++q) {
+        const int p = p0 + q * side_by_side;
+        const float gain = step * in[q];
+        float* const row = state + (unsigned)p * (unsigned)a.states;
+        float sum = 0.0f;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            const int n = (c + s * lpr) * V;
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                v[q][s][i] = fmaf(decay, v[q][s][i], gain * b[s][i]);
+                sum = fmaf(n < a.states ? v[q][s][i] : 0.0f, k[s][i], sum);
             }
+            if (p < a.dim && n < a.states) sel_store<float, V>(row + n, v[q][s]);
         }
         for (int d = lpr / 2; d > 0; d /= 2) sum += __shfl_xor(sum, d);
-        if (c == 0 && p < p1) y[p] = (T)(live ? fmaf(D, (float)x[p], sum) : 0.0f);
+        if (c == 0 && p < a.dim) y[p] = (T)fmaf(D, in[q], sum);
     }
 }
 
@@ -85,17 +108,21 @@ extern "C" int nhip_selective_step(void* stream, const nhip_scan_step_args* args
     const int v = vec ? 4 : 1;
     int lpr = 1;
     while (lpr < NHIP_WAVE && lpr * v < a.states) lpr *= 2;
+    // Eight rows to a lane where that leaves four work-groups to every compute unit, otherwise one.
     const int side_by_side = NHIP_WG / lpr;
-    const int rows = side_by_side * 2;
+    const bool many = (long long)a.n * a.n_heads * ((a.dim + 8 * side_by_side - 1) / (8 * side_by_side)) >= 1024;
+    const int rows = side_by_side * (many ? 8 : 1);
     const long long groups = (long long)a.n * a.n_heads * ((a.dim + rows - 1) / rows);
-    if (groups > 0x7fffffffLL) return NHIP_E_BADARG;
+    if (groups > 0x7fffffffLL || (long long)a.dim * a.states > 0x7fffffffLL) return NHIP_E_BADARG;
     int rc = NHIP_E_BADARG;
     sel_with_type(a.type, [&](auto t) {
         using T = decltype(t);
-        if (vec)
-            NHIP_LAUNCH((step_kernel<T, 4>), dim3((unsigned)groups), dim3(NHIP_WG), 0, static_cast<hipStream_t>(stream), a, lpr, rows);
-        else
-            NHIP_LAUNCH((step_kernel<T, 1>), dim3((unsigned)groups), dim3(NHIP_WG), 0, static_cast<hipStream_t>(stream), a, lpr, rows);
+        const dim3 g((unsigned)groups);
+        hipStream_t st = static_cast<hipStream_t>(stream);
+        if (vec && many) NHIP_LAUNCH((step_kernel<T, 4, 1, 8>), g, dim3(NHIP_WG), 0, st, a, lpr);
+        else if (vec) NHIP_LAUNCH((step_kernel<T, 4, 1, 1>), g, dim3(NHIP_WG), 0, st, a, lpr);
+        else if (many) NHIP_LAUNCH((step_kernel<T, 1, 4, 8>), g, dim3(NHIP_WG), 0, st, a, lpr);
+        else NHIP_LAUNCH((step_kernel<T, 1, 4, 1>), g, dim3(NHIP_WG), 0, st, a, lpr);
         rc = (int)hipGetLastError();
     });
     return rc;

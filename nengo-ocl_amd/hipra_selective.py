@@ -115,14 +115,14 @@ def _array(queue, name, t, shape, dtype, contiguous=False):
         t = t.tensor
     if dtype is not None and t.dtype != dtype:
         raise TypeError("%s is %s, not %s" % (name, t.dtype, dtype))
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError("%s has shape %s, not %s" % (name, tuple(t.shape), tuple(shape)))
     if t.device != queue.device:
         raise ValueError("%s is on %s, the queue on %s" % (name, t.device, queue.device))
     if contiguous:
         if not t.is_contiguous():
             raise ValueError("%s has to be contiguous" % name)
-    elif t.dim() and t.stride(-1) != 1 and t.shape[-1] > 1:
+    elif shape and shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError("%s has stride %d along its last axis, not 1" % (name, t.stride(-1)))
     return t
 
@@ -139,7 +139,7 @@ def _output(queue, name, t, shape, dtype):
 
 
 def _ptr(t):
-    return None if t is None else t.data_ptr() or None
+    return None if t is None else t.data_ptr()
 
 
 def _plain(t):
@@ -170,11 +170,11 @@ def _tokens(queue, x, starts, axes):
 
 
 def _rows(t, lead, heads=False):
-    """How the rows of `t` lie: [S, L, (heads,) ...] or [T, (heads,) ...]."""
+    """How the rows of `t` lie, as a `_Rows`: [S, L, (heads,) ...] or [T, (heads,) ...]."""
     st = t.stride()
     if lead == 2:
-        return _Rows(_ptr(t), st[0], st[1], st[2] if heads else 0)
-    return _Rows(_ptr(t), 0, st[0], st[1] if heads else 0)
+        return t.data_ptr(), st[0], st[1], st[2] if heads else 0
+    return t.data_ptr(), 0, st[0], st[1] if heads else 0
 
 
 def _activation(name):
@@ -201,23 +201,31 @@ def _workspace(queue, args, entry):
     return space
 
 
-def _plan(queue, entry, args, keep, name, tag, **results):
-    plan = Plan(queue, entry, (ctypes.byref(args),), gsize=(64,), full_args=(args,) + tuple(keep), name=name, tag=tag)
-    for key, value in results.items():
-        setattr(plan, key, value)
-    return plan
+class _Call:
+    """An entry point with its arguments, what they point into, and the arrays that it writes by name."""
 
+    __slots__ = ("entry", "args", "keep", "name", "results")
 
-def _enqueue(queue, plan):
-    """Enqueue once, in order with torch's current stream: the plan's arrays were made there, and are used there next."""
-    current = _torch().cuda.current_stream(queue.device)
-    if current.cuda_stream == queue.stream.cuda_stream:
-        plan.enqueue()
+    def __init__(self, entry, args, keep, name, **results):
+        self.entry, self.args, self.keep, self.name, self.results = entry, args, keep, name, results
+
+    def plan(self, queue, tag):
+        plan = Plan(queue, self.entry, (ctypes.byref(self.args),), gsize=(64,), full_args=(self,), name=self.name,
+                    tag=tag)
+        for key, value in self.results.items():
+            setattr(plan, key, value)
         return plan
-    queue.stream.wait_stream(current)
-    plan.enqueue()
-    current.wait_stream(queue.stream)
-    return plan
+
+    def now(self, queue):
+        """Enqueued once, in order with torch's current stream: the arrays were made there, and are used there next."""
+        current = _torch().cuda.current_stream(queue.device)
+        if current.cuda_stream == queue.stream.cuda_stream:
+            _lib.check(self.entry(queue.handle, ctypes.byref(self.args)), self.name)
+        else:
+            queue.stream.wait_stream(current)
+            _lib.check(self.entry(queue.handle, ctypes.byref(self.args)), self.name)
+            current.wait_stream(queue.stream)
+        return self.results
 
 
 # ----------------------------------------------------------------- short causal convolution
@@ -240,28 +248,31 @@ def _conv(queue, x, weight, bias, activation, initial, starts):
     return args, x, lead, (s, k - 1, d), [x, weight, bias, initial, starts]
 
 
+def _causal_conv(queue, x, weight, bias=None, activation=None, initial=None, starts=None, y=None, final=None):
+    args, x, lead, ends, keep = _conv(queue, x, weight, bias, activation, initial, starts)
+    y = _output(queue, "y", y, x.shape, x.dtype)
+    final = _output(queue, "final", final, ends, x.dtype)
+    args.y, args.final = _ptr(y), _ptr(final)
+    return _Call(queue.lib.nhip_causal_conv, args, keep + [y, final],
+                 "hip_causal_conv", y=y, final=final)
+
+
 def plan_causal_conv(queue, x, weight, bias=None, activation=None, initial=None, starts=None, y=None, final=None,
                      tag=None):
     """``y[t] = f(bias + sum_k weight[:, k] * x[t - width + 1 + k])``, channel by channel; f is the
     identity or (``activation="silu"``) v sigmoid(v).  In front of a sequence's first token lies
     `initial` ``[S, width - 1, channels]``, or zeros.  ``plan.y``, and ``plan.final``: the last
     width - 1 inputs of each sequence, what `causal_conv_step` goes on with."""
-    args, x, lead, ends, keep = _conv(queue, x, weight, bias, activation, initial, starts)
-    y = _output(queue, "y", y, x.shape, x.dtype)
-    final = _output(queue, "final", final, ends, x.dtype)
-    args.y, args.final = _ptr(y), _ptr(final)
-    return _plan(queue, queue.lib.nhip_causal_conv, args, keep + [y, final], "hip_causal_conv", tag, y=y, final=final)
+    return _causal_conv(queue, x, weight, bias, activation, initial, starts, y, final).plan(queue, tag)
 
 
 def causal_conv(queue, x, weight, bias=None, activation=None, initial=None, starts=None):
     """(y, final): see `plan_causal_conv`."""
-    plan = _enqueue(queue, plan_causal_conv(queue, x, weight, bias, activation, initial, starts))
-    return plan.y, plan.final
+    got = _causal_conv(queue, x, weight, bias, activation, initial, starts).now(queue)
+    return got["y"], got["final"]
 
 
-def plan_causal_conv_grad(queue, dy, x, weight, bias=None, activation=None, initial=None, starts=None, dfinal=None,
-                          tag=None):
-    """The gradient of `plan_causal_conv`, from `dy` and (where it went on) `dfinal`; ``plan.gradients``."""
+def _causal_conv_grad(queue, dy, x, weight, bias=None, activation=None, initial=None, starts=None, dfinal=None):
     torch = _torch()
     args, x, lead, ends, keep = _conv(queue, x, weight, bias, activation, initial, starts)
     dy = _array(queue, "dy", dy, x.shape, x.dtype)
@@ -275,20 +286,23 @@ def plan_causal_conv_grad(queue, dy, x, weight, bias=None, activation=None, init
     args.dx, args.dinitial, args.dweight, args.dbias = _ptr(dx), _ptr(dinitial), _ptr(dweight), _ptr(dbias)
     space = _workspace(queue, args, queue.lib.nhip_causal_conv_grad_workspace)
     got = ConvGradients(dx, dweight, None if bias is None else dbias, dinitial)
-    return _plan(queue, queue.lib.nhip_causal_conv_grad, args, keep + [dy, dfinal, dbias, space, got],
-                 "hip_causal_conv_grad", tag, gradients=got)
+    return _Call(queue.lib.nhip_causal_conv_grad, args, keep + [dy, dfinal, dbias, space, got],
+                 "hip_causal_conv_grad", gradients=got)
+
+
+def plan_causal_conv_grad(queue, dy, x, weight, bias=None, activation=None, initial=None, starts=None, dfinal=None,
+                          tag=None):
+    """The gradient of `plan_causal_conv`, from `dy` and (where it went on) `dfinal`; ``plan.gradients``."""
+    return _causal_conv_grad(queue, dy, x, weight, bias, activation, initial, starts, dfinal).plan(queue, tag)
 
 
 def causal_conv_grad(queue, dy, x, weight, bias=None, activation=None, initial=None, starts=None, dfinal=None):
     """`ConvGradients` (x, weight, bias, initial): see `plan_causal_conv_grad`."""
-    return _enqueue(queue, plan_causal_conv_grad(queue, dy, x, weight, bias, activation, initial, starts,
-                                                 dfinal)).gradients
+    got = _causal_conv_grad(queue, dy, x, weight, bias, activation, initial, starts, dfinal).now(queue)
+    return got["gradients"]
 
 
-def plan_causal_conv_step(queue, state, x, weight, bias=None, activation=None, slots=None, y=None, tag=None):
-    """One token each of n requests, `x` ``[n, channels]``: `state` ``[slots, width - 1, channels]`` holds
-    the inputs before it, oldest first, and moves on by one.  Request r has the slot ``slots[r]`` (int32;
-    each at most once), or r; one outside the state gets zeros.  ``plan.y``."""
+def _causal_conv_step(queue, state, x, weight, bias=None, activation=None, slots=None, y=None):
     state, x, weight = _plain(state), _plain(x), _plain(weight)
     code = _type_code("x", x)
     if weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_WIDTH:
@@ -309,13 +323,21 @@ def plan_causal_conv_step(queue, state, x, weight, bias=None, activation=None, s
     args = _ConvStepArgs(type=code, channels=d, width=k, silu=_activation(activation), n=n, n_slots=n_slots,
                          slots=_ptr(slots), x=_ptr(x), x_stride=x.stride(0), state_stride=state.stride(0),
                          weight=_ptr(weight), bias=_ptr(bias), state=_ptr(state), y=_ptr(y))
-    return _plan(queue, queue.lib.nhip_causal_conv_step, args, (state, x, weight, bias, slots, y),
-                 "hip_causal_conv_step", tag, y=y)
+    return _Call(queue.lib.nhip_causal_conv_step, args, (state, x, weight, bias, slots, y),
+                 "hip_causal_conv_step", y=y)
+
+
+def plan_causal_conv_step(queue, state, x, weight, bias=None, activation=None, slots=None, y=None, tag=None):
+    """One token each of n requests, `x` ``[n, channels]``: `state` ``[slots, width - 1, channels]`` holds
+    the inputs before it, oldest first, and moves on by one.  Request r has the slot ``slots[r]`` (int32;
+    each at most once), or r; one outside the state gets zeros.  ``plan.y``."""
+    return _causal_conv_step(queue, state, x, weight, bias, activation, slots, y).plan(queue, tag)
 
 
 def causal_conv_step(queue, state, x, weight, bias=None, activation=None, slots=None):
     """y: see `plan_causal_conv_step`."""
-    return _enqueue(queue, plan_causal_conv_step(queue, state, x, weight, bias, activation, slots)).y
+    got = _causal_conv_step(queue, state, x, weight, bias, activation, slots).now(queue)
+    return got["y"]
 
 
 # ------------------------------------------------------------------------- selective scan
@@ -335,7 +357,7 @@ def _scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts):
     B, C = _array(queue, "B", B, lead + (g, n), x.dtype), _array(queue, "C", C, lead + (g, n), x.dtype)
     dt = _plain(dt)
     dt_code = _type_code("dt", dt)
-    if tuple(dt.shape) != lead + (h,) or dt.device != queue.device:
+    if dt.shape != lead + (h,) or dt.device != queue.device:
         raise ValueError("dt has shape %s on %s, not %s on %s" % (tuple(dt.shape), dt.device, lead + (h,), queue.device))
     if A is None:
         raise TypeError("A is None")
@@ -348,8 +370,20 @@ def _scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts):
     return args, x, dt, B, lead, (s, h, p, n), [x, dt, A, B, C, D, dt_bias, initial, starts]
 
 
-def plan_selective_scan(queue, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None, starts=None, y=None,
-                        final=None, tag=None):
+def _selective_scan(queue, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None, starts=None, y=None,
+                    final=None):
+    torch = _torch()
+    args, x, _, _, _, ends, keep = _scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts)
+    y = _output(queue, "y", y, x.shape, x.dtype)
+    final = _output(queue, "final", final, ends, torch.float32)
+    args.y, args.final = _ptr(y), _ptr(final)
+    space = _workspace(queue, args, queue.lib.nhip_selective_scan_workspace)
+    return _Call(queue.lib.nhip_selective_scan, args, keep + [y, final, space],
+                 "hip_selective_scan", y=y, final=final)
+
+
+def plan_selective_scan(queue, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None, starts=None,
+                        y=None, final=None, tag=None):
     """The scan of `x` ``[..., heads, dim]``: with ``step = f(dt + dt_bias)`` (f: identity or softplus),
 
         S[t] = exp(step A) S[t - 1] + step x[t] (outer) B[t],     y[t] = S[t] C[t] + D x[t]
@@ -357,26 +391,17 @@ def plan_selective_scan(queue, x, dt, A, B, C, D=None, dt_bias=None, softplus=Fa
     per head, S of ``dim x states`` in float32.  `dt` ``[..., heads]``; `B`, `C` ``[..., groups, states]``,
     each for heads / groups heads; `A` (rates, below zero for a filter that forgets), `D`, `dt_bias`
     ``[heads]``.  `initial` ``[S, heads, dim, states]`` enters, or zeros.  ``plan.y``, ``plan.final``."""
-    torch = _torch()
-    args, x, _, _, _, ends, keep = _scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts)
-    y = _output(queue, "y", y, x.shape, x.dtype)
-    final = _output(queue, "final", final, ends, torch.float32)
-    args.y, args.final = _ptr(y), _ptr(final)
-    space = _workspace(queue, args, queue.lib.nhip_selective_scan_workspace)
-    return _plan(queue, queue.lib.nhip_selective_scan, args, keep + [y, final, space], "hip_selective_scan", tag, y=y,
-                 final=final)
+    return _selective_scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts, y, final).plan(queue, tag)
 
 
 def selective_scan(queue, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None, starts=None):
     """(y, final): see `plan_selective_scan`."""
-    plan = _enqueue(queue, plan_selective_scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts))
-    return plan.y, plan.final
+    got = _selective_scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts).now(queue)
+    return got["y"], got["final"]
 
 
-def plan_selective_scan_grad(queue, dy, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None,
-                             starts=None, dfinal=None, tag=None):
-    """The gradient of `plan_selective_scan`, from `dy` and (where the state went on) `dfinal`; it needs
-    nothing that the forward pass computed.  ``plan.gradients``: those of A, D and dt_bias are float32."""
+def _selective_scan_grad(queue, dy, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None, starts=None,
+                         dfinal=None):
     torch = _torch()
     args, x, dt, B, lead, ends, keep = _scan(queue, x, dt, A, B, C, D, dt_bias, softplus, initial, starts)
     dy = _array(queue, "dy", dy, x.shape, x.dtype)
@@ -391,22 +416,26 @@ def plan_selective_scan_grad(queue, dy, x, dt, A, B, C, D=None, dt_bias=None, so
     args.dA, args.dD, args.ddt_bias, args.dinitial = _ptr(dA), _ptr(dD), _ptr(dbias), _ptr(dinitial)
     space = _workspace(queue, args, queue.lib.nhip_selective_scan_grad_workspace)
     got = ScanGradients(dx, ddt, dA, dB, dC, None if D is None else dD, None if dt_bias is None else dbias, dinitial)
-    return _plan(queue, queue.lib.nhip_selective_scan_grad, args, keep + [dy, dfinal, dD, dbias, space, got],
-                 "hip_selective_scan_grad", tag, gradients=got)
+    return _Call(queue.lib.nhip_selective_scan_grad, args, keep + [dy, dfinal, dD, dbias, space, got],
+                 "hip_selective_scan_grad", gradients=got)
+
+
+def plan_selective_scan_grad(queue, dy, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None,
+                             starts=None, dfinal=None, tag=None):
+    """The gradient of `plan_selective_scan`, from `dy` and (where the state went on) `dfinal`; it needs
+    nothing that the forward pass computed.  ``plan.gradients``: those of A, D and dt_bias are float32."""
+    return _selective_scan_grad(queue, dy, x, dt, A, B, C, D, dt_bias, softplus, initial, starts,
+                                dfinal).plan(queue, tag)
 
 
 def selective_scan_grad(queue, dy, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, initial=None, starts=None,
                         dfinal=None):
     """`ScanGradients` (x, dt, A, B, C, D, dt_bias, initial): see `plan_selective_scan_grad`."""
-    return _enqueue(queue, plan_selective_scan_grad(queue, dy, x, dt, A, B, C, D, dt_bias, softplus, initial, starts,
-                                                    dfinal)).gradients
+    got = _selective_scan_grad(queue, dy, x, dt, A, B, C, D, dt_bias, softplus, initial, starts, dfinal).now(queue)
+    return got["gradients"]
 
 
-def plan_selective_step(queue, state, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, slots=None, y=None,
-                        tag=None):
-    """One token each of n requests: `x` ``[n, heads, dim]``, `dt` ``[n, heads]``, `B`, `C`
-    ``[n, groups, states]``; `state` ``[slots, heads, dim, states]`` (float32) is moved on by a token.  Slots
-    as for `plan_causal_conv_step`.  ``plan.y``."""
+def _selective_step(queue, state, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, slots=None, y=None):
     torch = _torch()
     state, x, B, dt = _plain(state), _plain(x), _plain(B), _plain(dt)
     code, dt_code = _type_code("x", x), _type_code("dt", dt)
@@ -421,13 +450,13 @@ def plan_selective_step(queue, state, x, dt, A, B, C, D=None, dt_bias=None, soft
     n_slots = state.shape[0]
     x = _array(queue, "x", x, (n, h, p), None)
     B, C = _array(queue, "B", B, (n, g, k), x.dtype), _array(queue, "C", C, (n, g, k), x.dtype)
-    if tuple(dt.shape) != (n, h) or dt.device != queue.device:
+    if dt.shape != (n, h) or dt.device != queue.device:
         raise ValueError("dt has shape %s on %s, not %s on %s" % (tuple(dt.shape), dt.device, (n, h), queue.device))
     if A is None:
         raise TypeError("A is None")
     A, D, dt_bias = (_parameter(queue, name, v, (h,)) for name, v in (("A", A), ("D", D), ("dt_bias", dt_bias)))
     state = _array(queue, "state", state, (n_slots, h, p, k), torch.float32)
-    if n_slots and not state[0].is_contiguous():
+    if state.stride()[1:] != (p * k, k, 1) and n_slots and not state[0].is_contiguous():
         raise ValueError("a slot of the state has to be contiguous")
     slots = _slots(queue, slots, n, n_slots)
     y = _output(queue, "y", y, (n, h, p), x.dtype)
@@ -435,13 +464,22 @@ def plan_selective_step(queue, state, x, dt, A, B, C, D=None, dt_bias=None, soft
                          states=k, n=n, n_slots=n_slots, slots=_ptr(slots), x=_rows(x, 1, True), dt=_rows(dt, 1, True),
                          B=_rows(B, 1, True), C=_rows(C, 1, True), A=_ptr(A), D=_ptr(D), dt_bias=_ptr(dt_bias),
                          state=_ptr(state), state_stride=state.stride(0), y=_ptr(y))
-    return _plan(queue, queue.lib.nhip_selective_step, args, (state, x, dt, A, B, C, D, dt_bias, slots, y),
-                 "hip_selective_step", tag, y=y)
+    return _Call(queue.lib.nhip_selective_step, args, (state, x, dt, A, B, C, D, dt_bias, slots, y),
+                 "hip_selective_step", y=y)
+
+
+def plan_selective_step(queue, state, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, slots=None, y=None,
+                        tag=None):
+    """One token each of n requests: `x` ``[n, heads, dim]``, `dt` ``[n, heads]``, `B`, `C`
+    ``[n, groups, states]``; `state` ``[slots, heads, dim, states]`` (float32) is moved on by a token.  Slots
+    as for `plan_causal_conv_step`.  ``plan.y``."""
+    return _selective_step(queue, state, x, dt, A, B, C, D, dt_bias, softplus, slots, y).plan(queue, tag)
 
 
 def selective_step(queue, state, x, dt, A, B, C, D=None, dt_bias=None, softplus=False, slots=None):
     """y: see `plan_selective_step`."""
-    return _enqueue(queue, plan_selective_step(queue, state, x, dt, A, B, C, D, dt_bias, softplus, slots)).y
+    got = _selective_step(queue, state, x, dt, A, B, C, D, dt_bias, softplus, slots).now(queue)
+    return got["y"]
 
 
 # ----------------------------------------------------------------------------- gated norm
@@ -484,6 +522,18 @@ def _norm(queue, x, weight, gate, residual, scale, groups, eps, after):
     return args, x, residual is not None and not after, keep
 
 
+def _block_norm(queue, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False, out=None,
+                v=None):
+    args, x, before, keep = _norm(queue, x, weight, gate, residual, scale, groups, eps, after)
+    out = _output(queue, "out", out, x.shape, x.dtype)
+    if v is not None and not before:
+        raise ValueError("v is written with a residual in front of a block only")
+    v = _output(queue, "v", v, x.shape, x.dtype) if before else None
+    args.out, args.v_out = _ptr(out), _ptr(v)
+    return _Call(queue.lib.nhip_block_norm, args, keep + [out, v],
+                 "hip_block_norm", out=out, v=v)
+
+
 def plan_block_norm(queue, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False, out=None,
                     v=None, tag=None):
     """The norm of ``u = x`` or ``x * gate * sigmoid(gate)``, in front of a block or (`after`) behind it:
@@ -493,25 +543,17 @@ def plan_block_norm(queue, x, weight, gate=None, residual=None, scale=None, grou
 
     with means over each of `groups` equal parts of the last axis.  `residual` (like x) and `scale`
     (``[channels]``, ones) are optional.  ``plan.out``, and ``plan.v`` where there is a residual in front."""
-    args, x, before, keep = _norm(queue, x, weight, gate, residual, scale, groups, eps, after)
-    out = _output(queue, "out", out, x.shape, x.dtype)
-    if v is not None and not before:
-        raise ValueError("v is written with a residual in front of a block only")
-    v = _output(queue, "v", v, x.shape, x.dtype) if before else None
-    args.out, args.v_out = _ptr(out), _ptr(v)
-    return _plan(queue, queue.lib.nhip_block_norm, args, keep + [out, v], "hip_block_norm", tag, out=out, v=v)
+    return _block_norm(queue, x, weight, gate, residual, scale, groups, eps, after, out, v).plan(queue, tag)
 
 
 def block_norm(queue, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False):
     """(out, v or None): see `plan_block_norm`."""
-    plan = _enqueue(queue, plan_block_norm(queue, x, weight, gate, residual, scale, groups, eps, after))
-    return plan.out, plan.v
+    got = _block_norm(queue, x, weight, gate, residual, scale, groups, eps, after).now(queue)
+    return got["out"], got["v"]
 
 
-def plan_block_norm_grad(queue, dout, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False,
-                         dv=None, tag=None):
-    """The gradient of `plan_block_norm`, from `dout` and (with a residual in front) `dv`;
-    ``plan.gradients``: those of weight and scale are float32."""
+def _block_norm_grad(queue, dout, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False,
+                     dv=None):
     torch = _torch()
     args, x, before, keep = _norm(queue, x, weight, gate, residual, scale, groups, eps, after)
     d = args.channels
@@ -532,12 +574,19 @@ def plan_block_norm_grad(queue, dout, x, weight, gate=None, residual=None, scale
     space = _workspace(queue, args, queue.lib.nhip_block_norm_grad_workspace)
     got = NormGradients(dx, dweight, dgate, None if residual is None else dresidual if before else plain_dout,
                         None if scale is None else dscale)
-    return _plan(queue, queue.lib.nhip_block_norm_grad, args, keep + [dout, dv, dscale, space, got],
-                 "hip_block_norm_grad", tag, gradients=got)
+    return _Call(queue.lib.nhip_block_norm_grad, args, keep + [dout, dv, dscale, space, got],
+                 "hip_block_norm_grad", gradients=got)
+
+
+def plan_block_norm_grad(queue, dout, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6,
+                         after=False, dv=None, tag=None):
+    """The gradient of `plan_block_norm`, from `dout` and (with a residual in front) `dv`;
+    ``plan.gradients``: those of weight and scale are float32."""
+    return _block_norm_grad(queue, dout, x, weight, gate, residual, scale, groups, eps, after, dv).plan(queue, tag)
 
 
 def block_norm_grad(queue, dout, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False,
                     dv=None):
     """`NormGradients` (x, weight, gate, residual, scale): see `plan_block_norm_grad`."""
-    return _enqueue(queue, plan_block_norm_grad(queue, dout, x, weight, gate, residual, scale, groups, eps, after,
-                                                dv)).gradients
+    got = _block_norm_grad(queue, dout, x, weight, gate, residual, scale, groups, eps, after, dv).now(queue)
+    return got["gradients"]
