@@ -381,7 +381,7 @@ extern "C" int nhip_block_norm_grad(void* stream, const nhip_norm_args* args) {
     hipStream_t st = static_cast<hipStream_t>(stream);
     sel_with_type(a.type, [&](auto t) {
         using T = decltype(t);
-        constexpr int V16 = 16 / sizeof(T);
+        constexpr int V16 = 4;  // (8 bytes of 16-bit types: what a lane holds of eight channels leaves too few waves)
         with_shape(wide(a), V16, width, [&](auto vec, auto lanes, auto held) {
             constexpr int V = decltype(vec)::value ? V16 : 1, L = decltype(lanes)::value, R = decltype(held)::value;
             NHIP_LAUNCH_FIRST((norm_grad_kernel<T, V, L, R>), dim3((unsigned)rows, (unsigned)a.groups),

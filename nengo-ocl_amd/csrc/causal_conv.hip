@@ -39,26 +39,42 @@ __device__ __forceinline__ void load_token(const nhip_conv_args& a, const SelSeq
     }
 }
 
+// Taps and bias of this lane's channels.  The group's lie back to back, V K floats to a lane: read by neighbouring
+// threads and handed over through the LDS (a lane's own V K reads touch as many lines as the inputs of
+// its whole strip).
+template <int V, int K> struct Taps {
+    static constexpr int kRow = NHIP_WAVE + 1;
+    float at[V * K][kRow];
+};
 template <int V, int K>
-__device__ __forceinline__ void load_taps(const nhip_conv_args& a, int c0, float (&w)[K][V],
-                                          float (&b)[V]) {
+__device__ __forceinline__ void load_taps(const nhip_conv_args& a, int c0, Taps<V, K>& s, float (&w)[K][V], float (&b)[V]) {
+    const long long first = (long long)blockIdx.y * NHIP_WAVE * V * K, end = (long long)a.channels * K;
+    constexpr int kAll = NHIP_WAVE * V * K;
 #pragma unroll
-    for (int i = 0; i < V; ++i) {
-        b[i] = a.bias ? a.bias[c0 + i] : 0.0f;
-#pragma unroll
-        for (int k = 0; k < K; ++k) w[k][i] = a.weight[(long long)(c0 + i) * K + k];
+    for (int q0 = 0; q0 < kAll; q0 += NHIP_WG) {
+        const int q = q0 + threadIdx.x;
+        const float v = a.weight[min(first + q, end - 1)];
+        if (q < kAll) s.at[q % (V * K)][q / (V * K)] = v;
     }
+#pragma unroll
+    for (int i = 0; i < V; ++i) b[i] = a.bias ? a.bias[min(c0 + i, a.channels - 1)] : 0.0f;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+#pragma unroll
+        for (int k = 0; k < K; ++k) w[k][i] = s.at[i * K + k][threadIdx.x & (NHIP_WAVE - 1)];
 }
 
 template <class T, int V, int K>
 __global__ __launch_bounds__(NHIP_WG) void conv_kernel(nhip_conv_args a) {
     const SelSeq s = sel_seq_of_chunk(a.tokens, blockIdx.x, kChunk);
     if (s.seq < 0) return;
+    __shared__ Taps<V, K> taps;
     const int c0 = first_channel<T, V>();
-    if (c0 >= a.channels) return;
     const int t0 = s.chunk * kChunk + (threadIdx.x / NHIP_WAVE) * kStrip;
     float w[K][V], b[V];
-    load_taps<V, K>(a, c0, w, b);
+    load_taps<V, K>(a, c0, taps, w, b);
+    if (c0 >= a.channels) return;
     const int t1 = min(t0 + kStrip, s.n);
     if (t0 < t1) {
         // All tokens of the strip are under way before the first is used.  (The loads are unconditional, the last
@@ -107,13 +123,17 @@ __global__ __launch_bounds__(NHIP_WG) void conv_kernel(nhip_conv_args a) {
 // launch in the order of the chunks: the same result on every call.
 template <class T, int V, int K>
 __global__ __launch_bounds__(NHIP_WG) void conv_grad_kernel(nhip_conv_args a, float* parts) {
-    __shared__ float sums[4][NHIP_WAVE * V];
+    __shared__ union {
+        Taps<V, K> taps;
+        float sums[4][NHIP_WAVE * V];
+    } lds;
     const int chunk = blockIdx.x;
     const SelSeq s = sel_seq_of_chunk(a.tokens, chunk, kChunk);
     const int c0 = first_channel<T, V>();
     const bool here = s.seq >= 0 && c0 < a.channels;
-    const int wave = threadIdx.x / NHIP_WAVE, lane = threadIdx.x & (NHIP_WAVE - 1);
-    float dw[K + 1][V];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NHIP_WAVE), lane = threadIdx.x & (NHIP_WAVE - 1);
+    float w[K][V], b[V], dw[K + 1][V];
+    load_taps<V, K>(a, c0, lds.taps, w, b);
 #pragma unroll
     for (int k = 0; k <= K; ++k)
 #pragma unroll
@@ -124,82 +144,99 @@ __global__ __launch_bounds__(NHIP_WG) void conv_grad_kernel(nhip_conv_args a, fl
         // the sequence's first strip also forms what goes to `initial`: rows of t < 0
         const int from = s.chunk == 0 && wave == 0 && a.dinitial ? 1 - K : t0;
         if (from < t1 || from < 0) {
-            float w[K][V], b[V], x[K][V], g[K][V];  // x[k], g[k]: token t - K + 1 + k
-            load_taps<V, K>(a, c0, w, b);
+            float x[K][V], g[K][V];  // x[k], g[k]: token t - K + 1 + k
 #pragma unroll
             for (int k = 0; k < K; ++k) {
                 if (k < K - 1) load_token<T, V, K>(a, s, t0 - K + 1 + k, c0, x[k]);
 #pragma unroll
                 for (int i = 0; i < V; ++i) g[k][i] = 0.0f;
             }
-#pragma unroll 4
-            for (int t = t0; t < max(t1, t0) + K - 1; ++t) {
-                load_token<T, V, K>(a, s, t, c0, x[K - 1]);
-                const bool in = t < s.n;
-                if (in) sel_load<T, V>(sel_row<T>(a.dy, a.tokens, s, t) + c0, g[K - 1]);
+            constexpr int kAhead = 4;  // tokens under way at once, from places cut to those that exist
+            const T* const x_at = s.n ? sel_row<T>(a.x, a.tokens, s, 0) + c0 : nullptr;
+            const T* const dy_at = s.n ? sel_row<T>(a.dy, a.tokens, s, 0) + c0 : nullptr;
+            const int t_end = max(t1, t0) + K - 1;
+            for (int t_first = t0; t_first < t_end; t_first += kAhead) {
+                SelPack<T, V> xs[kAhead], dys[kAhead];
+                if (s.n)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float u = b[i];
-#pragma unroll
-                    for (int k = 0; k < K; ++k) u = fmaf(w[k][i], x[k][i], u);
-                    float d = in ? g[K - 1][i] : 0.0f;
-                    if (a.silu && in) {
-                        const float sg = sel_sigmoid(u);
-                        d *= sg * fmaf(u, 1.0f - sg, 1.0f);
+                    for (int q = 0; q < kAhead; ++q) {
+                        const long long at = min(t_first + q, s.n - 1);
+                        xs[q] = *reinterpret_cast<const SelPack<T, V>*>(x_at + at * a.x.token);
+                        dys[q] = *reinterpret_cast<const SelPack<T, V>*>(dy_at + at * a.dy.token);
                     }
-                    g[K - 1][i] = d;
+#pragma unroll
+                for (int q = 0; q < kAhead; ++q) {
+                    const int t = t_first + q;
+                    const bool in = t < s.n;
+#pragma unroll
+                    for (int i = 0; i < V; ++i) {
+                        x[K - 1][i] = in ? (float)xs[q].v[i] : 0.0f;
+                        float d = (float)dys[q].v[i];
+                        if (a.silu) {
+                            float u = b[i];
+#pragma unroll
+                            for (int k = 0; k < K; ++k) u = fmaf(w[k][i], x[k][i], u);
+                            const float sg = sel_sigmoid(u);
+                            d *= sg * fmaf(u, 1.0f - sg, 1.0f);
+                        }
+                        g[K - 1][i] = in ? d : 0.0f;
+                    }
                     if (t < t1) {
 #pragma unroll
-                        for (int k = 0; k < K; ++k) dw[k][i] = fmaf(d, x[k][i], dw[k][i]);
-                        dw[K][i] += d;
+                        for (int i = 0; i < V; ++i) {
+#pragma unroll
+                            for (int k = 0; k < K; ++k) dw[k][i] = fmaf(g[K - 1][i], x[k][i], dw[k][i]);
+                            dw[K][i] += g[K - 1][i];
+                        }
                     }
+                    const int td = t - (K - 1);  // the token whose gradient is complete
+                    if (td >= from && t < t_end) {
+                        float dx[V];
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            dx[i] = 0.0f;
+#pragma unroll
+                            for (int k = 0; k < K; ++k) dx[i] = fmaf(w[k][i], g[K - 1 - k][i], dx[i]);
+                        }
+                        const int j = td + (K - 1) - s.n;  // its place among the last K - 1 inputs
+                        if (a.dfinal && j >= 0) {
+                            float more[V];
+                            sel_load<T, V>(static_cast<const T*>(a.dfinal) +
+                                               ((long long)s.seq * (K - 1) + j) * a.channels + c0, more);
+#pragma unroll
+                            for (int i = 0; i < V; ++i) dx[i] += more[i];
+                        }
+                        T* out = td >= 0 ? static_cast<T*>(a.dx) + (s.row0 + td) * a.channels + c0
+                                         : static_cast<T*>(a.dinitial) +
+                                               ((long long)s.seq * (K - 1) + (K - 1 + td)) * a.channels + c0;
+                        sel_store<T, V>(out, dx);
+                    }
+#pragma unroll
+                    for (int k = 0; k < K - 1; ++k)
+#pragma unroll
+                        for (int i = 0; i < V; ++i) {
+                            x[k][i] = x[k + 1][i];
+                            g[k][i] = g[k + 1][i];
+                        }
                 }
-                const int td = t - (K - 1);  // the token whose gradient is complete
-                if (td >= from) {
-                    float dx[V];
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        dx[i] = 0.0f;
-#pragma unroll
-                        for (int k = 0; k < K; ++k) dx[i] = fmaf(w[k][i], g[K - 1 - k][i], dx[i]);
-                    }
-                    const int j = td + (K - 1) - s.n;  // its place among the last K - 1 inputs
-                    if (a.dfinal && j >= 0) {
-                        float more[V];
-                        sel_load<T, V>(static_cast<const T*>(a.dfinal) +
-                                           ((long long)s.seq * (K - 1) + j) * a.channels + c0, more);
-#pragma unroll
-                        for (int i = 0; i < V; ++i) dx[i] += more[i];
-                    }
-                    T* out = td >= 0 ? static_cast<T*>(a.dx) + (s.row0 + td) * a.channels + c0
-                                     : static_cast<T*>(a.dinitial) +
-                                           ((long long)s.seq * (K - 1) + (K - 1 + td)) * a.channels + c0;
-                    sel_store<T, V>(out, dx);
-                }
-#pragma unroll
-                for (int k = 0; k < K - 1; ++k)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) {
-                        x[k][i] = x[k + 1][i];
-                        g[k][i] = g[k + 1][i];
-                    }
             }
         }
     }
+    __syncthreads();  // (the taps have been read)
     for (int k = 0; k <= K; ++k) {
 #pragma unroll
         for (int i = 0; i < V; ++i) {
             float v = dw[0][i];
 #pragma unroll
             for (int q = 1; q <= K; ++q) v = k == q ? dw[q][i] : v;
-            sums[wave][lane * V + i] = v;
+            lds.sums[wave][lane * V + i] = v;
         }
         __syncthreads();
         for (int c = threadIdx.x; c < NHIP_WAVE * V; c += NHIP_WG) {
             const int d = blockIdx.y * NHIP_WAVE * V + c;
             if (d < a.channels)
                 parts[((long long)chunk * (K + 1) + k) * a.channels + d] =
-                    (sums[0][c] + sums[1][c]) + (sums[2][c] + sums[3][c]);
+                    (lds.sums[0][c] + lds.sums[1][c]) + (lds.sums[2][c] + lds.sums[3][c]);
         }
         __syncthreads();
     }
@@ -323,7 +360,8 @@ extern "C" int nhip_causal_conv_grad(void* stream, const nhip_conv_args* args) {
     sel_with_type(a.type, [&](auto t) {
         using T = decltype(t);
         with_width(a.width, [&](auto k) {
-            constexpr int K = decltype(k)::value, V = 16 / sizeof(T);
+            // (four channels of 16 bits too: the window, its gradient and the sums of eight take all registers)
+            constexpr int K = decltype(k)::value, V = 4;
             dim3 g;
             if (wide(a.type, a.channels, {a.x.p, a.dy.p, a.initial, a.dfinal, a.dx, a.dinitial},
                      {a.x.seq, a.x.token, a.dy.seq, a.dy.token})) {
