@@ -132,9 +132,10 @@ template <class Tc> __device__ __forceinline__ SelFrag<Tc> sel_take_unfinite(Sel
     return ones;
 }
 
-// Row length in LDS of `n` elements (a multiple of 32).  Reads of rows (sel_rows) meet no bank twice with
-// 16 bytes more than the elements, reads across 16-bit rows (sel_cols) with 32.
-template <class Tc> __host__ __device__ constexpr int sel_stride(int n) { return n + 16 / (int)sizeof(Tc); }
+// Row length in LDS of `n` elements (a multiple of 32).  Reads of rows (sel_rows) go by 16 lanes of 8 bytes,
+// or 8 of 16, over 32 banks: they meet no bank twice with 8 bytes (16) more than the elements.  Reads across
+// 16-bit rows (sel_cols) take four rows of 32 bytes at once: 32 bytes more.
+template <class Tc> __host__ __device__ constexpr int sel_stride(int n) { return n + 4; }
 template <class Tc> __host__ __device__ constexpr int sel_stride_cols(int n) {
     return n + (sizeof(Tc) == 2 ? 16 : 4);
 }
@@ -161,13 +162,19 @@ template <class T, class Tc, int ROWS, int COLS, bool VEC> struct SelStage {
     __device__ __forceinline__ void load(const T* src, long long stride, int n_rows, int n_cols) {
         const int tid = thread(), row = tid / kRow, col = (tid % kRow) * V;
         if constexpr (VEC) {
-            const unsigned st = (unsigned)stride, last = (unsigned)(n_rows - 1) * st;
-            const unsigned r0 = row * st, c = (unsigned)min(col, n_cols - V);
+            const unsigned st = (unsigned)stride * (unsigned)sizeof(T), last = (unsigned)(n_rows - 1) * st;
+            const unsigned r0 = row * st, c = (unsigned)min(col, n_cols - V) * (unsigned)sizeof(T);
+            unsigned at[kPacks];
+            if (n_rows == ROWS) {
 #pragma unroll
-            for (int q = 0; q < kPacks; ++q) {
-                const unsigned at = min(r0 + (unsigned)(q * kRowStep) * st, last) + c;
-                held[q] = *reinterpret_cast<const SelPack<T, V>*>(reinterpret_cast<const char*>(src) + at * (unsigned)sizeof(T));
+                for (int q = 0; q < kPacks; ++q) at[q] = r0 + c + (unsigned)(q * kRowStep) * st;
+            } else {
+#pragma unroll
+                for (int q = 0; q < kPacks; ++q) at[q] = min(r0 + (unsigned)(q * kRowStep) * st, last) + c;
             }
+#pragma unroll
+            for (int q = 0; q < kPacks; ++q)
+                held[q] = *reinterpret_cast<const SelPack<T, V>*>(reinterpret_cast<const char*>(src) + at[q]);
         } else {
 #pragma unroll
             for (int q = 0; q < kPacks; ++q) {
@@ -187,8 +194,12 @@ template <class T, class Tc, int ROWS, int COLS, bool VEC> struct SelStage {
             SelPack<Tc, V> v;
 #pragma unroll
             for (int i = 0; i < V; ++i) v.v[i] = WHOLE || (VEC ? 0 : i) < there ? (Tc)held[q].v[i] : (Tc)0.0f;
-            if constexpr (sizeof(Tc) * V == 16) {
+            if constexpr (sizeof(Tc) * V == 16 && STRIDE * sizeof(Tc) % 16 == 0) {
                 *reinterpret_cast<SelPack<Tc, V>*>(out) = v;
+            } else if constexpr (sizeof(Tc) == 2) {
+#pragma unroll
+                for (int i = 0; i < V; i += 4)
+                    *reinterpret_cast<SelPack<Tc, 4>*>(out + i) = SelPack<Tc, 4>{{v.v[i], v.v[i + 1], v.v[i + 2], v.v[i + 3]}};
             } else {
 #pragma unroll
                 for (int i = 0; i < V; i += 4)
@@ -208,12 +219,12 @@ template <class T, class Tc, int ROWS, int COLS, bool VEC> struct SelStage {
 // units of log 2: what decays from token j to token i is 2^(c_i - c_j).  c is summed in 64 bits
 // and kept as a whole part, whose differences are exact, and a rest of at most 1/2: a large step
 // (c of thousands) costs the tokens behind it nothing, and no argument of an exponential is
-// rounded to less than 2^-24.
+// rounded to less than 2^-24.  The exponentials of all pairs of tokens are products of two of them.
 template <int Q> struct SelSteps {
     alignas(16) float step[Q];
     alignas(16) int whole[Q];
-    alignas(16) float rest[Q];
-    alignas(16) float raw[Q];
+    alignas(16) float to[Q];          // 2^rest_t, and 2^-rest_t step_t: e^{c_i - c_j} step_j is
+    alignas(16) float from_step[Q];   //   to_i from_step_j 2^(whole_i - whole_j)
     alignas(16) float from_start[Q];  // 2^c_t
     alignas(16) float to_end[Q];      // 2^(c_Q - c_t)
     alignas(16) float to_end_step[Q];
@@ -259,9 +270,9 @@ __device__ __forceinline__ float sel_dt(const nhip_scan_args& a, const SelSeq& s
 }
 
 // One wave; lane t: token t of the chunk, n of which there are, with dt as read.  Beyond them step is
-// zero and c goes on as it is.
+// zero and c goes on as it is.  Returns dt + bias.
 template <int Q>
-__device__ __forceinline__ void sel_steps(SelSteps<Q>& s, float dt, int n, float A, float bias, bool softplus) {
+__device__ __forceinline__ float sel_steps(SelSteps<Q>& s, float dt, int n, float A, float bias, bool softplus) {
     int lane = threadIdx.x & (NHIP_WAVE - 1);
     asm volatile("" : "+v"(lane));
     float step = 0.0f, raw = 0.0f;
@@ -281,12 +292,13 @@ __device__ __forceinline__ void sel_steps(SelSteps<Q>& s, float dt, int n, float
     const float rest_end = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(rest), Q - 1));
     if (lane < Q) {
         s.step[lane] = step;
-        s.raw[lane] = raw;
         s.whole[lane] = w;
-        s.rest[lane] = rest;
+        s.to[lane] = __builtin_amdgcn_exp2f(rest);
+        s.from_step[lane] = __builtin_amdgcn_exp2f(-rest) * step;
         s.from_start[lane] = sel_exp2(w, rest);
         const float to_end = sel_exp2(w_end - w, rest_end - rest);
         s.to_end[lane] = to_end;
         s.to_end_step[lane] = to_end * step;
     }
+    return raw;
 }

@@ -255,7 +255,6 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
             for (int m = 0; m < kMine; ++m) acc[m] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
-                sel_phase();
                 const SelFrag<Tc> c = sel_rows(s.C + (16 * row_a + l) * SC + 32 * ks, g);
 #pragma unroll
                 for (int m = 0; m < kMine; ++m)
@@ -270,12 +269,11 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
                 for (int m = 0; m < kMine; ++m) {
                     const int i = 16 * (m < 2 ? row_a : row_b) + l, j0 = 16 * col_of(m) + 4 * g;
                     const int whole = st.whole[i];
-                    const float rest = st.rest[i];
+                    const float to = st.to[i];
                     float v[4];
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
-                        const float decay = sel_exp2(whole - st.whole[j0 + r], rest - st.rest[j0 + r]);
-                        const float w = acc[m][r] * (decay * st.step[j0 + r]);
+                        const float w = __builtin_ldexpf(acc[m][r] * (to * st.from_step[j0 + r]), whole - st.whole[j0 + r]);
                         v[r] = j0 + r <= i ? w : 0.0f;
                     }
                     sel_store<Tc, 4>(s.weights[u] + i * SW + j0, v);
@@ -290,7 +288,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
                 for (int it = 0; it < QT; ++it) out[h][it] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
-                sel_phase();
+                if (ks % 2 == 0) sel_phase();
                 SelFrag<Tc> sf[2];  // the state that enters, over the states
 #pragma unroll
                 for (int h = 0; h < 2; ++h)
@@ -348,17 +346,29 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
             T* const y = static_cast<T*>(a.y) + ((seq.row0 + t0) * a.n_heads + head) * a.dim + p_tile;
             const unsigned row = (unsigned)(a.n_heads * a.dim);
 #pragma unroll
-            for (int it = 0; it < QT; ++it) {
-                const int i = 16 * it + l;
+            for (int it = 0; it < QT; ++it)
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
-                    const int c = p_wave + 16 * h + 4 * g;
                     float own[4];
-                    sel_load<Tc, 4>(xs + i * SX + c, own);
+                    sel_load<Tc, 4>(xs + (16 * it + l) * SX + p_wave + 16 * h + 4 * g, own);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) out[h][it][r] = fmaf(D, own[r], out[h][it][r]);
-                    if (i < n && writes) sel_store4<VEC>(y + (unsigned)i * row, c, cols, out[h][it]);
                 }
+            const unsigned at = l * row + 4 * g;
+            if (VEC && writes && n == Q && cols == 64) {
+                T* const to = y + p_wave;
+#pragma unroll
+                for (int it = 0; it < QT; ++it)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        sel_store<T, 4>(to + 16 * (it * row + h) + at, {out[h][it][0], out[h][it][1], out[h][it][2], out[h][it][3]});
+            } else if (writes) {
+#pragma unroll
+                for (int it = 0; it < QT; ++it)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        if (16 * it + l < n)
+                            sel_store4<VEC>(y + (unsigned)(16 * it + l) * row, p_wave + 16 * h + 4 * g, cols, out[h][it]);
             }
         }
         if (WALK == kSelStates) {
@@ -412,7 +422,6 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
             constexpr int kSide = 2;  // tiles side by side
 #pragma unroll
             for (int t0 = 0; t0 < NT; t0 += kSide) {
-                if (t0 % 4 == 0) sel_phase();
                 SelFrag<Tc> bf[kSide];
 #pragma unroll
                 for (int t = 0; t < kSide; ++t) bf[t] = sel_cols(s.B + 32 * ks * SB + 16 * (t0 + t), SB, l, g);
@@ -506,9 +515,10 @@ static inline int sel_scan_check(const nhip_scan_args* a) {
 
 static inline long long sel_round4(long long floats) { return (floats + 3) & ~3LL; }
 
-// How the sequences are cut, for a workspace that begins with the ends and the keeps.  A compute unit works best on
-// two walks at once; where the sequences, heads and tiles do not give that many, sequences are cut into segments
-// of at least four chunks.
+// How the sequences are cut, for a workspace that begins with the ends and the keeps.  A compute unit holds two walks
+// of the 16-bit kernel for up to 128 states, one of the others.  Sequences that give every unit a walk stay whole (8 x
+// 2048 tokens, 32 heads of 64, 128 states, both directions: 566 us for the gradient, cut in two 600); fewer are cut into
+// as many segments as walks fit, of at least four chunks (forward, with half as many walks: 152 us, cut in two 183).
 static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions, float* states) {
     SelWalkPlan p;
     const int q = sel_chunk_tokens(a.states);
@@ -520,8 +530,12 @@ static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions,
     const long long walks = (long long)directions * a.n_groups * p.pairs;
     const long long longest = a.tokens.starts ? (a.tokens.n_tokens + q - 1) / q : sel_chunks(a.tokens.length, q);
     const long long total = a.tokens.starts ? longest : longest * a.tokens.n_seqs;
-    long long wanted = (512 + walks - 1) / walks;  // segments
-    if (!a.tokens.starts && a.tokens.n_seqs) wanted = (wanted + a.tokens.n_seqs - 1) / a.tokens.n_seqs * a.tokens.n_seqs;
+    const long long target = a.type == NHIP_BF16 && a.states <= 128 ? 512 : 256;
+    long long wanted = (target + walks - 1) / walks;  // segments
+    if (!a.tokens.starts && a.tokens.n_seqs) {
+        if (a.tokens.n_seqs * walks >= 256) wanted = a.tokens.n_seqs;
+        wanted = (wanted + a.tokens.n_seqs - 1) / a.tokens.n_seqs * a.tokens.n_seqs;
+    }
     long long chunks = (total + wanted - 1) / wanted;
     if (chunks < 4) chunks = 4;
     const bool cut = chunks < longest;

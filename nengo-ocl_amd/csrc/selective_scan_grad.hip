@@ -134,6 +134,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
 #pragma unroll
         for (int t = 0; t < QT; ++t) dB[m][t] = dC[m][t] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
 
+    float raw = 0.0f;  // dt + dt_bias of token `lane` (the first wave)
     for (int head = head0; head < head1; ++head) {
         const float D = a.D ? a.D[head] : 0.0f;
         const float* const S = plan.S + ((long long)chunk * a.n_heads + head) * head_state;
@@ -160,7 +161,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
             stage_dy.template store<SX>(s.dy, n, cols);
             if (tile == 0) {
                 if (wave == 0)
-                    sel_steps<Q>(s.steps, sel_dt<Q>(a, seq, t0, head), n, a.A[head], a.dt_bias ? a.dt_bias[head] : 0.0f,
+                    raw = sel_steps<Q>(s.steps, sel_dt<Q>(a, seq, t0, head), n, a.A[head], a.dt_bias ? a.dt_bias[head] : 0.0f,
                                  a.softplus);
                 for (int q = tid; q < QT * Q; q += NHIP_WG) s.over[q / Q][q % Q] = s.col[q / Q][q % Q] = 0.0f;
                 for (int q = tid; q < 4 * Q; q += NHIP_WG) s.q[q / Q][q % Q] = s.r[q / Q][q % Q] = 0.0f;
@@ -184,20 +185,26 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
                     sel_mma(X, sel_rows(s.dy + (16 * it + l) * SX + 32 * ks, g), sel_rows(s.x + j * SX + 32 * ks, g));
                 sel_settle(X);
                 const float step = s.steps.step[j];
+                const int whole = s.steps.whole[j];
+                const float from = 1.0f / s.steps.to[j];
                 float kl[4], xl[4], ml[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = i0 + r;
-                    const float L = sel_exp2(s.steps.whole[i] - s.steps.whole[j], s.steps.rest[i] - s.steps.rest[j]);
-                    const float all = i >= j ? K[m][r] * X[r] * L : 0.0f;
-                    kl[r] = i >= j ? K[m][r] * L * step : 0.0f;
-                    xl[r] = i >= j ? X[r] * L * step : 0.0f;
-                    if (it == jt && i == j) {
-                        s.diag[j] += all;
-                        s.dot[j] += X[r];
-                    }
-                    ml[r] = i > j ? all : 0.0f;
+                    const bool in = i >= j;
+                    const float L = __builtin_ldexpf(s.steps.to[i] * from, s.steps.whole[i] - whole);
+                    const float both = X[r] * L, xl_r = both * step, kl_r = K[m][r] * (L * step), ml_r = K[m][r] * both;
+                    xl[r] = in ? xl_r : 0.0f;
+                    kl[r] = in ? kl_r : 0.0f;
+                    ml[r] = i > j ? ml_r : 0.0f;
                 }
+                if (it == jt)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (i0 + r == j) {
+                            s.diag[j] += K[m][r] * X[r];  // (L is one there)
+                            s.dot[j] += X[r];
+                        }
                 // sums over the rows from each on: this lane's four, and those of the quarters behind
 #pragma unroll
                 for (int r = 2; r >= 0; --r) ml[r] += ml[r + 1];
@@ -362,7 +369,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
             if (live) {
                 da = (float)(across + (all - sum + behind) + before + (double)z);
                 draw = fmaf(a.A[head], da, own);
-                if (a.softplus) draw *= 1.0f / (1.0f + expf(-s.steps.raw[lane]));
+                if (a.softplus) draw *= 1.0f / (1.0f + expf(-raw));
                 sel_set_element(a.ddt, a.dt_type, (seq.row0 + t0 + lane) * a.n_heads + head, draw);
             }
             const float dA = sel_wave_sum(da * step), dD = sel_wave_sum(dot), dbias = sel_wave_sum(draw);
