@@ -255,18 +255,29 @@ __device__ __forceinline__ float sel_exp2(int whole, float rest) {
     return __builtin_ldexpf(__builtin_amdgcn_exp2f(rest), whole);
 }
 
-// What lane t of a wave reads of token t0 + t of the sequence; zero beyond its end
-template <int Q>
-__device__ __forceinline__ float sel_dt(const nhip_scan_args& a, const SelSeq& seq, int t0, int head) {
+// What lane t of a wave reads for token t0 + t of the sequence, on its way: two halves of an element of 32
+// bits, or one of 16 twice, from a place cut to those that exist.  (No load is under a condition: one
+// is waited for where its branch ends, here a chunk before it is used.)
+struct SelDt {
+    unsigned lo, hi;
+    __device__ __forceinline__ float value(int type) const {
+        const float f32 = __uint_as_float((hi << 16) | lo), bf16 = __uint_as_float(lo << 16);
+        const float f16 = (float)__builtin_bit_cast(_Float16, (unsigned short)lo);
+        return type == NHIP_F32 ? f32 : type == NHIP_BF16 ? bf16 : f16;
+    }
+};
+__device__ __forceinline__ SelDt sel_dt(const nhip_scan_args& a, const SelSeq& seq, int t0, int head) {
     int lane = threadIdx.x & (NHIP_WAVE - 1);
     asm volatile("" : "+v"(lane));  // (the address is formed anew each time: kept, it takes two registers)
-    if (lane >= Q || t0 + lane >= seq.n) return 0.0f;
-    const long long first = (a.tokens.starts ? (seq.row0 + t0) * a.dt.token : seq.seq * a.dt.seq + t0 * a.dt.token) +
-                            head * a.dt.head;
-    const long long at = first + lane * a.dt.token;
-    if (a.dt_type == NHIP_F32) return static_cast<const float*>(a.dt.p)[at];
-    const unsigned short bits = static_cast<const unsigned short*>(a.dt.p)[at];
-    return a.dt_type == NHIP_BF16 ? (float)__builtin_bit_cast(__bf16, bits) : (float)__builtin_bit_cast(_Float16, bits);
+    const int t = max(0, min(t0 + lane, seq.n - 1));
+    const long long at = head * a.dt.head + (a.tokens.starts ? (seq.row0 + t) * a.dt.token
+                                                             : seq.seq * a.dt.seq + t * a.dt.token);
+    const int size = a.dt_type == NHIP_F32 ? 4 : 2;
+    const char* p = static_cast<const char*>(a.dt.p) + at * size;
+    SelDt d;
+    d.lo = *reinterpret_cast<const unsigned short*>(p);
+    d.hi = *reinterpret_cast<const unsigned short*>(p + (size - 2));
+    return d;
 }
 
 // One wave; lane t: token t of the chunk, n of which there are, with dt as read.  Beyond them step is

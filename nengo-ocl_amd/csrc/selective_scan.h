@@ -52,15 +52,16 @@ static inline int sel_chunk_tokens(int n) { return sel_chunk_of(n > 128 ? 256 : 
 // Four neighbouring elements of a row of `cols`; VEC: rows hold whole fours, at multiples of 16 bytes (states) or
 // of their size (outputs)
 template <bool VEC>
-__device__ __forceinline__ sel_f4 sel_state_load(const float* p, int n, int states) {
-    sel_f4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+__device__ __forceinline__ sel_f4 sel_state_load(const float* p, int n, int states) {  // (no load under a condition)
+    sel_f4 v;
     if constexpr (VEC) {
-        if (n < states) v = *reinterpret_cast<const sel_f4*>(p + n);
+        v = *reinterpret_cast<const sel_f4*>(p + min(n, states - 4));
     } else {
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            if (n + r < states) v[r] = p[n + r];
+        for (int r = 0; r < 4; ++r) v[r] = p[min(n + r, states - 1)];
     }
+#pragma unroll
+    for (int r = 0; r < 4; ++r) v[r] = n + r < states ? v[r] : 0.0f;
     return v;
 }
 template <bool VEC>
@@ -146,19 +147,20 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
     float* const ends = plan.ends ? plan.ends + back * plan.n_segments * all_states : nullptr;
 
     sel_f4 state[2][NT];
+    {
+        const float* from = WALK == kSelEnds ? nullptr
+                            : plan.ends      ? ends + segment * all_states
+                            : back           ? (a.dfinal ? a.dfinal + seq.seq * all_states : nullptr)
+                                             : (a.initial ? a.initial + seq.seq * all_states : nullptr);
+        // (rows that are not there: the last one again, for which nothing is written)
+        const int p = min(p_tile + p_wave + lane_l, a.dim - 1), q = min(p_tile + p_wave + 16 + lane_l, a.dim - 1);
+        const long long at[2] = {head * head_state + (long long)p * a.states, head * head_state + (long long)q * a.states};
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int t = 0; t < NT; ++t) state[h][t] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (WALK != kSelEnds && there[h]) {
-            const float* from = plan.ends ? ends + segment * all_states
-                                : back    ? (a.dfinal ? a.dfinal + seq.seq * all_states : nullptr)
-                                          : (a.initial ? a.initial + seq.seq * all_states : nullptr);
-            if (from)
-#pragma unroll
-                for (int t = 0; t < NT; ++t)
-                    state[h][t] = sel_state_load<VEC>(from + my_state + h * next_rows, 16 * t + 4 * lane_g, a.states);
-        }
+            for (int t = 0; t < NT; ++t)
+                if (from) state[h][t] = sel_state_load<VEC>(from + at[h], 16 * t + 4 * lane_g, a.states);
+                else state[h][t] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     if constexpr (kOut)  // (above the diagonal for good)
         for (int q = threadIdx.x; q < Q * SW; q += NHIP_WG) s.weights[0][q] = s.weights[1][q] = (Tc)0.0f;
@@ -188,11 +190,12 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
         stage_B.load(B_at, B.token, n, a.states);
         if constexpr (kOut) stage_C.load(C_at, a.C.token, n, a.states);
     };
-    float dt = 0.0f, keeps = 1.0f;
+    float keeps = 1.0f;
+    SelDt dt = {0, 0};
     const int ahead = wave & 1;  // which of two chunks this wave forms the steps of
     if (n_chunks > 0) {
         fetch(min(Q, seq.n - t_first));
-        if (ahead < n_chunks) dt = sel_dt<Q>(a, seq, token(ahead), head);
+        dt = sel_dt(a, seq, token(min(ahead, n_chunks - 1)), head);
     }
     for (int k = 0; k < n_chunks; ++k) {
         const int t0 = token(k), n = min(Q, seq.n - t0);
@@ -203,8 +206,8 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
         if constexpr (kOut) stage_C.template store<SC>(s.C, n, a.states);
         if ((k & 1) == 0) {
             if (k + ahead < n_chunks)
-                sel_steps<Q>(s.steps[mine][ahead], dt, seq.n - token(k + ahead), A, bias, a.softplus);
-            dt = k + 2 + ahead < n_chunks ? sel_dt<Q>(a, seq, token(k + 2 + ahead), head) : 0.0f;
+                sel_steps<Q>(s.steps[mine][ahead], dt.value(a.dt_type), seq.n - token(k + ahead), A, bias, a.softplus);
+            dt = sel_dt(a, seq, token(min(k + 2 + ahead, n_chunks - 1)), head);
         }
         __syncthreads();
         // (unconditional, as the loads are: the last chunk is fetched twice)

@@ -141,6 +141,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
         const float* const G = plan.G + ((long long)chunk * a.n_heads + head) * head_state;
         for (int tile = 0; tile < plan.n_tiles; ++tile) {
             const int p_tile = tile * 64, cols = min(64, a.dim - p_tile);
+            const SelDt dt = sel_dt(a, seq, t0, head);
             SelStage<T, Tc, Q, 64, VEC> stage_x, stage_dy;
             stage_x.load(sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n, cols);
             stage_dy.load(sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token, n, cols);
@@ -161,7 +162,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
             stage_dy.template store<SX>(s.dy, n, cols);
             if (tile == 0) {
                 if (wave == 0)
-                    raw = sel_steps<Q>(s.steps, sel_dt<Q>(a, seq, t0, head), n, a.A[head], a.dt_bias ? a.dt_bias[head] : 0.0f,
+                    raw = sel_steps<Q>(s.steps, dt.value(a.dt_type), n, a.A[head], a.dt_bias ? a.dt_bias[head] : 0.0f,
                                  a.softplus);
                 for (int q = tid; q < QT * Q; q += NHIP_WG) s.over[q / Q][q % Q] = s.col[q / Q][q % Q] = 0.0f;
                 for (int q = tid; q < 4 * Q; q += NHIP_WG) s.q[q / Q][q % Q] = s.r[q / Q][q % Q] = 0.0f;
