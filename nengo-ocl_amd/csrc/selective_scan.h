@@ -30,6 +30,7 @@ struct SelWalkPlan {
     int directions;         // 2: both halves
     long long n_segments, n_chunks;
     float* states;          // [direction][chunk][head][dim][states]
+    bool few;               // segments in a sequence: a walk adds up those before it itself
     float* ends;            // [direction][segment][head][dim][states], NULL: no sequence has two segments
     float* keeps;           // [direction][segment][head]: what a segment keeps of the state it begins with
 };
@@ -148,8 +149,9 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
 
     sel_f4 state[2][NT];
     {
+        const bool begun = plan.ends && !plan.few;
         const float* from = WALK == kSelEnds ? nullptr
-                            : plan.ends      ? ends + segment * all_states
+                            : begun          ? ends + segment * all_states
                             : back           ? (a.dfinal ? a.dfinal + seq.seq * all_states : nullptr)
                                              : (a.initial ? a.initial + seq.seq * all_states : nullptr);
         // (rows that are not there: the last one again, for which nothing is written)
@@ -161,6 +163,19 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
             for (int t = 0; t < NT; ++t)
                 if (from) state[h][t] = sel_state_load<VEC>(from + at[h], 16 * t + 4 * lane_g, a.states);
                 else state[h][t] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (WALK != kSelEnds && plan.ends && !begun) {
+            const int first = segment - seq.chunk, before = back ? n_segments - 1 - seq.chunk : seq.chunk;
+            for (int k = 0; k < before; ++k) {
+                const int other = first + (back ? n_segments - 1 - k : k);
+                const float keeps = plan.keeps[(back * plan.n_segments + other) * a.n_heads + head];
+                const float* const end = ends + other * all_states;
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        state[h][t] = state[h][t] * keeps + sel_state_load<VEC>(end + at[h], 16 * t + 4 * lane_g, a.states);
+            }
+        }
     }
     if constexpr (kOut)  // (above the diagonal for good)
         for (int q = threadIdx.x; q < Q * SW; q += NHIP_WG) s.weights[0][q] = s.weights[1][q] = (Tc)0.0f;
@@ -521,7 +536,9 @@ static inline long long sel_round4(long long floats) { return (floats + 3) & ~3L
 // How the sequences are cut, for a workspace that begins with the ends and the keeps.  A compute unit holds two walks
 // of the 16-bit kernel for up to 128 states, one of the others.  Sequences that give every unit a walk stay whole (8 x
 // 2048 tokens, 32 heads of 64, 128 states, both directions: 566 us for the gradient, cut in two 600); fewer are cut into
-// as many segments as walks fit, of at least four chunks (forward, with half as many walks: 152 us, cut in two 183).
+// as many segments as walks fit (forward, with half as many walks: 152 us, cut in two 183), down to a chunk each
+// (nine ragged sequences of 4001 tokens, 12 heads, 32 bits: 68 us, with four chunks at least 107).  Up to four segments are
+// added up by the walks themselves (32 x 32 KiB for each would be 100 us of 370; four save a launch of 12 us).
 static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions, float* states) {
     SelWalkPlan p;
     const int q = sel_chunk_tokens(a.states);
@@ -540,10 +557,10 @@ static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions,
         wanted = (wanted + a.tokens.n_seqs - 1) / a.tokens.n_seqs * a.tokens.n_seqs;
     }
     long long chunks = (total + wanted - 1) / wanted;
-    if (chunks < 4) chunks = 4;
     const bool cut = chunks < longest;
     p.chunks = (int)(cut ? chunks : longest > 0 ? longest : 1);
     p.n_segments = sel_max_chunks(a.tokens, q * p.chunks);
+    p.few = (longest + p.chunks - 1) / p.chunks <= 4;
     p.ends = cut ? reinterpret_cast<float*>(16) : nullptr;  // (its place is the caller's to fill in)
     p.keeps = nullptr;
     p.vec = sel_rows_wide(a.x, a.type, a.dim) && sel_rows_wide(a.B, a.type, a.states) &&
@@ -607,6 +624,8 @@ template <int WALK> static inline int sel_walk(hipStream_t stream, const nhip_sc
     if (plan.n_segments == 0) return 0;
     if (plan.ends) {
         if (int e = sel_walk_launch<kSelEnds>(stream, a, plan, true, false)) return e;
+    }
+    if (plan.ends && !plan.few) {
         const int v = plan.vec ? 4 : 1, per = NHIP_WG * v, q = sel_chunk_tokens(a.states);
         const long long blocks = ((long long)a.dim * a.states + per - 1) / per;
         const dim3 grid((unsigned)(blocks * a.n_heads * a.tokens.n_seqs * plan.directions));
