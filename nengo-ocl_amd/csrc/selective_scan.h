@@ -527,7 +527,7 @@ static inline int sel_scan_check(const nhip_scan_args* a) {
     if (chunks > most || chunks * a->n_heads > most || 2 * chunks * a->n_heads * tiles > most) return NHIP_E_BADARG;
     if (a->tokens.n_seqs * tiles * 64 * a->states / 256 * a->n_heads * 2 > most) return NHIP_E_BADARG;
     // (offsets of 32 bits within a chunk)
-    if ((long long)a->n_heads * a->dim >= (1 << 24)) return NHIP_E_BADARG;
+    if ((long long)a->n_heads * a->dim >= (1 << 24) || (long long)a->dim * a->states > (1 << 28)) return NHIP_E_BADARG;
     return 0;
 }
 

@@ -45,17 +45,24 @@ template <class Tc, int NP> struct GradLds {
 
 // Eight elements of a state across its rows: k over 32 rows from p0, column n.  Loads are unconditional (one
 // under a condition is waited for where its branch ends), from places cut to those that exist: what is too
-// much meets zeros of the other operand.
+// much meets zeros of the other operand.  WHOLE: all 32 rows exist; their places are then one offset from
+// places that the whole wave shares.
+template <bool WHOLE>
 __device__ __forceinline__ void state_cols(const float* s, int p0, int n, int dim, int states, int g, float (&v)[8]) {
     const unsigned c = (unsigned)min(n, states - 1);
+    const unsigned mine = 4 * (4 * g * (unsigned)states + c);
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-        const int p = min(p0 + 16 * (e >> 2) + 4 * g + (e & 3), dim - 1);
-        v[e] = s[(unsigned)p * (unsigned)states + c];
+        const int k = 16 * (e >> 2) + (e & 3);
+        if constexpr (WHOLE) {
+            v[e] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(s + (p0 + k) * states) + mine);
+        } else {
+            v[e] = s[(unsigned)min(p0 + k + 4 * g, dim - 1) * (unsigned)states + c];
+        }
     }
 }
 // Eight elements of row p, as a fragment over the states from n0
-template <class Tc, bool VEC>
+template <bool VEC>
 __device__ __forceinline__ void state_row(const float* s, int p, int n0, int dim, int states, int g, float (&v)[8]) {
     const float* row = s + (unsigned)min(p, dim - 1) * (unsigned)states;
 #pragma unroll
@@ -72,8 +79,9 @@ __device__ __forceinline__ void state_row(const float* s, int p, int n0, int dim
     }
 }
 
-template <class T, class Tc, int NP, bool VEC>
-__global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(nhip_scan_args a, GradPlan plan) {
+// WHOLE: the dimension is a multiple of 64
+template <class T, class Tc, int NP, bool VEC, bool WHOLE>
+__global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void grad_kernel(nhip_scan_args a, GradPlan plan) {
     using Lds = GradLds<Tc, NP>;
     constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
     constexpr int kTiles = QT * (QT + 1) / 2, kMyTiles = (kTiles + 3) / 4, kMyNT = (NT + 3) / 4;
@@ -135,16 +143,22 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
         for (int t = 0; t < QT; ++t) dB[m][t] = dC[m][t] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
 
     float raw = 0.0f;  // dt + dt_bias of token `lane` (the first wave)
+    SelStage<T, Tc, Q, 64, VEC> stage_x, stage_dy;
+    SelDt dt;
+    // (the next tile's inputs are on their way while one is worked on)
+    auto fetch = [&](int head, int p_tile) {
+        const int cols = min(64, a.dim - p_tile);
+        dt = sel_dt(a, seq, t0, head);
+        stage_x.load(sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n, cols);
+        stage_dy.load(sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token, n, cols);
+    };
+    fetch(head0, 0);
     for (int head = head0; head < head1; ++head) {
         const float D = a.D ? a.D[head] : 0.0f;
         const float* const S = plan.S + ((long long)chunk * a.n_heads + head) * head_state;
         const float* const G = plan.G + ((long long)chunk * a.n_heads + head) * head_state;
         for (int tile = 0; tile < plan.n_tiles; ++tile) {
             const int p_tile = tile * 64, cols = min(64, a.dim - p_tile);
-            const SelDt dt = sel_dt(a, seq, t0, head);
-            SelStage<T, Tc, Q, 64, VEC> stage_x, stage_dy;
-            stage_x.load(sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n, cols);
-            stage_dy.load(sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token, n, cols);
             // (addresses are formed anew in each tile: kept, they take the registers of the sums)
             int l = lane_l, g = lane_g;
             asm volatile("" : "+v"(l), "+v"(g));
@@ -154,8 +168,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
                     const int nt = min(wave + 4 * m, NT - 1);
-                    state_cols(S, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Sv[m][ks]);
-                    state_cols(G, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Gv[m][ks]);
+                    state_cols<WHOLE>(S, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Sv[m][ks]);
+                    state_cols<WHOLE>(G, p_tile + 32 * ks, 16 * nt + l, a.dim, a.states, g, Gv[m][ks]);
                 }
             __syncthreads();  // the tile before has been read
             stage_x.template store<SX>(s.x, n, cols);
@@ -170,10 +184,14 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
                 if (tid < 4) s.z[tid] = 0.0f;
             }
             __syncthreads();
+            {
+                const bool more = tile + 1 < plan.n_tiles;
+                fetch(more ? head : min(head + 1, head1 - 1), more ? p_tile + 64 : 0);
+            }
             float Gr[NK][8];  // row p of G
             const int p = p_tile + 16 * wave + l;
 #pragma unroll
-            for (int ks = 0; ks < NK; ++ks) state_row<Tc, VEC>(G, p, 32 * ks, a.dim, a.states, g, Gr[ks]);
+            for (int ks = 0; ks < NK; ++ks) state_row<VEC>(G, p, 32 * ks, a.dim, a.states, g, Gr[ks]);
 
 #pragma unroll
             for (int m = 0; m < kMyTiles; ++m) {
@@ -247,12 +265,14 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
 #pragma unroll
                     for (int ks = jt / 2; ks < QK; ++ks) sel_mma(acc, df[ks], sel_rows(s.kl + j * SW + 32 * ks, g));
                     sel_settle(acc);
-                    if (j < n) {
-                        const int c = 16 * wave + 4 * g;
+                    const int c = 16 * wave + 4 * g;
+                    float own[4];
+                    sel_load<Tc, 4>(s.dy + j * SX + c, own);
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) acc[r] = fmaf(D, (float)s.dy[j * SX + c + r], acc[r]);
-                        T* row = static_cast<T*>(a.dx) + ((seq.row0 + t0 + j) * a.n_heads + head) * a.dim + p_tile;
-                        sel_store4<VEC>(row, c, cols, acc);
+                    for (int r = 0; r < 4; ++r) acc[r] = fmaf(D, own[r], acc[r]);
+                    if (j < n) {
+                        T* row = static_cast<T*>(a.dx) + ((seq.row0 + t0) * a.n_heads + head) * a.dim + p_tile;
+                        sel_store4<VEC>(row + (unsigned)j * (unsigned)(a.n_heads * a.dim), c, cols, acc);
                     }
                 }
             }
@@ -266,14 +286,15 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 ? 2 : 1) void grad_kernel(
                 const int nt = wave + 4 * m;
                 if (nt >= NT) continue;
                 sel_phase();
+                float both = 0.0f;
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks)
 #pragma unroll
                     for (int e = 0; e < 8; ++e) {
-                        const int row = p_tile + 32 * ks + 16 * (e >> 2) + 4 * g + (e & 3);
-                        const float both = Sv[m][ks][e] * Gv[m][ks][e];
-                        z += row < a.dim && 16 * nt + l < a.states ? both : 0.0f;
+                        const float more = fmaf(Sv[m][ks][e], Gv[m][ks][e], both);
+                        both = WHOLE || p_tile + 32 * ks + 16 * (e >> 2) + 4 * g + (e & 3) < a.dim ? more : both;
                     }
+                z += 16 * nt + l < a.states ? both : 0.0f;
                 SelFrag<Tc> f[2][kSplits];
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Sv[m][ks], f[ks]);
@@ -477,7 +498,9 @@ extern "C" int nhip_selective_scan_grad(void* stream, const nhip_scan_args* args
             sel_with_states(a.states, [&](auto np) {
                 constexpr int NP = decltype(np)::value;
                 constexpr size_t lds = sizeof(GradLds<Tc, NP>);
-                auto kernel = m.walk.vec ? grad_kernel<T, Tc, NP, true> : grad_kernel<T, Tc, NP, false>;
+                auto kernel = !m.walk.vec       ? grad_kernel<T, Tc, NP, false, false>
+                              : a.dim % 64 == 0 ? grad_kernel<T, Tc, NP, true, true>
+                                                : grad_kernel<T, Tc, NP, true, false>;
                 rc = sel_allow_lds(kernel, lds);
                 if (rc) return;
                 hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(NHIP_WG), lds, st, a, plan);
