@@ -255,24 +255,32 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
 #pragma unroll
                 for (int ks = 0; ks < QK; ++ks) df[ks] = sel_cols(s.dy + 32 * ks * SX + 16 * wave, SX, l, g);
 #pragma unroll
-                for (int jt = 0; jt < QT; ++jt) {
+                for (int j2 = 0; j2 < QT; j2 += 2) {
                     sel_phase();
-                    const int j = 16 * jt + l;
-                    sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                    sel_f4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-                    for (int ks = 0; ks < NK; ++ks) sel_mma(acc, gf[ks], sel_rows(s.B + j * SN + 32 * ks, g));
-                    acc *= s.steps.to_end_step[j];
+                    for (int ks = 0; ks < NK; ++ks)
 #pragma unroll
-                    for (int ks = jt / 2; ks < QK; ++ks) sel_mma(acc, df[ks], sel_rows(s.kl + j * SW + 32 * ks, g));
+                        for (int u = 0; u < 2; ++u)
+                            sel_mma(acc[u], gf[ks], sel_rows(s.B + (16 * (j2 + u) + l) * SN + 32 * ks, g));
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) acc[u] *= s.steps.to_end_step[16 * (j2 + u) + l];
+#pragma unroll
+                    for (int ks = j2 / 2; ks < QK; ++ks)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            sel_mma(acc[u], df[ks], sel_rows(s.kl + (16 * (j2 + u) + l) * SW + 32 * ks, g));
                     sel_settle(acc);
                     const int c = 16 * wave + 4 * g;
-                    float own[4];
-                    sel_load<Tc, 4>(s.dy + j * SX + c, own);
+                    T* const row = static_cast<T*>(a.dx) + ((seq.row0 + t0) * a.n_heads + head) * a.dim + p_tile;
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) acc[r] = fmaf(D, own[r], acc[r]);
-                    if (j < n) {
-                        T* row = static_cast<T*>(a.dx) + ((seq.row0 + t0) * a.n_heads + head) * a.dim + p_tile;
-                        sel_store4<VEC>(row + (unsigned)j * (unsigned)(a.n_heads * a.dim), c, cols, acc);
+                    for (int u = 0; u < 2; ++u) {
+                        const int j = 16 * (j2 + u) + l;
+                        float own[4];
+                        sel_load<Tc, 4>(s.dy + j * SX + c, own);
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) acc[u][r] = fmaf(D, own[r], acc[u][r]);
+                        if (j < n) sel_store4<VEC>(row + (unsigned)j * (unsigned)(a.n_heads * a.dim), c, cols, acc[u]);
                     }
                 }
             }
@@ -298,50 +306,73 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                 SelFrag<Tc> f[2][kSplits];
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Sv[m][ks], f[ks]);
+                // (two tiles of tokens at once: the products of one wait for each other)
 #pragma unroll
-                for (int it = 0; it < QT; ++it) {
+                for (int i2 = 0; i2 < QT; i2 += 2) {
                     sel_phase();
-                    const int i = 16 * it + l;
-                    sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                    sel_f4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
                     for (int ks = 0; ks < 2; ++ks) {
-                        const SelFrag<Tc> d = sel_rows(s.dy + i * SX + 32 * ks, g);
+                        SelFrag<Tc> d[2];
 #pragma unroll
-                        for (int q = 0; q < kSplits; ++q) sel_mma(acc, f[ks][q], d);
+                        for (int u = 0; u < 2; ++u) d[u] = sel_rows(s.dy + (16 * (i2 + u) + l) * SX + 32 * ks, g);
+#pragma unroll
+                        for (int q = 0; q < kSplits; ++q)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) sel_mma(acc[u], f[ks][q], d[u]);
                     }
-                    acc *= s.steps.from_start[i];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        qs[it] = fmaf(acc[r], (float)s.C[i * SN + 16 * nt + 4 * g + r], qs[it]);
-                    dC[m][it] += acc;
+                    for (int u = 0; u < 2; ++u) {
+                        const int i = 16 * (i2 + u) + l;
+                        acc[u] *= s.steps.from_start[i];
+                        float c[4];
+                        sel_load<Tc, 4>(s.C + i * SN + 16 * nt + 4 * g, c);
 #pragma unroll
-                    for (int ks = 0; ks <= it / 2; ++ks)
-                        sel_mma(dC[m][it], sel_cols(s.B + 32 * ks * SN + 16 * nt, SN, l, g),
-                                sel_cols(s.xl + 32 * ks * SW + 16 * it, SW, l, g));
+                        for (int r = 0; r < 4; ++r) qs[i2 + u] = fmaf(acc[u][r], c[r], qs[i2 + u]);
+                        dC[m][i2 + u] += acc[u];
+                    }
+#pragma unroll
+                    for (int ks = 0; ks <= i2 / 2; ++ks) {
+                        const SelFrag<Tc> b = sel_cols(s.B + 32 * ks * SN + 16 * nt, SN, l, g);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            sel_mma(dC[m][i2 + u], b, sel_cols(s.xl + 32 * ks * SW + 16 * (i2 + u), SW, l, g));
+                    }
                 }
                 sel_settle(dC[m]);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Gv[m][ks], f[ks]);
 #pragma unroll
-                for (int jt = 0; jt < QT; ++jt) {
+                for (int j2 = 0; j2 < QT; j2 += 2) {
                     sel_phase();
-                    const int j = 16 * jt + l;
-                    sel_f4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+                    sel_f4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
                     for (int ks = 0; ks < 2; ++ks) {
-                        const SelFrag<Tc> d = sel_rows(s.x + j * SX + 32 * ks, g);
+                        SelFrag<Tc> d[2];
 #pragma unroll
-                        for (int q = 0; q < kSplits; ++q) sel_mma(acc, f[ks][q], d);
+                        for (int u = 0; u < 2; ++u) d[u] = sel_rows(s.x + (16 * (j2 + u) + l) * SX + 32 * ks, g);
+#pragma unroll
+                        for (int q = 0; q < kSplits; ++q)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) sel_mma(acc[u], f[ks][q], d[u]);
                     }
-                    acc *= s.steps.to_end[j];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        rs[jt] = fmaf(acc[r], (float)s.B[j * SN + 16 * nt + 4 * g + r], rs[jt]);
-                    dB[m][jt] += acc * s.steps.step[j];
+                    for (int u = 0; u < 2; ++u) {
+                        const int j = 16 * (j2 + u) + l;
+                        acc[u] *= s.steps.to_end[j];
+                        float b[4];
+                        sel_load<Tc, 4>(s.B + j * SN + 16 * nt + 4 * g, b);
 #pragma unroll
-                    for (int ks = jt / 2; ks < QK; ++ks)
-                        sel_mma(dB[m][jt], sel_cols(s.C + 32 * ks * SN + 16 * nt, SN, l, g),
-                                sel_rows(s.xl + j * SW + 32 * ks, g));
+                        for (int r = 0; r < 4; ++r) rs[j2 + u] = fmaf(acc[u][r], b[r], rs[j2 + u]);
+                        dB[m][j2 + u] += acc[u] * s.steps.step[j];
+                    }
+#pragma unroll
+                    for (int ks = j2 / 2; ks < QK; ++ks) {
+                        const SelFrag<Tc> c = sel_cols(s.C + 32 * ks * SN + 16 * nt, SN, l, g);
+#pragma unroll
+                        for (int u = 0; u < 2; ++u)
+                            sel_mma(dB[m][j2 + u], c, sel_rows(s.xl + (16 * (j2 + u) + l) * SW + 32 * ks, g));
+                    }
                 }
                 sel_settle(dB[m]);
             }
