@@ -124,7 +124,8 @@ __global__ __launch_bounds__(NHIP_WG) void norm_kernel(nhip_norm_args a) {
 // With n = v inv (inv = 1 / sqrt(mean(v^2) + eps)) and e the gradient of n weight (dout, times
 // scale behind a block): dweight = sum over rows of e n;  dv = inv (e weight - n mean(e weight n)).
 // Each group of lanes keeps its channels over its rows (every gridDim.x-th) and the sums for
-// weight and scale with them; a second launch adds the groups' sums up in their order.
+// weight and scale with them; a second launch adds the groups' sums up in their order.  The next row is on its
+// way while one is worked on (8192 rows of 2048, bfloat16, residual: 53 us without).
 template <class T, int V, int L, int R>
 __global__ __launch_bounds__(NHIP_WG) void norm_grad_kernel(nhip_norm_args a, float* parts) {
     __shared__ float s[8];
@@ -133,144 +134,134 @@ __global__ __launch_bounds__(NHIP_WG) void norm_grad_kernel(nhip_norm_args a, fl
     const int lane = threadIdx.x % L, mine = threadIdx.x / L, width = a.channels / a.groups;
     const int base = blockIdx.y * width;
     const bool before = a.residual && !a.after, behind = a.residual && a.after;
-    constexpr int kHeld = R ? R : 1;
-    float dw[kHeld][V], ds[kHeld][V];
     float* const row_w = parts + (long long)blockIdx.x * 2 * a.channels + base;
     float* const row_s = row_w + a.channels;
+    const long long step = (long long)gridDim.x * kWaves;
+
+    // What a lane needs of V channels of a row
+    struct Raw {
+        SelPack<T, V> x, gate, residual, dout, dv;
+    };
+    // loads are unconditional, from channels and rows cut to those that exist: one under a condition is waited
+    // for where its branch ends
+    auto fetch = [&](Raw& raw, long long row, int c) {
+        const long long r = min(row, a.rows - 1);
+        const int at = base + min(c, width - V);
+        auto get = [&](const void* p, long long stride) {
+            return *reinterpret_cast<const SelPack<T, V>*>(static_cast<const T*>(p) + r * stride + at);
+        };
+        raw.x = get(a.x, a.x_stride);
+        raw.dout = get(a.dout, a.dout_stride);
+        if (a.gate) raw.gate = get(a.gate, a.gate_stride);
+        if (before) raw.residual = get(a.residual, a.residual_stride);
+        if (a.dv) raw.dv = get(a.dv, a.dv_stride);
+    };
+    struct Values {
+        float v[V], e[V], x[V], f[V], slope[V], more[V];  // normed, dout, x, gate sigmoid(gate), its derivative, dv
+    };
+    auto params = [&](int c, float(&w)[V], float(&k)[V]) {
 #pragma unroll
-    for (int r = 0; r < kHeld; ++r)
+        for (int i = 0; i < V; ++i) {
+            w[i] = a.weight[base + min(c, width - V) + i];
+            k[i] = a.scale ? a.scale[base + min(c, width - V) + i] : 1.0f;
+        }
+    };
+    auto open = [&](const Raw& raw, const float(&k)[V], Values& u) {
 #pragma unroll
-        for (int i = 0; i < V; ++i) dw[r][i] = ds[r][i] = 0.0f;
-    if constexpr (R == 0) {
-        for (int c = lane * V; c < width; c += L * V)
-#pragma unroll
-            for (int i = 0; i < V; ++i) row_w[c + i] = row_s[c + i] = 0.0f;
-    }
-    for (long long row = (long long)blockIdx.x * kWaves + mine; row < a.rows;
-         row += (long long)gridDim.x * kWaves) {
-        const Operands<T, V> op{a, row, base, before};
-        float v[kHeld][V], e[kHeld][V];
-        float sum = 0.0f, dot = 0.0f;
-        auto first = [&](int c, float(&u)[V], float(&g)[V]) {
-            float w[V];
-            op.normed(c, u);
-            op.read(a.dout, a.dout_stride, c, g);
-            op.param(a.weight, c, w);
-            if (behind && a.scale) {
-                float k[V];
-                op.param(a.scale, c, k);
-#pragma unroll
-                for (int i = 0; i < V; ++i) w[i] *= k[i];
+        for (int i = 0; i < V; ++i) {
+            u.x[i] = (float)raw.x.v[i];
+            u.e[i] = (float)raw.dout.v[i];
+            u.f[i] = 1.0f;
+            u.slope[i] = 0.0f;
+            if (a.gate) {
+                const float g = (float)raw.gate.v[i], sg = sel_sigmoid(g);
+                u.f[i] = g * sg;
+                u.slope[i] = sg * fmaf(g, 1.0f - sg, 1.0f);
             }
+            u.v[i] = u.x[i] * u.f[i];
+            if (before) u.v[i] = fmaf(k[i], u.v[i], (float)raw.residual.v[i]);
+            u.more[i] = a.dv ? (float)raw.dv.v[i] : 0.0f;
+        }
+    };
+    auto sums = [&](int c, const Values& u, const float(&w)[V], const float(&k)[V], float& sum, float& dot) {
+        if (c >= width) return;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            sum = fmaf(u.v[i], u.v[i], sum);
+            dot = fmaf(u.e[i] * (behind ? w[i] * k[i] : w[i]), u.v[i], dot);
+        }
+    };
+    auto close = [&](long long row, int c, const Values& u, const float(&w)[V], const float(&k)[V], float inv, float mean,
+                     float(&dw)[V], float(&ds)[V]) {
+        if (c >= width) return;
+        const long long at = row * a.channels + base + c;
+        float d[V], dg[V];
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const float n = u.v[i] * inv;
+            const float to_w = behind ? u.e[i] * k[i] : u.e[i];  // gradient of n weight
+            dw[i] = fmaf(to_w, n, dw[i]);
+            d[i] = fmaf(inv, fmaf(-n, mean, to_w * w[i]), u.more[i]);
+            if (behind) ds[i] = fmaf(u.e[i], n * w[i], ds[i]);
+        }
+        if (before) {
+            if (a.dresidual) sel_store<T, V>(static_cast<T*>(a.dresidual) + at, d);
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                sum = fmaf(u[i], u[i], sum);
-                dot = fmaf(g[i] * w[i], u[i], dot);
+                ds[i] = fmaf(d[i], u.x[i] * u.f[i], ds[i]);
+                d[i] *= k[i];
             }
-        };
-        if constexpr (R > 0) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int c = (r * L + lane) * V;
-                if (c < width) first(c, v[r], e[r]);
-            }
-        } else {
-            for (int c = lane * V; c < width; c += L * V) first(c, v[0], e[0]);
         }
-        sum = sum_over<L>(sum, s);
-        dot = sum_over<L>(dot, s + 4);
-        const float inv = 1.0f / sqrtf(sum / (float)width + a.eps);
-        const float mean = dot * inv / (float)width;
-        const long long at = row * a.channels + base;
-        auto second = [&](int c, float(&u)[V], float(&g)[V], float(&w_sum)[V], float(&s_sum)[V]) {
-            float w[V], k[V], d[V];
-            op.param(a.weight, c, w);
-#pragma unroll
-            for (int i = 0; i < V; ++i) k[i] = 1.0f;
-            if (a.scale) op.param(a.scale, c, k);
+        if (a.gate) {
 #pragma unroll
             for (int i = 0; i < V; ++i) {
-                const float n = u[i] * inv;
-                const float to_w = behind ? g[i] * k[i] : g[i];  // gradient of n weight
-                w_sum[i] = fmaf(to_w, n, w_sum[i]);
-                if (behind) s_sum[i] = fmaf(g[i], n * w[i], s_sum[i]);
-                d[i] = inv * fmaf(-n, mean, to_w * w[i]);
+                dg[i] = d[i] * u.x[i] * u.slope[i];
+                d[i] *= u.f[i];
             }
-            float x[V], gate[V], f[V];
-            if (before || a.gate) op.read(a.x, a.x_stride, c, x);
-#pragma unroll
-            for (int i = 0; i < V; ++i) f[i] = 1.0f;
-            if (a.gate) {
-                op.read(a.gate, a.gate_stride, c, gate);
-#pragma unroll
-                for (int i = 0; i < V; ++i) f[i] = sel_sigmoid(gate[i]);
-            }
-            if (before) {
-                if (a.dv) {
-                    float more[V];
-                    op.read(a.dv, a.dv_stride, c, more);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) d[i] += more[i];
-                }
-                if (a.dresidual) sel_store<T, V>(static_cast<T*>(a.dresidual) + at + c, d);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    s_sum[i] = fmaf(d[i], a.gate ? x[i] * (gate[i] * f[i]) : x[i], s_sum[i]);
-                    d[i] *= k[i];
-                }
-            }
-            if (a.gate) {
-                float dg[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    dg[i] = d[i] * x[i] * (f[i] * fmaf(gate[i], 1.0f - f[i], 1.0f));
-                    d[i] *= gate[i] * f[i];
-                }
-                sel_store<T, V>(static_cast<T*>(a.dgate) + at + c, dg);
-            }
-            sel_store<T, V>(static_cast<T*>(a.dx) + at + c, d);
-        };
-        if constexpr (R > 0) {
-#pragma unroll
-            for (int r = 0; r < R; ++r) {
-                const int c = (r * L + lane) * V;
-                if (c < width) second(c, v[r], e[r], dw[r], ds[r]);
-            }
-        } else {
-            for (int c = lane * V; c < width; c += L * V) {
-                op.normed(c, v[0]);
-                op.read(a.dout, a.dout_stride, c, e[0]);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    dw[0][i] = row_w[c + i];
-                    ds[0][i] = row_s[c + i];
-                }
-                second(c, v[0], e[0], dw[0], ds[0]);
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    row_w[c + i] = dw[0][i];
-                    row_s[c + i] = ds[0][i];
-                }
-            }
+            sel_store<T, V>(static_cast<T*>(a.dgate) + at, dg);
         }
-    }
+        sel_store<T, V>(static_cast<T*>(a.dx) + at, d);
+    };
+    auto channel = [&](int r) { return (r * L + lane) * V; };
+    const long long row0 = (long long)blockIdx.x * kWaves + mine;
+
     if constexpr (R > 0) {
+        float w[R][V], k[R][V], dw[R][V], ds[R][V];
+        Raw raw[R];
+#pragma unroll
         for (int r = 0; r < R; ++r) {
+            params(channel(r), w[r], k[r]);
+            if (a.rows) fetch(raw[r], row0, channel(r));
+#pragma unroll
+            for (int i = 0; i < V; ++i) dw[r][i] = ds[r][i] = 0.0f;
+        }
+        for (long long row = row0; row < a.rows; row += step) {
+            Values u[R];
+            float sum = 0.0f, dot = 0.0f;
+#pragma unroll
+            for (int r = 0; r < R; ++r) open(raw[r], k[r], u[r]);
+#pragma unroll
+            for (int r = 0; r < R; ++r) fetch(raw[r], row + step, channel(r));
+#pragma unroll
+            for (int r = 0; r < R; ++r) sums(channel(r), u[r], w[r], k[r], sum, dot);
+            sum = sum_over<L>(sum, s);
+            dot = sum_over<L>(dot, s + 4);
+            const float inv = 1.0f / sqrtf(sum / (float)width + a.eps);
+            const float mean = dot * inv / (float)width;
+#pragma unroll
+            for (int r = 0; r < R; ++r) close(row, channel(r), u[r], w[r], k[r], inv, mean, dw[r], ds[r]);
+        }
+        // the waves' sums, or the group's own
+#pragma unroll
+        for (int r = 0; r < R; ++r)
 #pragma unroll
             for (int which = 0; which < 2; ++which) {
-                float m[V];
-#pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    m[i] = which ? ds[0][i] : dw[0][i];
-#pragma unroll
-                    for (int q = 1; q < R; ++q) m[i] = r == q ? (which ? ds[q][i] : dw[q][i]) : m[i];
-                }
                 float* const out = which ? row_s : row_w;
-                const int c = (r * L + lane) * V;
+                const int c = channel(r);
                 if constexpr (L == NHIP_WAVE) {
                     __syncthreads();
 #pragma unroll
-                    for (int i = 0; i < V; ++i) both[(mine * NHIP_WAVE + lane) * V + i] = m[i];
+                    for (int i = 0; i < V; ++i) both[(mine * NHIP_WAVE + lane) * V + i] = which ? ds[r][i] : dw[r][i];
                     __syncthreads();
                     if (mine == 0 && c < width)
 #pragma unroll
@@ -281,7 +272,41 @@ __global__ __launch_bounds__(NHIP_WG) void norm_grad_kernel(nhip_norm_args a, fl
                         }
                 } else if (c < width) {
 #pragma unroll
-                    for (int i = 0; i < V; ++i) out[c + i] = m[i];
+                    for (int i = 0; i < V; ++i) out[c + i] = which ? ds[r][i] : dw[r][i];
+                }
+            }
+    } else {
+        for (int c = lane * V; c < width; c += L * V)
+#pragma unroll
+            for (int i = 0; i < V; ++i) row_w[c + i] = row_s[c + i] = 0.0f;
+        for (long long row = row0; row < a.rows; row += step) {
+            float sum = 0.0f, dot = 0.0f, w[V], k[V], dw[V], ds[V];
+            Raw raw;
+            Values u;
+            for (int c = lane * V; c < width; c += L * V) {
+                params(c, w, k);
+                fetch(raw, row, c);
+                open(raw, k, u);
+                sums(c, u, w, k, sum, dot);
+            }
+            sum = sum_over<L>(sum, s);
+            dot = sum_over<L>(dot, s + 4);
+            const float inv = 1.0f / sqrtf(sum / (float)width + a.eps);
+            const float mean = dot * inv / (float)width;
+            for (int c = lane * V; c < width; c += L * V) {
+                params(c, w, k);
+                fetch(raw, row, c);
+                open(raw, k, u);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    dw[i] = row_w[c + i];
+                    ds[i] = row_s[c + i];
+                }
+                close(row, c, u, w, k, inv, mean, dw, ds);
+#pragma unroll
+                for (int i = 0; i < V; ++i) {
+                    row_w[c + i] = dw[i];
+                    row_s[c + i] = ds[i];
                 }
             }
         }
