@@ -26,7 +26,9 @@ typedef struct nhip_rows {
 
 /* Which tokens there are.  starts == NULL: n_seqs sequences of `length` tokens.  Otherwise
  * sequence s holds the tokens starts[s] ... starts[s + 1] - 1 of `n_tokens` (int32, device;
- * offsets outside 0 ... n_tokens are cut to that range, lengths below zero are zero). */
+ * offsets outside 0 ... n_tokens are cut to that range, lengths below zero are zero; results of
+ * tokens that no sequence holds are not written, those of sequences that overlap are undefined).
+ * n_tokens is at most 0x7fff0000. */
 typedef struct nhip_tokens {
     const int *starts;
     long long n_tokens;

@@ -64,7 +64,7 @@ template <class T, int V, int L, int R>
 __global__ __launch_bounds__(NHIP_WG) void norm_kernel(nhip_norm_args a) {
     __shared__ float s[8];
     const int lane = threadIdx.x % L, width = a.channels / a.groups;
-    const long long part = (long long)blockIdx.x * (NHIP_WG / L) + threadIdx.x / L;
+    const long long part = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * (NHIP_WG / L) + threadIdx.x / L;
     if (part >= a.rows * a.groups) return;  // uniform over the lanes that share a part
     const Operands<T, V> op{a, part / a.groups, (int)(part % a.groups) * width, a.residual && !a.after};
     constexpr int kHeld = R ? R : 1;
@@ -377,8 +377,10 @@ extern "C" int nhip_block_norm(void* stream, const nhip_norm_args* args) {
             constexpr int V = decltype(vec)::value ? V16 : 1, L = decltype(lanes)::value, R = decltype(held)::value;
             const long long parts = a.rows * a.groups;
             constexpr int per = NHIP_WG / L;
-            NHIP_LAUNCH((norm_kernel<T, V, L, R>), dim3((unsigned)((parts + per - 1) / per)), dim3(NHIP_WG), 0,
-                        static_cast<hipStream_t>(stream), a);
+            // (an axis of a grid has fewer than 2^32 threads)
+            const long long n = (parts + per - 1) / per, across = n < 65536 ? n : 65536;
+            NHIP_LAUNCH((norm_kernel<T, V, L, R>), dim3((unsigned)across, (unsigned)((n + across - 1) / across)),
+                        dim3(NHIP_WG), 0, static_cast<hipStream_t>(stream), a);
             rc = (int)hipGetLastError();
         });
     });

@@ -9,6 +9,7 @@
 typedef float sel_f4 __attribute__((ext_vector_type(4)));
 
 #define SEL_MAX_GRID_Y 65535
+#define SEL_MAX_TOKENS 0x7fff0000LL  // (room for a chunk behind the last token in 32 bits)
 
 // ------------------------------------------------------------------------------ element types
 // Sums, states and statistics are float32; a value is rounded to a 16-bit type once, when it
@@ -109,6 +110,10 @@ static inline long long sel_max_chunks(const nhip_tokens& t, int q) {
     return t.n_tokens / q + t.n_seqs;
 }
 
+// Sequences that overlap (offsets that go back) can make more chunks than sel_max_chunks: those
+// beyond it have no work-group, and whoever counts to them stays below 2^31.
+__device__ __forceinline__ int sel_add_chunks(int a, int b) { return (int)min((unsigned)a + (unsigned)b, 0x7fffffffu); }
+
 // Which sequence chunk c belongs to.  Ragged: the 64 lanes of a wave take a sequence each and
 // add up their chunks (uniform over the wave, no table, no launch of its own; 64 sequences
 // cost about as much as a read of memory).
@@ -134,17 +139,17 @@ __device__ __forceinline__ SelSeq sel_seq_of_chunk(const nhip_tokens& t, int c, 
 #pragma unroll
         for (int d = 1; d < NHIP_WAVE; d *= 2) {
             const int other = __shfl_up(sum, d);
-            if (lane >= d) sum += other;
+            if (lane >= d) sum = sel_add_chunks(sum, other);
         }
         const int total = __builtin_amdgcn_readlane(sum, NHIP_WAVE - 1);
-        if (c < before + total) {
-            const unsigned long long past = __ballot(before + sum > c);
+        if (c < sel_add_chunks(before, total)) {
+            const unsigned long long past = __ballot(sel_add_chunks(before, sum) > c);
             const int at = __ffsll((long long)past) - 1;
             // (in scalar registers: they are the same in all lanes, which the compiler cannot see)
             const int lane_of = __builtin_amdgcn_readfirstlane(at);
             r.seq = s0 + lane_of;
             r.n = __builtin_amdgcn_readlane(n, lane_of);
-            r.chunk = c - (before + __builtin_amdgcn_readlane(sum - mine, lane_of));
+            r.chunk = c - before - (__builtin_amdgcn_readlane(sum, lane_of) - __builtin_amdgcn_readlane(mine, lane_of));
             r.row0 = __builtin_amdgcn_readfirstlane(sel_bound(t, r.seq));
             return r;
         }
@@ -165,9 +170,9 @@ __device__ __forceinline__ SelSeq sel_seq(const nhip_tokens& t, int s, int q) {
     }
     const int lane = threadIdx.x & (NHIP_WAVE - 1);
     int sum = 0;
-    for (int i = lane; i < s; i += NHIP_WAVE) sum += sel_chunks(sel_length(t, i), q);
+    for (int i = lane; i < s; i += NHIP_WAVE) sum = sel_add_chunks(sum, sel_chunks(sel_length(t, i), q));
 #pragma unroll
-    for (int d = 1; d < NHIP_WAVE; d *= 2) sum += __shfl_xor(sum, d);
+    for (int d = 1; d < NHIP_WAVE; d *= 2) sum = sel_add_chunks(sum, __shfl_xor(sum, d));
     r.chunk = __builtin_amdgcn_readfirstlane(sum);
     r.n = __builtin_amdgcn_readfirstlane(sel_length(t, s));
     r.row0 = __builtin_amdgcn_readfirstlane(sel_bound(t, s));
@@ -249,7 +254,7 @@ static inline int sel_reduce(hipStream_t stream, const SelReduce& a) {
 }
 
 static inline bool sel_tokens_ok(const nhip_tokens& t) {
-    if (t.n_seqs < 0 || t.n_tokens < 0 || t.n_tokens > 0x7fffffffLL) return false;
+    if (t.n_seqs < 0 || t.n_tokens < 0 || t.n_tokens > SEL_MAX_TOKENS) return false;
     if (!t.starts) return t.length >= 0 && (long long)t.n_seqs * t.length == t.n_tokens;
     return true;
 }

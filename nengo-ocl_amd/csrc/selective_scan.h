@@ -166,7 +166,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
         if (WALK != kSelEnds && plan.ends && !begun) {
             const int first = segment - seq.chunk, before = back ? n_segments - 1 - seq.chunk : seq.chunk;
             for (int k = 0; k < before; ++k) {
-                const int other = first + (back ? n_segments - 1 - k : k);
+                const long long other = min((long long)first + (back ? n_segments - 1 - k : k), plan.n_segments - 1);
                 const float keeps = plan.keeps[(back * plan.n_segments + other) * a.n_heads + head];
                 const float* const end = ends + other * all_states;
 #pragma unroll
@@ -187,7 +187,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
     const int chunk0 = seq.chunk * plan.chunks;
     const int n_chunks = min(plan.chunks, (seq.n + Q - 1) / Q - chunk0);
     auto token = [&](int k) { return (chunk0 + (back ? n_chunks - 1 - k : k)) * Q; };
-    const int first_chunk = WALK == kSelStates ? sel_seq(a.tokens, seq.seq, Q).chunk : 0;
+    const long long first_chunk = WALK == kSelStates ? sel_seq(a.tokens, seq.seq, Q).chunk : 0;
 
     SelStage<T, Tc, Q, 64, VEC> stage_x[2];
     SelStage<T, Tc, Q, NP, VEC> stage_B, stage_C;
@@ -480,8 +480,9 @@ static __global__ __launch_bounds__(NHIP_WG) void sel_begin_kernel(nhip_scan_arg
     const int block = blockIdx.x % blocks, head = (blockIdx.x / blocks) % a.n_heads;
     const int which = blockIdx.x / (blocks * a.n_heads), s = which % a.tokens.n_seqs, back = which / a.tokens.n_seqs;
     const SelSeq seq = sel_seq(a.tokens, s, q * plan.chunks);
-    const int at = (block * NHIP_WG + threadIdx.x) * V, n = sel_chunks(seq.n, q * plan.chunks);
-    if (at >= head_state) return;
+    const int at = (block * NHIP_WG + threadIdx.x) * V;
+    const int n = (int)min((long long)sel_chunks(seq.n, q * plan.chunks), plan.n_segments - seq.chunk);
+    if (at >= head_state || n <= 0) return;
     const long long all_states = (long long)a.n_heads * head_state, mine = (long long)head * head_state + at;
     float state[V];
     const float* from = back ? a.dfinal : a.initial;
@@ -514,7 +515,7 @@ static __global__ __launch_bounds__(NHIP_WG) void sel_begin_kernel(nhip_scan_arg
 static inline bool sel_rows_wide(const nhip_rows& r, int type, int cols) {
     const int v = 16 / sel_size(type);
     return sel_aligned(r.p, 16) && cols % v == 0 && r.seq % v == 0 && r.token % v == 0 && r.head % v == 0 &&
-           r.token < (1 << 23);
+           r.token >= 0 && r.token < (1 << 23);
 }
 
 static inline int sel_scan_check(const nhip_scan_args* a) {

@@ -29,6 +29,13 @@ float16 (parameters and states: float32).  Sequences lie side by side, ``[S, L, 
 with ``starts`` (int32, S + 1 offsets on the device, the layout of a ragged array's
 ``starts``), back to back, ``[T, ...]``; sequences may be empty.  Rows may have any
 strides, the last axis has stride one.  ValueError and TypeError say what does not fit.
+
+What the offsets on the device hold is not checked: they are cut to the tokens that there are,
+results of tokens that no sequence holds are not written, and those of sequences that overlap
+are undefined.  Outputs may not overlap inputs.  Sums, states and parameters' gradients are
+float32 and added up in the same order on every call.  An input that is no finite number reaches
+what depends on it, no earlier token and no other sequence; in the scan's gradient, all tokens of
+its chunk of 64 (32 with more than 128 states).
 """
 
 import collections
@@ -42,6 +49,7 @@ c_int, c_ll, c_float, c_p = ctypes.c_int, ctypes.c_longlong, ctypes.c_float, cty
 
 MAX_WIDTH = 8     # taps of the convolution
 MAX_STATES = 256  # states per row of a head
+MAX_TOKENS = 0x7fff0000  # of a call
 
 ConvGradients = collections.namedtuple("ConvGradients", "x weight bias initial")
 ScanGradients = collections.namedtuple("ScanGradients", "x dt A B C D dt_bias initial")
@@ -154,8 +162,8 @@ def _tokens(queue, x, starts, axes):
             raise ValueError("x has %d axes: [S, L, ...] needs %d, back-to-back sequences need `starts`"
                              % (x.dim(), 2 + axes))
         s, n = x.shape[0], x.shape[1]
-        if s * n > 0x7fffffff:
-            raise ValueError("%d tokens: at most 2**31 - 1 in a call" % (s * n))
+        if s * n > MAX_TOKENS:
+            raise ValueError("%d tokens: at most %d in a call" % (s * n, MAX_TOKENS))
         return _Tokens(None, s * n, s, n), (s, n), s, None
     if lead != 1:
         raise ValueError("x has %d axes: with `starts` it has %d, [T, ...]" % (x.dim(), 1 + axes))
@@ -164,8 +172,8 @@ def _tokens(queue, x, starts, axes):
         raise ValueError("starts has shape %s: S + 1 offsets are wanted" % (tuple(starts.shape),))
     starts = _array(queue, "starts", starts, starts.shape, _torch().int32, contiguous=True)
     t, s = x.shape[0], starts.shape[0] - 1
-    if t > 0x7fffffff:
-        raise ValueError("%d tokens: at most 2**31 - 1 in a call" % t)
+    if t > MAX_TOKENS:
+        raise ValueError("%d tokens: at most %d in a call" % (t, MAX_TOKENS))
     return _Tokens(starts.data_ptr(), t, s, 0), (t,), s, starts
 
 

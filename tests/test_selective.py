@@ -494,6 +494,39 @@ def test_offsets_beyond_the_tokens(queue, ops):
     assert torch.equal(y[:20], want[:20])
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,copies", [(700, 3), (9000, 5)])
+def test_offsets_that_go_back(queue, ops, tokens, copies):
+    """Sequences that overlap make more chunks than there are places: those that have one hold."""
+    given, _, _ = scan_inputs(22, F32, [tokens], 2, 8, 1, 8, False)
+    given.pop("initial", None)
+    starts = torch.tensor([0, tokens] * copies, dtype=torch.int32).cuda()
+    s = 2 * copies - 1
+    plans = [ops.plan_selective_scan(queue, softplus=True, starts=starts, **given),
+             ops.plan_selective_scan_grad(queue, given["x"], softplus=True, starts=starts, **given)]
+    torch.cuda.synchronize()
+    for plan in plans:
+        plan()
+    want, end = ops.selective_scan(queue, softplus=True, starts=starts[:2].contiguous(), **given)
+    assert plans[0].final.shape[0] == s and torch.isfinite(plans[0].y[:64]).all()
+    assert torch.equal(plans[0].y[:64], want[:64])
+    conv, _, _ = conv_inputs(23, F32, [tokens], 8, 3, False)
+    conv.pop("initial", None)
+    y, _ = ops.causal_conv(queue, starts=starts, **conv)
+    want, _ = ops.causal_conv(queue, starts=starts[:2].contiguous(), **conv)
+    assert torch.equal(y, want)
+
+
+@pytest.mark.gpu
+def test_norm_of_more_parts_than_an_axis_of_a_grid_has(queue, ops):
+    """2**26 + 3 rows of one channel: 64 threads each."""
+    n = 2 ** 26 + 3
+    x = torch.full((n, 1), 3.0, dtype=BF16, device="cuda")
+    x[-1] = -3.0
+    out, _ = ops.block_norm(queue, x, torch.full((1,), 2.0, device="cuda"), eps=0.0)
+    assert float(out[0]) == 2.0 and float(out[-1]) == -2.0 and int((out == 2.0).sum()) == n - 1
+
+
 # -------------------------------------------------------------------------------- refusals
 @pytest.fixture
 def host(monkeypatch):
