@@ -91,34 +91,50 @@ __device__ __forceinline__ SelFrag<float> sel_cols(const float* at, int stride, 
     return f;
 }
 
-// Eight float32 values as fragments that add up to them
-template <class Tc>
-__device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<Tc> (&f)[SelSplit<Tc>::n]) {
+// Eight float32 values as fragments that add up to them.  (bfloat16: two values at a time, which is one
+// instruction to round them and one for each to widen it; element by element the compiler rounds each alone)
+__device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<float> (&f)[1]) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        float rest = x[e];
+    for (int e = 0; e < 8; ++e) f[0].v[e] = x[e];
+}
+__device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<__bf16> (&f)[3]) {
+    typedef float two __attribute__((ext_vector_type(2)));
+    typedef __bf16 two_b __attribute__((ext_vector_type(2)));
+    unsigned out[3][4];
 #pragma unroll
-        for (int s = 0; s < SelSplit<Tc>::n; ++s) {
-            f[s].set(e, rest);
-            rest -= f[s].get(e);
+    for (int e = 0; e < 4; ++e) {
+        two rest = {x[2 * e], x[2 * e + 1]};
+#pragma unroll
+        for (int s = 0; s < 3; ++s) {
+            out[s][e] = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, two_b));
+            rest.x -= __uint_as_float(out[s][e] << 16);
+            rest.y -= __uint_as_float(out[s][e] & 0xffff0000u);
         }
     }
+#pragma unroll
+    for (int s = 0; s < 3; ++s) f[s].v = __builtin_bit_cast(sel_b8, out[s]);
 }
 
-// Whether all eight are finite, and what is left with zeros in the place of those that are not; ones in their place
-__device__ __forceinline__ bool sel_finite(const SelFrag<__bf16>& f) {
-    typedef unsigned short us8 __attribute__((ext_vector_type(8)));
-    typedef unsigned short us4 __attribute__((ext_vector_type(4)));
+// Whether all elements are finite (magnitudes of 16 bits are compared as whole numbers, two at a time), and
+// what is left with zeros in the place of those that are not; ones in their place
+template <int H, int K> __device__ __forceinline__ bool sel_finite(const SelFrag<__bf16> (&f)[H][K]) {
     typedef unsigned short us2 __attribute__((ext_vector_type(2)));
-    const us8 m = __builtin_bit_cast(us8, f.v) & (unsigned short)0x7fff;
-    const us4 a = __builtin_elementwise_max(m.lo, m.hi);
-    const us2 b = __builtin_elementwise_max(a.lo, a.hi);
-    return b.x < 0x7f80 && b.y < 0x7f80;
-}
-__device__ __forceinline__ bool sel_finite(const SelFrag<float>& f) {
-    float m = fabsf(f.v[0]) * 0.0f;
+    typedef unsigned u4 __attribute__((ext_vector_type(4)));
+    us2 most = {0, 0};
 #pragma unroll
-    for (int e = 1; e < 8; ++e) m = fmaf(f.v[e], 0.0f, m);
+    for (int q = 0; q < H * K; ++q) {
+        const u4 m = __builtin_bit_cast(u4, f[q / K][q % K].v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = __builtin_elementwise_max(most, __builtin_bit_cast(us2, m[e] & 0x7fff7fffu));
+    }
+    return most.x < 0x7f80 && most.y < 0x7f80;
+}
+template <int H, int K> __device__ __forceinline__ bool sel_finite(const SelFrag<float> (&f)[H][K]) {
+    float m = 0.0f;
+#pragma unroll
+    for (int q = 0; q < H * K; ++q)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) m = fmaf(f[q / K][q % K].v[e], 0.0f, m);
     return m == 0.0f;
 }
 template <class Tc> __device__ __forceinline__ SelFrag<Tc> sel_take_unfinite(SelFrag<Tc>& f) {

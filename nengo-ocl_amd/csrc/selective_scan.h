@@ -236,6 +236,8 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
         // (addresses are formed anew in each chunk: kept, they take the registers of the state)
         int l = lane_l, g = lane_g;
         asm volatile("" : "+v"(l), "+v"(g));
+        // (24 bits: products of 32 take four times as long)
+        const int l_X = __mul24(l, SX), l_B = __mul24(l, SB), l_C = __mul24(l, SC), l_W = __mul24(l, SW);
 
         SelFrag<Tc> xf[2][QK];  // rows p of x transposed, over the tokens
 #pragma unroll
@@ -249,13 +251,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
             SelFrag<Tc> f = sel_cols(xs + 32 * ks * SX + p_wave + 16 * h, SX, l, g);
             return sel_take_unfinite(f);
         };
-        if constexpr (kOut) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int ks = 0; ks < QK; ++ks) finite = sel_finite(xf[h][ks]) && finite;
-            finite = __all(finite);
-        }
+        if constexpr (kOut) finite = __all(sel_finite(xf));
         if (!finite)
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -273,11 +269,11 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
             for (int m = 0; m < kMine; ++m) acc[m] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) {
-                const SelFrag<Tc> c = sel_rows(s.C + (16 * row_a + l) * SC + 32 * ks, g);
+                const SelFrag<Tc> c = sel_rows(s.C + 16 * row_a * SC + l_C + 32 * ks, g);
 #pragma unroll
                 for (int m = 0; m < kMine; ++m)
-                    sel_mma(acc[m], sel_rows(s.B + (16 * col_of(m) + l) * SB + 32 * ks, g),
-                            m < 2 ? c : sel_rows(s.C + (16 * row_b + l) * SC + 32 * ks, g));
+                    sel_mma(acc[m], sel_rows(s.B + 16 * col_of(m) * SB + l_B + 32 * ks, g),
+                            m < 2 ? c : sel_rows(s.C + 16 * row_b * SC + l_C + 32 * ks, g));
             }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
@@ -294,7 +290,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
                         const float w = __builtin_ldexpf(acc[m][r] * (to * st.from_step[j0 + r]), whole - st.whole[j0 + r]);
                         v[r] = j0 + r <= i ? w : 0.0f;
                     }
-                    sel_store<Tc, 4>(s.weights[u] + i * SW + j0, v);
+                    sel_store<Tc, 4>(s.weights[u] + 16 * (m < 2 ? row_a : row_b) * SW + l_W + j0, v);
                 }
             }
             __syncthreads();
@@ -314,7 +310,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
                     for (int e = 0; e < 8; ++e) sf[h].set(e, state[h][2 * ks + (e >> 2)][e & 3]);
 #pragma unroll
                 for (int it = 0; it < QT; ++it) {
-                    const SelFrag<Tc> c = sel_rows(s.C + (16 * it + l) * SC + 32 * ks, g);
+                    const SelFrag<Tc> c = sel_rows(s.C + 16 * it * SC + l_C + 32 * ks, g);
                     sel_mma(out[0][it], sf[0], c);
                     sel_mma(out[1][it], sf[1], c);
                 }
@@ -330,7 +326,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
             for (int ks = 0; ks < QK; ++ks)
 #pragma unroll
                 for (int it = 2 * ks; it < QT; ++it) {
-                    const SelFrag<Tc> w = sel_rows(s.weights[mine] + (16 * it + l) * SW + 32 * ks, g);
+                    const SelFrag<Tc> w = sel_rows(s.weights[mine] + 16 * it * SW + l_W + 32 * ks, g);
                     sel_mma(out[0][it], xf[0][ks], w);
                     sel_mma(out[1][it], xf[1][ks], w);
                 }
@@ -368,18 +364,19 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     float own[4];
-                    sel_load<Tc, 4>(xs + (16 * it + l) * SX + p_wave + 16 * h + 4 * g, own);
+                    sel_load<Tc, 4>(xs + 16 * it * SX + l_X + p_wave + 16 * h + 4 * g, own);
 #pragma unroll
                     for (int r = 0; r < 4; ++r) out[h][it][r] = fmaf(D, own[r], out[h][it][r]);
                 }
             const unsigned at = l * row + 4 * g;
             if (VEC && writes && n == Q && cols == 64) {
-                T* const to = y + p_wave;
+                char* const to = reinterpret_cast<char*>(y + p_wave);  // (one place for the wave, and 32 bits from it)
 #pragma unroll
                 for (int it = 0; it < QT; ++it)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        sel_store<T, 4>(to + 16 * (it * row + h) + at, {out[h][it][0], out[h][it][1], out[h][it][2], out[h][it][3]});
+                        sel_store<T, 4>(reinterpret_cast<T*>(to + (at + 16 * it * row) * (unsigned)sizeof(T)) + 16 * h,
+                                        {out[h][it][0], out[h][it][1], out[h][it][2], out[h][it][3]});
             } else if (writes) {
 #pragma unroll
                 for (int it = 0; it < QT; ++it)
@@ -435,7 +432,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
                 float v[8];
 #pragma unroll
                 for (int e = 0; e < 8; ++e) v[e] = xf[h][ks].get(e) * w[e];
-                sel_split<Tc>(v, split[h]);
+                sel_split(v, split[h]);
             }
             constexpr int kSide = 2;  // tiles side by side
 #pragma unroll
@@ -528,7 +525,7 @@ static inline int sel_scan_check(const nhip_scan_args* a) {
     if (chunks > most || chunks * a->n_heads > most || 2 * chunks * a->n_heads * tiles > most) return NHIP_E_BADARG;
     if (a->tokens.n_seqs * tiles * 64 * a->states / 256 * a->n_heads * 2 > most) return NHIP_E_BADARG;
     // (offsets of 32 bits within a chunk)
-    if ((long long)a->n_heads * a->dim >= (1 << 24) || (long long)a->dim * a->states > (1 << 28)) return NHIP_E_BADARG;
+    if ((long long)a->n_heads * a->dim >= (1 << 23) || (long long)a->dim * a->states > (1 << 28)) return NHIP_E_BADARG;
     return 0;
 }
 

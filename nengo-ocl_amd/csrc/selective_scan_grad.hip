@@ -305,7 +305,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                 z += 16 * nt + l < a.states ? both : 0.0f;
                 SelFrag<Tc> f[2][kSplits];
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Sv[m][ks], f[ks]);
+                for (int ks = 0; ks < 2; ++ks) sel_split(Sv[m][ks], f[ks]);
                 // (two tiles of tokens at once: the products of one wait for each other)
 #pragma unroll
                 for (int i2 = 0; i2 < QT; i2 += 2) {
@@ -341,7 +341,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                 }
                 sel_settle(dC[m]);
 #pragma unroll
-                for (int ks = 0; ks < 2; ++ks) sel_split<Tc>(Gv[m][ks], f[ks]);
+                for (int ks = 0; ks < 2; ++ks) sel_split(Gv[m][ks], f[ks]);
 #pragma unroll
                 for (int j2 = 0; j2 < QT; j2 += 2) {
                     sel_phase();
