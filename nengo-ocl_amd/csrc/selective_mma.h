@@ -169,17 +169,18 @@ template <class T, class Tc, int ROWS, int COLS, bool VEC> struct SelStage {
     SelPack<T, V> held[kPacks];
 
     // (formed anew each time: kept over a loop, the places take the registers of what is worked on)
-    static __device__ __forceinline__ int thread() {
-        int tid = threadIdx.x;
+    static __device__ __forceinline__ unsigned thread() {
+        unsigned tid = threadIdx.x;
         asm volatile("" : "+v"(tid));
         return tid;
     }
 
     __device__ __forceinline__ void load(const T* src, long long stride, int n_rows, int n_cols) {
-        const int tid = thread(), row = tid / kRow, col = (tid % kRow) * V;
+        const unsigned tid = thread();
+        const int row = tid / kRow, col = (tid % kRow) * V;
         if constexpr (VEC) {
             const unsigned st = (unsigned)stride * (unsigned)sizeof(T), last = (unsigned)(n_rows - 1) * st;
-            const unsigned r0 = row * st, c = (unsigned)min(col, n_cols - V) * (unsigned)sizeof(T);
+            const unsigned r0 = (unsigned)row * st, c = (unsigned)min(col, n_cols - V) * (unsigned)sizeof(T);
             unsigned at[kPacks];
             if (n_rows == ROWS) {
 #pragma unroll
@@ -201,11 +202,13 @@ template <class T, class Tc, int ROWS, int COLS, bool VEC> struct SelStage {
         }
     }
     template <int STRIDE, bool WHOLE> __device__ __forceinline__ void put(Tc* dst, int n_rows, int n_cols) const {
-        const int tid = thread(), row = tid / kRow, col = (tid % kRow) * V;
+        const unsigned tid = thread();
+        const int row = tid / kRow, col = (tid % kRow) * V;
+        Tc* const first = dst + __mul24(row, STRIDE) + col;
 #pragma unroll
         for (int q = 0; q < kPacks; ++q) {
             const int r = row + q * kRowStep;
-            Tc* out = dst + r * STRIDE + col;
+            Tc* const out = first + q * kRowStep * STRIDE;
             const int there = r < n_rows ? n_cols - col : 0;
             SelPack<Tc, V> v;
 #pragma unroll
@@ -282,17 +285,23 @@ struct SelDt {
         return type == NHIP_F32 ? f32 : type == NHIP_BF16 ? bf16 : f16;
     }
 };
-__device__ __forceinline__ SelDt sel_dt(const nhip_scan_args& a, const SelSeq& seq, int t0, int head) {
+struct SelDtRow {  // where a head's begin, and the bytes from token to token and from half to half
+    const char* p;
+    long long token;
+    int half;
+};
+__device__ __forceinline__ SelDtRow sel_dt_row(const nhip_scan_args& a, const SelSeq& seq, int head) {
+    const int size = a.dt_type == NHIP_F32 ? 4 : 2;
+    const long long first = a.tokens.starts ? seq.row0 * a.dt.token : seq.seq * a.dt.seq;
+    return {static_cast<const char*>(a.dt.p) + (head * a.dt.head + first) * size, a.dt.token * size, size - 2};
+}
+__device__ __forceinline__ SelDt sel_dt(const SelDtRow& row, int t0, int n) {
     int lane = threadIdx.x & (NHIP_WAVE - 1);
     asm volatile("" : "+v"(lane));  // (the address is formed anew each time: kept, it takes two registers)
-    const int t = max(0, min(t0 + lane, seq.n - 1));
-    const long long at = head * a.dt.head + (a.tokens.starts ? (seq.row0 + t) * a.dt.token
-                                                             : seq.seq * a.dt.seq + t * a.dt.token);
-    const int size = a.dt_type == NHIP_F32 ? 4 : 2;
-    const char* p = static_cast<const char*>(a.dt.p) + at * size;
+    const char* p = row.p + max(0, min(t0 + lane, n - 1)) * row.token;
     SelDt d;
     d.lo = *reinterpret_cast<const unsigned short*>(p);
-    d.hi = *reinterpret_cast<const unsigned short*>(p + (size - 2));
+    d.hi = *reinterpret_cast<const unsigned short*>(p + row.half);
     return d;
 }
 

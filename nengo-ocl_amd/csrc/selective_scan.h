@@ -207,10 +207,11 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
     };
     float keeps = 1.0f;
     SelDt dt = {0, 0};
+    const SelDtRow dt_row = sel_dt_row(a, seq, head);
     const int ahead = wave & 1;  // which of two chunks this wave forms the steps of
     if (n_chunks > 0) {
         fetch(min(Q, seq.n - t_first));
-        dt = sel_dt(a, seq, token(min(ahead, n_chunks - 1)), head);
+        dt = sel_dt(dt_row, token(min(ahead, n_chunks - 1)), seq.n);
     }
     for (int k = 0; k < n_chunks; ++k) {
         const int t0 = token(k), n = min(Q, seq.n - t0);
@@ -222,7 +223,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
         if ((k & 1) == 0) {
             if (k + ahead < n_chunks)
                 sel_steps<Q>(s.steps[mine][ahead], dt.value(a.dt_type), seq.n - token(k + ahead), A, bias, a.softplus);
-            dt = sel_dt(a, seq, token(min(k + 2 + ahead, n_chunks - 1)), head);
+            dt = sel_dt(dt_row, token(min(k + 2 + ahead, n_chunks - 1)), seq.n);
         }
         __syncthreads();
         // (unconditional, as the loads are: the last chunk is fetched twice)

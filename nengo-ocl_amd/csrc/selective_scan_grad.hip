@@ -148,7 +148,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
     // (the next tile's inputs are on their way while one is worked on)
     auto fetch = [&](int head, int p_tile) {
         const int cols = min(64, a.dim - p_tile);
-        dt = sel_dt(a, seq, t0, head);
+        dt = sel_dt(sel_dt_row(a, seq, head), t0, seq.n);
         stage_x.load(sel_row<T>(a.x, a.tokens, seq, t0) + head * a.x.head + p_tile, a.x.token, n, cols);
         stage_dy.load(sel_row<T>(a.dy, a.tokens, seq, t0) + head * a.dy.head + p_tile, a.dy.token, n, cols);
     };
