@@ -40,6 +40,7 @@ its chunk of 64 (32 with more than 128 states).
 
 import collections
 import ctypes
+import struct
 
 from . import _lib
 from .hipraggedarray import DeviceArray, _torch
@@ -103,6 +104,29 @@ class _NormArgs(ctypes.Structure):
                 ("workspace_bytes", c_ll)]
 
 
+def _packer(kind):
+    """A function of all fields of a struct in their order, those of structs in it among them, to the struct: where
+    a call takes ten microseconds, to set 20 fields by their names takes four of them."""
+    form, at = "@", 0
+
+    def add(fields, base):
+        nonlocal form, at
+        for name, t in fields._fields_:
+            place = base + getattr(fields, name).offset
+            if issubclass(t, ctypes.Structure):
+                add(t, place)
+            else:
+                form += "%dx" % (place - at) * (place > at) + {c_int: "i", c_ll: "q", c_p: "P", c_float: "f"}[t]
+                at = place + ctypes.sizeof(t)
+
+    add(kind, 0)
+    form = struct.Struct("=" + form[1:].replace("P", "Q") + "%dx" % (ctypes.sizeof(kind) - at))
+    return lambda *values: kind.from_buffer_copy(form.pack(*values))
+
+
+_conv_step_args, _scan_step_args = _packer(_ConvStepArgs), _packer(_ScanStepArgs)
+
+
 # ------------------------------------------------------------------------ argument checks
 _codes = {}
 
@@ -130,13 +154,13 @@ def _array(queue, name, t, shape, dtype, contiguous=False):
     if contiguous:
         if not t.is_contiguous():
             raise ValueError("%s has to be contiguous" % name)
-    elif shape and shape[-1] > 1 and t.stride(-1) != 1:
+    elif not t.is_contiguous() and shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError("%s has stride %d along its last axis, not 1" % (name, t.stride(-1)))
     return t
 
 
 def _parameter(queue, name, t, shape):
-    return None if t is None else _array(queue, name, t, shape, _torch().float32, contiguous=True)
+    return None if t is None else _array(queue, name, t, shape, _torch().float32, True)
 
 
 def _output(queue, name, t, shape, dtype):
@@ -146,8 +170,13 @@ def _output(queue, name, t, shape, dtype):
     return _array(queue, name, t, shape, dtype, contiguous=True)
 
 
+def _like(x):
+    """A new array of the shape and type of `x`, contiguous."""
+    return _torch().empty_like(x) if x.is_contiguous() else x.new_empty(x.shape)
+
+
 def _ptr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _plain(t):
@@ -209,6 +238,16 @@ def _workspace(queue, args, entry):
     return space
 
 
+def _current_stream(device):
+    """The handle of torch's current stream.  (Where torch has the function that gives the handle alone: an object for
+    the stream costs two microseconds, as much as half a launch.)"""
+    torch = _torch()
+    try:
+        return torch._C._cuda_getCurrentRawStream(device)
+    except AttributeError:
+        return torch.cuda.current_stream(device).cuda_stream
+
+
 class _Call:
     """An entry point with its arguments, what they point into, and the arrays that it writes by name."""
 
@@ -226,10 +265,10 @@ class _Call:
 
     def now(self, queue):
         """Enqueued once, in order with torch's current stream: the arrays were made there, and are used there next."""
-        current = _torch().cuda.current_stream(queue.device)
-        if current.cuda_stream == queue.stream.cuda_stream:
+        if _current_stream(queue.device.index) == queue.stream.cuda_stream:
             _lib.check(self.entry(queue.handle, ctypes.byref(self.args)), self.name)
         else:
+            current = _torch().cuda.current_stream(queue.device)
             queue.stream.wait_stream(current)
             _lib.check(self.entry(queue.handle, ctypes.byref(self.args)), self.name)
             current.wait_stream(queue.stream)
@@ -325,12 +364,11 @@ def _causal_conv_step(queue, state, x, weight, bias=None, activation=None, slots
         raise ValueError("a slot of the state has to be contiguous")
     weight, bias = _parameter(queue, "weight", weight, (d, k)), _parameter(queue, "bias", bias, (d,))
     slots = _slots(queue, slots, n, n_slots)
-    y = _output(queue, "y", y, (n, d), x.dtype)
+    y = _like(x) if y is None else _output(queue, "y", y, (n, d), x.dtype)
     if d < 1:
         raise ValueError("x has no channels")
-    args = _ConvStepArgs(type=code, channels=d, width=k, silu=_activation(activation), n=n, n_slots=n_slots,
-                         slots=_ptr(slots), x=_ptr(x), x_stride=x.stride(0), state_stride=state.stride(0),
-                         weight=_ptr(weight), bias=_ptr(bias), state=_ptr(state), y=_ptr(y))
+    args = _conv_step_args(code, d, k, _activation(activation), n, n_slots, _ptr(slots), x.data_ptr(), x.stride(0),
+                           state.stride(0), weight.data_ptr(), _ptr(bias), state.data_ptr(), y.data_ptr())
     return _Call(queue.lib.nhip_causal_conv_step, args, (state, x, weight, bias, slots, y),
                  "hip_causal_conv_step", y=y)
 
@@ -462,16 +500,16 @@ def _selective_step(queue, state, x, dt, A, B, C, D=None, dt_bias=None, softplus
         raise ValueError("dt has shape %s on %s, not %s on %s" % (tuple(dt.shape), dt.device, (n, h), queue.device))
     if A is None:
         raise TypeError("A is None")
-    A, D, dt_bias = (_parameter(queue, name, v, (h,)) for name, v in (("A", A), ("D", D), ("dt_bias", dt_bias)))
+    A = _array(queue, "A", A, (h,), torch.float32, True)
+    D, dt_bias = _parameter(queue, "D", D, (h,)), _parameter(queue, "dt_bias", dt_bias, (h,))
     state = _array(queue, "state", state, (n_slots, h, p, k), torch.float32)
-    if state.stride()[1:] != (p * k, k, 1) and n_slots and not state[0].is_contiguous():
+    if not state.is_contiguous() and n_slots and not state[0].is_contiguous():
         raise ValueError("a slot of the state has to be contiguous")
     slots = _slots(queue, slots, n, n_slots)
-    y = _output(queue, "y", y, (n, h, p), x.dtype)
-    args = _ScanStepArgs(type=code, dt_type=dt_code, softplus=int(bool(softplus)), n_heads=h, dim=p, n_groups=g,
-                         states=k, n=n, n_slots=n_slots, slots=_ptr(slots), x=_rows(x, 1, True), dt=_rows(dt, 1, True),
-                         B=_rows(B, 1, True), C=_rows(C, 1, True), A=_ptr(A), D=_ptr(D), dt_bias=_ptr(dt_bias),
-                         state=_ptr(state), state_stride=state.stride(0), y=_ptr(y))
+    y = _like(x) if y is None else _output(queue, "y", y, (n, h, p), x.dtype)
+    args = _scan_step_args(code, dt_code, bool(softplus), h, p, g, k, n, n_slots, _ptr(slots), *_rows(x, 1, True),
+                           *_rows(dt, 1, True), *_rows(B, 1, True), *_rows(C, 1, True), A.data_ptr(), _ptr(D),
+                           _ptr(dt_bias), state.data_ptr(), state.stride(0), y.data_ptr())
     return _Call(queue.lib.nhip_selective_step, args, (state, x, dt, A, B, C, D, dt_bias, slots, y),
                  "hip_selective_step", y=y)
 
@@ -533,7 +571,7 @@ def _norm(queue, x, weight, gate, residual, scale, groups, eps, after):
 def _block_norm(queue, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6, after=False, out=None,
                 v=None):
     args, x, before, keep = _norm(queue, x, weight, gate, residual, scale, groups, eps, after)
-    out = _output(queue, "out", out, x.shape, x.dtype)
+    out = _like(x) if out is None else _output(queue, "out", out, x.shape, x.dtype)
     if v is not None and not before:
         raise ValueError("v is written with a residual in front of a block only")
     v = _output(queue, "v", v, x.shape, x.dtype) if before else None
