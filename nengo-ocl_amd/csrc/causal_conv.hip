@@ -99,7 +99,7 @@ __global__ __launch_bounds__(NHIP_WG) void conv_kernel(nhip_conv_args a) {
                 for (int k = 0; k < K; ++k) u[i] = fmaf(w[k][i], x[k][i], u[i]);
                 if (a.silu) u[i] *= sel_sigmoid(u[i]);
             }
-            if (q < t1 - t0) sel_store<T, V>(out + (long long)q * a.channels, u);
+            if (q < t1 - t0) sel_store_past<T, V>(out + (long long)q * a.channels, u);
 #pragma unroll
             for (int k = 0; k < K - 1; ++k)
 #pragma unroll

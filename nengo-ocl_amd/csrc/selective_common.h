@@ -31,6 +31,21 @@ __device__ __forceinline__ void sel_store(T* p, const float (&in)[N]) {
     *reinterpret_cast<SelPack<T, N>*>(p) = q;
 }
 
+// The same past the caches, for results of many megabytes: a launch ends when the L2s' written lines are in
+// memory, and these are there already.
+template <class T, int N>
+__device__ __forceinline__ void sel_store_past(T* p, const float (&in)[N]) {
+    typedef unsigned words __attribute__((ext_vector_type(4)));
+    if constexpr (sizeof(T) * N == 16) {
+        SelPack<T, N> q;
+#pragma unroll
+        for (int i = 0; i < N; ++i) q.v[i] = (T)in[i];
+        __builtin_nontemporal_store(__builtin_bit_cast(words, q), reinterpret_cast<words*>(p));
+    } else {
+        sel_store<T, N>(p, in);
+    }
+}
+
 // Calls f(element type) for the type code; false where there is no such type.
 template <class F> static inline bool sel_with_type(int type, F&& f) {
     switch (type) {

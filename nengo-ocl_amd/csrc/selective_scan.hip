@@ -68,7 +68,7 @@ __global__ __launch_bounds__(NHIP_WG) void step_kernel(nhip_scan_step_args a, in
                 v[q][s][i] = fmaf(decay, v[q][s][i], gain * b[s][i]);
                 sum = fmaf(n < a.states ? v[q][s][i] : 0.0f, k[s][i], sum);
             }
-            if (p < a.dim && n < a.states) sel_store<float, V>(row + n, v[q][s]);
+            if (p < a.dim && n < a.states) sel_store_past<float, V>(row + n, v[q][s]);
         }
         for (int d = lpr / 2; d > 0; d /= 2) sum += __shfl_xor(sum, d);
         if (c == 0 && p < a.dim) y[p] = (T)fmaf(D, in[q], sum);
