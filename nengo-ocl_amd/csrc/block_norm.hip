@@ -125,9 +125,9 @@ __global__ __launch_bounds__(NHIP_WG) void norm_kernel(nhip_norm_args a) {
 // scale behind a block): dweight = sum over rows of e n;  dv = inv (e weight - n mean(e weight n)).
 // Each group of lanes keeps its channels over its rows (every gridDim.x-th) and the sums for
 // weight and scale with them; a second launch adds the groups' sums up in their order.  The next row is on its
-// way while one is worked on (8192 rows of 2048, bfloat16, residual: 53 us without).
+// way while one is worked on (8192 rows of 2048, bfloat16, residual: 37 us for 201 MB, 53 without).
 template <class T, int V, int L, int R>
-__global__ __launch_bounds__(NHIP_WG) void norm_grad_kernel(nhip_norm_args a, float* parts) {
+__global__ __launch_bounds__(NHIP_WG, 2) void norm_grad_kernel(nhip_norm_args a, float* parts) {
     __shared__ float s[8];
     __shared__ float both[R > 0 && L == NHIP_WAVE ? 4 * NHIP_WAVE * V : 1];
     constexpr int kWaves = NHIP_WG / L;  // rows side by side
@@ -226,12 +226,14 @@ __global__ __launch_bounds__(NHIP_WG) void norm_grad_kernel(nhip_norm_args a, fl
     const long long row0 = (long long)blockIdx.x * kWaves + mine;
 
     if constexpr (R > 0) {
+        // (more channels to a lane leave no registers for the next row: 4096 rows of 4096, 32 bits, 169 us with it, 59.5 without)
+        constexpr bool kAhead = R * V * sizeof(T) <= 32;
         float w[R][V], k[R][V], dw[R][V], ds[R][V];
         Raw raw[R];
 #pragma unroll
         for (int r = 0; r < R; ++r) {
             params(channel(r), w[r], k[r]);
-            if (a.rows) fetch(raw[r], row0, channel(r));
+            if (kAhead && a.rows) fetch(raw[r], row0, channel(r));
 #pragma unroll
             for (int i = 0; i < V; ++i) dw[r][i] = ds[r][i] = 0.0f;
         }
@@ -239,9 +241,13 @@ __global__ __launch_bounds__(NHIP_WG) void norm_grad_kernel(nhip_norm_args a, fl
             Values u[R];
             float sum = 0.0f, dot = 0.0f;
 #pragma unroll
+            for (int r = 0; r < R; ++r)
+                if (!kAhead) fetch(raw[r], row, channel(r));
+#pragma unroll
             for (int r = 0; r < R; ++r) open(raw[r], k[r], u[r]);
 #pragma unroll
-            for (int r = 0; r < R; ++r) fetch(raw[r], row + step, channel(r));
+            for (int r = 0; r < R; ++r)
+                if (kAhead) fetch(raw[r], row + step, channel(r));
 #pragma unroll
             for (int r = 0; r < R; ++r) sums(channel(r), u[r], w[r], k[r], sum, dot);
             sum = sum_over<L>(sum, s);
@@ -313,8 +319,8 @@ __global__ __launch_bounds__(NHIP_WG) void norm_grad_kernel(nhip_norm_args a, fl
     }
 }
 
-// How a part of `width` channels is held: a wave up to 1024 16-bit channels (512 of 32 bits),
-// a group of four waves up to four times as many, and longer ones are read twice.
+// How a part of `width` channels is held, `per16` of them side by side in a lane (one where rows do not allow
+// wide reads): by a wave up to 128 times as many, by a group of four waves up to 1024 times; longer ones are read twice.
 template <class F> void with_shape(bool vec, int per16, int width, F&& f) {
     const int v = vec ? per16 : 1;
     auto go = [&](auto lanes, auto held) {
@@ -352,13 +358,19 @@ int check(const nhip_norm_args* a) {
     return 0;
 }
 
-// Rows of the table of sums: one per group of waves along the rows.  2048 groups over all parts
-// give each of the 256 compute units eight; a few rows each, or the table costs more than the rows.
-int sum_rows(const nhip_norm_args& a) {
-    long long n = a.rows / 8;
-    const long long most = 2048 / a.groups > 1 ? 2048 / a.groups : 1;
-    if (n > most) n = most;
-    return n < 1 ? 1 : (int)n;
+// Rows of the table of sums: one per group of waves along the rows.  `groups` over all parts; eight rows each
+// at least, or the table costs more than the rows.
+int sum_rows(const nhip_norm_args& a, int groups) {
+    const long long n = a.rows / 8, most = groups / a.groups > 1 ? groups / a.groups : 1;
+    return (int)(n > most ? most : n < 1 ? 1 : n);
+}
+constexpr int kMostGroups = 2048;
+// As many groups as run at once, by the registers that a lane takes, where it takes many (8192 rows of 2048 with a
+// residual: bfloat16, three to a compute unit, 56.7 us with 1024 groups, 48.9 with 768, 48.4 with 512, 60.3 with
+// 256; 32 bits, two to a unit, 44.9 us with 1024, 49.9 with 768, 41.3 with 512), otherwise twice as many, which
+// share the rows more evenly (parts of 256, bfloat16, with a gate: 42.2 us with 1024, 39.4 with 2048).
+template <class T, int V, int R> constexpr int groups_at_once() {
+    return 256 * (V == 1 || R < 2 ? 8 : R == 2 && sizeof(T) == 2 ? 3 : 2);
 }
 
 }  // namespace
@@ -390,7 +402,7 @@ extern "C" int nhip_block_norm(void* stream, const nhip_norm_args* args) {
 extern "C" int nhip_block_norm_grad_workspace(const nhip_norm_args* args, long long* bytes_out) {
     if (int e = check(args)) return e;
     if (!bytes_out) return NHIP_E_BADARG;
-    *bytes_out = (long long)sum_rows(*args) * 2 * args->channels * 4;
+    *bytes_out = (long long)sum_rows(*args, kMostGroups) * 2 * args->channels * 4;
     return 0;
 }
 
@@ -403,7 +415,8 @@ extern "C" int nhip_block_norm_grad(void* stream, const nhip_norm_args* args) {
     if (need > a.workspace_bytes) return NHIP_E_TOOBIG;
     if (!a.workspace) return NHIP_E_BADARG;
     int rc = NHIP_E_BADARG;
-    const int width = a.channels / a.groups, rows = sum_rows(a);
+    const int width = a.channels / a.groups;
+    int rows = 0;
     float* parts = static_cast<float*>(a.workspace);
     hipStream_t st = static_cast<hipStream_t>(stream);
     sel_with_type(a.type, [&](auto t) {
@@ -411,6 +424,7 @@ extern "C" int nhip_block_norm_grad(void* stream, const nhip_norm_args* args) {
         constexpr int V16 = 4;  // (8 bytes of 16-bit types: what a lane holds of eight channels leaves too few waves)
         with_shape(wide(a), V16, width, [&](auto vec, auto lanes, auto held) {
             constexpr int V = decltype(vec)::value ? V16 : 1, L = decltype(lanes)::value, R = decltype(held)::value;
+            rows = sum_rows(a, groups_at_once<T, V, R>());
             NHIP_LAUNCH_FIRST((norm_grad_kernel<T, V, L, R>), dim3((unsigned)rows, (unsigned)a.groups),
                               dim3(NHIP_WG), 0, st, a, parts);
             rc = (int)hipGetLastError();
