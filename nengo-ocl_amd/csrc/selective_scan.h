@@ -109,6 +109,10 @@ template <class Tc, int NP, bool OUTPUTS> struct SelWalkLds {
 // operands but the state come from, was busy for as long as a chunk took.  The inputs of the next chunk
 // are fetched while one is worked on, the steps of two chunks formed at once, by a wave each.  A
 // work-group of the bfloat16 kernel with 128 states takes half of a compute unit's LDS and registers.
+// 8 x 2048 tokens, 32 heads of 64, 128 states, bfloat16: 88 us for 175 MB and 40 GFLOP, 38 for the ends (53 MB in, 25
+// out).  Bound by issue: the matrix cores work for 22 % of the time, the LDS for 39 %, and a chunk takes a wave about
+// a thousand vector instructions beside 152 matrix ones (two thirds of these for the state's three parts).  Chunks of
+// 32 tokens, at which four work-groups fit a unit, took 96 us when these took 95.
 template <class T, class Tc, int NP, int WALK, bool VEC>
 __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1)
 void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
@@ -533,11 +537,12 @@ static inline int sel_scan_check(const nhip_scan_args* a) {
 static inline long long sel_round4(long long floats) { return (floats + 3) & ~3LL; }
 
 // How the sequences are cut, for a workspace that begins with the ends and the keeps.  A compute unit holds two walks
-// of the 16-bit kernel for up to 128 states, one of the others.  Sequences that give every unit a walk stay whole (8 x
-// 2048 tokens, 32 heads of 64, 128 states, both directions: 566 us for the gradient, cut in two 600); fewer are cut into
-// as many segments as walks fit (forward, with half as many walks: 152 us, cut in two 183), down to a chunk each
-// (nine ragged sequences of 4001 tokens, 12 heads, 32 bits: 68 us, with four chunks at least 107).  Up to four segments are
-// added up by the walks themselves (32 x 32 KiB for each would be 100 us of 370; four save a launch of 12 us).
+// of the bfloat16 kernel for up to 128 states, one of the others.  Sequences that give every unit a walk stay whole
+// (gradient of 8 x 2048 tokens, 32 heads of 64, 128 states, both directions: 482 us, cut in two 489); fewer are cut
+// into as many segments as walks fit (8 x 2048 tokens forward: 121 us with 512 walks, 157 with 256), down to a chunk
+// each (nine ragged sequences of 4001 tokens, 12 heads, 32 bits: 64 us, with four chunks 104).  Up to four segments are
+// added up by the walks themselves (the same 8 x 2048 tokens: 114 us, by a launch of its own 133), more by that launch
+// (32768 tokens in 32 segments: 222 us, by the walks 301).
 static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions, float* states) {
     SelWalkPlan p;
     const int q = sel_chunk_tokens(a.states);

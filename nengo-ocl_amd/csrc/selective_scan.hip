@@ -8,7 +8,8 @@ namespace {
 // One token: S <- e^{step A} S + step x (x) B, y = S C + D x.  The state is read and written, 8 bytes
 // per element for 5 operations: memory bound.  Lanes of a wave share the rows of a head's state: LPR
 // (a power of two) to a row, V neighbouring states NS times over; each takes ROWS rows, whose loads are all
-// under way before the first is used, and B and C stay in registers for all of them.
+// under way before the first is used, and B and C stay in registers for all of them.  128 requests, 64 heads of 64,
+// 128 states: 537 MB in 96 us, 5.6 TB/s; one request, 24 heads of 64, 64 states: 4.0 us.
 template <class T, int V, int NS, int ROWS>
 __global__ __launch_bounds__(NHIP_WG) void step_kernel(nhip_scan_step_args a, int lpr) {
     const int side_by_side = NHIP_WG / lpr, per_group = side_by_side * ROWS;
