@@ -339,6 +339,19 @@ def test_scan_gradient(queue, ops, dtype, heads, dim, groups, states):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("lengths", [[230], [700, 3, 0, 420]])
+def test_scan_gradient_over_many_chunks(queue, ops, dtype, lengths):
+    """States and their gradients go through several segments, few and many."""
+    given, starts, m = scan_inputs(24, dtype, lengths, 2, 16, 1, 16, True)
+    dy, dfinal = m.normal(sum(lengths), 2, 16, dtype=dtype), m.normal(len(lengths), 2, 16, 16)
+    got = ops.selective_scan_grad(queue, dy, softplus=True, starts=starts, dfinal=dfinal, **given)
+    want = gradients(lambda **v: scan_definition(softplus=True, starts=starts, **v), given, (dy, dfinal))
+    for k in want:
+        near(getattr(got, k), want[k], k)
+
+
+@pytest.mark.gpu
 def test_scan_gradient_without_the_optional(queue, ops):
     given, _, m = scan_inputs(13, BF16, None, 8, 32, 2, 32, False, dense=(2, 200))
     dy = m.normal(2, 200, 8, 32, dtype=BF16)
