@@ -540,7 +540,7 @@ static inline long long sel_round4(long long floats) { return (floats + 3) & ~3L
 // of the bfloat16 kernel for up to 128 states, one of the others.  Sequences that give every unit a walk stay whole
 // (gradient of 8 x 2048 tokens, 32 heads of 64, 128 states, both directions: 482 us, cut in two 489); fewer are cut
 // into as many segments as walks fit (8 x 2048 tokens forward: 121 us with 512 walks, 157 with 256), down to a chunk
-// each (nine ragged sequences of 4001 tokens, 12 heads, 32 bits: 64 us, with four chunks 104).  Up to four segments are
+// each (4001 tokens in nine ragged sequences, 12 heads, 32 bits: 64 us, with four chunks 104).  Up to four segments are
 // added up by the walks themselves (the same 8 x 2048 tokens: 114 us, by a launch of its own 133), more by that launch
 // (32768 tokens in 32 segments: 222 us, by the walks 301).
 static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions, float* states) {
