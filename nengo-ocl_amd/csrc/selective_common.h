@@ -80,11 +80,14 @@ __device__ __forceinline__ float sel_sigmoid(float v) {
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896341f));
 }
 
-// exp(v): 2^v' with the whole part of v' = v log2(e) set aside, so that its rounding costs nothing
+// exp(v): 2^v' with the whole part of v' = v log2(e) set aside, so that its rounding costs nothing.  v is cut first, far
+// beyond what 32 bits hold (what is no number stays none): the product of a larger one is rounded to more than
+// the 128 that its rest may have, and that of an infinite one has no rest.
 __device__ __forceinline__ float sel_exp(float v) {
+    v = v < -200.0f ? -200.0f : (v > 200.0f ? 200.0f : v);
     const float whole = rintf(v * 1.44269504088896341f);
     const float rest = fmaf(v, 1.925963033500e-8f, fmaf(v, 1.44269502162933349609f, -whole));  // log2(e) in two parts
-    return __builtin_ldexpf(__builtin_amdgcn_exp2f(rest), (int)fmaxf(fminf(whole, 300.0f), -300.0f));
+    return __builtin_ldexpf(__builtin_amdgcn_exp2f(rest), (int)fmaxf(whole, -300.0f));  // (a number in any case)
 }
 
 // max(v, 0) + log(1 + exp(-|v|)), without loss for large negative v: with u = exp(-|v|) and w = 1 + u as
