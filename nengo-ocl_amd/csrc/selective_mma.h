@@ -29,9 +29,10 @@ template <> struct SelFrag<float> {
 };
 
 // How many fragments stand for float32 values without loss: three bfloat16 hold 24 bits between
-// them.  The other operand holds inputs, which are exact.
-template <class Tc> struct SelSplit { static constexpr int n = 1; };
-template <> struct SelSplit<__bf16> { static constexpr int n = 3; };
+// them.  The other operand holds inputs, which are exact.  What leads to a result of 16 bits and to nothing else goes in as
+// `out` parts: two bfloat16 hold 16 bits, off by 2^-16 at most where the result's own rounding is 2^-8.
+template <class Tc> struct SelSplit { static constexpr int n = 1, out = 1; };
+template <> struct SelSplit<__bf16> { static constexpr int n = 3, out = 2; };
 
 // acc += first second over 32 values of k.  32-bit elements: eight products of four k.
 __device__ __forceinline__ void sel_mma(sel_f4& acc, const SelFrag<__bf16>& a, const SelFrag<__bf16>& b) {
@@ -91,28 +92,41 @@ __device__ __forceinline__ SelFrag<float> sel_cols(const float* at, int stride, 
     return f;
 }
 
-// Eight float32 values as fragments that add up to them.  (bfloat16: two values at a time, which is one
-// instruction to round them and one for each to widen it; element by element the compiler rounds each alone)
-__device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<float> (&f)[1]) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) f[0].v[e] = x[e];
-}
-__device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<__bf16> (&f)[3]) {
+// Float32 values as parts that add up to them.  (bfloat16: two values at a time, which is one instruction to
+// round them and one for each to widen it; element by element the compiler rounds each alone)
+template <int N, int P> __device__ __forceinline__ void sel_parts(const float (&x)[N], unsigned (&out)[P][N / 2]) {
     typedef float two __attribute__((ext_vector_type(2)));
     typedef __bf16 two_b __attribute__((ext_vector_type(2)));
-    unsigned out[3][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
+    for (int e = 0; e < N / 2; ++e) {
         two rest = {x[2 * e], x[2 * e + 1]};
 #pragma unroll
-        for (int s = 0; s < 3; ++s) {
+        for (int s = 0; s < P; ++s) {
             out[s][e] = __builtin_bit_cast(unsigned, __builtin_convertvector(rest, two_b));
             rest.x -= __uint_as_float(out[s][e] << 16);
             rest.y -= __uint_as_float(out[s][e] & 0xffff0000u);
         }
     }
+}
+__device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<float> (&f)[1]) {
 #pragma unroll
-    for (int s = 0; s < 3; ++s) f[s].v = __builtin_bit_cast(sel_b8, out[s]);
+    for (int e = 0; e < 8; ++e) f[0].v[e] = x[e];
+}
+template <int P> __device__ __forceinline__ void sel_split(const float (&x)[8], SelFrag<__bf16> (&f)[P]) {
+    unsigned out[P][4];
+    sel_parts(x, out);
+#pragma unroll
+    for (int s = 0; s < P; ++s) f[s].v = __builtin_bit_cast(sel_b8, out[s]);
+}
+// Four of them to LDS, the parts of each at `to` and `rest`
+__device__ __forceinline__ void sel_store_parts(float* to, float*, const float (&x)[4]) {
+    *reinterpret_cast<sel_f4*>(to) = sel_f4{x[0], x[1], x[2], x[3]};
+}
+__device__ __forceinline__ void sel_store_parts(__bf16* to, __bf16* rest, const float (&x)[4]) {
+    unsigned out[2][2];
+    sel_parts(x, out);
+    *reinterpret_cast<uint2*>(to) = uint2{out[0][0], out[0][1]};
+    *reinterpret_cast<uint2*>(rest) = uint2{out[1][0], out[1][1]};
 }
 
 // Whether all elements are finite (magnitudes of 16 bits are compared as whole numbers, two at a time), and

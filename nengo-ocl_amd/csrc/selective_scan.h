@@ -96,8 +96,11 @@ template <class Tc, int NP, bool OUTPUTS> struct SelWalkLds {
                          SW = sel_stride<Tc>(Q);
     alignas(16) Tc x[2][Q * SX];
     alignas(16) Tc B[Q * SB];
-    alignas(16) Tc C[OUTPUTS ? Q * SC : 8];
-    alignas(16) Tc weights[OUTPUTS ? 2 : 1][OUTPUTS ? Q * SW : 8];  // [i][j]: (C_i . B_j) e^{c_i - c_j} step_j
+    // weights [i][j]: (C_i . B_j) e^{c_i - c_j} step_j of each unit; their second parts (bfloat16) take the place of C
+    static constexpr int kParts = SelSplit<Tc>::out, kRest = (kParts - 1) * 2 * Q * SW;
+    alignas(16) Tc C[OUTPUTS ? (Q * SC > kRest ? Q * SC : kRest) : 8];
+    alignas(16) Tc weights[OUTPUTS ? 2 : 1][OUTPUTS ? Q * SW : 8];
+    __device__ __forceinline__ Tc* rest(int unit) { return C + unit * Q * SW; }
     SelSteps<Q> steps[2][2];                                        // [unit][chunk % 2]
 };
 
@@ -109,10 +112,11 @@ template <class Tc, int NP, bool OUTPUTS> struct SelWalkLds {
 // operands but the state come from, was busy for as long as a chunk took.  The inputs of the next chunk
 // are fetched while one is worked on, the steps of two chunks formed at once, by a wave each.  A
 // work-group of the bfloat16 kernel with 128 states takes half of a compute unit's LDS and registers.
-// 8 x 2048 tokens, 32 heads of 64, 128 states, bfloat16: 88 us for 175 MB and 40 GFLOP, 38 for the ends (53 MB in, 25
+// 8 x 2048 tokens, 32 heads of 64, 128 states, bfloat16: 96 us for 175 MB and 40 GFLOP, 38 for the ends (53 MB in, 25
 // out).  Bound by issue: the matrix cores work for 22 % of the time, the LDS for 39 %, and a chunk takes a wave about
-// a thousand vector instructions beside 152 matrix ones (two thirds of these for the state's three parts).  Chunks of
-// 32 tokens, at which four work-groups fit a unit, took 96 us when these took 95.
+// a thousand vector instructions beside 196 matrix ones (half of these for the three parts of what the state gains).  Chunks of
+// 32 tokens, at which four work-groups fit a unit, took 96 us when these took 95.  The state that enters and the
+// weights go in as two parts: as one, the walk took 88 us and y was off by 2^-8 of the terms' magnitudes, not of itself.
 template <class T, class Tc, int NP, int WALK, bool VEC>
 __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1)
 void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
@@ -120,7 +124,7 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
     using Lds = SelWalkLds<Tc, NP, kOut>;
     constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
     constexpr int SX = Lds::SX, SB = Lds::SB, SC = Lds::SC, SW = Lds::SW;
-    constexpr int kSplits = SelSplit<Tc>::n;
+    constexpr int kSplits = SelSplit<Tc>::n, kParts = Lds::kParts;
     extern __shared__ __align__(16) char lds_bytes[];
     Lds& s = *reinterpret_cast<Lds*>(lds_bytes);
 
@@ -181,9 +185,6 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
             }
         }
     }
-    if constexpr (kOut)  // (above the diagonal for good)
-        for (int q = threadIdx.x; q < Q * SW; q += NHIP_WG) s.weights[0][q] = s.weights[1][q] = (Tc)0.0f;
-
     const nhip_rows& x = back ? a.dy : a.x;
     const nhip_rows& B = back ? a.C : a.B;
     const float D = kOut && a.D ? a.D[head] : 0.0f, A = a.A[head], bias = a.dt_bias ? a.dt_bias[head] : 0.0f;
@@ -264,11 +265,13 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
                 for (int ks = 0; ks < QK; ++ks) (void)sel_take_unfinite(xf[h][ks]);
 
         if constexpr (kOut) {
-            // Weights: tiles of the lower triangle of C . B, for both units.  A wave's tiles are in rows
-            // (3: 0, 1, 2), (2: 0, 1, 2), (1: 0, 1; 3: 3), (0: 0): the first two share the rows of C.
+            // Weights: tiles of the lower triangle of C . B, for both units, and those above it that a read of 32 tokens
+            // takes along.  A wave's tiles are in rows (3: 0, 1, 2), (2: 0, 1, 2), (1: 0, 1; 3: 3), (0: 0, 1; 2: 3): the
+            // first two share the rows of C.
             constexpr int kMine = QT == 4 ? 3 : 1;
-            const int row_a = QT == 4 ? 3 - wave : (wave > 0), row_b = QT == 4 && wave == 2 ? 3 : row_a;
-            auto col_of = [&](int m) { return QT == 4 ? (wave == 3 ? 0 : wave == 2 && m == 2 ? 3 : m) : (wave > 1); };
+            const int row_a = QT == 4 ? 3 - wave : (wave == 1 || wave == 2);
+            const int row_b = QT == 4 && wave >= 2 ? 5 - wave : row_a;
+            auto col_of = [&](int m) { return QT == 4 ? (wave >= 2 && m == 2 ? 3 : m) : (wave > 1); };
             sel_f4 acc[kMine];
 #pragma unroll
             for (int m = 0; m < kMine; ++m) acc[m] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -280,14 +283,53 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
                     sel_mma(acc[m], sel_rows(s.B + 16 * col_of(m) * SB + l_B + 32 * ks, g),
                             m < 2 ? c : sel_rows(s.C + 16 * row_b * SC + l_C + 32 * ks, g));
             }
+
+            sel_f4 out[2][QT];
+            auto read_state = [&] {
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int it = 0; it < QT; ++it) out[h][it] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int ks = 0; ks < NK; ++ks) {
+                    if (ks % 2 == 0) sel_phase();
+                    SelFrag<Tc> sf[2][kParts];  // the state that enters, over the states
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        float v[8];
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) v[e] = state[h][2 * ks + (e >> 2)][e & 3];
+                        sel_split(v, sf[h]);
+                    }
+#pragma unroll
+                    for (int it = 0; it < QT; ++it) {
+                        const SelFrag<Tc> c = sel_rows(s.C + 16 * it * SC + l_C + 32 * ks, g);
+#pragma unroll
+                        for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                            for (int h = 0; h < 2; ++h) sel_mma(out[h][it], sf[h][q], c);
+                    }
+                }
+                sel_phase();
+#pragma unroll
+                for (int it = 0; it < QT; ++it) {
+                    const float e = steps.from_start[16 * it + l];
+                    out[0][it] *= e;
+                    out[1][it] *= e;
+                }
+            };
+            if constexpr (kParts > 1) {  // (nobody reads C any more when the second parts are stored)
+                read_state();
+                __syncthreads();
+            }
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 sel_phase();
                 const SelSteps<Q>& st = s.steps[u][k & 1];
 #pragma unroll
                 for (int m = 0; m < kMine; ++m) {
-                    const int i = 16 * (m < 2 ? row_a : row_b) + l, j0 = 16 * col_of(m) + 4 * g;
-                    const int whole = st.whole[i];
+                    const int row = 16 * (m < 2 ? row_a : row_b), i = row + l, j0 = 16 * col_of(m) + 4 * g;
+                    const int whole = st.whole[i], at = row * SW + l_W + j0;
                     const float to = st.to[i];
                     float v[4];
 #pragma unroll
@@ -295,46 +337,21 @@ void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
                         const float w = __builtin_ldexpf(acc[m][r] * (to * st.from_step[j0 + r]), whole - st.whole[j0 + r]);
                         v[r] = j0 + r <= i ? w : 0.0f;
                     }
-                    sel_store<Tc, 4>(s.weights[u] + 16 * (m < 2 ? row_a : row_b) * SW + l_W + j0, v);
+                    sel_store_parts(s.weights[u] + at, s.rest(u) + at, v);
                 }
             }
             __syncthreads();
-
-            sel_f4 out[2][QT];
-#pragma unroll
-            for (int h = 0; h < 2; ++h)
-#pragma unroll
-                for (int it = 0; it < QT; ++it) out[h][it] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int ks = 0; ks < NK; ++ks) {
-                if (ks % 2 == 0) sel_phase();
-                SelFrag<Tc> sf[2];  // the state that enters, over the states
-#pragma unroll
-                for (int h = 0; h < 2; ++h)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) sf[h].set(e, state[h][2 * ks + (e >> 2)][e & 3]);
-#pragma unroll
-                for (int it = 0; it < QT; ++it) {
-                    const SelFrag<Tc> c = sel_rows(s.C + 16 * it * SC + l_C + 32 * ks, g);
-                    sel_mma(out[0][it], sf[0], c);
-                    sel_mma(out[1][it], sf[1], c);
-                }
-            }
-            sel_phase();
-#pragma unroll
-            for (int it = 0; it < QT; ++it) {
-                const float e = steps.from_start[16 * it + l];
-                out[0][it] *= e;
-                out[1][it] *= e;
-            }
+            if constexpr (kParts == 1) read_state();
 #pragma unroll
             for (int ks = 0; ks < QK; ++ks)
 #pragma unroll
-                for (int it = 2 * ks; it < QT; ++it) {
-                    const SelFrag<Tc> w = sel_rows(s.weights[mine] + 16 * it * SW + l_W + 32 * ks, g);
-                    sel_mma(out[0][it], xf[0][ks], w);
-                    sel_mma(out[1][it], xf[1][ks], w);
-                }
+                for (int it = 2 * ks; it < QT; ++it)
+#pragma unroll
+                    for (int q = 0; q < kParts; ++q) {
+                        const SelFrag<Tc> w = sel_rows((q ? s.rest(mine) : s.weights[mine]) + 16 * it * SW + l_W + 32 * ks, g);
+                        sel_mma(out[0][it], xf[0][ks], w);
+                        sel_mma(out[1][it], xf[1][ks], w);
+                    }
             sel_settle(out[0]);
             sel_settle(out[1]);
             if (!finite)
