@@ -35,8 +35,9 @@ template <class Tc, int NP> struct GradLds {
     alignas(16) Tc dy[Q * sel_stride<Tc>(64)];
     alignas(16) Tc B[Q * sel_stride<Tc>(NP)];
     alignas(16) Tc C[Q * sel_stride<Tc>(NP)];
-    alignas(16) Tc xl[Q * sel_stride<Tc>(Q)];  // [j][i]: X_ij L_ij step_j
-    alignas(16) Tc kl[Q * sel_stride<Tc>(Q)];  // [j][i]: K_ij L_ij step_j
+    // [j][i]: X_ij L_ij step_j and K_ij L_ij step_j.  bfloat16: both parts of K's, and when dx has been formed both of X's
+    static constexpr int kParts = SelSplit<Tc>::out;
+    alignas(16) Tc pairs[2][Q * sel_stride<Tc>(Q)];
     SelSteps<Q> steps;
     // Sums of a head.  over[jt][t]: of K X L step over i >= t in t's own tile of 16 and j < t in tile jt;
     // col[it][j]: of K X L over the i > j of tile it;  q, r, z: by wave
@@ -91,7 +92,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
     constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
     constexpr int kTiles = QT * (QT + 1) / 2, kMyTiles = (kTiles + 3) / 4, kMyNT = (NT + 3) / 4;
     constexpr int SX = Lds::SX, SN = Lds::SN, SW = Lds::SW;
-    constexpr int kSplits = SelSplit<Tc>::n;
+    constexpr int kSplits = SelSplit<Tc>::n, kParts = Lds::kParts;
     extern __shared__ __align__(16) char lds_bytes[];
     Lds& s = *reinterpret_cast<Lds*>(lds_bytes);
 
@@ -120,7 +121,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
         stage_B.template store<SN>(s.B, n, a.states);
         stage_C.template store<SN>(s.C, n, a.states);
     }
-    for (int q = tid; q < Q * SW; q += NHIP_WG) s.xl[q] = s.kl[q] = (Tc)0.0f;  // (i < j for good)
+    for (int q = tid; q < Q * SW; q += NHIP_WG) s.pairs[0][q] = s.pairs[1][q] = (Tc)0.0f;  // (i < j for good)
     __syncthreads();
 
     int tile_i[kMyTiles], tile_j[kMyTiles];  // this wave's tiles of the lower triangle
@@ -198,6 +199,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) state_row<VEC>(G, p, 32 * ks, a.dim, a.states, g, Gr[ks]);
 
+            float x_pairs[kMyTiles][4];
 #pragma unroll
             for (int m = 0; m < kMyTiles; ++m) {
                 if (tile_i[m] < 0) continue;
@@ -211,7 +213,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                 const float step = s.steps.step[j];
                 const int whole = s.steps.whole[j];
                 const float from = 1.0f / s.steps.to[j];
-                float kl[4], xl[4], ml[4];
+                float kl[4], ml[4];
+                float(&xl)[4] = x_pairs[m];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = i0 + r;
@@ -244,18 +247,21 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                     const float over = sel_row_sum(i > j ? (ml[r] + (g < 3 ? other : 0.0f)) * step : 0.0f);
                     if (l == 0) s.over[jt][i] += over;
                 }
-                sel_store<Tc, 4>(s.kl + j * SW + i0, kl);
-                sel_store<Tc, 4>(s.xl + j * SW + i0, xl);
+                const int at = j * SW + i0;
+                if constexpr (kParts > 1) {
+                    sel_store_parts(s.pairs[0] + at, s.pairs[1] + at, kl);
+                } else {
+                    sel_store<Tc, 4>(s.pairs[0] + at, xl);
+                    sel_store<Tc, 4>(s.pairs[1] + at, kl);
+                }
             }
             __syncthreads();
 
             // dx: 16 of the dimension to a wave
             if (16 * wave < cols) {
-                SelFrag<Tc> gf[NK];
+                SelFrag<Tc> gf[NK][kParts];
 #pragma unroll
-                for (int ks = 0; ks < NK; ++ks)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) gf[ks].set(e, Gr[ks][e]);
+                for (int ks = 0; ks < NK; ++ks) sel_split(Gr[ks], gf[ks]);
                 SelFrag<Tc> df[QK];
 #pragma unroll
                 for (int ks = 0; ks < QK; ++ks) df[ks] = sel_cols(s.dy + 32 * ks * SX + 16 * wave, SX, l, g);
@@ -264,17 +270,25 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                     sel_phase();
                     sel_f4 acc[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-                    for (int ks = 0; ks < NK; ++ks)
+                    for (int ks = 0; ks < NK; ++ks) {
+                        SelFrag<Tc> b[2];
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            sel_mma(acc[u], gf[ks], sel_rows(s.B + (16 * (j2 + u) + l) * SN + 32 * ks, g));
+                        for (int u = 0; u < 2; ++u) b[u] = sel_rows(s.B + (16 * (j2 + u) + l) * SN + 32 * ks, g);
+#pragma unroll
+                        for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) sel_mma(acc[u], gf[ks][q], b[u]);
+                    }
 #pragma unroll
                     for (int u = 0; u < 2; ++u) acc[u] *= s.steps.to_end_step[16 * (j2 + u) + l];
 #pragma unroll
                     for (int ks = j2 / 2; ks < QK; ++ks)
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            sel_mma(acc[u], df[ks], sel_rows(s.kl + (16 * (j2 + u) + l) * SW + 32 * ks, g));
+                        for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+                                sel_mma(acc[u], df[ks],
+                                        sel_rows(s.pairs[kParts > 1 ? q : 1] + (16 * (j2 + u) + l) * SW + 32 * ks, g));
                     sel_settle(acc);
                     const int c = 16 * wave + 4 * g;
                     T* const row = static_cast<T*>(a.dx) + ((seq.row0 + t0) * a.n_heads + head) * a.dim + p_tile;
@@ -288,6 +302,16 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                         if (j < n) sel_store4<VEC>(row + (unsigned)j * (unsigned)(a.n_heads * a.dim), c, cols, acc[u]);
                     }
                 }
+            }
+
+            if constexpr (kParts > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int m = 0; m < kMyTiles; ++m) {
+                    const int at = (16 * tile_j[m] + l) * SW + 16 * tile_i[m] + 4 * g;
+                    if (tile_i[m] >= 0) sel_store_parts(s.pairs[0] + at, s.pairs[1] + at, x_pairs[m]);
+                }
+                __syncthreads();
             }
 
             // dB, dC: every fourth tile of the states to a wave
@@ -340,8 +364,10 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                     for (int ks = 0; ks <= i2 / 2; ++ks) {
                         const SelFrag<Tc> b = sel_cols(s.B + 32 * ks * SN + 16 * nt, SN, l, g);
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            sel_mma(dC[m][i2 + u], b, sel_cols(s.xl + 32 * ks * SW + 16 * (i2 + u), SW, l, g));
+                        for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+                                sel_mma(dC[m][i2 + u], b, sel_cols(s.pairs[q] + 32 * ks * SW + 16 * (i2 + u), SW, l, g));
                     }
                 }
                 sel_settle(dC[m]);
@@ -375,8 +401,10 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                     for (int ks = j2 / 2; ks < QK; ++ks) {
                         const SelFrag<Tc> c = sel_cols(s.C + 32 * ks * SN + 16 * nt, SN, l, g);
 #pragma unroll
-                        for (int u = 0; u < 2; ++u)
-                            sel_mma(dB[m][j2 + u], c, sel_rows(s.xl + (16 * (j2 + u) + l) * SW + 32 * ks, g));
+                        for (int q = 0; q < kParts; ++q)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u)
+                                sel_mma(dB[m][j2 + u], c, sel_rows(s.pairs[q] + (16 * (j2 + u) + l) * SW + 32 * ks, g));
                     }
                 }
                 sel_settle(dB[m]);

@@ -11,7 +11,7 @@ bfloat16 parts by r r = 2**-16.  Together less than 2**-15 `size`, r of it inclu
 import pytest
 import torch
 
-from test_selective import BF16, F16, ops, scan_definition, scan_inputs, wide  # noqa: F401
+from test_selective import BF16, F16, gradients, ops, scan_definition, scan_inputs, wide  # noqa: F401
 
 ROUNDED = {BF16: 2.0 ** -8, F16: 2.0 ** -11}
 SMALLEST = {BF16: 2.0 ** -134, F16: 2.0 ** -25}
@@ -58,3 +58,20 @@ def test_scan_of_a_large_state_that_the_output_does_not_see(queue, ops, dtype): 
     want, size = scan64(given, starts), scan64(magnitudes(given), starts)
     assert float((size[:5] / want[:5].abs()).median()) > 100.0  # (what the case is for: terms that cancel)
     rounded_once(y, want, size, "y")
+
+
+def gradients64(given, starts, dy, dfinal):
+    return gradients(lambda **v: scan_definition(softplus=True, starts=starts, **v), given, (dy, dfinal))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("lengths, heads, dim, groups, states", CASES)
+def test_gradient_of_the_scan_is_rounded_once(queue, ops, dtype, lengths, heads, dim, groups, states):  # noqa: F811
+    given, starts, m = scan_inputs(53, dtype, lengths, heads, dim, groups, states, True)
+    dy, dfinal = m.normal(sum(lengths), heads, dim, dtype=dtype), m.normal(len(lengths), heads, dim, states)
+    got = ops.selective_scan_grad(queue, dy, softplus=True, starts=starts, dfinal=dfinal, **given)
+    want = gradients64(given, starts, dy, dfinal)
+    size = gradients64(magnitudes(given), starts, dy.abs(), dfinal.abs())
+    for k in ("x", "B", "C"):
+        rounded_once(getattr(got, k), want[k], size[k], k)
