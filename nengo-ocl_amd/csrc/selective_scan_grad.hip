@@ -488,16 +488,25 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
     }
 }
 
-// dB and dC from the blocks of heads, in their order
+// dB and dC from the blocks of heads, in their order: a chunk's rows by `pieces` work-groups.  (By chunk, so that tokens
+// of no sequence are left as they are: no block has anything of them.)
 template <class T>
-__global__ __launch_bounds__(NHIP_WG) void add_blocks_kernel(const float* shared, int blocks, long long n, T* dB, T* dC) {
-    const long long i = (long long)blockIdx.x * NHIP_WG + threadIdx.x;
-    if (i >= 2 * n) return;
-    float sum = 0.0f;
+__global__ __launch_bounds__(NHIP_WG) void add_blocks_kernel(nhip_scan_args a, const float* shared, int blocks, int pieces,
+                                                             int q) {
+    const int piece = blockIdx.x % pieces;
+    const SelSeq seq = sel_seq_of_chunk(a.tokens, blockIdx.x / pieces, q);
+    const int t0 = seq.chunk * q, n = seq.seq < 0 ? 0 : min(q, seq.n - t0);
+    const long long row = (long long)a.n_groups * a.states, all = a.tokens.n_tokens * row;
+    const long long first = (seq.row0 + t0) * row, count = n * row;
+    for (long long e = (long long)piece * NHIP_WG + threadIdx.x; e < 2 * count; e += (long long)pieces * NHIP_WG) {
+        const bool of_C = e >= count;
+        const long long i = first + (of_C ? e - count : e);
+        const float* const from = shared + (of_C ? all : 0) + i;
+        float sum = 0.0f;
 #pragma unroll 8
-    for (int b = 0; b < blocks; ++b) sum += shared[(long long)b * 2 * n + i];
-    if (i < n) dB[i] = (T)sum;
-    else dC[i - n] = (T)sum;
+        for (int b = 0; b < blocks; ++b) sum += from[(long long)b * 2 * all];
+        static_cast<T*>(of_C ? a.dC : a.dB)[i] = (T)sum;
+    }
 }
 
 struct Layout {
@@ -571,13 +580,12 @@ extern "C" int nhip_selective_scan_grad(void* stream, const nhip_scan_args* args
                 rc = (int)hipGetLastError();
             });
             if (!rc && m.blocks > 1) {
-                const long long n = a.tokens.n_tokens * a.n_groups * a.states;
-                if (n) {
-                    hipLaunchKernelGGL(add_blocks_kernel<T>, dim3((unsigned)((2 * n + NHIP_WG - 1) / NHIP_WG)),
-                                       dim3(NHIP_WG), 0, st, shared, m.blocks, n, static_cast<T*>(a.dB),
-                                       static_cast<T*>(a.dC));
-                    rc = (int)hipGetLastError();
-                }
+                // (there are fewer than 512 chunks and groups, so this is a small grid)
+                const int q = sel_chunk_tokens(a.states);
+                const int pieces = (int)((2LL * q * a.n_groups * a.states + NHIP_WG - 1) / NHIP_WG);
+                hipLaunchKernelGGL(add_blocks_kernel<T>, dim3((unsigned)(m.n_chunks * pieces)), dim3(NHIP_WG), 0, st, a,
+                                   shared, m.blocks, pieces, q);
+                rc = (int)hipGetLastError();
             }
         });
     }

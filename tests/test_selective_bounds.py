@@ -1,0 +1,89 @@
+"""Tokens that no sequence holds, calls without any sequence, calls of more work than a launch takes, queues and streams of two
+devices: what is left as it was, what does nothing, and what is refused.  Definitions and tolerances are those of
+test_selective.py.
+"""
+
+import pytest
+import torch
+
+from test_selective import (BF16, F32, conv_definition, conv_inputs, gradients, near, ops, scan_definition,  # noqa: F401
+                            scan_inputs, wide)
+
+LEFT = 7.0  # what outputs hold before the call
+
+
+def spread(plan, *outputs):
+    """Outputs filled, the workspace without a number in it; then the plan runs."""
+    for v in outputs:
+        v.fill_(LEFT)
+    for v in plan.full_args[0].keep:
+        if isinstance(v, torch.Tensor) and v.dtype == torch.uint8:
+            v.fill_(255)
+    torch.cuda.synchronize()
+    plan()
+    plan.queue.finish()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("heads, groups, lengths", [
+    (4, 1, [5, 70, 0, 64]),  # the heads of a group in blocks, whose sums are added up by a launch of their own
+    (4, 4, [5, 70, 0, 64]),  # one work-group to a group
+    (6, 2, [900])])          # several segments
+def test_scan_leaves_tokens_of_no_sequence(queue, ops, dtype, heads, groups, lengths):  # noqa: F811
+    front, back = 37, 90
+    n = sum(lengths)
+    padded, _, m = scan_inputs(61, dtype, [front + n + back], heads, 16, groups, 16, False)
+    padded.pop("initial")
+    starts = torch.tensor([front] + lengths, dtype=torch.int32).cumsum(0).int().cuda()
+    held = slice(front, front + n)
+    given = {k: v[held] if k in ("x", "dt", "B", "C") else v for k, v in padded.items()}
+    at = (starts - front).cpu()
+
+    def function(**v):
+        return scan_definition(softplus=True, initial=None, starts=at, **v)
+
+    plan = ops.plan_selective_scan(queue, softplus=True, starts=starts, **padded)
+    spread(plan, plan.y)
+    near(plan.y[held], function(**dict(zip(given, wide(*given.values()))))[0], "y")
+    assert (plan.y[:front] == LEFT).all() and (plan.y[front + n:] == LEFT).all()
+
+    dy = m.normal(*padded["x"].shape, dtype=dtype)
+    plan = ops.plan_selective_scan_grad(queue, dy, softplus=True, starts=starts, **padded)
+    got = plan.gradients
+    rows = ("x", "dt", "B", "C")
+    spread(plan, *(getattr(got, k) for k in rows))
+    want = gradients(function, given, (dy[held], None))
+    for k in want:
+        v = getattr(got, k)
+        near(v[held] if k in rows else v, want[k], k)
+    for k in rows:
+        assert (getattr(got, k)[:front] == LEFT).all() and (getattr(got, k)[front + n:] == LEFT).all(), k
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, channels", [(F32, 20), (BF16, 64)])
+def test_convolution_leaves_tokens_of_no_sequence(queue, ops, dtype, channels):  # noqa: F811
+    front, lengths, back = 20, [3, 0, 130], 70
+    n = sum(lengths)
+    padded, _, m = conv_inputs(62, dtype, [front + n + back], channels, 4, False)
+    padded.pop("initial")
+    starts = torch.tensor([front] + lengths, dtype=torch.int32).cumsum(0).int().cuda()
+    held = slice(front, front + n)
+    given = dict(padded, x=padded["x"][held])
+
+    def function(**v):
+        return conv_definition(silu_=True, initial=None, starts=(starts - front).cpu(), **v)
+
+    plan = ops.plan_causal_conv(queue, activation="silu", starts=starts, **padded)
+    spread(plan, plan.y)
+    near(plan.y[held], function(**dict(zip(given, wide(*given.values()))))[0], "y")
+    dy = m.normal(front + n + back, channels, dtype=dtype)
+    grad = ops.plan_causal_conv_grad(queue, dy, activation="silu", starts=starts, **padded)
+    spread(grad, grad.gradients.x)
+    want = gradients(function, given, (dy[held], None))
+    near(grad.gradients.x[held], want["x"], "x")
+    near(grad.gradients.weight, want["weight"], "weight")
+    near(grad.gradients.bias, want["bias"], "bias")
+    for v in (plan.y, grad.gradients.x):
+        assert (v[:front] == LEFT).all() and (v[front + n:] == LEFT).all()
