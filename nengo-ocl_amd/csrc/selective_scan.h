@@ -642,7 +642,7 @@ template <int WALK> static inline int sel_walk_launch(hipStream_t stream, const 
 // WALK over all sequences, after a launch for the segments' ends where they are cut; `last`: nothing
 // follows in this entry point.
 template <int WALK> static inline int sel_walk(hipStream_t stream, const nhip_scan_args& a, const SelWalkPlan& plan, bool last) {
-    if (plan.n_segments == 0) return 0;
+    if (plan.n_segments == 0 || a.tokens.n_seqs == 0) return 0;  // (tokens of no sequence have segments, too)
     if (plan.ends) {
         if (int e = sel_walk_launch<kSelEnds>(stream, a, plan, true, false)) return e;
     }

@@ -87,3 +87,30 @@ def test_convolution_leaves_tokens_of_no_sequence(queue, ops, dtype, channels): 
     near(grad.gradients.bias, want["bias"], "bias")
     for v in (plan.y, grad.gradients.x):
         assert (v[:front] == LEFT).all() and (v[front + n:] == LEFT).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("tokens", [0, 100, 3000])
+def test_calls_without_sequences(queue, ops, dtype, tokens):  # noqa: F811
+    """One offset, no sequence, any number of tokens: nothing is written, the parameters' gradients are zero."""
+    starts = torch.zeros(1, dtype=torch.int32, device="cuda")
+    given, _, m = scan_inputs(63, dtype, [tokens], 4, 16, 2, 16, False)
+    given.pop("initial")
+    plan = ops.plan_selective_scan(queue, softplus=True, starts=starts, **given)
+    grad = ops.plan_selective_scan_grad(queue, given["x"], softplus=True, starts=starts, **given)
+    got = grad.gradients
+    rows = [plan.y] + [getattr(got, k) for k in ("x", "dt", "B", "C")]
+    spread(plan, *rows)
+    spread(grad, got.A, got.D, got.dt_bias)
+    assert plan.final.shape == (0, 4, 16, 16)
+    assert all((v == LEFT).all() for v in rows)
+    assert not got.A.any() and not got.D.any() and not got.dt_bias.any()
+    given, _, _ = conv_inputs(64, dtype, [tokens], 24, 4, False)
+    given.pop("initial")
+    plan = ops.plan_causal_conv(queue, starts=starts, **given)
+    grad = ops.plan_causal_conv_grad(queue, given["x"], starts=starts, **given)
+    spread(plan, plan.y)
+    spread(grad, *grad.gradients[:3])
+    assert (plan.y == LEFT).all() and (grad.gradients.x == LEFT).all()
+    assert not grad.gradients.weight.any() and not grad.gradients.bias.any()
