@@ -859,7 +859,9 @@ int nhip_rtc_launch_direct(void *stream, void *function, int n, const int *t_sta
 
 /* ---- blocks that filter selectively ------------------------------------------
  * The arguments are described in nengo_hip_selective.h.  Sizes: width 1 ... 8; states 1 ...
- * 256; any others from 1 (tokens, sequences and requests from 0).  The `*_workspace` functions give
+ * 256; any others from 1 (tokens, sequences and requests from 0).  What would take a launch of 2^24
+ * work-groups (of 64 tokens of a channel block, a segment and two heads, 256 lanes of a step) is
+ * refused before any launch with NHIP_E_BADARG.  The `*_workspace` functions give
  * the bytes of workspace that a call with these arguments needs (a smaller one is refused
  * with NHIP_E_TOOBIG); its contents need not be kept between calls. */
 int nhip_causal_conv(void *stream, const nhip_conv_args *args);

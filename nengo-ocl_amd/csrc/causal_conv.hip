@@ -315,7 +315,7 @@ int check(const nhip_conv_args* a) {
     if (!a || !a->weight || a->channels <= 0 || a->width < 1 || a->width > kMaxWidth) return NHIP_E_BADARG;
     if (a->type < NHIP_F32 || a->type > NHIP_F16 || !sel_tokens_ok(a->tokens)) return NHIP_E_BADARG;
     if (a->tokens.n_tokens && !a->x.p) return NHIP_E_BADARG;
-    if (sel_max_chunks(a->tokens, kChunk) > 0x7fffffffLL || a->channels > SEL_MAX_GRID_Y * NHIP_WAVE)
+    if (sel_max_chunks(a->tokens, kChunk) > SEL_MAX_GROUPS || a->channels > SEL_MAX_GRID_Y * NHIP_WAVE)
         return NHIP_E_BADARG;
     return 0;
 }
@@ -400,15 +400,17 @@ extern "C" int nhip_causal_conv_step(void* stream, const nhip_conv_step_args* ar
     if (a.type < NHIP_F32 || a.type > NHIP_F16) return NHIP_E_BADARG;
     if (a.n == 0) return 0;
     if (!a.x || !a.y || (!a.state && a.width > 1)) return NHIP_E_BADARG;
+    const bool w = wide(a.type, a.channels, {a.x, a.state, a.y}, {a.x_stride, a.state_stride});
+    const long long lanes = (long long)a.n * (w ? a.channels / (16 / sel_size(a.type)) : a.channels);
+    const long long groups = (lanes + NHIP_WG - 1) / NHIP_WG;
+    if (groups > SEL_MAX_GROUPS) return NHIP_E_BADARG;
     int rc = NHIP_E_BADARG;
     sel_with_type(a.type, [&](auto t) {
         using T = decltype(t);
         with_width(a.width, [&](auto k) {
             constexpr int K = decltype(k)::value, V = 16 / sizeof(T);
             hipStream_t st = static_cast<hipStream_t>(stream);
-            const bool w = wide(a.type, a.channels, {a.x, a.state, a.y}, {a.x_stride, a.state_stride});
-            const long long lanes = (long long)a.n * (w ? a.channels / V : a.channels);
-            const dim3 g((unsigned)((lanes + NHIP_WG - 1) / NHIP_WG));
+            const dim3 g((unsigned)groups);
             if (w) NHIP_LAUNCH((conv_step_kernel<T, V, K>), g, dim3(NHIP_WG), 0, st, a);
             else NHIP_LAUNCH((conv_step_kernel<T, 1, K>), g, dim3(NHIP_WG), 0, st, a);
             rc = (int)hipGetLastError();

@@ -9,6 +9,7 @@
 typedef float sel_f4 __attribute__((ext_vector_type(4)));
 
 #define SEL_MAX_GRID_Y 65535
+#define SEL_MAX_GROUPS ((1LL << 32) / NHIP_WG - 1)  // work-groups along x: an axis has fewer than 2^32 threads
 #define SEL_MAX_TOKENS 0x7fff0000LL  // (room for a chunk behind the last token in 32 bits)
 
 // ------------------------------------------------------------------------------ element types

@@ -545,7 +545,6 @@ static inline int sel_scan_check(const nhip_scan_args* a) {
     // (work-groups: at most one per chunk, head and tile of the dimension in each direction)
     const long long most = 0x7fffffffLL, chunks = sel_max_chunks(a->tokens, 32), tiles = (a->dim + 63) / 64;
     if (chunks > most || chunks * a->n_heads > most || 2 * chunks * a->n_heads * tiles > most) return NHIP_E_BADARG;
-    if (a->tokens.n_seqs * tiles * 64 * a->states / 256 * a->n_heads * 2 > most) return NHIP_E_BADARG;
     // (offsets of 32 bits within a chunk)
     if ((long long)a->n_heads * a->dim >= (1 << 23) || (long long)a->dim * a->states > (1 << 28)) return NHIP_E_BADARG;
     return 0;
@@ -592,6 +591,20 @@ static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions,
     return p;
 }
 
+// Work-groups, for V elements of a state to a lane, of the launch that turns segments' ends into beginnings
+static inline long long sel_begin_groups(const nhip_scan_args& a, const SelWalkPlan& p, int v) {
+    const long long per = NHIP_WG * v, blocks = ((long long)a.dim * a.states + per - 1) / per;
+    return blocks * a.n_heads * a.tokens.n_seqs * p.directions;
+}
+static inline long long sel_walk_groups(const nhip_scan_args& a, const SelWalkPlan& p) {
+    return (long long)p.directions * p.n_segments * a.n_groups * p.pairs;
+}
+// Whether the launches of a walk are ones
+static inline bool sel_walk_fits(const nhip_scan_args& a, const SelWalkPlan& p) {
+    return sel_walk_groups(a, p) <= SEL_MAX_GROUPS &&
+           (!p.ends || p.few || sel_begin_groups(a, p, p.vec ? 4 : 1) <= SEL_MAX_GROUPS);
+}
+
 // Floats of workspace that the cut needs (a multiple of 4), and its place
 static inline long long sel_walk_space(const nhip_scan_args& a, const SelWalkPlan& p) {
     if (!p.ends) return 0;
@@ -618,7 +631,7 @@ template <> struct SelCompute<__bf16> { using type = __bf16; };
 
 template <int WALK> static inline int sel_walk_launch(hipStream_t stream, const nhip_scan_args& a, const SelWalkPlan& plan,
                                                       bool first, bool last) {
-    const unsigned grid = (unsigned)(plan.directions * plan.n_segments * a.n_groups * plan.pairs);
+    const unsigned grid = (unsigned)sel_walk_groups(a, plan);
     int rc = NHIP_E_BADARG;
     sel_with_type(a.type, [&](auto t) {
         using T = decltype(t);
@@ -647,9 +660,8 @@ template <int WALK> static inline int sel_walk(hipStream_t stream, const nhip_sc
         if (int e = sel_walk_launch<kSelEnds>(stream, a, plan, true, false)) return e;
     }
     if (plan.ends && !plan.few) {
-        const int v = plan.vec ? 4 : 1, per = NHIP_WG * v, q = sel_chunk_tokens(a.states);
-        const long long blocks = ((long long)a.dim * a.states + per - 1) / per;
-        const dim3 grid((unsigned)(blocks * a.n_heads * a.tokens.n_seqs * plan.directions));
+        const int q = sel_chunk_tokens(a.states);
+        const dim3 grid((unsigned)sel_begin_groups(a, plan, plan.vec ? 4 : 1));
         if (plan.vec) hipLaunchKernelGGL(sel_begin_kernel<4>, grid, dim3(NHIP_WG), 0, stream, a, plan, q);
         else hipLaunchKernelGGL(sel_begin_kernel<1>, grid, dim3(NHIP_WG), 0, stream, a, plan, q);
         NHIP_LAUNCH_CHECK();

@@ -81,7 +81,9 @@ __global__ __launch_bounds__(NHIP_WG) void step_kernel(nhip_scan_step_args a, in
 extern "C" int nhip_selective_scan_workspace(const nhip_scan_args* args, long long* bytes_out) {
     if (int e = sel_scan_check(args)) return e;
     if (!bytes_out) return NHIP_E_BADARG;
-    *bytes_out = 4 * sel_walk_space(*args, sel_walk_plan(*args, 1, nullptr));
+    const SelWalkPlan plan = sel_walk_plan(*args, 1, nullptr);
+    if (!sel_walk_fits(*args, plan)) return NHIP_E_BADARG;
+    *bytes_out = 4 * sel_walk_space(*args, plan);
     return 0;
 }
 
@@ -90,6 +92,7 @@ extern "C" int nhip_selective_scan(void* stream, const nhip_scan_args* args) {
     const nhip_scan_args& a = *args;
     if (a.tokens.n_tokens && !a.y) return NHIP_E_BADARG;
     SelWalkPlan plan = sel_walk_plan(a, 1, nullptr);
+    if (!sel_walk_fits(a, plan)) return NHIP_E_BADARG;
     const long long need = 4 * sel_walk_space(a, plan);
     if (need > a.workspace_bytes) return NHIP_E_TOOBIG;
     if (need && (!a.workspace || !sel_aligned(a.workspace, 16))) return NHIP_E_BADARG;
@@ -114,7 +117,7 @@ extern "C" int nhip_selective_step(void* stream, const nhip_scan_step_args* args
     const bool many = (long long)a.n * a.n_heads * ((a.dim + 8 * side_by_side - 1) / (8 * side_by_side)) >= 1024;
     const int rows = side_by_side * (many ? 8 : 1);
     const long long groups = (long long)a.n * a.n_heads * ((a.dim + rows - 1) / rows);
-    if (groups > 0x7fffffffLL || (long long)a.dim * a.states > 0x7fffffffLL) return NHIP_E_BADARG;
+    if (groups > SEL_MAX_GROUPS || (long long)a.dim * a.states > 0x7fffffffLL) return NHIP_E_BADARG;
     int rc = NHIP_E_BADARG;
     sel_with_type(a.type, [&](auto t) {
         using T = decltype(t);

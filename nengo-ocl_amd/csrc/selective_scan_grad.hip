@@ -539,6 +539,7 @@ extern "C" int nhip_selective_scan_grad_workspace(const nhip_scan_args* args, lo
     if (int e = sel_scan_check(args)) return e;
     if (!bytes_out) return NHIP_E_BADARG;
     const Layout m = layout(*args);
+    if (!sel_walk_fits(*args, m.walk) || m.n_chunks * args->n_groups * m.blocks > SEL_MAX_GROUPS) return NHIP_E_BADARG;
     *bytes_out = 4 * (sel_round4(2 * m.states) + m.walk_space + sel_round4(m.parts) + m.shared);
     return 0;
 }
@@ -553,7 +554,6 @@ extern "C" int nhip_selective_scan_grad(void* stream, const nhip_scan_args* args
     if (need && (!a.workspace || !sel_aligned(a.workspace, 16))) return NHIP_E_BADARG;
     Layout m = layout(a);
     const long long groups = m.n_chunks * a.n_groups * m.blocks;
-    if (groups > 0x7fffffffLL) return NHIP_E_BADARG;
     hipStream_t st = static_cast<hipStream_t>(stream);
     m.walk.states = static_cast<float*>(a.workspace);
     float* space = m.walk.states + sel_round4(2 * m.states);

@@ -114,3 +114,50 @@ def test_calls_without_sequences(queue, ops, dtype, tokens):  # noqa: F811
     spread(grad, *grad.gradients[:3])
     assert (plan.y == LEFT).all() and (grad.gradients.x == LEFT).all()
     assert not grad.gradients.weight.any() and not grad.gradients.bias.any()
+
+
+def test_more_work_than_a_launch_takes_is_refused_before_any(ops):  # noqa: F811
+    """2**24 work-groups of 256 threads are one more than an axis of a grid has; a workspace is told up to there."""
+    import ctypes
+
+    from nengo_ocl_amd import _lib
+
+    lib, bad, ref, need, one = _lib.lib(), -1, ctypes.byref, ctypes.c_longlong(), 1 << 20
+
+    def told(entry, args):
+        return entry(ref(args), ref(need))
+
+    conv = ops._ConvArgs(channels=1, width=2, weight=one, y=one, dx=one, dweight=one, dbias=one, workspace=one,
+                         workspace_bytes=1 << 60)
+    conv.x.p = conv.dy.p = one
+    conv.tokens.n_seqs = 1
+    conv.tokens.length = conv.tokens.n_tokens = 2 ** 30 - 64
+    assert told(lib.nhip_causal_conv_grad_workspace, conv) == 0
+    conv.tokens.length = conv.tokens.n_tokens = 2 ** 30
+    assert told(lib.nhip_causal_conv_grad_workspace, conv) == bad
+    assert lib.nhip_causal_conv(None, ref(conv)) == bad and lib.nhip_causal_conv_grad(None, ref(conv)) == bad
+
+    scan = ops._ScanArgs(n_heads=1, dim=1, n_groups=1, states=1, A=one, y=one, dx=one, ddt=one, dB=one, dC=one, dA=one,
+                         dD=one, ddt_bias=one, workspace=one, workspace_bytes=1 << 60)
+    scan.x.p = scan.dt.p = scan.B.p = scan.C.p = scan.dy.p = one
+    for seqs, forward, gradient in ((2 ** 23 - 1, 0, 0), (2 ** 23, 0, bad), (2 ** 24 - 1, 0, bad), (2 ** 24, bad, bad)):
+        scan.tokens.n_seqs, scan.tokens.length, scan.tokens.n_tokens = seqs, 1, seqs
+        assert told(lib.nhip_selective_scan_workspace, scan) == forward
+        assert told(lib.nhip_selective_scan_grad_workspace, scan) == gradient
+    assert lib.nhip_selective_scan(None, ref(scan)) == bad and lib.nhip_selective_scan_grad(None, ref(scan)) == bad
+    # sequences back to back, cut into segments: a lane to four elements of each one's state
+    scan.n_heads, scan.dim, scan.states, scan.tokens.starts = 8, 64, 128, one
+    scan.tokens.length, scan.tokens.n_tokens = 0, 2 ** 26
+    for seqs, code in ((2 ** 18 - 1, 0), (2 ** 18, bad)):
+        scan.tokens.n_seqs = seqs
+        assert told(lib.nhip_selective_scan_workspace, scan) == code
+    assert lib.nhip_selective_scan(None, ref(scan)) == bad
+
+    step = ops._ScanStepArgs(n_heads=1, dim=1, n_groups=1, states=1, n=2 ** 24, n_slots=2 ** 24, A=one, state=one, y=one)
+    step.x.p = step.dt.p = step.B.p = step.C.p = one
+    assert lib.nhip_selective_step(None, ref(step)) == bad
+    step = ops._ConvStepArgs(channels=256, width=1, n=2 ** 24, n_slots=2 ** 24, x=one, x_stride=257, weight=one, y=one)
+    assert lib.nhip_causal_conv_step(None, ref(step)) == bad
+    norm = ops._NormArgs(channels=2 ** 27, groups=1, rows=1, weight=one, x=one, dout=one, dx=one, dweight=one,
+                         workspace=one, workspace_bytes=1 << 60)
+    assert lib.nhip_block_norm_grad(None, ref(norm)) == bad
