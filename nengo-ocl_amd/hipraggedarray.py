@@ -36,12 +36,14 @@ def _torch():
 
 
 class Queue:
-    """An in-order HIP stream on one device (default priority): a new one, or a torch stream of the caller's (a
-    program whose torch operations and plans take turns saves the waits between two streams)."""
+    """An in-order HIP stream on one device (default priority): a new one, or a torch stream of the caller's on
+    that device (a program whose torch operations and plans take turns saves the waits between two streams)."""
 
     def __init__(self, device=0, stream=None):
         torch = _torch()
         self.device = torch.device("cuda", device)
+        if stream is not None and stream.device != self.device:
+            raise ValueError("the stream is on %s, the queue on %s" % (stream.device, self.device))
         self.stream = torch.cuda.Stream(device=self.device) if stream is None else stream
         self.handle = ctypes.c_void_p(self.stream.cuda_stream)
         self.lib = _lib.lib()

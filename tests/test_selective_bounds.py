@@ -161,3 +161,14 @@ def test_more_work_than_a_launch_takes_is_refused_before_any(ops):  # noqa: F811
     norm = ops._NormArgs(channels=2 ** 27, groups=1, rows=1, weight=one, x=one, dout=one, dx=one, dweight=one,
                          workspace=one, workspace_bytes=1 << 60)
     assert lib.nhip_block_norm_grad(None, ref(norm)) == bad
+
+
+def test_a_queue_takes_no_stream_of_another_device(monkeypatch):
+    import types
+
+    from nengo_ocl_amd import hipraggedarray
+
+    monkeypatch.setattr(hipraggedarray, "_TORCH", torch)
+    other = types.SimpleNamespace(device=torch.device("cuda", 1), cuda_stream=0)
+    with pytest.raises(ValueError, match="cuda:1"):
+        hipraggedarray.Queue(0, stream=other)
