@@ -574,7 +574,7 @@ extern "C" int nhip_selective_scan_grad(void* stream, const nhip_scan_args* args
                 auto kernel = !m.walk.vec       ? grad_kernel<T, Tc, NP, false, false>
                               : a.dim % 64 == 0 ? grad_kernel<T, Tc, NP, true, true>
                                                 : grad_kernel<T, Tc, NP, true, false>;
-                rc = sel_allow_lds(kernel, lds);
+                rc = sel_allow_lds(st, kernel, lds);
                 if (rc) return;
                 hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(NHIP_WG), lds, st, a, plan);
                 rc = (int)hipGetLastError();

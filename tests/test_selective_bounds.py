@@ -172,3 +172,52 @@ def test_a_queue_takes_no_stream_of_another_device(monkeypatch):
     other = types.SimpleNamespace(device=torch.device("cuda", 1), cuda_stream=0)
     with pytest.raises(ValueError, match="cuda:1"):
         hipraggedarray.Queue(0, stream=other)
+
+
+@pytest.mark.gpu
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two devices")
+def test_scan_on_a_device_that_is_not_the_current_one(ops):  # noqa: F811
+    """Its launches take more LDS than a kernel has without being asked for, on the queue's device."""
+    from nengo_ocl_amd.hipraggedarray import Queue
+
+    given, starts, m = scan_inputs(65, BF16, [70, 200], 2, 64, 1, 128, False)
+    given.pop("initial")
+    there = {k: v.to("cuda:1") for k, v in dict(given, starts=starts).items()}
+    queue = Queue(1)
+    assert torch.cuda.current_device() == 0
+    y, _ = ops.selective_scan(queue, softplus=True, **there)
+    got = ops.selective_scan_grad(queue, there["x"], softplus=True, **there)
+    assert torch.cuda.current_device() == 0
+    want, _ = ops.selective_scan(Queue(0), softplus=True, starts=starts, **given)
+    assert torch.equal(y.cpu(), want.cpu()) and torch.isfinite(got.A).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_recorded_scans(queue, ops, dtype):  # noqa: F811
+    """A scan, its gradient and a convolution's as a list of plans, recorded once and replayed."""
+    from nengo_ocl_amd.plan import Plans
+
+    given, starts, m = scan_inputs(66, dtype, [300, 0, 700, 1], 8, 32, 2, 128, True)
+    conv, _, _ = conv_inputs(67, dtype, [300, 0, 700, 1], 256, 4, False)
+    conv.pop("initial")
+    dy = m.normal(1001, 8, 32, dtype=dtype)
+    want = ops.selective_scan(queue, softplus=True, starts=starts, **given)
+    grad = ops.selective_scan_grad(queue, dy, softplus=True, starts=starts, **given)
+    of_conv = ops.causal_conv_grad(queue, grad.x.flatten(1), activation="silu", starts=starts, **conv)
+    torch.cuda.synchronize()
+    scan = ops.plan_selective_scan(queue, softplus=True, starts=starts, **given)
+    back = ops.plan_selective_scan_grad(queue, dy, softplus=True, starts=starts, **given)
+    last = ops.plan_causal_conv_grad(queue, back.gradients.x.flatten(1), activation="silu", starts=starts, **conv)
+    plans = Plans([scan, back, last], profiling=False)
+    plans.prepare()
+    for steps in (1, 2, 3):
+        for v in (scan.y, scan.final, back.gradients.x, back.gradients.A, last.gradients.x, last.gradients.weight):
+            v.fill_(LEFT)
+        torch.cuda.synchronize()
+        plans.call_n_times(steps)
+        torch.cuda.synchronize()
+        assert torch.equal(scan.y, want[0]) and torch.equal(scan.final, want[1])
+        assert all(torch.equal(a, b) for a, b in zip(back.gradients, grad))
+        assert all(torch.equal(a, b) for a, b in zip(last.gradients[:3], of_conv[:3]))
+    plans.close()
