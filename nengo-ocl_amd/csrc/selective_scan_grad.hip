@@ -488,9 +488,9 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
     }
 }
 
-// dB and dC from the blocks of heads, in their order: a chunk's rows by `pieces` work-groups.  (By chunk, so that tokens
-// of no sequence are left as they are: no block has anything of them.)
-template <class T>
+// dB and dC from the blocks of heads, in their order: a chunk's rows by `pieces` work-groups, V elements to a lane.  (By
+// chunk, so that tokens of no sequence are left as they are: no block has anything of them.)
+template <class T, int V>
 __global__ __launch_bounds__(NHIP_WG) void add_blocks_kernel(nhip_scan_args a, const float* shared, int blocks, int pieces,
                                                              int q) {
     const int piece = blockIdx.x % pieces;
@@ -498,15 +498,21 @@ __global__ __launch_bounds__(NHIP_WG) void add_blocks_kernel(nhip_scan_args a, c
     const int t0 = seq.chunk * q, n = seq.seq < 0 ? 0 : min(q, seq.n - t0);
     const long long row = (long long)a.n_groups * a.states, all = a.tokens.n_tokens * row;
     const long long first = (seq.row0 + t0) * row, count = n * row;
-    for (long long e = (long long)piece * NHIP_WG + threadIdx.x; e < 2 * count; e += (long long)pieces * NHIP_WG) {
-        const bool of_C = e >= count;
-        const long long i = first + (of_C ? e - count : e);
-        const float* const from = shared + (of_C ? all : 0) + i;
-        float sum = 0.0f;
-#pragma unroll 8
-        for (int b = 0; b < blocks; ++b) sum += from[(long long)b * 2 * all];
-        static_cast<T*>(of_C ? a.dC : a.dB)[i] = (T)sum;
+    const long long e = ((long long)piece * NHIP_WG + threadIdx.x) * V;
+    if (e >= 2 * count) return;
+    const bool of_C = e >= count;
+    const long long i = first + (of_C ? e - count : e);
+    const float* const from = shared + (of_C ? all : 0) + i;
+    float sum[V];
+    sel_load<float, V>(from, sum);
+#pragma unroll 4
+    for (int b = 1; b < blocks; ++b) {
+        float more[V];
+        sel_load<float, V>(from + (long long)b * 2 * all, more);
+#pragma unroll
+        for (int k = 0; k < V; ++k) sum[k] += more[k];
     }
+    sel_store<T, V>(static_cast<T*>(of_C ? a.dC : a.dB) + i, sum);
 }
 
 struct Layout {
@@ -581,10 +587,11 @@ extern "C" int nhip_selective_scan_grad(void* stream, const nhip_scan_args* args
             });
             if (!rc && m.blocks > 1) {
                 // (there are fewer than 512 chunks and groups, so this is a small grid)
-                const int q = sel_chunk_tokens(a.states);
-                const int pieces = (int)((2LL * q * a.n_groups * a.states + NHIP_WG - 1) / NHIP_WG);
-                hipLaunchKernelGGL(add_blocks_kernel<T>, dim3((unsigned)(m.n_chunks * pieces)), dim3(NHIP_WG), 0, st, a,
-                                   shared, m.blocks, pieces, q);
+                const int q = sel_chunk_tokens(a.states), per = NHIP_WG * (m.walk.vec ? 4 : 1);
+                const int pieces = (int)((2LL * q * a.n_groups * a.states + per - 1) / per);
+                auto add = m.walk.vec ? add_blocks_kernel<T, 4> : add_blocks_kernel<T, 1>;
+                hipLaunchKernelGGL(add, dim3((unsigned)(m.n_chunks * pieces)), dim3(NHIP_WG), 0, st, a, shared, m.blocks,
+                                   pieces, q);
                 rc = (int)hipGetLastError();
             }
         });
