@@ -30,14 +30,21 @@ struct GradPlan {
 
 template <class Tc, int NP> struct GradLds {
     static constexpr int Q = sel_chunk_of(NP);
-    static constexpr int SX = sel_stride<Tc>(64), SN = sel_stride<Tc>(NP), SW = sel_stride<Tc>(Q);
+    static constexpr int SX = sel_stride<Tc>(64), SN = sel_stride<Tc>(NP);
     alignas(16) Tc x[Q * sel_stride<Tc>(64)];
     alignas(16) Tc dy[Q * sel_stride<Tc>(64)];
     alignas(16) Tc B[Q * sel_stride<Tc>(NP)];
     alignas(16) Tc C[Q * sel_stride<Tc>(NP)];
-    // [j][i]: X_ij L_ij step_j and K_ij L_ij step_j.  bfloat16: both parts of K's, and when dx has been formed both of X's
-    static constexpr int kParts = SelSplit<Tc>::out;
-    alignas(16) Tc pairs[2][Q * sel_stride<Tc>(Q)];
+    // The parts of X_ij L_ij step_j, then those of K_ij L_ij step_j: tiles [16 of j][16 of i] of the lower triangle, and one
+    // of zeros in the place of all others.  (Rows of 32 bytes, or of 64 with 16 between them, meet no bank twice, however
+    // they are read; whole rows of the tables would leave no room for two parts beside another work-group.)
+    static constexpr int kParts = SelSplit<Tc>::out, kTiles = Q / 16 * (Q / 16 + 1) / 2, kZeros = 2 * kParts * kTiles;
+    static constexpr int ST = sizeof(Tc) == 2 ? 16 : 20;
+    alignas(16) Tc pairs[kZeros + 1][16 * ST];
+    static constexpr int X(int part, int it, int jt) {
+        return it < jt ? kZeros : part * kTiles + it * (it + 1) / 2 + jt;
+    }
+    static constexpr int K(int part, int it, int jt) { return it < jt ? kZeros : kParts * kTiles + X(part, it, jt); }
     SelSteps<Q> steps;
     // Sums of a head.  over[jt][t]: of K X L step over i >= t in t's own tile of 16 and j < t in tile jt;
     // col[it][j]: of K X L over the i > j of tile it;  q, r, z: by wave
@@ -90,8 +97,8 @@ template <class T, class Tc, int NP, bool VEC, bool WHOLE>
 __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void grad_kernel(nhip_scan_args a, GradPlan plan) {
     using Lds = GradLds<Tc, NP>;
     constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
-    constexpr int kTiles = QT * (QT + 1) / 2, kMyTiles = (kTiles + 3) / 4, kMyNT = (NT + 3) / 4;
-    constexpr int SX = Lds::SX, SN = Lds::SN, SW = Lds::SW;
+    constexpr int kTiles = Lds::kTiles, kMyTiles = (kTiles + 3) / 4, kMyNT = (NT + 3) / 4;
+    constexpr int SX = Lds::SX, SN = Lds::SN, ST = Lds::ST;
     constexpr int kSplits = SelSplit<Tc>::n, kParts = Lds::kParts;
     extern __shared__ __align__(16) char lds_bytes[];
     Lds& s = *reinterpret_cast<Lds*>(lds_bytes);
@@ -121,7 +128,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
         stage_B.template store<SN>(s.B, n, a.states);
         stage_C.template store<SN>(s.C, n, a.states);
     }
-    for (int q = tid; q < Q * SW; q += NHIP_WG) s.pairs[0][q] = s.pairs[1][q] = (Tc)0.0f;  // (i < j for good)
+    for (int q = tid; q < 16 * ST; q += NHIP_WG) s.pairs[Lds::kZeros][q] = (Tc)0.0f;
     __syncthreads();
 
     int tile_i[kMyTiles], tile_j[kMyTiles];  // this wave's tiles of the lower triangle
@@ -199,7 +206,6 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
 #pragma unroll
             for (int ks = 0; ks < NK; ++ks) state_row<VEC>(G, p, 32 * ks, a.dim, a.states, g, Gr[ks]);
 
-            float x_pairs[kMyTiles][4];
 #pragma unroll
             for (int m = 0; m < kMyTiles; ++m) {
                 if (tile_i[m] < 0) continue;
@@ -213,8 +219,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                 const float step = s.steps.step[j];
                 const int whole = s.steps.whole[j];
                 const float from = 1.0f / s.steps.to[j];
-                float kl[4], ml[4];
-                float(&xl)[4] = x_pairs[m];
+                float kl[4], xl[4], ml[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int i = i0 + r;
@@ -247,13 +252,10 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                     const float over = sel_row_sum(i > j ? (ml[r] + (g < 3 ? other : 0.0f)) * step : 0.0f);
                     if (l == 0) s.over[jt][i] += over;
                 }
-                const int at = j * SW + i0;
-                if constexpr (kParts > 1) {
-                    sel_store_parts(s.pairs[0] + at, s.pairs[1] + at, kl);
-                } else {
-                    sel_store<Tc, 4>(s.pairs[0] + at, xl);
-                    sel_store<Tc, 4>(s.pairs[1] + at, kl);
-                }
+                Tc* const to = s.pairs[wave + 4 * m] + ST * l + 4 * g;
+                constexpr int kTable = kTiles * 16 * ST;
+                sel_store_parts(to, to + kTable, xl);
+                sel_store_parts(to + kParts * kTable, to + (kParts + 1) * kTable, kl);
             }
             __syncthreads();
 
@@ -287,8 +289,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                         for (int q = 0; q < kParts; ++q)
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
-                                sel_mma(acc[u], df[ks],
-                                        sel_rows(s.pairs[kParts > 1 ? q : 1] + (16 * (j2 + u) + l) * SW + 32 * ks, g));
+                                sel_mma(acc[u], df[ks], sel_rows(s.pairs[Lds::K(q, 2 * ks, j2 + u)] + ST * l,
+                                                                 s.pairs[Lds::K(q, 2 * ks + 1, j2 + u)] + ST * l, g));
                     sel_settle(acc);
                     const int c = 16 * wave + 4 * g;
                     T* const row = static_cast<T*>(a.dx) + ((seq.row0 + t0) * a.n_heads + head) * a.dim + p_tile;
@@ -302,16 +304,6 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                         if (j < n) sel_store4<VEC>(row + (unsigned)j * (unsigned)(a.n_heads * a.dim), c, cols, acc[u]);
                     }
                 }
-            }
-
-            if constexpr (kParts > 1) {
-                __syncthreads();
-#pragma unroll
-                for (int m = 0; m < kMyTiles; ++m) {
-                    const int at = (16 * tile_j[m] + l) * SW + 16 * tile_i[m] + 4 * g;
-                    if (tile_i[m] >= 0) sel_store_parts(s.pairs[0] + at, s.pairs[1] + at, x_pairs[m]);
-                }
-                __syncthreads();
             }
 
             // dB, dC: every fourth tile of the states to a wave
@@ -367,7 +359,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                         for (int q = 0; q < kParts; ++q)
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
-                                sel_mma(dC[m][i2 + u], b, sel_cols(s.pairs[q] + 32 * ks * SW + 16 * (i2 + u), SW, l, g));
+                                sel_mma(dC[m][i2 + u], b, sel_cols(s.pairs[Lds::X(q, i2 + u, 2 * ks)],
+                                                                   s.pairs[Lds::X(q, i2 + u, 2 * ks + 1)], ST, l, g));
                     }
                 }
                 sel_settle(dC[m]);
@@ -404,7 +397,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                         for (int q = 0; q < kParts; ++q)
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
-                                sel_mma(dB[m][j2 + u], c, sel_rows(s.pairs[q] + (16 * (j2 + u) + l) * SW + 32 * ks, g));
+                                sel_mma(dB[m][j2 + u], c, sel_rows(s.pairs[Lds::X(q, 2 * ks, j2 + u)] + ST * l,
+                                                                   s.pairs[Lds::X(q, 2 * ks + 1, j2 + u)] + ST * l, g));
                     }
                 }
                 sel_settle(dB[m]);
