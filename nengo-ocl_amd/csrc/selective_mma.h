@@ -55,46 +55,82 @@ template <int N> __device__ __forceinline__ void sel_settle(sel_f4 (&a)[N]) {
 }
 __device__ __forceinline__ void sel_settle(sel_f4& a) { asm volatile("s_nop 15" : "+v"(a)); }
 
-// Fragment of a matrix in LDS whose rows run along k: `row` is this lane's row, at the first k, `next` 16 of k behind.
-__device__ __forceinline__ SelFrag<__bf16> sel_rows(const __bf16* row, const __bf16* next, int g) {
+// Fragment of a matrix in LDS whose rows run along k: `row` is this lane's row, at the first k.
+__device__ __forceinline__ SelFrag<__bf16> sel_rows(const __bf16* row, int g) {
     const sel_b4 lo = *reinterpret_cast<const sel_b4*>(row + 4 * g);
-    const sel_b4 hi = *reinterpret_cast<const sel_b4*>(next + 4 * g);
+    const sel_b4 hi = *reinterpret_cast<const sel_b4*>(row + 16 + 4 * g);
     SelFrag<__bf16> f;
     f.v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return f;
 }
-__device__ __forceinline__ SelFrag<float> sel_rows(const float* row, const float* next, int g) {
+__device__ __forceinline__ SelFrag<float> sel_rows(const float* row, int g) {
     const sel_f4 lo = *reinterpret_cast<const sel_f4*>(row + 4 * g);
-    const sel_f4 hi = *reinterpret_cast<const sel_f4*>(next + 4 * g);
+    const sel_f4 hi = *reinterpret_cast<const sel_f4*>(row + 16 + 4 * g);
     SelFrag<float> f;
 #pragma unroll
     for (int e = 0; e < 4; ++e) { f.v[e] = lo[e]; f.v[4 + e] = hi[e]; }
     return f;
 }
-template <class Tc> __device__ __forceinline__ SelFrag<Tc> sel_rows(const Tc* row, int g) { return sel_rows(row, row + 16, g); }
 
 // Fragment of a matrix in LDS whose rows run across: `at` is its element (first k, first row or
-// column of the tile), `next` that 16 of k behind, `stride` the length of its rows (a multiple of 4).  16-bit elements: the
+// column of the tile), `stride` the length of its rows (a multiple of 4).  16-bit elements: the
 // 16 lanes of a quarter of the wave name four rows of 16 elements, four to a lane, and each gets
 // its column of them (ds_read_b64_tr_b16).
-__device__ __forceinline__ SelFrag<__bf16> sel_cols(const __bf16* at, const __bf16* next, int stride, int l, int g) {
+__device__ __forceinline__ SelFrag<__bf16> sel_cols(const __bf16* at, int stride, int l, int g) {
     typedef __attribute__((address_space(3))) sel_b4* lds;
-    const int mine = (4 * g + (l >> 2)) * stride + 4 * (l & 3);
-    const sel_b4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds)(at + mine));
-    const sel_b4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds)(next + mine));
+    const __bf16* p = at + (4 * g + (l >> 2)) * stride + 4 * (l & 3);
+    const sel_b4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds)(p));
+    const sel_b4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds)(p + 16 * stride));
     SelFrag<__bf16> f;
     f.v = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
     return f;
 }
-__device__ __forceinline__ SelFrag<float> sel_cols(const float* at, const float* next, int stride, int l, int g) {
+__device__ __forceinline__ SelFrag<float> sel_cols(const float* at, int stride, int l, int g) {
     SelFrag<float> f;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) f.v[e] = (e < 4 ? at : next)[(4 * g + (e & 3)) * stride + l];
+    for (int e = 0; e < 8; ++e) f.v[e] = at[(16 * (e >> 2) + 4 * g + (e & 3)) * stride + l];
     return f;
 }
-template <class Tc> __device__ __forceinline__ SelFrag<Tc> sel_cols(const Tc* at, int stride, int l, int g) {
-    return sel_cols(at, at + 16 * stride, stride, l, g);
-}
+
+// A matrix in LDS kept as tiles of 16 x 16, of which only some are held: where the four elements `four` of a row of a
+// tile lie, and fragments over two tiles, along their rows and across.  16-bit elements: 512 bytes without gaps, fours of
+// rows 4 apart in other places, so that 16 lanes meet no bank twice (rows of 32 bytes in their order do, four
+// times).  32-bit elements: 16 bytes between the rows.
+template <class Tc> struct SelTile {
+    static constexpr bool kSwapped = sizeof(Tc) == 2;
+    static constexpr int kRow = kSwapped ? 16 : 20, kSize = 16 * kRow;
+    static __device__ __forceinline__ int at(int row, int four) {
+        return kRow * row + 4 * (kSwapped ? four ^ (row >> 2) : four);
+    }
+    static __device__ __forceinline__ SelFrag<__bf16> rows(const __bf16* lo, const __bf16* hi, int l, int g) {
+        const sel_b4 a = *reinterpret_cast<const sel_b4*>(lo + at(l, g)), b = *reinterpret_cast<const sel_b4*>(hi + at(l, g));
+        SelFrag<__bf16> f;
+        f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        return f;
+    }
+    static __device__ __forceinline__ SelFrag<float> rows(const float* lo, const float* hi, int l, int g) {
+        const sel_f4 a = *reinterpret_cast<const sel_f4*>(lo + at(l, g)), b = *reinterpret_cast<const sel_f4*>(hi + at(l, g));
+        SelFrag<float> f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) { f.v[e] = a[e]; f.v[4 + e] = b[e]; }
+        return f;
+    }
+    static __device__ __forceinline__ SelFrag<__bf16> cols(const __bf16* lo, const __bf16* hi, int l, int g) {
+        typedef __attribute__((address_space(3))) sel_b4* lds;
+        const int mine = at(4 * g + (l >> 2), l & 3);
+        const sel_b4 a = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds)(lo + mine));
+        const sel_b4 b = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds)(hi + mine));
+        SelFrag<__bf16> f;
+        f.v = __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+        return f;
+    }
+    static __device__ __forceinline__ SelFrag<float> cols(const float* lo, const float* hi, int l, int g) {
+        SelFrag<float> f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f.v[e] = (e < 4 ? lo : hi)[kRow * (4 * g + (e & 3)) + l];
+        return f;
+    }
+};
 
 // Float32 values as parts that add up to them.  (bfloat16: two values at a time, which is one instruction to
 // round them and one for each to widen it; element by element the compiler rounds each alone)

@@ -36,11 +36,10 @@ template <class Tc, int NP> struct GradLds {
     alignas(16) Tc B[Q * sel_stride<Tc>(NP)];
     alignas(16) Tc C[Q * sel_stride<Tc>(NP)];
     // The parts of X_ij L_ij step_j, then those of K_ij L_ij step_j: tiles [16 of j][16 of i] of the lower triangle, and one
-    // of zeros in the place of all others.  (Rows of 32 bytes, or of 64 with 16 between them, meet no bank twice, however
-    // they are read; whole rows of the tables would leave no room for two parts beside another work-group.)
+    // of zeros in the place of all others.  (Whole rows of the tables would leave no room for two parts beside another
+    // work-group.)
     static constexpr int kParts = SelSplit<Tc>::out, kTiles = Q / 16 * (Q / 16 + 1) / 2, kZeros = 2 * kParts * kTiles;
-    static constexpr int ST = sizeof(Tc) == 2 ? 16 : 20;
-    alignas(16) Tc pairs[kZeros + 1][16 * ST];
+    alignas(16) Tc pairs[kZeros + 1][SelTile<Tc>::kSize];
     static constexpr int X(int part, int it, int jt) {
         return it < jt ? kZeros : part * kTiles + it * (it + 1) / 2 + jt;
     }
@@ -98,7 +97,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
     using Lds = GradLds<Tc, NP>;
     constexpr int Q = Lds::Q, QT = Q / 16, QK = Q / 32, NT = NP / 16, NK = NP / 32;
     constexpr int kTiles = Lds::kTiles, kMyTiles = (kTiles + 3) / 4, kMyNT = (NT + 3) / 4;
-    constexpr int SX = Lds::SX, SN = Lds::SN, ST = Lds::ST;
+    constexpr int SX = Lds::SX, SN = Lds::SN;
+    using Tile = SelTile<Tc>;
     constexpr int kSplits = SelSplit<Tc>::n, kParts = Lds::kParts;
     extern __shared__ __align__(16) char lds_bytes[];
     Lds& s = *reinterpret_cast<Lds*>(lds_bytes);
@@ -128,7 +128,7 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
         stage_B.template store<SN>(s.B, n, a.states);
         stage_C.template store<SN>(s.C, n, a.states);
     }
-    for (int q = tid; q < 16 * ST; q += NHIP_WG) s.pairs[Lds::kZeros][q] = (Tc)0.0f;
+    for (int q = tid; q < Tile::kSize; q += NHIP_WG) s.pairs[Lds::kZeros][q] = (Tc)0.0f;
     __syncthreads();
 
     int tile_i[kMyTiles], tile_j[kMyTiles];  // this wave's tiles of the lower triangle
@@ -252,8 +252,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                     const float over = sel_row_sum(i > j ? (ml[r] + (g < 3 ? other : 0.0f)) * step : 0.0f);
                     if (l == 0) s.over[jt][i] += over;
                 }
-                Tc* const to = s.pairs[wave + 4 * m] + ST * l + 4 * g;
-                constexpr int kTable = kTiles * 16 * ST;
+                Tc* const to = s.pairs[wave + 4 * m] + Tile::at(l, g);
+                constexpr int kTable = kTiles * Tile::kSize;
                 sel_store_parts(to, to + kTable, xl);
                 sel_store_parts(to + kParts * kTable, to + (kParts + 1) * kTable, kl);
             }
@@ -289,8 +289,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                         for (int q = 0; q < kParts; ++q)
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
-                                sel_mma(acc[u], df[ks], sel_rows(s.pairs[Lds::K(q, 2 * ks, j2 + u)] + ST * l,
-                                                                 s.pairs[Lds::K(q, 2 * ks + 1, j2 + u)] + ST * l, g));
+                                sel_mma(acc[u], df[ks], Tile::rows(s.pairs[Lds::K(q, 2 * ks, j2 + u)],
+                                                                   s.pairs[Lds::K(q, 2 * ks + 1, j2 + u)], l, g));
                     sel_settle(acc);
                     const int c = 16 * wave + 4 * g;
                     T* const row = static_cast<T*>(a.dx) + ((seq.row0 + t0) * a.n_heads + head) * a.dim + p_tile;
@@ -359,8 +359,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                         for (int q = 0; q < kParts; ++q)
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
-                                sel_mma(dC[m][i2 + u], b, sel_cols(s.pairs[Lds::X(q, i2 + u, 2 * ks)],
-                                                                   s.pairs[Lds::X(q, i2 + u, 2 * ks + 1)], ST, l, g));
+                                sel_mma(dC[m][i2 + u], b, Tile::cols(s.pairs[Lds::X(q, i2 + u, 2 * ks)],
+                                                                     s.pairs[Lds::X(q, i2 + u, 2 * ks + 1)], l, g));
                     }
                 }
                 sel_settle(dC[m]);
@@ -397,8 +397,8 @@ __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void
                         for (int q = 0; q < kParts; ++q)
 #pragma unroll
                             for (int u = 0; u < 2; ++u)
-                                sel_mma(dB[m][j2 + u], c, sel_rows(s.pairs[Lds::X(q, 2 * ks, j2 + u)] + ST * l,
-                                                                   s.pairs[Lds::X(q, 2 * ks + 1, j2 + u)] + ST * l, g));
+                                sel_mma(dB[m][j2 + u], c, Tile::rows(s.pairs[Lds::X(q, 2 * ks, j2 + u)],
+                                                                     s.pairs[Lds::X(q, 2 * ks + 1, j2 + u)], l, g));
                     }
                 }
                 sel_settle(dB[m]);
