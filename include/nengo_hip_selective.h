@@ -72,7 +72,8 @@ typedef struct nhip_conv_step_args {
  *     y[t] = S[t] C[t] + D[h] x[t]
  * for each of n_heads heads; B and C are shared by the n_heads / n_groups heads of a group.
  * S before a sequence's first token: initial[s, n_heads, dim, states], or zeros; final: after
- * its last.  Gradients (nhip_selective_scan_grad): dy, dfinal -> dx, ddt, dB, dC (contiguous,
+ * its last.  softplus(-inf), like that of the lowest value of a type, is zero: such a token reads the
+ * state and leaves it as it is.  Gradients (nhip_selective_scan_grad): dy, dfinal -> dx, ddt, dB, dC (contiguous,
  * types of x, dt, x, x), dA, dD, ddt_bias (float32, [n_heads]), dinitial (float32). */
 typedef struct nhip_scan_args {
     nhip_tokens tokens;

@@ -336,6 +336,8 @@ template <class F> void with_shape(bool vec, int per16, int width, F&& f) {
     else go(integral_constant<int, 256>(), integral_constant<int, 0>());
 }
 
+// Whether every part of a row begins at a multiple of 16 bytes and holds whole packs of 16.  (The gradient's lanes, which
+// take 8 bytes of 16-bit types, go by the same rule.)
 bool wide(const nhip_norm_args& a) {
     const int v = 16 / sel_size(a.type);
     if ((a.channels / a.groups) % v) return false;

@@ -299,7 +299,7 @@ template <class F> bool with_width(int width, F&& f) {
 }
 
 // A lane reads 16 bytes of neighbouring channels where every row begins at a multiple of 16 bytes,
-// otherwise one channel.
+// otherwise one channel.  (The gradient's lanes, which take 8 bytes of 16-bit types, go by the same rule.)
 bool wide(int type, int channels, std::initializer_list<const void*> pointers,
           std::initializer_list<long long> strides) {
     const int v = 16 / sel_size(type);

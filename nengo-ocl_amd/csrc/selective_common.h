@@ -14,7 +14,8 @@ typedef float sel_f4 __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------------------------ element types
 // Sums, states and statistics are float32; a value is rounded to a 16-bit type once, when it
-// is stored (to nearest, ties to even).
+// is stored (to nearest, ties to even).  Operands of matrix products that are no inputs go in as
+// several parts of 16 bits (SelSplit).
 template <class T, int N> struct alignas(sizeof(T) * N) SelPack { T v[N]; };
 
 template <class T, int N>
@@ -32,8 +33,9 @@ __device__ __forceinline__ void sel_store(T* p, const float (&in)[N]) {
     *reinterpret_cast<SelPack<T, N>*>(p) = q;
 }
 
-// The same past the caches, for results of many megabytes: a launch ends when the L2s' written lines are in
-// memory, and these are there already.
+// The same past the caches: a launch ends when the L2s' written lines are in memory, and these are there already
+// (the convolution of 8 x 2048 tokens, 2304 channels, bfloat16: 41.7 -> 30.9 us).  At any size: a small call takes what its
+// launch takes either way.
 template <class T, int N>
 __device__ __forceinline__ void sel_store_past(T* p, const float (&in)[N]) {
     typedef unsigned words __attribute__((ext_vector_type(4)));

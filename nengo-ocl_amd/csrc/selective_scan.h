@@ -38,7 +38,7 @@ struct SelWalkPlan {
 // Tokens of a chunk: 64, or 32 where 256 states would not fit the LDS otherwise.
 constexpr int sel_chunk_of(int np) { return np > 128 ? 32 : 64; }
 
-// States are kept in multiples of 32; f(std::integral_constant) for the smallest that holds n.
+// States are worked on as 32, 64, 128 or 256; f(std::integral_constant) for the smallest of these that holds n.
 template <class F> static inline bool sel_with_states(int n, F&& f) {
     using std::integral_constant;
     if (n <= 32) f(integral_constant<int, 32>());
@@ -112,11 +112,12 @@ template <class Tc, int NP, bool OUTPUTS> struct SelWalkLds {
 // operands but the state come from, was busy for as long as a chunk took.  The inputs of the next chunk
 // are fetched while one is worked on, the steps of two chunks formed at once, by a wave each.  A
 // work-group of the bfloat16 kernel with 128 states takes half of a compute unit's LDS and registers.
-// 8 x 2048 tokens, 32 heads of 64, 128 states, bfloat16: 96 us for 175 MB and 40 GFLOP, 38 for the ends (53 MB in, 25
-// out).  Bound by issue: the matrix cores work for 22 % of the time, the LDS for 39 %, and a chunk takes a wave about
-// a thousand vector instructions beside 196 matrix ones (half of these for the three parts of what the state gains).  Chunks of
-// 32 tokens, at which four work-groups fit a unit, took 96 us when these took 95.  The state that enters and the
-// weights go in as two parts: as one, the walk took 88 us and y was off by 2^-8 of the terms' magnitudes, not of itself.
+// 8 x 2048 tokens, 32 heads of 64, 128 states, bfloat16: 103 us for 175 MB and 40 GFLOP, 39 for the ends (53 MB in, 25
+// out), 93 and 36 behind a hundred calls.  Bound by issue: the matrix cores work for 24 % of the time, the LDS for 36 %,
+// and a chunk takes a wave about 1,300 vector instructions beside 196 matrix ones (half of these for the three parts of
+// what the state gains).  Chunks of 32 tokens, at which four work-groups fit a unit, took 96 us when these took 95.  The
+// state that enters and the weights go in as two parts: as one, the walk took 88 us and y was off by 2^-8 of the terms'
+// magnitudes, not of itself.
 template <class T, class Tc, int NP, int WALK, bool VEC>
 __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1)
 void sel_walk_kernel(nhip_scan_args a, SelWalkPlan plan) {
@@ -558,7 +559,7 @@ static inline long long sel_round4(long long floats) { return (floats + 3) & ~3L
 // into as many segments as walks fit (8 x 2048 tokens forward: 121 us with 512 walks, 157 with 256), down to a chunk
 // each (4001 tokens in nine ragged sequences, 12 heads, 32 bits: 64 us, with four chunks 104).  Up to four segments are
 // added up by the walks themselves (the same 8 x 2048 tokens: 114 us, by a launch of its own 133), more by that launch
-// (32768 tokens in 32 segments: 222 us, by the walks 301).
+// (32768 tokens in 32 segments: 222 us, by the walks 301; all of these with the weights of pairs as one part).
 static inline SelWalkPlan sel_walk_plan(const nhip_scan_args& a, int directions, float* states) {
     SelWalkPlan p;
     const int q = sel_chunk_tokens(a.states);

@@ -88,10 +88,11 @@ __device__ __forceinline__ void state_row(const float* s, int p, int n0, int dim
 
 // A work-group takes a chunk through a block of its group's heads, 64 of the dimension at a time: the sums for dB
 // and dC of 16 states per wave (twice over for 128) stay in registers over all of them, B and C in the LDS.  WHOLE: the
-// dimension is a multiple of 64.  4 x 2048 tokens, 32 heads of 64, 128 states, bfloat16: 161 us, of which the
-// walks' states, 269 MB once and one half of them again as rows, would take 70 by themselves; the matrix cores work
-// for 11 % of the time, the LDS for 28 %, and half of it the two waves of a unit both wait.  The walks before it take 41
-// (ends) and 88 (269 MB written).
+// dimension is a multiple of 64.  4 x 2048 tokens, 32 heads of 64, 128 states, bfloat16: 187 us, 170 behind a
+// hundred calls, of which the walks' states, 269 MB once and one half of them again as rows, would take 70 by themselves;
+// the matrix cores work for 13 % of the time, the LDS for 26 %, and half of it the two waves of a unit both wait.  The
+// walks before it take 41 (ends) and 90 (269 MB written).  With one part of the pairs' weights and of G it took 169,
+// and dx, dB and dC were off by 2^-8 of their terms' magnitudes.
 template <class T, class Tc, int NP, bool VEC, bool WHOLE>
 __global__ __launch_bounds__(NHIP_WG, sizeof(Tc) == 2 && NP <= 128 ? 2 : 1) void grad_kernel(nhip_scan_args a, GradPlan plan) {
     using Lds = GradLds<Tc, NP>;

@@ -32,10 +32,21 @@ strides, the last axis has stride one.  ValueError and TypeError say what does n
 
 What the offsets on the device hold is not checked: they are cut to the tokens that there are,
 results of tokens that no sequence holds are not written, and those of sequences that overlap
-are undefined.  Outputs may not overlap inputs.  Sums, states and parameters' gradients are
-float32 and added up in the same order on every call.  An input that is no finite number reaches
-what depends on it, no earlier token and no other sequence; in the scan's gradient, all tokens of
-its chunk of 64 (32 with more than 128 states).
+are undefined.  Outputs may not overlap inputs.  What would take a launch of 2**24 work-groups is
+refused (`HipError`) before any.
+
+Sums, states and parameters' gradients are float32 and added up in the same order on every call.
+A result of 16 bits is rounded once: besides that rounding it is off by less than 2**-15 of the
+magnitudes of the terms that it is the sum of (bfloat16 scans, whose states and weights go into
+the matrix products as two bfloat16 parts; the state itself gains float32 values).
+
+An input that is no finite number reaches what depends on it, no earlier token and no other
+sequence; in the scan's gradient, all tokens of its chunk of 64 (32 with more than 128 states).
+With `softplus`, a `dt` of -inf or of the lowest value of its type masks a token: its step is zero,
+and the state passes it unchanged.
+
+Nothing is recorded for torch's autograd, also where an input has `requires_grad`: gradients come
+from the ``*_grad`` functions.
 """
 
 import collections
@@ -627,7 +638,8 @@ def _block_norm_grad(queue, dout, x, weight, gate=None, residual=None, scale=Non
 def plan_block_norm_grad(queue, dout, x, weight, gate=None, residual=None, scale=None, groups=1, eps=1e-6,
                          after=False, dv=None, tag=None):
     """The gradient of `plan_block_norm`, from `dout` and (with a residual in front) `dv`;
-    ``plan.gradients``: those of weight and scale are float32."""
+    ``plan.gradients``: those of weight and scale are float32.  Behind a block (`after`) the residual's is
+    `dout` itself, the caller's array and no copy."""
     return _block_norm_grad(queue, dout, x, weight, gate, residual, scale, groups, eps, after, dv).plan(queue, tag)
 
 
