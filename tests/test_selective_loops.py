@@ -116,3 +116,32 @@ def test_norm_gradient_of_rows_in_several_packs(queue, ops, dtype, rows, channel
         want = gradients(function, given, (dout, dv))
         for k in want:
             near(getattr(got, k), want[k], (k, gate, residual, scale, after))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf"), -float("inf")])
+def test_what_is_no_number_over_several_chunks(queue, ops, dtype, bad):  # noqa: F811
+    """In a walk over six chunks it reaches no earlier token and no other sequence, from C its own token alone; in the
+    gradient, the other sequences' parts stay as they are."""
+    given, _, m = given_for(45, dtype, *WALKS[0])
+    dy = m.normal(*given["x"].shape, dtype=dtype)
+    clean, _ = ops.selective_scan(queue, softplus=True, **given)
+    grads = ops.selective_scan_grad(queue, dy, softplus=True, **given)
+    others = [0, 1, 2, 4, 5, 6, 7]
+    for name in ("x", "B", "C"):
+        odd = dict(given)
+        odd[name] = given[name].clone()
+        odd[name][3, 200, 0, 3] = bad
+        y, final = ops.selective_scan(queue, softplus=True, **odd)
+        assert torch.equal(y[others], clean[others]) and torch.equal(y[3, :200], clean[3, :200]), name
+        assert torch.isfinite(final[others]).all()
+        assert not torch.isfinite(y[3, 200]).all(), name
+        if name == "C":
+            assert torch.equal(y[3, 201:], clean[3, 201:]) and torch.isfinite(final).all()
+        if name == "x":  # head 0, element 3 of its dimension
+            rest = [0, 1, 2, 4, 5, 6, 7]
+            assert torch.equal(y[3, :, 1:], clean[3, :, 1:]) and torch.equal(y[3, :, 0][:, rest], clean[3, :, 0][:, rest])
+        got = ops.selective_scan_grad(queue, dy, softplus=True, **odd)
+        for k in ("x", "dt", "B", "C", "initial"):
+            assert torch.equal(getattr(got, k)[others], getattr(grads, k)[others]), (name, k)
