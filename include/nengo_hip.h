@@ -30,6 +30,7 @@
 #define NENGO_HIP_H
 
 #include "nengo_hip_selective.h"
+#include "nengo_hip_tokens.h"
 
 #ifdef __cplusplus
 extern "C" {
@@ -876,6 +877,22 @@ int nhip_selective_step(void *stream, const nhip_scan_step_args *args);
 int nhip_block_norm(void *stream, const nhip_norm_args *args);
 int nhip_block_norm_grad(void *stream, const nhip_norm_args *args);
 int nhip_block_norm_grad_workspace(const nhip_norm_args *args, long long *bytes_out);
+
+/* ---- operators over tokens ---------------------------------------------------
+ * The arguments are described in nengo_hip_tokens.h.  Sizes: channels, features and words from 1, rows from
+ * 0 to 2^24, top up to 256.  The `*_workspace` functions give the bytes of workspace that a call with these
+ * arguments needs (a smaller one is refused with NHIP_E_TOOBIG); its contents need not be kept between calls. */
+int nhip_layer_norm(void *stream, const nhip_layer_norm_args *args);
+int nhip_layer_norm_grad(void *stream, const nhip_layer_norm_args *args);
+int nhip_layer_norm_grad_workspace(const nhip_layer_norm_args *args, long long *bytes_out);
+int nhip_gated_projection(void *stream, const nhip_gated_args *args);
+int nhip_gated_projection_workspace(const nhip_gated_args *args, long long *bytes_out);
+int nhip_gated_projection_grad(void *stream, const nhip_gated_args *args);
+int nhip_gated_projection_grad_workspace(const nhip_gated_args *args, long long *bytes_out);
+int nhip_vocabulary_loss(void *stream, const nhip_loss_args *args);
+int nhip_vocabulary_loss_workspace(const nhip_loss_args *args, long long *bytes_out);
+int nhip_vocabulary_loss_grad(void *stream, const nhip_loss_args *args);
+int nhip_vocabulary_loss_grad_workspace(const nhip_loss_args *args, long long *bytes_out);
 
 /* ---- executor ----------------------------------------------------------
  * replaces the Python launch loop of `Plans.enqueue_n_times` (plan.py:137-149):

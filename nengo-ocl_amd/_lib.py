@@ -112,6 +112,17 @@ SIGNATURES = {
     "nhip_block_norm": [P, P],
     "nhip_block_norm_grad": [P, P],
     "nhip_block_norm_grad_workspace": [P, P],
+    "nhip_layer_norm": [P, P],
+    "nhip_layer_norm_grad": [P, P],
+    "nhip_layer_norm_grad_workspace": [P, P],
+    "nhip_gated_projection": [P, P],
+    "nhip_gated_projection_workspace": [P, P],
+    "nhip_gated_projection_grad": [P, P],
+    "nhip_gated_projection_grad_workspace": [P, P],
+    "nhip_vocabulary_loss": [P, P],
+    "nhip_vocabulary_loss_workspace": [P, P],
+    "nhip_vocabulary_loss_grad": [P, P],
+    "nhip_vocabulary_loss_grad_workspace": [P, P],
     "nhip_capture_begin": [P],
     "nhip_capture_end": [P, ctypes.POINTER(c_void_p)],
     "nhip_graph_upload": [P, P],

@@ -7,9 +7,7 @@
 // (means over each of `groups` equal parts of a row) and its gradient.  All of it moves memory:
 // every array is read or written once, a part of a row stays in registers between the sum of
 // its squares and its use.  16384 rows of 2048 in four groups with a gate, bfloat16: 201 MB in 37 us, 5.4 TB/s.
-#include <type_traits>
-
-#include "selective_common.h"
+#include "norm_rows.h"
 
 namespace {
 
@@ -47,19 +45,6 @@ struct Operands {
     }
 };
 
-template <int L>
-__device__ __forceinline__ float sum_over(float v, float* s) {
-    v = sel_wave_sum(v);
-    if constexpr (L > NHIP_WAVE) {
-        const int wave = threadIdx.x / NHIP_WAVE;
-        __syncthreads();
-        if ((threadIdx.x & (NHIP_WAVE - 1)) == 0) s[wave] = v;
-        __syncthreads();
-        v = (s[0] + s[1]) + (s[2] + s[3]);
-    }
-    return v;
-}
-
 template <class T, int V, int L, int R>
 __global__ __launch_bounds__(NHIP_WG) void norm_kernel(nhip_norm_args a) {
     __shared__ float s[8];
@@ -90,7 +75,7 @@ __global__ __launch_bounds__(NHIP_WG) void norm_kernel(nhip_norm_args a) {
             if (v_out) sel_store<T, V>(v_out + c, v[0]);
         }
     }
-    sum = sum_over<L>(sum, s);
+    sum = norm_sum<L>(sum, s);
     const float inv = 1.0f / sqrtf(sum / (float)width + a.eps);
     T* const out = static_cast<T*>(a.out) + op.row * a.channels + op.base;
     auto finish = [&](int c, float(&u)[V]) {
@@ -250,8 +235,8 @@ __global__ __launch_bounds__(NHIP_WG, 2) void norm_grad_kernel(nhip_norm_args a,
                 if (kAhead) fetch(raw[r], row + step, channel(r));
 #pragma unroll
             for (int r = 0; r < R; ++r) sums(channel(r), u[r], w[r], k[r], sum, dot);
-            sum = sum_over<L>(sum, s);
-            dot = sum_over<L>(dot, s + 4);
+            sum = norm_sum<L>(sum, s);
+            dot = norm_sum<L>(dot, s + 4);
             const float inv = 1.0f / sqrtf(sum / (float)width + a.eps);
             const float mean = dot * inv / (float)width;
 #pragma unroll
@@ -295,8 +280,8 @@ __global__ __launch_bounds__(NHIP_WG, 2) void norm_grad_kernel(nhip_norm_args a,
                 open(raw, k, u);
                 sums(c, u, w, k, sum, dot);
             }
-            sum = sum_over<L>(sum, s);
-            dot = sum_over<L>(dot, s + 4);
+            sum = norm_sum<L>(sum, s);
+            dot = norm_sum<L>(dot, s + 4);
             const float inv = 1.0f / sqrtf(sum / (float)width + a.eps);
             const float mean = dot * inv / (float)width;
             for (int c = lane * V; c < width; c += L * V) {
@@ -317,23 +302,6 @@ __global__ __launch_bounds__(NHIP_WG, 2) void norm_grad_kernel(nhip_norm_args a,
             }
         }
     }
-}
-
-// How a part of `width` channels is held, `per16` of them side by side in a lane (one where rows do not allow
-// wide reads): by a wave up to 128 times as many, by a group of four waves up to 1024 times; longer ones are read twice.
-template <class F> void with_shape(bool vec, int per16, int width, F&& f) {
-    const int v = vec ? per16 : 1;
-    auto go = [&](auto lanes, auto held) {
-        if (vec) f(std::true_type(), lanes, held);
-        else f(std::false_type(), lanes, held);
-    };
-    using std::integral_constant;
-    if (width <= 64 * v) go(integral_constant<int, 64>(), integral_constant<int, 1>());
-    else if (width <= 128 * v) go(integral_constant<int, 64>(), integral_constant<int, 2>());
-    else if (width <= 256 * v) go(integral_constant<int, 256>(), integral_constant<int, 1>());
-    else if (width <= 512 * v) go(integral_constant<int, 256>(), integral_constant<int, 2>());
-    else if (width <= 1024 * v) go(integral_constant<int, 256>(), integral_constant<int, 4>());
-    else go(integral_constant<int, 256>(), integral_constant<int, 0>());
 }
 
 // Whether every part of a row begins at a multiple of 16 bytes and holds whole packs of 16.  (The gradient's lanes, which
@@ -387,7 +355,7 @@ extern "C" int nhip_block_norm(void* stream, const nhip_norm_args* args) {
     sel_with_type(a.type, [&](auto t) {
         using T = decltype(t);
         constexpr int V16 = 16 / sizeof(T);
-        with_shape(wide(a), V16, width, [&](auto vec, auto lanes, auto held) {
+        norm_with_shape(wide(a), V16, width, [&](auto vec, auto lanes, auto held) {
             constexpr int V = decltype(vec)::value ? V16 : 1, L = decltype(lanes)::value, R = decltype(held)::value;
             const long long parts = a.rows * a.groups;
             constexpr int per = NHIP_WG / L;
@@ -425,7 +393,7 @@ extern "C" int nhip_block_norm_grad(void* stream, const nhip_norm_args* args) {
     sel_with_type(a.type, [&](auto t) {
         using T = decltype(t);
         constexpr int V16 = 4;  // (8 bytes of 16-bit types: what a lane holds of eight channels leaves too few waves)
-        with_shape(wide(a), V16, width, [&](auto vec, auto lanes, auto held) {
+        norm_with_shape(wide(a), V16, width, [&](auto vec, auto lanes, auto held) {
             constexpr int V = decltype(vec)::value ? V16 : 1, L = decltype(lanes)::value, R = decltype(held)::value;
             rows = sum_rows(a, groups_at_once<T, V, R>());
             NHIP_LAUNCH_FIRST((norm_grad_kernel<T, V, L, R>), dim3((unsigned)rows, (unsigned)a.groups),

@@ -1,0 +1,279 @@
+// The gated projection of a feed-forward block, y = act(x gate') (x up'), and its gradient:
+//
+//     g = x gate',  u = x up',  y = act(g) u
+//     dg = dy u act'(g),  du = dy act(g);   dx = dg gate + du up,   dgate = dg' x,   dup = du' x
+//
+// A wave's tile holds equal features of both weights, so that activation and product happen in its registers.  The
+// backward pass forms g and u again and keeps dg and du, in the type of x, for the two products that read them.
+#include "token_layout.h"
+
+namespace {
+
+constexpr long long kMostRows = 1 << 20, kMostChannels = 1 << 20, kMostFeatures = 1 << 20;
+
+// act(g) and its derivative
+__device__ __forceinline__ void activate(int kind, float g, float& f, float& slope) {
+    if (kind == NHIP_ACT_SILU) {
+        const float s = sel_sigmoid(g);
+        f = g * s;
+        slope = s * fmaf(g, 1.0f - s, 1.0f);
+    } else {
+        const float cdf = 0.5f * erfcf(g * -0.70710678118654752f);
+        f = g * cdf;
+        slope = fmaf(g * 0.39894228040143268f, sel_exp(-0.5f * g * g), cdf);
+    }
+}
+
+struct Forward {
+    void* y;
+    long long features, f0, n_features;  // of a row; the piece's first, and how many it has
+    int activation;
+    template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
+        constexpr int H = S::MI / 2;
+        const bool wide = tok_fours(y, features, sizeof(T));
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+            const long long n = (long long)at.n_tile * S::BN + at.wave_n * S::kWaveN + 16 * j + at.l;
+            if (n >= at.live) continue;
+            T* const to = static_cast<T*>(y) + n * features + f0;
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                const long long f = ((long long)at.m_tile * S::BM + at.wave_m * S::kWaveM) / 2 + 16 * i + 4 * at.g;
+                float v[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float act, slope;
+                    activate(activation, acc[i][j][r], act, slope);
+                    v[r] = act * acc[i + H][j][r];
+                }
+                if (wide && f + 4 <= n_features) {
+                    sel_store<T, 4>(to + f, v);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (f + r < n_features) to[f + r] = (T)v[r];
+                }
+            }
+        }
+    }
+};
+
+// dg and du of the tile, in both layouts: columns (rows) of du come `second` behind those of dg
+struct Backward {
+    const void* dy;
+    long long dy_ld, f0, n_features, second;
+    void *g, *gt;
+    long long g_ld, gt_ld;
+    int activation;
+    template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
+        constexpr int H = S::MI / 2;
+        const bool wide = tok_fours(dy, dy_ld, sizeof(T));
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+            const long long n = (long long)at.n_tile * S::BN + at.wave_n * S::kWaveN + 16 * j + at.l;
+            const bool counts = n < at.live;
+            const T* const from = static_cast<const T*>(dy) + (counts ? n : 0) * dy_ld + f0;
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                const long long f = ((long long)at.m_tile * S::BM + at.wave_m * S::kWaveM) / 2 + 16 * i + 4 * at.g;
+                float d[4], dg[4], du[4];
+                if (wide && f + 4 <= n_features) {
+                    sel_load<T, 4>(from + f, d);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) d[r] = f + r < n_features ? (float)from[f + r] : 0.0f;
+                }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    float act, slope;
+                    activate(activation, acc[i][j][r], act, slope);
+                    const bool is = counts && f + r < n_features;
+                    dg[r] = is ? d[r] * acc[i + H][j][r] * slope : 0.0f;
+                    du[r] = is ? d[r] * act : 0.0f;
+                }
+                T* const to = static_cast<T*>(g) + n * g_ld + f;
+                sel_store<T, 4>(to, dg);
+                sel_store<T, 4>(to + second, du);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    static_cast<T*>(gt)[(f + r) * gt_ld + n] = (T)dg[r];
+                    static_cast<T*>(gt)[(second + f + r) * gt_ld + n] = (T)du[r];
+                }
+            }
+        }
+    }
+};
+
+int check(const nhip_gated_args* a) {
+    if (!a || a->channels <= 0 || a->features <= 0 || a->rows < 0) return NHIP_E_BADARG;
+    if (a->type < NHIP_F32 || a->type > NHIP_F16) return NHIP_E_BADARG;
+    if (a->activation != NHIP_ACT_SILU && a->activation != NHIP_ACT_GELU) return NHIP_E_BADARG;
+    if (a->rows > kMostRows || a->channels > kMostChannels || a->features > kMostFeatures) return NHIP_E_BADARG;
+    return 0;
+}
+
+struct Space : TokSpace {
+    long long padded, x_ld, piece, g_ld, gt_ld, dx_ld;
+    long long x = 0, gate = 0, up = 0, xt, wt, g, gt, dx;
+    bool pad_x, pad_w;
+    TokCut cut;
+    Space(const nhip_gated_args& a, bool grad) {
+        const long long size = sel_size(a.type), d = a.channels, rows = a.rows > 0 ? a.rows : 1;
+        padded = tok_round(rows, TOK_MOST_TILE);
+        x_ld = tok_round(d, 64);
+        cut = tok_cut(a.rows, d, 2 * tok_round(a.features, 128), (int)size);  // rows of both weights, whole tiles of each
+        piece = cut.piece / 2;
+        if (!grad) {
+            // as many features as a launch's grid holds
+            const long long most = (1LL << 21) / (padded / 256) * 128;
+            piece = tok_round(a.features, 128) < most ? tok_round(a.features, 128) : most;
+        }
+        pad_x = !tok_rows_wide(a.x, a.x_stride * size, d * size);
+        pad_w = !tok_rows_wide(a.gate, a.gate_stride * size, d * size) || !tok_rows_wide(a.up, a.up_stride * size, d * size) ||
+                a.gate_stride != a.up_stride;
+        if (pad_x) x = take(rows * x_ld * size);
+        if (pad_w) {
+            gate = take(piece * x_ld * size);
+            up = take(piece * x_ld * size);
+        }
+        if (grad) {
+            g_ld = tok_ld(2 * piece);
+            gt_ld = tok_ld(padded);
+            dx_ld = tok_round(d, TOK_MOST_TILE);
+            xt = take(d * gt_ld * size);
+            wt = take(d * g_ld * size);
+            g = take(padded * g_ld * size);
+            gt = take(2 * piece * gt_ld * size);
+            dx = take(cut.splits * padded * dx_ld * 4);
+        }
+    }
+};
+
+#define TOK_TRY(call) do { if (int e_ = (call)) return e_; } while (0)
+
+// x as the products read it
+template <class T> int x_rows(hipStream_t st, const nhip_gated_args& a, const Space& s, char* w, TokRows& rows) {
+    rows = TokRows{static_cast<const char*>(a.x), nullptr, a.x_stride * (long long)sizeof(T), a.rows};
+    if (s.pad_x) {
+        TOK_TRY(tok_pad<T>(st, TokPad{a.x, a.x_stride, w + s.x, s.x_ld, a.rows, a.channels}));
+        rows.p = w + s.x;
+        rows.ld = s.x_ld * (long long)sizeof(T);
+    }
+    return 0;
+}
+
+// n features from f0 on, of both weights
+template <class T>
+int weight_rows(hipStream_t st, const nhip_gated_args& a, const Space& s, char* w, long long f0, long long n, TokRows& rows) {
+    const T* const gate = static_cast<const T*>(a.gate) + f0 * a.gate_stride;
+    const T* const up = static_cast<const T*>(a.up) + f0 * a.up_stride;
+    rows = TokRows{reinterpret_cast<const char*>(gate), reinterpret_cast<const char*>(up), a.gate_stride * (long long)sizeof(T), n};
+    if (s.pad_w) {
+        TOK_TRY(tok_pad<T>(st, TokPad{gate, a.gate_stride, w + s.gate, s.x_ld, n, a.channels}));
+        TOK_TRY(tok_pad<T>(st, TokPad{up, a.up_stride, w + s.up, s.x_ld, n, a.channels}));
+        rows.p = w + s.gate;
+        rows.p2 = w + s.up;
+        rows.ld = s.x_ld * (long long)sizeof(T);
+    }
+    return 0;
+}
+
+template <class T> int forward(hipStream_t st, const nhip_gated_args& a, const Space& s) {
+    char* const w = static_cast<char*>(a.workspace);
+    if (!a.rows) return 0;
+    TokRows x, rows;
+    TOK_TRY(x_rows<T>(st, a, s, w, x));
+    for (long long f0 = 0; f0 < a.features; f0 += s.piece) {
+        const long long n = a.features - f0 < s.piece ? a.features - f0 : s.piece;
+        TOK_TRY(weight_rows<T>(st, a, s, w, f0, n, rows));
+        TOK_TRY(tok_with_shape(2 * n, a.rows, [&](auto shape) {
+            using S = decltype(shape);
+            TokProduct p{rows, x, nullptr, nullptr, a.channels * (long long)sizeof(T), (int)((2 * n + S::BM - 1) / S::BM),
+                         (int)((a.rows + S::BN - 1) / S::BN), 1};
+            return tok_product<T, S, S::kWaveM / 2>(st, p, Forward{a.y, a.features, f0, n, a.activation});
+        }));
+    }
+    return 0;
+}
+
+template <class T> int backward(hipStream_t st, const nhip_gated_args& a, const Space& s) {
+    constexpr long long size = sizeof(T);
+    char* const w = static_cast<char*>(a.workspace);
+    const long long d = a.channels;
+    TokRows x, rows;
+    TOK_TRY(x_rows<T>(st, a, s, w, x));
+    TOK_TRY(tok_transpose<T>(st, TokTranspose{a.x, a.x_stride, w + s.xt, s.gt_ld, a.rows, d, s.padded, nullptr, 0}));
+    for (long long f0 = 0; f0 < a.features; f0 += s.piece) {
+        const long long n = a.features - f0 < s.piece ? a.features - f0 : s.piece;
+        // the second weights' part begins behind the last tile of the first one's, whose zeros lie between
+        const long long second = tok_round(n, tok_with_shape(2 * n, a.rows, [](auto shape) { return decltype(shape)::BM / 2; }));
+        const long long both = second + tok_round(n, 64);
+        TOK_TRY(weight_rows<T>(st, a, s, w, f0, n, rows));
+        if (a.rows)
+            TOK_TRY(tok_with_shape(2 * n, a.rows, [&](auto shape) {
+                using S = decltype(shape);
+                TokProduct p{rows, x, nullptr, nullptr, d * size, (int)((2 * n + S::BM - 1) / S::BM),
+                             (int)((a.rows + S::BN - 1) / S::BN), 1};
+                return tok_product<T, S, S::kWaveM / 2>(st, p, Backward{a.dy, a.dy_stride, f0, n, second, w + s.g, w + s.gt, s.g_ld,
+                                                                        s.gt_ld, a.activation});
+            }));
+        TOK_TRY(tok_with_shape(d, 2 * n, [&](auto shape) {
+            using S = decltype(shape);
+            TokProduct p{TokRows{w + s.xt, nullptr, s.gt_ld * size, d}, TokRows{w + s.gt, nullptr, s.gt_ld * size, second + n},
+                         nullptr, nullptr, a.rows * size, (int)((d + S::BM - 1) / S::BM), (int)((second + n + S::BN - 1) / S::BN), 1};
+            return tok_product<T, S, 0>(st, p, TokStoreRows{static_cast<T*>(a.dgate) + f0 * d, static_cast<T*>(a.dup) + f0 * d, d, n,
+                                                            second, nullptr});
+        }));
+        if (!a.rows) continue;
+        for (int k = 0; k < 2; ++k) {
+            const long long ld = k ? a.up_stride : a.gate_stride;
+            const T* const from = static_cast<const T*>(k ? a.up : a.gate) + f0 * ld;
+            TOK_TRY(tok_transpose<T>(st, TokTranspose{from, ld, static_cast<T*>(static_cast<void*>(w + s.wt)) + k * second, s.g_ld, n, d,
+                                                      k ? tok_round(n, 64) : second, nullptr, 0}));
+        }
+        TOK_TRY(tok_with_shape(d, a.rows, [&](auto shape) {
+            using S = decltype(shape);
+            TokProduct p{TokRows{w + s.wt, nullptr, s.g_ld * size, d}, TokRows{w + s.g, nullptr, s.g_ld * size, a.rows}, nullptr, nullptr,
+                         both * size, (int)((d + S::BM - 1) / S::BM), (int)((a.rows + S::BN - 1) / S::BN), s.cut.splits};
+            return tok_product<T, S, 0>(st, p, TokAddParts{reinterpret_cast<float*>(w + s.dx), s.dx_ld, s.padded * s.dx_ld, f0 > 0});
+        }));
+    }
+    return tok_join<T>(st, TokJoin{reinterpret_cast<float*>(w + s.dx), s.dx_ld, s.padded * s.dx_ld, s.cut.splits, nullptr, nullptr,
+                                   a.dx, a.rows, d});
+}
+
+int run(void* stream, const nhip_gated_args* args, bool grad) {
+    if (int e = check(args)) return e;
+    const nhip_gated_args& a = *args;
+    if (!a.gate || !a.up || (a.rows && !a.x)) return NHIP_E_BADARG;
+    if (grad ? !a.dgate || !a.dup || (a.rows && (!a.dy || !a.dx)) : a.rows && !a.y) return NHIP_E_BADARG;
+    const Space s(a, grad);
+    if (s.bytes > a.workspace_bytes) return NHIP_E_TOOBIG;
+    if (s.bytes && (!a.workspace || !sel_aligned(a.workspace, 256))) return NHIP_E_BADARG;
+    int rc = NHIP_E_BADARG;
+    sel_with_type(a.type, [&](auto t) {
+        using T = decltype(t);
+        rc = grad ? backward<T>(static_cast<hipStream_t>(stream), a, s) : forward<T>(static_cast<hipStream_t>(stream), a, s);
+    });
+    return rc;
+}
+
+}  // namespace
+
+extern "C" int nhip_gated_projection_workspace(const nhip_gated_args* args, long long* bytes_out) {
+    if (int e = check(args)) return e;
+    if (!bytes_out) return NHIP_E_BADARG;
+    *bytes_out = Space(*args, false).bytes;
+    return 0;
+}
+
+extern "C" int nhip_gated_projection(void* stream, const nhip_gated_args* args) { return run(stream, args, false); }
+
+extern "C" int nhip_gated_projection_grad_workspace(const nhip_gated_args* args, long long* bytes_out) {
+    if (int e = check(args)) return e;
+    if (!bytes_out) return NHIP_E_BADARG;
+    *bytes_out = Space(*args, true).bytes;
+    return 0;
+}
+
+extern "C" int nhip_gated_projection_grad(void* stream, const nhip_gated_args* args) { return run(stream, args, true); }

@@ -274,6 +274,25 @@ static inline int sel_reduce(hipStream_t stream, const SelReduce& a) {
     return 0;
 }
 
+// The LDS of a launch above 64 KiB has to be asked for, once per kernel and device (again with each call, which changes
+// nothing and costs less than to look it up): on the stream's device, which need not be the current one.
+template <class K> static inline int sel_allow_lds(hipStream_t stream, K kernel, size_t bytes) {
+    if (bytes <= 65536) return 0;
+    int current = 0;
+    hipDevice_t device = 0;
+    if (int e = (int)hipGetDevice(&current)) return e;
+    if (int e = (int)hipStreamGetDevice(stream, &device)) return e;
+    if (device != current)
+        if (int e = (int)hipSetDevice(device)) return e;
+    int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                      (int)bytes);
+    if (device != current) {
+        const int back = (int)hipSetDevice(current);
+        rc = rc ? rc : back;
+    }
+    return rc;
+}
+
 static inline bool sel_tokens_ok(const nhip_tokens& t) {
     if (t.n_seqs < 0 || t.n_tokens < 0 || t.n_tokens > SEL_MAX_TOKENS) return false;
     if (!t.starts) return t.length >= 0 && (long long)t.n_seqs * t.length == t.n_tokens;

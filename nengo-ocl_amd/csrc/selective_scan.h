@@ -618,25 +618,6 @@ static inline void sel_walk_place(const nhip_scan_args& a, SelWalkPlan& p, float
     p.keeps = space + sel_round4((long long)p.directions * p.n_segments * a.n_heads * a.dim * a.states);
 }
 
-// The LDS of a launch above 64 KiB has to be asked for, once per kernel and device (again with each call, which changes
-// nothing and costs less than to look it up): on the stream's device, which need not be the current one.
-template <class K> static inline int sel_allow_lds(hipStream_t stream, K kernel, size_t bytes) {
-    if (bytes <= 65536) return 0;
-    int current = 0;
-    hipDevice_t device = 0;
-    if (int e = (int)hipGetDevice(&current)) return e;
-    if (int e = (int)hipStreamGetDevice(stream, &device)) return e;
-    if (device != current)
-        if (int e = (int)hipSetDevice(device)) return e;
-    int rc = (int)hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                      (int)bytes);
-    if (device != current) {
-        const int back = (int)hipSetDevice(current);
-        rc = rc ? rc : back;
-    }
-    return rc;
-}
-
 // 16-bit floats have their own products on the matrix cores only in their own type; bfloat16's range does
 // not hold their precision, so they take the 32-bit ones.
 template <class T> struct SelCompute { using type = float; };

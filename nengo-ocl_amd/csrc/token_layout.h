@@ -1,0 +1,237 @@
+// Layouts that the products of token_products.h read: rows without the tokens that do not count, rows of whole stages,
+// transposed matrices; and the sum of the parts of a product's result.
+#pragma once
+
+#include "token_products.h"
+
+static inline long long tok_round(long long v, long long to) { return (v + to - 1) / to * to; }
+// Elements of a row in the workspace: rows whose distance is a power of two meet in few channels of the memory
+static inline long long tok_ld(long long v) { return tok_round(v, 64) + 64; }
+
+// Whether rows may be read 16 bytes at a time
+static inline bool tok_rows_wide(const void* p, long long ld_bytes, long long row_bytes) {
+    return sel_aligned(p, 16) && ld_bytes % 16 == 0 && row_bytes % 16 == 0;
+}
+
+// Whether rows of elements of `size` bytes may be read and written four at a time, from columns that are multiples of four
+static __host__ __device__ __forceinline__ bool tok_fours(const void* p, long long ld, int size) {
+    return ld % 4 == 0 && (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(4 * size - 1)) == 0;
+}
+
+// Offsets of a workspace
+struct TokSpace {
+    long long bytes = 0;
+    long long take(long long n) {
+        const long long at = bytes;
+        bytes += tok_round(n, 256);
+        return at;
+    }
+};
+
+// ------------------------------------------------------------------------------------ transposed
+// out[c, r] = in[r, c] for r < rows (or *live of them) and c < cols; zeros for rows up to out_rows (a multiple of 64).
+struct TokTranspose {
+    const void* in;
+    long long ld;
+    void* out;
+    long long out_ld;
+    long long rows, cols, out_rows;
+    const int* live;
+    int wide;
+};
+
+template <class T> __global__ __launch_bounds__(NHIP_WG) void tok_transpose_kernel(TokTranspose a) {
+    constexpr int V = 16 / (int)sizeof(T), kPacks = 64 / V;
+    __shared__ T s[64][64 + 2];
+    const long long r0 = (long long)blockIdx.x * 64, c0 = (long long)blockIdx.y * 64;
+    const long long rows = a.live ? min((long long)*a.live, a.rows) : a.rows;
+    const T* const in = static_cast<const T*>(a.in);
+    for (int q = threadIdx.x; q < 64 * kPacks; q += NHIP_WG) {
+        const int r = q / kPacks, c = q % kPacks * V;
+        SelPack<T, V> v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v.v[e] = (T)0.0f;
+        if (r0 + r < rows) {
+            const T* const from = in + (r0 + r) * a.ld + c0 + c;
+            if (a.wide && c0 + c + V <= a.cols) {
+                v = *reinterpret_cast<const SelPack<T, V>*>(from);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e)
+                    if (c0 + c + e < a.cols) v.v[e] = from[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) s[c + e][r] = v.v[e];
+    }
+    __syncthreads();
+    T* const out = static_cast<T*>(a.out);
+    for (int q = threadIdx.x; q < 64 * kPacks; q += NHIP_WG) {
+        const int c = q / kPacks, r = q % kPacks * V;
+        if (c0 + c >= a.cols) continue;
+        SelPack<T, V> v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v.v[e] = s[c][r + e];
+        *reinterpret_cast<SelPack<T, V>*>(out + (c0 + c) * a.out_ld + r0 + r) = v;
+    }
+}
+
+template <class T> static inline int tok_transpose(hipStream_t stream, TokTranspose a) {
+    if (a.cols <= 0 || a.out_rows <= 0) return 0;
+    const long long x = a.out_rows / 64, y = (a.cols + 63) / 64;
+    if (x > 0xffffff || y > SEL_MAX_GRID_Y) return NHIP_E_BADARG;
+    a.wide = tok_rows_wide(a.in, a.ld * (long long)sizeof(T), 16);
+    NHIP_LAUNCH((tok_transpose_kernel<T>), dim3((unsigned)x, (unsigned)y), dim3(NHIP_WG), 0, stream, a);
+    NHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+// ------------------------------------------------------------------------------- rows of whole stages
+// out[r, c] = in[r, c], zeros for c up to out_ld (a multiple of 64)
+struct TokPad {
+    const void* in;
+    long long ld;
+    void* out;
+    long long out_ld, rows, cols;
+};
+
+template <class T> __global__ __launch_bounds__(NHIP_WG) void tok_pad_kernel(TokPad a) {
+    constexpr int V = 16 / (int)sizeof(T);
+    const long long packs = a.out_ld / V, all = a.rows * packs;
+    for (long long q = (long long)blockIdx.x * NHIP_WG + threadIdx.x; q < all; q += (long long)gridDim.x * NHIP_WG) {
+        const long long r = q / packs, c = q % packs * V;
+        const T* const from = static_cast<const T*>(a.in) + r * a.ld + c;
+        SelPack<T, V> v;
+#pragma unroll
+        for (int e = 0; e < V; ++e) v.v[e] = c + e < a.cols ? from[e] : (T)0.0f;
+        *reinterpret_cast<SelPack<T, V>*>(static_cast<T*>(a.out) + r * a.out_ld + c) = v;
+    }
+}
+
+template <class T> static inline int tok_pad(hipStream_t stream, const TokPad& a) {
+    if (a.rows <= 0) return 0;
+    const long long groups = (a.rows * (a.out_ld * (long long)sizeof(T) / 16) + NHIP_WG - 1) / NHIP_WG;
+    NHIP_LAUNCH((tok_pad_kernel<T>), dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(NHIP_WG), 0, stream, a);
+    NHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+// --------------------------------------------------------------------------- gradients of x and of the weights
+// dW[w, d] = sum_n G[n, w] x[n, d] for the rows w of a piece of the weights: rows below `first` of them go to out, those from
+// `second` on (the other weights of a gated projection) to out2.
+struct TokStoreRows {
+    void *out, *out2;
+    long long ld, rows, second;  // ld: elements of a row of the result, its channels; rows: of each
+    const float* scale;          // 1 / that of G, or NULL
+    template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
+        const float k = scale ? *scale : 1.0f;
+        const bool wide = tok_fours(out, ld, sizeof(T)) && (!out2 || tok_fours(out2, ld, sizeof(T)));
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+            long long w = (long long)at.n_tile * S::BN + at.wave_n * S::kWaveN + 16 * j + at.l;
+            T* to = static_cast<T*>(out);
+            if (second && w >= second) {
+                w -= second;
+                to = static_cast<T*>(out2);
+            }
+            if (w >= rows) continue;
+            to += w * ld;
+#pragma unroll
+            for (int i = 0; i < S::MI; ++i) {
+                const long long d = (long long)at.m_tile * S::BM + at.wave_m * S::kWaveM + 16 * i + 4 * at.g;
+                const float v[4] = {acc[i][j][0] * k, acc[i][j][1] * k, acc[i][j][2] * k, acc[i][j][3] * k};
+                if (wide && d + 4 <= ld) {
+                    sel_store<T, 4>(to + d, v);
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (d + r < ld) to[d + r] = (T)v[r];
+                }
+            }
+        }
+    }
+};
+
+// dx[n, d] = sum_w G[n, w] W[w, d], added up over pieces of the weights in 32 bits, in parts (splits of k)
+struct TokAddParts {
+    float* parts;
+    long long ld, part;  // elements of a row, of a part
+    int add;
+    template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
+        float* const mine = parts + at.split * part;
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+            const long long n = (long long)at.n_tile * S::BN + at.wave_n * S::kWaveN + 16 * j + at.l;
+            if (n >= at.live) continue;
+#pragma unroll
+            for (int i = 0; i < S::MI; ++i) {
+                const long long d = (long long)at.m_tile * S::BM + at.wave_m * S::kWaveM + 16 * i + 4 * at.g;
+                sel_f4* const to = reinterpret_cast<sel_f4*>(mine + n * ld + d);
+                *to = add ? *to + acc[i][j] : acc[i][j];
+            }
+        }
+    }
+};
+
+// dx[r] = the sum of the parts of row where[r] (zeros where it is below zero; NULL: r)
+struct TokJoin {
+    const float* parts;
+    long long ld, part;
+    int n_parts;
+    const int* where;
+    const float* scale;
+    void* out;
+    long long rows, cols;
+};
+
+template <class T, int V> __global__ __launch_bounds__(NHIP_WG) void tok_join_kernel(TokJoin a) {
+    const float k = a.scale ? *a.scale : 1.0f;
+    const long long packs = (a.cols + V - 1) / V, all = a.rows * packs;
+    for (long long q = (long long)blockIdx.x * NHIP_WG + threadIdx.x; q < all; q += (long long)gridDim.x * NHIP_WG) {
+        const long long r = q / packs, c = q % packs * V, from = a.where ? a.where[r] : r;
+        float v[V], sum[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] = 0.0f;
+        if (from >= 0) {
+            const float* p = a.parts + from * a.ld + c;
+            for (int s = 0; s < a.n_parts; ++s) {
+                sel_load<float, V>(p + s * a.part, v);
+#pragma unroll
+                for (int e = 0; e < V; ++e) sum[e] += v[e];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) sum[e] *= k;
+        sel_store<T, V>(static_cast<T*>(a.out) + r * a.cols + c, sum);
+    }
+}
+
+template <class T> static inline int tok_join(hipStream_t stream, const TokJoin& a) {
+    if (a.rows <= 0) return 0;
+    const int v = tok_fours(a.out, a.cols, sizeof(T)) ? 4 : 1;
+    const long long groups = (a.rows * (a.cols / v) + NHIP_WG - 1) / NHIP_WG;
+    const dim3 grid((unsigned)(groups < 16384 ? groups : 16384));
+    if (v == 4) NHIP_LAUNCH((tok_join_kernel<T, 4>), grid, dim3(NHIP_WG), 0, stream, a);
+    else NHIP_LAUNCH((tok_join_kernel<T, 1>), grid, dim3(NHIP_WG), 0, stream, a);
+    NHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+// How the gradient's work is cut: pieces of `piece` weights' rows (a multiple of 256), the dx product in `splits` parts of k
+struct TokCut {
+    long long piece;
+    int splits;
+};
+static inline TokCut tok_cut(long long rows, long long channels, long long weights, int size) {
+    TokCut c;
+    const long long padded = tok_round(rows > 0 ? rows : 1, 256);
+    long long most = (512LL << 20) / (padded * size) / 256 * 256;
+    most = most < 256 ? 256 : most;
+    const long long pieces = (weights + most - 1) / most;
+    c.piece = tok_round((weights + pieces - 1) / pieces, 256);
+    const long long tiles = ((channels + 127) / 128) * ((rows + 127) / 128), stages = c.piece * size / TOK_KB;
+    long long s = 1;
+    while (s < 64 && tiles * s * 2 <= 512 && stages / (s * 2) >= 16 && s * 2 * padded * tok_round(channels, 256) * 4 <= (256LL << 20)) s *= 2;
+    c.splits = (int)s;
+    return c;
+}

@@ -1,0 +1,656 @@
+// Losses over a vocabulary, and their gradients, without the logits in memory:
+//
+//     z[n, v] = x[n] . weight[v] / temperature,   lse[n] = log sum_v exp(z[n, v])
+//     loss[n] = lse[n] - z[n, label[n]],  or  sum_k q[n, k] (log q[n, k] - z[n, word[n, k]] + lse[n])
+//     G[n, v] = dloss[n] / temperature (exp(z[n, v] - lse[n]) - q[n, v]),   dx = G weight,   dweight = G' x
+//
+// The forward pass forms tiles of z and leaves of each the maximum and the sum of a token's exponentials and the
+// logits of its targets.  The backward pass goes over the vocabulary in pieces: a piece's part of G is formed from z again and kept,
+// in the type of x, for the two products that read it.
+#include "token_layout.h"
+
+namespace {
+
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
+constexpr int kNoWord = 0x7fffffff;
+constexpr int kMostTop = 256;
+constexpr long long kMostRows = 1 << 20, kMostChannels = 1 << 20;
+
+__device__ __forceinline__ long long word_at(const void* p, int wide, long long i) {
+    return wide ? static_cast<const long long*>(p)[i] : (long long)static_cast<const int*>(p)[i];
+}
+
+// ------------------------------------------------------------------------- a teacher's shares
+// A wave takes a row: shares of its entries, sorted by word, equal words added up, so that a tile finds its targets in one
+// range and no element of G has two.
+struct Shares {
+    const void *words, *logits;
+    int wide, logits_type, top, n_words;
+    long long rows;
+    float per_temperature;
+    int* word;      // [rows, top], kNoWord behind the last
+    float* share;
+    float* self;    // sum q log q
+    int* flag;      // 0: the row counts, -1: it has no entries
+};
+
+template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares a) {
+    constexpr int kMost = Q * NHIP_WAVE;
+    __shared__ int s_word[4][kMost], s_sorted[4][kMost];
+    __shared__ float s_share[4][kMost], s_sorted_share[4][kMost];
+    const int wave = threadIdx.x / NHIP_WAVE, lane = threadIdx.x % NHIP_WAVE;
+    const long long row = (long long)blockIdx.x * 4 + wave, r = min(row, a.rows - 1);
+    int id[Q];
+    float t[Q];
+    float most = -INFINITY;
+    bool nan = false;
+    int any = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int e = lane + q * NHIP_WAVE;
+        id[q] = kNoWord;
+        t[q] = -INFINITY;
+        if (e < a.top) {
+            const long long w = word_at(a.words, a.wide, r * a.top + e);
+            const float v = sel_element(a.logits, a.logits_type, r * a.top + e) * a.per_temperature;
+            if (w >= 0 && w < a.n_words && !(v == -INFINITY)) {
+                id[q] = (int)w;
+                t[q] = v;
+                any = 1;
+            }
+        }
+        nan |= t[q] != t[q];
+        most = fmaxf(most, t[q]);
+    }
+#pragma unroll
+    for (int d = 1; d < NHIP_WAVE; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+    any = __any(any);
+    nan = __any(nan);
+    float sum = 0.0f, x[Q];
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        x[q] = id[q] == kNoWord ? 0.0f : sel_exp(t[q] - most);
+        sum += x[q];
+    }
+    sum = sel_wave_sum(sum);
+    if (nan) sum = NAN;
+    const float log_sum = logf(sum);
+    float self = 0.0f;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int e = lane + q * NHIP_WAVE;
+        const float share = id[q] == kNoWord ? 0.0f : x[q] / sum;
+        self += share == 0.0f ? 0.0f : share * (t[q] - most - log_sum);
+        s_word[wave][e] = id[q];
+        s_share[wave][e] = x[q] = share;
+    }
+    self = sel_wave_sum(self);
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int e = lane + q * NHIP_WAVE;
+        int rank = 0;
+        for (int o = 0; o < kMost; ++o) {
+            const int w = s_word[wave][o];
+            rank += w < id[q] || (w == id[q] && o < e);
+        }
+        s_sorted[wave][rank] = id[q];
+        s_sorted_share[wave][rank] = x[q];
+    }
+    __syncthreads();
+    if (row >= a.rows) return;
+    int before = 0;
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int e = lane + q * NHIP_WAVE, w = s_sorted[wave][e];
+        const bool first = w != kNoWord && (e == 0 || s_sorted[wave][e - 1] != w);
+        const unsigned long long all = __ballot(first);
+        if (first) {
+            float share = s_sorted_share[wave][e];
+            for (int o = e + 1; o < kMost && s_sorted[wave][o] == w; ++o) share += s_sorted_share[wave][o];
+            const int at = before + __popcll(all & ((1ULL << lane) - 1));
+            a.word[row * a.top + at] = w;
+            a.share[row * a.top + at] = share;
+        }
+        before += __popcll(all);
+    }
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        const int e = lane + q * NHIP_WAVE;
+        if (e >= before && e < a.top) {
+            a.word[row * a.top + e] = kNoWord;
+            a.share[row * a.top + e] = 0.0f;
+        }
+    }
+    if (lane == 0) {
+        a.self[row] = self;
+        a.flag[row] = any ? 0 : -1;
+    }
+}
+
+// ------------------------------------------------------------------------------ rows that count
+// The rows whose label is a word move together, rows of whole stages.  A group takes 64 rows and counts those before them itself
+// (8192 labels are 64 KB in the L2; a launch of its own for the sums would take longer).
+struct Gather {
+    const void *x, *labels;
+    int wide_labels, n_words, type, wide;
+    long long ld, rows;
+    int channels, out_ld;
+    void* out;
+    int *row, *where, *label, *count;  // [rows padded], [rows], [rows padded], 1
+    float *loss, *lse;                 // zeros where a row does not count; NULL in the backward pass
+};
+constexpr int kGatherRows = 64;
+
+template <class T> __global__ __launch_bounds__(NHIP_WG) void gather_kernel(Gather a) {
+    constexpr int V = 16 / (int)sizeof(T);
+    __shared__ int s_sum[4], s_at[kGatherRows];
+    const int wave = threadIdx.x / NHIP_WAVE, lane = threadIdx.x % NHIP_WAVE;
+    const long long r0 = (long long)blockIdx.x * kGatherRows;
+    auto label_of = [&](long long r) {
+        const long long w = word_at(a.labels, a.wide_labels, r);
+        return w >= 0 && w < a.n_words ? (int)w : -1;
+    };
+    int sum = 0;
+    for (long long r = threadIdx.x; r < r0; r += NHIP_WG) sum += label_of(r) >= 0;
+#pragma unroll
+    for (int d = 1; d < NHIP_WAVE; d *= 2) sum += __shfl_xor(sum, d);
+    if (lane == 0) s_sum[wave] = sum;
+    __syncthreads();
+    const int before = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+    if (wave == 0) {
+        const long long r = r0 + lane;
+        const int label = r < a.rows ? label_of(r) : -1;
+        const unsigned long long all = __ballot(label >= 0);
+        const int at = before + __popcll(all & ((1ULL << lane) - 1));
+        s_at[lane] = label >= 0 ? at : -1;
+        if (label >= 0) {
+            a.row[at] = (int)r;
+            a.label[at] = label;
+        }
+        if (r < a.rows) {
+            a.where[r] = label >= 0 ? at : -1;
+            if (a.loss && label < 0) a.loss[r] = a.lse[r] = 0.0f;
+        }
+        if (blockIdx.x == gridDim.x - 1 && lane == 0) *a.count = before + __popcll(all);
+    }
+    __syncthreads();
+    for (int k = wave; k < kGatherRows; k += 4) {
+        const int at = s_at[k];
+        if (at < 0) continue;
+        const T* const from = static_cast<const T*>(a.x) + (r0 + k) * a.ld;
+        T* const to = static_cast<T*>(a.out) + (long long)at * a.out_ld;
+        for (int c = lane * V; c < a.out_ld; c += NHIP_WAVE * V) {
+            SelPack<T, V> v;
+            if (a.wide && c + V <= a.channels) {
+                v = *reinterpret_cast<const SelPack<T, V>*>(from + c);
+            } else {
+#pragma unroll
+                for (int e = 0; e < V; ++e) v.v[e] = c + e < a.channels ? from[c + e] : (T)0.0f;
+            }
+            *reinterpret_cast<SelPack<T, V>*>(to + c) = v;
+        }
+    }
+}
+
+// What G is scaled by in float16, whose range does not hold the gradient of a mean over many tokens: a power of two that
+// brings its largest magnitude to 2^13 ... 2^14; and the reverse.
+__global__ __launch_bounds__(1024) void scale_kernel(const float* dloss, const int* row, const int* count, float per_temperature,
+                                                     float* scale) {
+    __shared__ float s[16];
+    float most = 0.0f;
+    for (int n = threadIdx.x; n < *count; n += 1024) {
+        const float v = fabsf(dloss[row[n]] * per_temperature);
+        if (v < INFINITY) most = fmaxf(most, v);
+    }
+#pragma unroll
+    for (int d = 1; d < NHIP_WAVE; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
+    if (threadIdx.x % NHIP_WAVE == 0) s[threadIdx.x / NHIP_WAVE] = most;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int w = 1; w < 16; ++w) most = fmaxf(most, s[w]);
+        int e = 14;
+        if (most > 0.0f) frexpf(most, &e);
+        e = e < -100 ? -100 : e > 100 ? 100 : e;
+        scale[0] = ldexpf(1.0f, 14 - e);
+        scale[1] = ldexpf(1.0f, e - 14);
+    }
+}
+
+// ----------------------------------------------------------------------------------- tiles of z
+struct Targets {
+    const int* label;   // [live], or
+    const int* word;    // [rows, top], sorted, with
+    const float* share;
+    const int* row;     // of a live token
+    int top;
+};
+
+// Where the targets of the tile's tokens lie among their sorted entries: [lo, hi), for the BN tokens from n0
+template <class S>
+__device__ __forceinline__ void find_targets(const Targets& t, long long n0, int live, int w0, int w1, int* lo, int* hi) {
+    const int wave = threadIdx.x / NHIP_WAVE, lane = threadIdx.x % NHIP_WAVE;
+    for (int k = wave; k < S::BN; k += S::kWaves) {
+        int below = 0, above = 0;
+        if (n0 + k < live) {
+            const int* const from = t.word + (long long)t.row[n0 + k] * t.top;
+            for (int e = lane; e < t.top; e += NHIP_WAVE) {
+                const int w = from[e];
+                below += w < w0;
+                above += w < w1;
+            }
+        }
+#pragma unroll
+        for (int d = 1; d < NHIP_WAVE; d *= 2) {
+            below += __shfl_xor(below, d);
+            above += __shfl_xor(above, d);
+        }
+        if (lane == 0) {
+            lo[k] = below;
+            hi[k] = above;
+        }
+    }
+}
+
+// Forward: of each token in the tile the maximum of z and the sum of exp(z - maximum), in powers of two, and the logits of
+// its targets.
+template <bool TOP> struct Statistics {
+    Targets targets;
+    float2* part;      // [tiles of the whole vocabulary, ld]
+    float* logits;     // [live, top]
+    long long ld;
+    int words, word0, tile0;  // words of the piece, its first word, its first tile
+    float per_temperature;
+
+    template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
+        float2* const s_part = reinterpret_cast<float2*>(at.lds);              // [WM][BN]
+        int* const s_lo = reinterpret_cast<int*>(s_part + S::WM * S::BN), *const s_hi = s_lo + S::BN;
+        const long long n0 = (long long)at.n_tile * S::BN;
+        const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g;  // within the piece
+        __syncthreads();
+        if constexpr (TOP) {
+            find_targets<S>(targets, n0, at.live, word0 + at.m_tile * S::BM, word0 + (at.m_tile + 1) * S::BM, s_lo, s_hi);
+            __syncthreads();
+        }
+        const float c = kLog2e * per_temperature;
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+            const int local = at.wave_n * S::kWaveN + 16 * j + at.l;
+            const long long n = n0 + local;
+            float most = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (m0 + 16 * i + r < words) most = fmaxf(most, acc[i][j][r]);
+            most = fmaxf(most, __shfl_xor(most, 16));
+            most = fmaxf(most, __shfl_xor(most, 32));
+            float top2 = most * c;
+            if (!(fabsf(top2) < INFINITY)) top2 = 0.0f;  // (infinities then reach the sum as they are)
+            float sum = 0.0f;
+#pragma unroll
+            for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    if (m0 + 16 * i + r < words) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -top2));
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (at.g == 0) s_part[at.wave_m * S::BN + local] = float2{top2, sum};
+            auto pick = [&](int word, float* to) {
+                const int rel = word - word0 - m0;
+                if (rel < 0 || rel >= S::kWaveM || (rel & 15) >= 4) return;
+#pragma unroll
+                for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (rel == 16 * i + r) *to = acc[i][j][r] * per_temperature;
+            };
+            if (n < at.live) {
+                if constexpr (TOP) {
+                    const long long from = (long long)targets.row[n] * targets.top;
+                    for (int k = s_lo[local]; k < s_hi[local]; ++k) pick(targets.word[from + k], logits + n * targets.top + k);
+                } else {
+                    pick(targets.label[n], logits + n);
+                }
+            }
+        }
+        __syncthreads();
+        for (int k = threadIdx.x; k < S::BN; k += S::kThreads) {
+            float2 a = s_part[k];
+#pragma unroll
+            for (int w = 1; w < S::WM; ++w) a = joined(a, s_part[w * S::BN + k]);
+            if (n0 + k < at.live) part[(long long)(tile0 + at.m_tile) * ld + n0 + k] = a;
+        }
+    }
+    // of two parts, neither of which is more than infinite
+    static __device__ __forceinline__ float2 joined(float2 a, float2 b) {
+        if (b.y == 0.0f) return a;
+        if (a.y == 0.0f) return b;
+        const float top = fmaxf(a.x, b.x);
+        const float x = a.y == INFINITY ? a.y : a.y * __builtin_amdgcn_exp2f(a.x - top);
+        const float y = b.y == INFINITY ? b.y : b.y * __builtin_amdgcn_exp2f(b.x - top);
+        return float2{top, x + y};
+    }
+};
+
+// loss and lse of the live tokens: 16 lanes to a token
+struct Finish {
+    const float2* part;
+    const float* logits;
+    Targets targets;
+    const float* self;
+    const int* count;
+    long long ld;
+    int tiles;
+    float *loss, *lse;
+};
+
+__global__ __launch_bounds__(NHIP_WG) void finish_kernel(Finish a) {
+    __shared__ float2 s[16][16];
+    __shared__ float s_loss[16][16];
+    const int k = threadIdx.x % 16, q = threadIdx.x / 16, live = *a.count;
+    if ((long long)blockIdx.x * 16 >= live) return;
+    const int n = min((int)blockIdx.x * 16 + k, live - 1), row = a.targets.row[n];
+    float2 v = {0.0f, 0.0f};
+    for (int t = q; t < a.tiles; t += 16) v = Statistics<false>::joined(v, a.part[(long long)t * a.ld + n]);
+    s[q][k] = v;
+    __syncthreads();
+    v = s[0][k];
+#pragma unroll
+    for (int o = 1; o < 16; ++o) v = Statistics<false>::joined(v, s[o][k]);
+    const float lse = (v.x + __builtin_amdgcn_logf(v.y)) * kLn2;
+    float loss = 0.0f;
+    if (a.targets.top) {
+        for (int e = q; e < a.targets.top; e += 16) {
+            const long long at = (long long)row * a.targets.top + e;
+            if (a.targets.word[at] != kNoWord) {
+                const float share = a.targets.share[at];
+                loss += share == 0.0f ? 0.0f : share * (lse - a.logits[(long long)n * a.targets.top + e]);
+            }
+        }
+        s_loss[q][k] = loss;
+        __syncthreads();
+        loss = a.self[row];
+#pragma unroll
+        for (int o = 0; o < 16; ++o) loss += s_loss[o][k];
+    } else {
+        loss = lse - a.logits[n];
+    }
+    if (q == 0 && (int)blockIdx.x * 16 + k < live) {
+        a.loss[row] = loss;
+        a.lse[row] = lse;
+    }
+}
+
+// Backward: G of the tile, in both layouts
+template <bool TOP> struct Gradient {
+    Targets targets;
+    const float *dloss, *lse, *scale;
+    void *g, *gt;             // [live, g_ld], [words, gt_ld]
+    long long g_ld, gt_ld;
+    int words, word0;
+    float per_temperature;
+
+    template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
+        int* const s_lo = reinterpret_cast<int*>(at.lds), *const s_hi = s_lo + S::BN;
+        const long long n0 = (long long)at.n_tile * S::BN;
+        const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g;
+        if constexpr (TOP) {
+            __syncthreads();
+            find_targets<S>(targets, n0, at.live, word0 + at.m_tile * S::BM, word0 + (at.m_tile + 1) * S::BM, s_lo, s_hi);
+            __syncthreads();
+        }
+        const float c = kLog2e * per_temperature, k = scale ? *scale * per_temperature : per_temperature;
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+            const int local = at.wave_n * S::kWaveN + 16 * j + at.l;
+            const long long n = n0 + local;
+            const bool counts = n < at.live;
+            const int row = counts ? targets.row[n] : 0;
+            const float d = counts ? dloss[row] * k : 0.0f, lse2 = counts ? lse[row] * kLog2e : 0.0f;
+#pragma unroll
+            for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    acc[i][j][r] = counts && m0 + 16 * i + r < words ? d * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -lse2)) : 0.0f;
+            auto take = [&](int word, float share) {
+                const int rel = word - word0 - m0;
+                if (rel < 0 || rel >= S::kWaveM || (rel & 15) >= 4) return;
+#pragma unroll
+                for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (rel == 16 * i + r) acc[i][j][r] -= d * share;
+            };
+            if (counts) {
+                if constexpr (TOP) {
+                    const long long from = (long long)row * targets.top;
+                    for (int e = s_lo[local]; e < s_hi[local]; ++e) take(targets.word[from + e], targets.share[from + e]);
+                } else {
+                    take(targets.label[n], 1.0f);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < S::MI; ++i) {
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                sel_store<T, 4>(static_cast<T*>(g) + n * g_ld + m0 + 16 * i, v);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) static_cast<T*>(gt)[(m0 + 16 * i + r) * gt_ld + n] = (T)v[r];
+            }
+        }
+    }
+};
+
+// --------------------------------------------------------------------------------------- host
+int check(const nhip_loss_args* a) {
+    if (!a || a->channels <= 0 || a->words <= 0 || a->rows < 0 || a->top < 0) return NHIP_E_BADARG;
+    if (a->type < NHIP_F32 || a->type > NHIP_F16 || a->rows > kMostRows || a->top > kMostTop) return NHIP_E_BADARG;
+    if (a->top && (a->logits_type < NHIP_F32 || a->logits_type > NHIP_F16)) return NHIP_E_BADARG;
+    if (!(a->temperature > 0.0f) || !(a->temperature < INFINITY)) return NHIP_E_BADARG;
+    if (a->words > kNoWord - 4096 || a->channels > kMostChannels) return NHIP_E_BADARG;
+    return 0;
+}
+
+bool wide_weight(const nhip_loss_args& a) {
+    const long long size = sel_size(a.type);
+    return tok_rows_wide(a.weight, a.weight_stride * size, a.channels * size);
+}
+
+struct Space : TokSpace {
+    long long padded, x_ld, piece, g_ld, gt_ld, dx_ld;
+    long long row, where, label, count, flag, word, share, self, x, weight, part, logits, xt, wt, g, gt, dx;
+    TokCut cut;
+    Space(const nhip_loss_args& a, bool grad) {
+        const long long size = sel_size(a.type), rows = a.rows > 0 ? a.rows : 1, top = a.top;
+        padded = tok_round(rows, TOK_MOST_TILE);
+        x_ld = tok_round(a.channels, 64);
+        cut = tok_cut(a.rows, a.channels, a.words, (int)size);
+        piece = cut.piece;
+        row = take(padded * 4);
+        where = take(rows * 4);
+        label = take(padded * 4);
+        count = take(256);
+        flag = word = share = self = 0;
+        if (top) {
+            flag = take(rows * 4);
+            word = take(rows * top * 4);
+            share = take(rows * top * 4);
+            self = take(rows * 4);
+        }
+        x = take(padded * x_ld * size);
+        weight = wide_weight(a) ? 0 : take(piece * x_ld * size);
+        if (!grad) {
+            part = take((tok_round(a.words, piece) / TOK_LEAST_BM) * padded * 8);
+            logits = take(padded * (top ? top : 1) * 4);
+        } else {
+            g_ld = tok_ld(piece);
+            gt_ld = tok_ld(padded);
+            dx_ld = tok_round(a.channels, TOK_MOST_TILE);
+            xt = take((long long)a.channels * gt_ld * size);
+            wt = take((long long)a.channels * g_ld * size);
+            g = take(padded * g_ld * size);
+            gt = take(piece * gt_ld * size);
+            dx = take(cut.splits * padded * dx_ld * 4);
+        }
+    }
+};
+
+#define TOK_TRY(call) do { if (int e_ = (call)) return e_; } while (0)
+
+// The rows that count, and the targets of all rows
+template <class T> int prepare(hipStream_t st, const nhip_loss_args& a, const Space& s, char* w, bool grad, Targets& t) {
+    t = Targets{reinterpret_cast<int*>(w + s.label), reinterpret_cast<int*>(w + s.word), reinterpret_cast<float*>(w + s.share),
+                reinterpret_cast<int*>(w + s.row), a.top};
+    Gather gather{a.x, a.targets, a.wide_targets, a.words, a.type, 0, a.x_stride, a.rows, a.channels, (int)s.x_ld, w + s.x,
+                  reinterpret_cast<int*>(w + s.row), reinterpret_cast<int*>(w + s.where), reinterpret_cast<int*>(w + s.label),
+                  reinterpret_cast<int*>(w + s.count), grad ? nullptr : a.loss, grad ? nullptr : a.lse};
+    gather.wide = tok_rows_wide(a.x, a.x_stride * (long long)sizeof(T), 16);
+    if (a.top && a.rows) {
+        Shares sh{a.targets, a.target_logits, a.wide_targets, a.logits_type, a.top, a.words, a.rows, 1.0f / a.temperature,
+                  reinterpret_cast<int*>(w + s.word), reinterpret_cast<float*>(w + s.share), reinterpret_cast<float*>(w + s.self),
+                  reinterpret_cast<int*>(w + s.flag)};
+        const dim3 grid((unsigned)((a.rows + 3) / 4));
+        if (a.top <= 64) NHIP_LAUNCH((shares_kernel<1>), grid, dim3(NHIP_WG), 0, st, sh);
+        else if (a.top <= 128) NHIP_LAUNCH((shares_kernel<2>), grid, dim3(NHIP_WG), 0, st, sh);
+        else NHIP_LAUNCH((shares_kernel<4>), grid, dim3(NHIP_WG), 0, st, sh);
+        NHIP_LAUNCH_CHECK();
+        gather.labels = w + s.flag;  // 0 or -1
+        gather.wide_labels = 0;
+    }
+    const long long groups = (a.rows + kGatherRows - 1) / kGatherRows;
+    NHIP_LAUNCH((gather_kernel<T>), dim3((unsigned)(groups ? groups : 1)), dim3(NHIP_WG), 0, st, gather);
+    NHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+// The rows of a piece of the weights as the products read them
+template <class T> int piece_rows(hipStream_t st, const nhip_loss_args& a, const Space& s, char* w, long long v0, long long words,
+                                  TokRows& rows) {
+    const T* const from = static_cast<const T*>(a.weight) + v0 * a.weight_stride;
+    rows = TokRows{reinterpret_cast<const char*>(from), nullptr, a.weight_stride * (long long)sizeof(T), words};
+    if (s.weight) {
+        TOK_TRY(tok_pad<T>(st, TokPad{from, a.weight_stride, w + s.weight, s.x_ld, words, a.channels}));
+        rows.p = w + s.weight;
+        rows.ld = s.x_ld * (long long)sizeof(T);
+    }
+    return 0;
+}
+
+template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Space& s) {
+    char* const w = static_cast<char*>(a.workspace);
+    Targets t;
+    TOK_TRY(prepare<T>(st, a, s, w, false, t));
+    const int* const count = reinterpret_cast<int*>(w + s.count);
+    int tiles = 0;
+    for (long long v0 = 0; v0 < a.words; v0 += s.piece) {
+        const long long words = a.words - v0 < s.piece ? a.words - v0 : s.piece;
+        TokRows rows;
+        TOK_TRY(piece_rows<T>(st, a, s, w, v0, words, rows));
+        TOK_TRY(tok_with_shape(words, a.rows, [&](auto shape) {
+            using S = decltype(shape);
+            TokProduct p{rows, TokRows{w + s.x, nullptr, s.x_ld * (long long)sizeof(T), a.rows}, count, nullptr,
+                         a.channels * (long long)sizeof(T), (int)((words + S::BM - 1) / S::BM),
+                         (int)((a.rows + S::BN - 1) / S::BN), 1};
+            auto go = [&](auto top) {
+                Statistics<decltype(top)::value> e{t, reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits),
+                                                   s.padded, (int)words, (int)v0, tiles, 1.0f / a.temperature};
+                return tok_product<T, S, 0>(st, p, e);
+            };
+            const int rc = a.top ? go(std::true_type()) : go(std::false_type());
+            tiles += p.m_tiles;
+            return rc;
+        }));
+    }
+    if (!a.rows) return 0;
+    Finish f{reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits), t, reinterpret_cast<float*>(w + s.self),
+             count, s.padded, tiles, a.loss, a.lse};
+    NHIP_LAUNCH(finish_kernel, dim3((unsigned)((a.rows + 15) / 16)), dim3(NHIP_WG), 0, st, f);
+    NHIP_LAUNCH_CHECK();
+    return 0;
+}
+
+template <class T> int backward(hipStream_t st, const nhip_loss_args& a, const Space& s) {
+    constexpr long long size = sizeof(T);
+    char* const w = static_cast<char*>(a.workspace);
+    Targets t;
+    TOK_TRY(prepare<T>(st, a, s, w, true, t));
+    const int* const count = reinterpret_cast<int*>(w + s.count);
+    TOK_TRY(tok_transpose<T>(st, TokTranspose{w + s.x, s.x_ld, w + s.xt, s.gt_ld, a.rows, a.channels, s.padded, count, 0}));
+    float* scale = nullptr;
+    if constexpr (std::is_same<T, _Float16>::value) {
+        scale = reinterpret_cast<float*>(w + s.count) + 16;
+        NHIP_LAUNCH(scale_kernel, dim3(1), dim3(1024), 0, st, a.dloss, t.row, count, 1.0f / a.temperature, scale);
+        NHIP_LAUNCH_CHECK();
+    }
+    const long long d = a.channels;
+    for (long long v0 = 0; v0 < a.words; v0 += s.piece) {
+        const long long words = a.words - v0 < s.piece ? a.words - v0 : s.piece;
+        TokRows rows;
+        TOK_TRY(piece_rows<T>(st, a, s, w, v0, words, rows));
+        const TokRows g{w + s.g, nullptr, s.g_ld * size, a.rows};
+        TOK_TRY(tok_with_shape(words, a.rows, [&](auto shape) {
+            using S = decltype(shape);
+            TokProduct p{rows, TokRows{w + s.x, nullptr, s.x_ld * size, a.rows}, count, nullptr, d * size,
+                         (int)((words + S::BM - 1) / S::BM), (int)((a.rows + S::BN - 1) / S::BN), 1};
+            auto go = [&](auto top) {
+                Gradient<decltype(top)::value> e{t, a.dloss, a.lse, scale, w + s.g, w + s.gt, s.g_ld, s.gt_ld, (int)words, (int)v0,
+                                                 1.0f / a.temperature};
+                return tok_product<T, S, 0>(st, p, e);
+            };
+            return a.top ? go(std::true_type()) : go(std::false_type());
+        }));
+        TOK_TRY(tok_with_shape(d, words, [&](auto shape) {
+            using S = decltype(shape);
+            TokProduct p{TokRows{w + s.xt, nullptr, s.gt_ld * size, d}, TokRows{w + s.gt, nullptr, s.gt_ld * size, words}, nullptr,
+                         count, 0, (int)((d + S::BM - 1) / S::BM), (int)((words + S::BN - 1) / S::BN), 1};
+            return tok_product<T, S, 0>(st, p, TokStoreRows{static_cast<T*>(a.dweight) + v0 * d, nullptr, d, words, 0,
+                                                            scale ? scale + 1 : nullptr});
+        }));
+        const T* const from = static_cast<const T*>(a.weight) + v0 * a.weight_stride;
+        TOK_TRY(tok_transpose<T>(st, TokTranspose{from, a.weight_stride, w + s.wt, s.g_ld, words, d, tok_round(words, 64), nullptr, 0}));
+        TOK_TRY(tok_with_shape(d, a.rows, [&](auto shape) {
+            using S = decltype(shape);
+            TokProduct p{TokRows{w + s.wt, nullptr, s.g_ld * size, d}, g, count, nullptr, words * size,
+                         (int)((d + S::BM - 1) / S::BM), (int)((a.rows + S::BN - 1) / S::BN), s.cut.splits};
+            return tok_product<T, S, 0>(st, p, TokAddParts{reinterpret_cast<float*>(w + s.dx), s.dx_ld, s.padded * s.dx_ld, v0 > 0});
+        }));
+    }
+    return tok_join<T>(st, TokJoin{reinterpret_cast<float*>(w + s.dx), s.dx_ld, s.padded * s.dx_ld, s.cut.splits,
+                                   reinterpret_cast<int*>(w + s.where), scale ? scale + 1 : nullptr, a.dx, a.rows, d});
+}
+
+int run(void* stream, const nhip_loss_args* args, bool grad) {
+    if (int e = check(args)) return e;
+    const nhip_loss_args& a = *args;
+    if (!a.weight || (a.rows && (!a.x || !a.targets || (a.top && !a.target_logits) || !a.lse))) return NHIP_E_BADARG;
+    if (grad ? !a.dweight || (a.rows && (!a.dloss || !a.dx)) : a.rows && !a.loss) return NHIP_E_BADARG;
+    const Space s(a, grad);
+    if (s.bytes > a.workspace_bytes) return NHIP_E_TOOBIG;
+    if (!a.workspace || !sel_aligned(a.workspace, 256)) return NHIP_E_BADARG;
+    int rc = NHIP_E_BADARG;
+    sel_with_type(a.type, [&](auto t) {
+        using T = decltype(t);
+        rc = grad ? backward<T>(static_cast<hipStream_t>(stream), a, s) : forward<T>(static_cast<hipStream_t>(stream), a, s);
+    });
+    return rc;
+}
+
+}  // namespace
+
+extern "C" int nhip_vocabulary_loss_workspace(const nhip_loss_args* args, long long* bytes_out) {
+    if (int e = check(args)) return e;
+    if (!bytes_out) return NHIP_E_BADARG;
+    *bytes_out = Space(*args, false).bytes;
+    return 0;
+}
+
+extern "C" int nhip_vocabulary_loss(void* stream, const nhip_loss_args* args) { return run(stream, args, false); }
+
+extern "C" int nhip_vocabulary_loss_grad_workspace(const nhip_loss_args* args, long long* bytes_out) {
+    if (int e = check(args)) return e;
+    if (!bytes_out) return NHIP_E_BADARG;
+    *bytes_out = Space(*args, true).bytes;
+    return 0;
+}
+
+extern "C" int nhip_vocabulary_loss_grad(void* stream, const nhip_loss_args* args) { return run(stream, args, true); }
