@@ -409,18 +409,27 @@ template <bool TOP> struct Gradient {
             const int row = counts ? targets.row[n] : 0;
             const float d = counts ? dloss[row] * k : 0.0f, lse2 = counts ? lse[row] * kLog2e : 0.0f;
 #pragma unroll
-            for (int i = 0; i < S::MI; ++i)
+            for (int i = 0; i < S::MI; ++i) {
+                float v[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    acc[i][j][r] = counts && m0 + 16 * i + r < words ? d * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -lse2)) : 0.0f;
+                    v[r] = counts && m0 + 16 * i + r < words ? d * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -lse2)) : 0.0f;
+                sel_store<T, 4>(static_cast<T*>(g) + n * g_ld + m0 + 16 * i, v);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) static_cast<T*>(gt)[(m0 + 16 * i + r) * gt_ld + n] = (T)v[r];
+            }
+            // the targets' elements once more, by the lane that has just stored them
             auto take = [&](int word, float share) {
                 const int rel = word - word0 - m0;
                 if (rel < 0 || rel >= S::kWaveM || (rel & 15) >= 4) return;
+                float z = 0.0f;
 #pragma unroll
                 for (int i = 0; i < S::MI; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (rel == 16 * i + r) acc[i][j][r] -= d * share;
+                    for (int r = 0; r < 4; ++r) z = rel == 16 * i + r ? acc[i][j][r] : z;
+                const T v = (T)(d * (__builtin_amdgcn_exp2f(fmaf(z, c, -lse2)) - share));
+                static_cast<T*>(g)[n * g_ld + m0 + rel] = v;
+                static_cast<T*>(gt)[(m0 + rel) * gt_ld + n] = v;
             };
             if (counts) {
                 if constexpr (TOP) {
@@ -429,13 +438,6 @@ template <bool TOP> struct Gradient {
                 } else {
                     take(targets.label[n], 1.0f);
                 }
-            }
-#pragma unroll
-            for (int i = 0; i < S::MI; ++i) {
-                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
-                sel_store<T, 4>(static_cast<T*>(g) + n * g_ld + m0 + 16 * i, v);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) static_cast<T*>(gt)[(m0 + 16 * i + r) * gt_ld + n] = (T)v[r];
             }
         }
     }
