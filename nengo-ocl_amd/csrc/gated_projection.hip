@@ -91,14 +91,8 @@ struct Backward {
                     dg[r] = is ? d[r] * acc[i + H][j][r] * slope : 0.0f;
                     du[r] = is ? d[r] * act : 0.0f;
                 }
-                T* const to = static_cast<T*>(g) + n * g_ld + f;
-                sel_store<T, 4>(to, dg);
-                sel_store<T, 4>(to + second, du);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    static_cast<T*>(gt)[(f + r) * gt_ld + n] = (T)dg[r];
-                    static_cast<T*>(gt)[(second + f + r) * gt_ld + n] = (T)du[r];
-                }
+                tok_store_both<T>(static_cast<T*>(g), g_ld, static_cast<T*>(gt), gt_ld, n, f, dg);
+                tok_store_both<T>(static_cast<T*>(g), g_ld, static_cast<T*>(gt), gt_ld, n, second + f, du);
             }
         }
     }

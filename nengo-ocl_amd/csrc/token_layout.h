@@ -10,7 +10,7 @@ static inline long long tok_ld(long long v) { return tok_round(v, 64) + 64; }
 
 // Whether rows may be read 16 bytes at a time
 static inline bool tok_rows_wide(const void* p, long long ld_bytes, long long row_bytes) {
-    return sel_aligned(p, 16) && ld_bytes % 16 == 0 && row_bytes % 16 == 0;
+    return sel_aligned(p, 16) && ld_bytes % 16 == 0 && row_bytes % 16 == 0 && ld_bytes <= TOK_MOST_LD;
 }
 
 // Whether rows of elements of `size` bytes may be read and written four at a time, from columns that are multiples of four

@@ -19,6 +19,7 @@ typedef unsigned tok_u4 __attribute__((ext_vector_type(4)));
 typedef __bf16 tok_b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 tok_h8 __attribute__((ext_vector_type(8)));
 
+#define TOK_MOST_LD (1 << 23)  // 256 rows lie within 2^31 bytes
 #define TOK_KB 128  // bytes of k in a stage: 64 elements of 16 bits, 32 of 32
 
 // acc += a b over 64 bytes of k: lane group g = lane / 16 holds k = 8 g ... 8 g + 7 (16 bits), or four products of
@@ -35,8 +36,8 @@ template <class T> __device__ __forceinline__ void tok_mma(sel_f4& acc, tok_u4 a
     }
 }
 
-// An operand: rows of `ld` bytes at p (multiples of 16 both).  `half` != 0: two matrices side by side, the second at p2; of
-// every 2 `half` rows of a tile the first half are the first one's, so that a wave holds equal rows of both.
+// An operand: rows of `ld` bytes at p (multiples of 16 both; TOK_MOST_LD at most).  HALF != 0: two matrices side by side, the
+// second at p2; of every 2 HALF rows of a tile the first half are the first one's, so that a wave holds equal rows of both.
 struct TokRows {
     const char *p, *p2;
     long long ld;
@@ -49,14 +50,17 @@ struct TokProduct {
     const int* k_live; // how many elements of k count (device), or NULL
     long long k_bytes; // of a row
     int m_tiles, n_tiles;
-    int splits;        // parts that k is cut into (gridDim.y)
+    int splits;        // parts that k is cut into
 };
 
 template <int BM_, int BN_, int WM_, int WN_> struct TokShape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;     // tile, waves along m and n
     static constexpr int kWaves = WM * WN, kThreads = kWaves * NHIP_WAVE;
     static constexpr int kWaveM = BM / WM, kWaveN = BN / WN, MI = kWaveM / 16, NI = kWaveN / 16;
-    static constexpr int kStage = (BM + BN) * TOK_KB, kLds = 2 * kStage;
+    static constexpr int kStage = (BM + BN) * TOK_KB;
+    static constexpr int kEpilogue = 8 * WM * BN, kLds = 2 * kStage + kEpilogue;  // an epilogue has 8 bytes per column and wave of m
+    // work-groups to a compute unit, by the LDS and the registers of eight waves
+    static constexpr int kAtOnce = (160 << 10) / kLds < 8 / kWaves ? (160 << 10) / kLds : 8 / kWaves;
     static_assert(kWaveM % 16 == 0 && kWaveN % 16 == 0, "waves hold whole tiles");
 };
 
@@ -65,7 +69,7 @@ struct TokPlace {
     int m_tile, n_tile, split;
     int wave_m, wave_n, l, g;   // lane % 16, lane / 16
     int live;                   // rows of B that count
-    char* lds;                  // free for the epilogue after a barrier
+    char* lds;                  // S::kEpilogue bytes, the epilogue's own
 };
 
 static __device__ const tok_u4 tok_zeros = {0, 0, 0, 0};  // what lies behind the end of a row
@@ -77,23 +81,23 @@ static __device__ __forceinline__ void tok_load_lds(const char* from, char* to) 
 
 // One operand's part of a stage: instruction i of a wave brings rows 8 i ... 8 i + 7.  Row r's 16 bytes c lie at c ^ (r % 8),
 // so that 8 rows' same bytes lie in different banks.
-template <int ROWS, int WAVES> struct TokLoader {
+template <int ROWS, int WAVES, int HALF> struct TokLoader {
     static constexpr int kAll = ROWS / 8, kMine = (kAll + WAVES - 1) / WAVES;
     const char* at[kMine];
 
-    __device__ __forceinline__ void begin(const TokRows& t, long long row0, int half, int wave, int lane, long long k0) {
+    __device__ __forceinline__ void begin(const TokRows& t, long long row0, int wave, int lane, long long k0) {
+        const long long first = HALF ? row0 / 2 : row0;
+        const int last = (int)min((long long)ROWS, t.rows - first) - 1;
+        const unsigned c = 16 * ((lane % 8) ^ (lane / 8));
 #pragma unroll
         for (int q = 0; q < kMine; ++q) {
-            const int row = 8 * (wave + q * WAVES) + lane / 8;
-            long long r = row0 + row;
+            int row = 8 * (wave + q * WAVES) + lane / 8;
             const char* p = t.p;
-            if (half) {
-                const int of = row % (2 * half);
-                r = row0 / 2 + row / (2 * half) * half + of % half;
-                p = of < half ? t.p : t.p2;
+            if constexpr (HALF > 0) {
+                p = row / HALF % 2 ? t.p2 : t.p;
+                row = row / (2 * HALF) * HALF + row % HALF;
             }
-            r = r < t.rows ? r : t.rows - 1;
-            at[q] = p + r * t.ld + k0 + 16 * ((lane % 8) ^ (lane / 8));
+            at[q] = p + first * t.ld + k0 + (unsigned)min(row, last) * (unsigned)t.ld + c;
         }
     }
     // `left`: bytes of k from here on
@@ -136,35 +140,46 @@ static __device__ __forceinline__ void tok_tile(int id, int m_tiles, int n_tiles
     n = at / wide;
 }
 
+// As many work-groups as run at once go over the tiles, those of a die over neighbouring ones.  The first stage of the next
+// tile is on its way during the last one of a tile and its epilogue.  Tiles of rows that do not count are no tiles.
 template <class T, class S, int HALF, class Epilogue>
 __global__ __launch_bounds__(S::kThreads) void tok_product_kernel(TokProduct p, Epilogue epilogue) {
     extern __shared__ __attribute__((aligned(16))) char tok_lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NHIP_WAVE), lane = threadIdx.x % NHIP_WAVE;
     TokPlace at;
-    tok_tile(nhip_xcd_remap(blockIdx.x, gridDim.x), p.m_tiles, p.n_tiles, at.m_tile, at.n_tile);
-    at.live = p.live ? min((long long)*p.live, p.b.rows) : (int)p.b.rows;
-    at.split = blockIdx.y;
-    if ((long long)at.n_tile * S::BN >= at.live) return;  // uniform over the work-group
+    at.live = (int)(p.live ? min((long long)*p.live, p.b.rows) : p.b.rows);
     at.wave_m = wave % S::WM;
     at.wave_n = wave / S::WM;
     at.l = lane % 16;
     at.g = lane / 16;
-    at.lds = tok_lds;
-
-    long long bytes = p.k_live ? (long long)*p.k_live * (int)sizeof(T) : p.k_bytes;
+    at.lds = tok_lds + 2 * S::kStage;
+    const int n_tiles = (at.live + S::BN - 1) / S::BN, tiles = p.m_tiles * n_tiles, total = tiles * p.splits;
+    const long long bytes = p.k_live ? (long long)*p.k_live * (int)sizeof(T) : p.k_bytes;
     const int all = (int)((bytes + TOK_KB - 1) / TOK_KB), per = (all + p.splits - 1) / p.splits;
-    const int k0 = min(all, at.split * per), n = min(all, k0 + per) - k0;
-    long long left = bytes - (long long)k0 * TOK_KB;
+    const int dies = min(NHIP_NXCD, (int)gridDim.x), die = blockIdx.x % dies, step = ((int)gridDim.x - die + dies - 1) / dies;
+    const int end = (int)((long long)total * (die + 1) / dies);
+    int id = (int)((long long)total * die / dies) + blockIdx.x / dies;
 
-    sel_f4 acc[S::MI][S::NI];
-#pragma unroll
-    for (int i = 0; i < S::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < S::NI; ++j) acc[i][j] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    TokLoader<S::BM, S::kWaves> la;
-    TokLoader<S::BN, S::kWaves> lb;
-    la.begin(p.a, (long long)at.m_tile * S::BM, HALF, wave, lane, (long long)k0 * TOK_KB);
-    lb.begin(p.b, (long long)at.n_tile * S::BN, 0, wave, lane, (long long)k0 * TOK_KB);
+    struct Tile {
+        int m, n, split, k0, stages;
+    };
+    auto tile = [&](int i) {
+        Tile t;
+        t.split = i / max(tiles, 1);
+        tok_tile(i - t.split * tiles, p.m_tiles, n_tiles, t.m, t.n);
+        t.k0 = min(all, t.split * per);
+        t.stages = min(all, t.k0 + per) - t.k0;
+        return t;
+    };
+    TokLoader<S::BM, S::kWaves, HALF> la;
+    TokLoader<S::BN, S::kWaves, 0> lb;
+    long long left = 0;
+    auto begin = [&](const Tile& t) {
+        const long long k0 = (long long)t.k0 * TOK_KB;
+        left = bytes - k0;
+        la.begin(p.a, (long long)t.m * S::BM, wave, lane, k0);
+        lb.begin(p.b, (long long)t.n * S::BN, wave, lane, k0);
+    };
     auto fetch = [&](int stage) {
         char* const to = tok_lds + stage * S::kStage;
         const int some = (int)min(left, (long long)TOK_KB);
@@ -172,34 +187,94 @@ __global__ __launch_bounds__(S::kThreads) void tok_product_kernel(TokProduct p, 
         lb.load(to + S::BM * TOK_KB, wave, lane, some);
         left -= TOK_KB;
     };
-    if (n > 0) fetch(0);
-    for (int k = 0; k < n; ++k) {
-        __syncthreads();  // this stage has come, the other one is read
-        if (k + 1 < n) fetch((k + 1) & 1);
-        const char* const a = tok_lds + (k & 1) * S::kStage;
-        tok_stage<T, S>(acc, a + at.wave_m * S::kWaveM * TOK_KB, a + (S::BM + at.wave_n * S::kWaveN) * TOK_KB, at.l, at.g);
+
+    int stage = 0;
+    bool ready = false;  // the tile's first stage is on its way
+    Tile next = tile(id);
+    while (id < end) {
+        const Tile now = next;
+        at.m_tile = now.m;
+        at.n_tile = now.n;
+        at.split = now.split;
+        id += step;
+        next = tile(id);
+        const bool more = id < end && next.stages > 0;
+        sel_f4 acc[S::MI][S::NI];
+#pragma unroll
+        for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::NI; ++j) acc[i][j] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+        if (!ready && now.stages > 0) {
+            __syncthreads();  // (both stages are read)
+            begin(now);
+            fetch(stage);
+        }
+        ready = now.stages > 0 && more;
+        for (int k = 0; k < now.stages; ++k) {
+            __syncthreads();  // this stage has come, the other one is read
+            const bool last = k + 1 == now.stages;
+            if (last && more) begin(next);
+            if (!last || more) fetch(stage ^ 1);
+            const char* const a = tok_lds + stage * S::kStage;
+            tok_stage<T, S>(acc, a + at.wave_m * S::kWaveM * TOK_KB, a + (S::BM + at.wave_n * S::kWaveN) * TOK_KB, at.l, at.g);
+            stage ^= 1;
+        }
+        // (a result that is read behind the loop's branch: see sel_settle)
+#pragma unroll
+        for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::NI; ++j) asm volatile("" : "+v"(acc[i][j]));
+        asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::NI; ++j) asm volatile("" : "+v"(acc[i][j]));
+        epilogue.template run<T, S>(at, acc);
     }
-    // (a result that is read behind the loop's branch: see sel_settle)
+}
+
+// Four values of column n in rows m ... m + 3 (a lane's part of a tile), stored along m at g[n, m] and along n at gt[m, n].
+// 16 bits: the four lanes of neighbouring columns exchange theirs, so that each stores four neighbours along n, too.
+template <class T>
+__device__ __forceinline__ void tok_store_both(T* g, long long g_ld, T* gt, long long gt_ld, long long n, long long m,
+                                               const float (&v)[4]) {
+    T* const to = g + n * g_ld + m;
+    if constexpr (sizeof(T) == 2) {
+        typedef unsigned pair __attribute__((ext_vector_type(2)));
+        SelPack<T, 4> q;
 #pragma unroll
-    for (int i = 0; i < S::MI; ++i)
+        for (int r = 0; r < 4; ++r) q.v[r] = (T)v[r];
+        const pair p = __builtin_bit_cast(pair, q);
+        *reinterpret_cast<pair*>(to) = p;
+        const int lane = threadIdx.x & 3;
+        auto from = [](unsigned x, auto order) {
+            return (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, decltype(order)::value, 0xf, 0xf, true);
+        };
+        // with the neighbour: rows 0 and 2 in even lanes, 1 and 3 in odd ones, of two columns
+        const unsigned which = lane & 1 ? 0x03020706u : 0x05040100u;
+        const unsigned a0 = __builtin_amdgcn_perm(from(p.x, std::integral_constant<int, 0xb1>()), p.x, which);
+        const unsigned a1 = __builtin_amdgcn_perm(from(p.y, std::integral_constant<int, 0xb1>()), p.y, which);
+        // with the lane two further: of four columns
+        const unsigned other = from(lane & 2 ? a0 : a1, std::integral_constant<int, 0x4e>());
+        pair t;
+        t.x = lane & 2 ? other : a0;
+        t.y = lane & 2 ? a1 : other;
+        *reinterpret_cast<pair*>(gt + (m + lane) * gt_ld + n - lane) = t;
+    } else {
+        sel_store<T, 4>(to, v);
 #pragma unroll
-        for (int j = 0; j < S::NI; ++j) asm volatile("" : "+v"(acc[i][j]));
-    asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
-#pragma unroll
-    for (int i = 0; i < S::MI; ++i)
-#pragma unroll
-        for (int j = 0; j < S::NI; ++j) asm volatile("" : "+v"(acc[i][j]));
-    epilogue.template run<T, S>(at, acc);
+        for (int r = 0; r < 4; ++r) gt[(m + r) * gt_ld + n] = v[r];
+    }
 }
 
 template <class T, class S, int HALF, class E>
 static inline int tok_product(hipStream_t stream, const TokProduct& p, const E& epilogue) {
-    const long long tiles = (long long)p.m_tiles * p.n_tiles;
+    const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits, groups = 256 * S::kAtOnce;
     if (tiles == 0) return 0;
-    if (tiles > 0x7fffff || p.splits < 1 || p.splits > SEL_MAX_GRID_Y) return NHIP_E_BADARG;
+    if (tiles > 0x3fffffff) return NHIP_E_BADARG;
     auto kernel = tok_product_kernel<T, S, HALF, E>;
     if (int e = sel_allow_lds(stream, kernel, S::kLds)) return e;
-    NHIP_LAUNCH(kernel, dim3((unsigned)tiles, (unsigned)p.splits), dim3(S::kThreads), S::kLds, stream, p, epilogue);
+    NHIP_LAUNCH(kernel, dim3((unsigned)(tiles < groups ? tiles : groups)), dim3(S::kThreads), S::kLds, stream, p, epilogue);
     NHIP_LAUNCH_CHECK();
     return 0;
 }

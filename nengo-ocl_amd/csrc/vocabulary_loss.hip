@@ -13,7 +13,7 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr int kNoWord = 0x7fffffff;
-constexpr int kMostTop = 256;
+constexpr int kMostTop = 256, kBlock = TOK_LEAST_BM;
 constexpr long long kMostRows = 1 << 20, kMostChannels = 1 << 20;
 
 __device__ __forceinline__ long long word_at(const void* p, int wide, long long i) {
@@ -32,11 +32,13 @@ struct Shares {
     float* share;
     float* self;    // sum q log q
     int* flag;      // 0: the row counts, -1: it has no entries
+    unsigned short* first;  // [rows, blocks]: entries below the first word of each block of kBlock words
+    int blocks;
 };
 
 template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares a) {
     constexpr int kMost = Q * NHIP_WAVE;
-    __shared__ int s_word[4][kMost], s_sorted[4][kMost];
+    __shared__ int s_word[4][kMost], s_sorted[4][kMost], s_merged[4][kMost];
     __shared__ float s_share[4][kMost], s_sorted_share[4][kMost];
     const int wave = threadIdx.x / NHIP_WAVE, lane = threadIdx.x % NHIP_WAVE;
     const long long row = (long long)blockIdx.x * 4 + wave, r = min(row, a.rows - 1);
@@ -98,7 +100,7 @@ template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares
         s_sorted_share[wave][rank] = x[q];
     }
     __syncthreads();
-    if (row >= a.rows) return;
+    if (row >= a.rows) return;  // (a wave: what follows is within waves, whose LDS accesses stay in their order)
     int before = 0;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
@@ -109,6 +111,7 @@ template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares
             float share = s_sorted_share[wave][e];
             for (int o = e + 1; o < kMost && s_sorted[wave][o] == w; ++o) share += s_sorted_share[wave][o];
             const int at = before + __popcll(all & ((1ULL << lane) - 1));
+            s_merged[wave][at] = w;
             a.word[row * a.top + at] = w;
             a.share[row * a.top + at] = share;
         }
@@ -126,10 +129,20 @@ template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares
         a.self[row] = self;
         a.flag[row] = any ? 0 : -1;
     }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    for (int b = lane; b < a.blocks; b += NHIP_WAVE) {
+        int lo = 0, hi = before;  // (b kBlock stays below 2^31: so do the words)
+        while (lo < hi) {
+            const int mid = (lo + hi) / 2;
+            if (s_merged[wave][mid] < b * kBlock) lo = mid + 1;
+            else hi = mid;
+        }
+        a.first[row * a.blocks + b] = (unsigned short)lo;
+    }
 }
 
 // ------------------------------------------------------------------------------ rows that count
-// The rows whose label is a word move together, rows of whole stages.  A group takes 64 rows and counts those before them itself
+// The rows whose label is a word move together, rows of whole stages.  A group takes some rows and counts those before them itself
 // (8192 labels are 64 KB in the L2; a launch of its own for the sums would take longer).
 struct Gather {
     const void *x, *labels;
@@ -139,56 +152,79 @@ struct Gather {
     void* out;
     int *row, *where, *label, *count;  // [rows padded], [rows], [rows padded], 1
     float *loss, *lse;                 // zeros where a row does not count; NULL in the backward pass
+    int per;                           // rows of a group
 };
-constexpr int kGatherRows = 64;
+constexpr int kMostPer = 1024;
+// Rows of a group: as few as give every compute unit some, more where counting would cost more than moving
+int gather_rows(long long rows) { return rows <= 1024 * 8 ? 8 : rows <= 1024 * 64 ? 64 : kMostPer; }
+static_assert(kMostRows <= 1024 * kMostPer, "");
 
 template <class T> __global__ __launch_bounds__(NHIP_WG) void gather_kernel(Gather a) {
     constexpr int V = 16 / (int)sizeof(T);
-    __shared__ int s_sum[4], s_at[kGatherRows];
+    __shared__ int s_sum[4], s_at[kMostPer];
     const int wave = threadIdx.x / NHIP_WAVE, lane = threadIdx.x % NHIP_WAVE;
-    const long long r0 = (long long)blockIdx.x * kGatherRows;
+    const long long r0 = (long long)blockIdx.x * a.per;
     auto label_of = [&](long long r) {
         const long long w = word_at(a.labels, a.wide_labels, r);
         return w >= 0 && w < a.n_words ? (int)w : -1;
     };
     int sum = 0;
-    for (long long r = threadIdx.x; r < r0; r += NHIP_WG) sum += label_of(r) >= 0;
+    for (long long r = threadIdx.x; r < r0; r += 8 * NHIP_WG) {
+        int some[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) some[e] = label_of(min(r + e * NHIP_WG, r0 - 1));
+#pragma unroll
+        for (int e = 0; e < 8; ++e) sum += some[e] >= 0 && r + e * NHIP_WG < r0;
+    }
 #pragma unroll
     for (int d = 1; d < NHIP_WAVE; d *= 2) sum += __shfl_xor(sum, d);
     if (lane == 0) s_sum[wave] = sum;
     __syncthreads();
-    const int before = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
     if (wave == 0) {
-        const long long r = r0 + lane;
-        const int label = r < a.rows ? label_of(r) : -1;
-        const unsigned long long all = __ballot(label >= 0);
-        const int at = before + __popcll(all & ((1ULL << lane) - 1));
-        s_at[lane] = label >= 0 ? at : -1;
-        if (label >= 0) {
-            a.row[at] = (int)r;
-            a.label[at] = label;
+        int before = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        for (int k = lane; k < a.per; k += NHIP_WAVE) {
+            const long long r = r0 + k;
+            const int label = r < a.rows ? label_of(r) : -1;
+            const unsigned long long all = __ballot(label >= 0);
+            const int at = before + __popcll(all & ((1ULL << lane) - 1));
+            s_at[k] = label >= 0 ? at : -1;
+            if (label >= 0) {
+                a.row[at] = (int)r;
+                a.label[at] = label;
+            }
+            if (r < a.rows) {
+                a.where[r] = label >= 0 ? at : -1;
+                if (a.loss && label < 0) a.loss[r] = a.lse[r] = 0.0f;
+            }
+            before += __popcll(all);
         }
-        if (r < a.rows) {
-            a.where[r] = label >= 0 ? at : -1;
-            if (a.loss && label < 0) a.loss[r] = a.lse[r] = 0.0f;
-        }
-        if (blockIdx.x == gridDim.x - 1 && lane == 0) *a.count = before + __popcll(all);
+        if (blockIdx.x == gridDim.x - 1 && lane == 0) *a.count = before;
     }
     __syncthreads();
-    for (int k = wave; k < kGatherRows; k += 4) {
-        const int at = s_at[k];
-        if (at < 0) continue;
-        const T* const from = static_cast<const T*>(a.x) + (r0 + k) * a.ld;
-        T* const to = static_cast<T*>(a.out) + (long long)at * a.out_ld;
-        for (int c = lane * V; c < a.out_ld; c += NHIP_WAVE * V) {
-            SelPack<T, V> v;
-            if (a.wide && c + V <= a.channels) {
-                v = *reinterpret_cast<const SelPack<T, V>*>(from + c);
+    if (r0 >= a.rows) return;
+    // loads are unconditional, from places that exist: those under a condition are waited for one by one
+    const int packs = a.out_ld / V, all = a.per * packs;
+    for (int q = threadIdx.x; q < all; q += 4 * NHIP_WG) {
+        SelPack<T, V> v[4];
+#pragma unroll
+        for (int o = 0; o < 4; ++o) {
+            const int k = min(q + o * NHIP_WG, all - 1), c = k % packs * V;
+            const T* const from = static_cast<const T*>(a.x) + min(r0 + k / packs, a.rows - 1) * a.ld;
+            if (a.wide && a.channels % V == 0) {
+                v[o] = *reinterpret_cast<const SelPack<T, V>*>(from + min(c, a.channels - V));
             } else {
 #pragma unroll
-                for (int e = 0; e < V; ++e) v.v[e] = c + e < a.channels ? from[c + e] : (T)0.0f;
+                for (int e = 0; e < V; ++e) v[o].v[e] = from[min(c + e, a.channels - 1)];
             }
-            *reinterpret_cast<SelPack<T, V>*>(to + c) = v;
+        }
+#pragma unroll
+        for (int o = 0; o < 4; ++o) {
+            const int k = q + o * NHIP_WG, c = k % packs * V;
+            const int at = k < all ? s_at[k / packs] : -1;
+            if (at < 0) continue;
+#pragma unroll
+            for (int e = 0; e < V; ++e) v[o].v[e] = c + e < a.channels ? v[o].v[e] : (T)0.0f;
+            *reinterpret_cast<SelPack<T, V>*>(static_cast<T*>(a.out) + (long long)at * a.out_ld + c) = v[o];
         }
     }
 }
@@ -223,34 +259,15 @@ struct Targets {
     const int* word;    // [rows, top], sorted, with
     const float* share;
     const int* row;     // of a live token
-    int top;
-};
-
-// Where the targets of the tile's tokens lie among their sorted entries: [lo, hi), for the BN tokens from n0
-template <class S>
-__device__ __forceinline__ void find_targets(const Targets& t, long long n0, int live, int w0, int w1, int* lo, int* hi) {
-    const int wave = threadIdx.x / NHIP_WAVE, lane = threadIdx.x % NHIP_WAVE;
-    for (int k = wave; k < S::BN; k += S::kWaves) {
-        int below = 0, above = 0;
-        if (n0 + k < live) {
-            const int* const from = t.word + (long long)t.row[n0 + k] * t.top;
-            for (int e = lane; e < t.top; e += NHIP_WAVE) {
-                const int w = from[e];
-                below += w < w0;
-                above += w < w1;
-            }
-        }
-#pragma unroll
-        for (int d = 1; d < NHIP_WAVE; d *= 2) {
-            below += __shfl_xor(below, d);
-            above += __shfl_xor(above, d);
-        }
-        if (lane == 0) {
-            lo[k] = below;
-            hi[k] = above;
-        }
+    const unsigned short* first;
+    int top, blocks;
+    // where the entries of words w0 ... w1 - 1 (multiples of kBlock) begin and end among a row's
+    __device__ __forceinline__ void range(long long r, int w0, int w1, int& lo, int& hi) const {
+        const unsigned short* const of = first + r * blocks;
+        lo = of[min(w0 / kBlock, blocks - 1)];
+        hi = of[min(w1 / kBlock, blocks - 1)];
     }
-}
+};
 
 // Forward: of each token in the tile the maximum of z and the sum of exp(z - maximum), in powers of two, and the logits of
 // its targets.
@@ -264,14 +281,10 @@ template <bool TOP> struct Statistics {
 
     template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
         float2* const s_part = reinterpret_cast<float2*>(at.lds);              // [WM][BN]
-        int* const s_lo = reinterpret_cast<int*>(s_part + S::WM * S::BN), *const s_hi = s_lo + S::BN;
         const long long n0 = (long long)at.n_tile * S::BN;
         const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g;  // within the piece
-        __syncthreads();
-        if constexpr (TOP) {
-            find_targets<S>(targets, n0, at.live, word0 + at.m_tile * S::BM, word0 + (at.m_tile + 1) * S::BM, s_lo, s_hi);
-            __syncthreads();
-        }
+        const int w0 = word0 + at.m_tile * S::BM;
+        __syncthreads();  // (the tile before is done with the LDS)
         const float c = kLog2e * per_temperature;
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
@@ -308,7 +321,9 @@ template <bool TOP> struct Statistics {
             if (n < at.live) {
                 if constexpr (TOP) {
                     const long long from = (long long)targets.row[n] * targets.top;
-                    for (int k = s_lo[local]; k < s_hi[local]; ++k) pick(targets.word[from + k], logits + n * targets.top + k);
+                    int lo, hi;
+                    targets.range(targets.row[n], w0, w0 + S::BM, lo, hi);
+                    for (int k = lo; k < hi; ++k) pick(targets.word[from + k], logits + n * targets.top + k);
                 } else {
                     pick(targets.label[n], logits + n);
                 }
@@ -333,7 +348,8 @@ template <bool TOP> struct Statistics {
     }
 };
 
-// loss and lse of the live tokens: 16 lanes to a token
+// loss and lse of the live tokens: 64 lanes to a token
+constexpr int kFinishLanes = 64;
 struct Finish {
     const float2* part;
     const float* logits;
@@ -345,38 +361,43 @@ struct Finish {
     float *loss, *lse;
 };
 
-__global__ __launch_bounds__(NHIP_WG) void finish_kernel(Finish a) {
-    __shared__ float2 s[16][16];
-    __shared__ float s_loss[16][16];
+__global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
+    __shared__ float2 s[kFinishLanes][16];
+    __shared__ float s_loss[kFinishLanes][16];
     const int k = threadIdx.x % 16, q = threadIdx.x / 16, live = *a.count;
     if ((long long)blockIdx.x * 16 >= live) return;
     const int n = min((int)blockIdx.x * 16 + k, live - 1), row = a.targets.row[n];
     float2 v = {0.0f, 0.0f};
-    for (int t = q; t < a.tiles; t += 16) v = Statistics<false>::joined(v, a.part[(long long)t * a.ld + n]);
-    s[q][k] = v;
-    __syncthreads();
-    v = s[0][k];
+    for (int t = q; t < a.tiles; t += 4 * kFinishLanes) {
+        float2 some[4];
 #pragma unroll
-    for (int o = 1; o < 16; ++o) v = Statistics<false>::joined(v, s[o][k]);
-    const float lse = (v.x + __builtin_amdgcn_logf(v.y)) * kLn2;
+        for (int o = 0; o < 4; ++o) some[o] = a.part[(long long)min(t + o * kFinishLanes, a.tiles - 1) * a.ld + n];
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+            if (t + o * kFinishLanes < a.tiles) v = Statistics<false>::joined(v, some[o]);
+    }
+    s[q][k] = v;
     float loss = 0.0f;
-    if (a.targets.top) {
-        for (int e = q; e < a.targets.top; e += 16) {
+    if (a.targets.top) {  // sum q (lse - z), whose sum of q times lse follows
+        for (int e = q; e < a.targets.top; e += kFinishLanes) {
             const long long at = (long long)row * a.targets.top + e;
-            if (a.targets.word[at] != kNoWord) {
-                const float share = a.targets.share[at];
-                loss += share == 0.0f ? 0.0f : share * (lse - a.logits[(long long)n * a.targets.top + e]);
-            }
+            const float share = a.targets.share[at];
+            if (a.targets.word[at] != kNoWord && share != 0.0f) loss = fmaf(share, a.logits[(long long)n * a.targets.top + e], loss);
         }
         s_loss[q][k] = loss;
-        __syncthreads();
-        loss = a.self[row];
-#pragma unroll
-        for (int o = 0; o < 16; ++o) loss += s_loss[o][k];
+    }
+    __syncthreads();
+    if (q) return;
+#pragma unroll 8
+    for (int o = 1; o < kFinishLanes; ++o) v = Statistics<false>::joined(v, s[o][k]);
+    const float lse = (v.x + __builtin_amdgcn_logf(v.y)) * kLn2;
+    if (a.targets.top) {
+        for (int o = 1; o < kFinishLanes; ++o) loss += s_loss[o][k];
+        loss = a.self[row] + (lse - loss);  // (the shares' sum is one)
     } else {
         loss = lse - a.logits[n];
     }
-    if (q == 0 && (int)blockIdx.x * 16 + k < live) {
+    if ((int)blockIdx.x * 16 + k < live) {
         a.loss[row] = loss;
         a.lse[row] = lse;
     }
@@ -392,19 +413,12 @@ template <bool TOP> struct Gradient {
     float per_temperature;
 
     template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
-        int* const s_lo = reinterpret_cast<int*>(at.lds), *const s_hi = s_lo + S::BN;
         const long long n0 = (long long)at.n_tile * S::BN;
-        const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g;
-        if constexpr (TOP) {
-            __syncthreads();
-            find_targets<S>(targets, n0, at.live, word0 + at.m_tile * S::BM, word0 + (at.m_tile + 1) * S::BM, s_lo, s_hi);
-            __syncthreads();
-        }
+        const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g, w0 = word0 + at.m_tile * S::BM;
         const float c = kLog2e * per_temperature, k = scale ? *scale * per_temperature : per_temperature;
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
-            const int local = at.wave_n * S::kWaveN + 16 * j + at.l;
-            const long long n = n0 + local;
+            const long long n = n0 + at.wave_n * S::kWaveN + 16 * j + at.l;
             const bool counts = n < at.live;
             const int row = counts ? targets.row[n] : 0;
             const float d = counts ? dloss[row] * k : 0.0f, lse2 = counts ? lse[row] * kLog2e : 0.0f;
@@ -414,11 +428,9 @@ template <bool TOP> struct Gradient {
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
                     v[r] = counts && m0 + 16 * i + r < words ? d * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -lse2)) : 0.0f;
-                sel_store<T, 4>(static_cast<T*>(g) + n * g_ld + m0 + 16 * i, v);
-#pragma unroll
-                for (int r = 0; r < 4; ++r) static_cast<T*>(gt)[(m0 + 16 * i + r) * gt_ld + n] = (T)v[r];
+                tok_store_both<T>(static_cast<T*>(g), g_ld, static_cast<T*>(gt), gt_ld, n, m0 + 16 * i, v);
             }
-            // the targets' elements once more, by the lane that has just stored them
+            // the targets' elements once more, when what the wave has stored there has arrived
             auto take = [&](int word, float share) {
                 const int rel = word - word0 - m0;
                 if (rel < 0 || rel >= S::kWaveM || (rel & 15) >= 4) return;
@@ -427,6 +439,7 @@ template <bool TOP> struct Gradient {
                 for (int i = 0; i < S::MI; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) z = rel == 16 * i + r ? acc[i][j][r] : z;
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 const T v = (T)(d * (__builtin_amdgcn_exp2f(fmaf(z, c, -lse2)) - share));
                 static_cast<T*>(g)[n * g_ld + m0 + rel] = v;
                 static_cast<T*>(gt)[(m0 + rel) * gt_ld + n] = v;
@@ -434,7 +447,9 @@ template <bool TOP> struct Gradient {
             if (counts) {
                 if constexpr (TOP) {
                     const long long from = (long long)row * targets.top;
-                    for (int e = s_lo[local]; e < s_hi[local]; ++e) take(targets.word[from + e], targets.share[from + e]);
+                    int lo, hi;
+                    targets.range(row, w0, w0 + S::BM, lo, hi);
+                    for (int e = lo; e < hi; ++e) take(targets.word[from + e], targets.share[from + e]);
                 } else {
                     take(targets.label[n], 1.0f);
                 }
@@ -460,7 +475,7 @@ bool wide_weight(const nhip_loss_args& a) {
 
 struct Space : TokSpace {
     long long padded, x_ld, piece, g_ld, gt_ld, dx_ld;
-    long long row, where, label, count, flag, word, share, self, x, weight, part, logits, xt, wt, g, gt, dx;
+    long long row, where, label, count, flag, word, share, self, first, blocks, x, weight, part, logits, xt, wt, g, gt, dx;
     TokCut cut;
     Space(const nhip_loss_args& a, bool grad) {
         const long long size = sel_size(a.type), rows = a.rows > 0 ? a.rows : 1, top = a.top;
@@ -472,12 +487,14 @@ struct Space : TokSpace {
         where = take(rows * 4);
         label = take(padded * 4);
         count = take(256);
-        flag = word = share = self = 0;
+        flag = word = share = self = first = blocks = 0;
         if (top) {
             flag = take(rows * 4);
             word = take(rows * top * 4);
             share = take(rows * top * 4);
             self = take(rows * 4);
+            blocks = (a.words + kBlock - 1) / kBlock + 1;  // (the last one: all entries)
+            first = take(rows * blocks * 2);
         }
         x = take(padded * x_ld * size);
         weight = wide_weight(a) ? 0 : take(piece * x_ld * size);
@@ -502,15 +519,15 @@ struct Space : TokSpace {
 // The rows that count, and the targets of all rows
 template <class T> int prepare(hipStream_t st, const nhip_loss_args& a, const Space& s, char* w, bool grad, Targets& t) {
     t = Targets{reinterpret_cast<int*>(w + s.label), reinterpret_cast<int*>(w + s.word), reinterpret_cast<float*>(w + s.share),
-                reinterpret_cast<int*>(w + s.row), a.top};
+                reinterpret_cast<int*>(w + s.row), reinterpret_cast<unsigned short*>(w + s.first), a.top, (int)s.blocks};
     Gather gather{a.x, a.targets, a.wide_targets, a.words, a.type, 0, a.x_stride, a.rows, a.channels, (int)s.x_ld, w + s.x,
                   reinterpret_cast<int*>(w + s.row), reinterpret_cast<int*>(w + s.where), reinterpret_cast<int*>(w + s.label),
-                  reinterpret_cast<int*>(w + s.count), grad ? nullptr : a.loss, grad ? nullptr : a.lse};
+                  reinterpret_cast<int*>(w + s.count), grad ? nullptr : a.loss, grad ? nullptr : a.lse, gather_rows(a.rows)};
     gather.wide = tok_rows_wide(a.x, a.x_stride * (long long)sizeof(T), 16);
     if (a.top && a.rows) {
         Shares sh{a.targets, a.target_logits, a.wide_targets, a.logits_type, a.top, a.words, a.rows, 1.0f / a.temperature,
                   reinterpret_cast<int*>(w + s.word), reinterpret_cast<float*>(w + s.share), reinterpret_cast<float*>(w + s.self),
-                  reinterpret_cast<int*>(w + s.flag)};
+                  reinterpret_cast<int*>(w + s.flag), reinterpret_cast<unsigned short*>(w + s.first), (int)s.blocks};
         const dim3 grid((unsigned)((a.rows + 3) / 4));
         if (a.top <= 64) NHIP_LAUNCH((shares_kernel<1>), grid, dim3(NHIP_WG), 0, st, sh);
         else if (a.top <= 128) NHIP_LAUNCH((shares_kernel<2>), grid, dim3(NHIP_WG), 0, st, sh);
@@ -519,7 +536,7 @@ template <class T> int prepare(hipStream_t st, const nhip_loss_args& a, const Sp
         gather.labels = w + s.flag;  // 0 or -1
         gather.wide_labels = 0;
     }
-    const long long groups = (a.rows + kGatherRows - 1) / kGatherRows;
+    const long long groups = (a.rows + gather.per - 1) / gather.per;
     NHIP_LAUNCH((gather_kernel<T>), dim3((unsigned)(groups ? groups : 1)), dim3(NHIP_WG), 0, st, gather);
     NHIP_LAUNCH_CHECK();
     return 0;
@@ -566,7 +583,7 @@ template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Sp
     if (!a.rows) return 0;
     Finish f{reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits), t, reinterpret_cast<float*>(w + s.self),
              count, s.padded, tiles, a.loss, a.lse};
-    NHIP_LAUNCH(finish_kernel, dim3((unsigned)((a.rows + 15) / 16)), dim3(NHIP_WG), 0, st, f);
+    NHIP_LAUNCH(finish_kernel, dim3((unsigned)((a.rows + 15) / 16)), dim3(16 * kFinishLanes), 0, st, f);
     NHIP_LAUNCH_CHECK();
     return 0;
 }
