@@ -148,6 +148,7 @@ struct TokStoreRows {
                         if (d + r < ld) to[d + r] = (T)v[r];
                 }
             }
+            asm volatile("" ::: "memory");
         }
     }
 };
@@ -169,6 +170,7 @@ struct TokAddParts {
                 sel_f4* const to = reinterpret_cast<sel_f4*>(mine + n * ld + d);
                 *to = add ? *to + acc[i][j] : acc[i][j];
             }
+            asm volatile("" ::: "memory");  // (a column's sums at a time: all of them at once are more than the registers hold)
         }
     }
 };

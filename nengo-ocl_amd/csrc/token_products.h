@@ -3,8 +3,8 @@
 //     D[m, n] = sum_k A[m, k] B[n, k],     rows of A and B along k, sums in 32 bits
 //
 // and what becomes of D is the caller's: an epilogue gets it in registers.  A work-group forms a tile of BM x BN; tiles of A
-// and B of 128 bytes along k lie in the LDS in two stages, and the next stage is on its way, straight from memory into the
-// LDS, while one is multiplied.
+// and B of 128 bytes along k (a stage) go straight from memory into one of two places in the LDS.  While half a stage is
+// multiplied the next half is read into registers; a place is filled again as soon as it has been read.
 //
 // D lies as the matrix instructions leave it: tile (i, j) of 16 x 16 of a wave holds column n = 16 j + lane % 16 and
 // rows m = 16 i + 4 (lane / 16) + r in its four registers.  So m runs along what is contiguous in the result, and a
@@ -23,16 +23,15 @@ typedef _Float16 tok_h8 __attribute__((ext_vector_type(8)));
 #define TOK_KB 128  // bytes of k in a stage: 64 elements of 16 bits, 32 of 32
 
 // acc += a b over 64 bytes of k: lane group g = lane / 16 holds k = 8 g ... 8 g + 7 (16 bits), or four products of
-// k = 4 g + e, which the hardware sums over g (32 bits; both operands agree on the order).
-template <class T> __device__ __forceinline__ void tok_mma(sel_f4& acc, tok_u4 a, tok_u4 b) {
+// k = 4 g + part, which the hardware sums over g (32 bits; both operands agree on the order).
+template <class T> __device__ __forceinline__ void tok_mma(sel_f4& acc, tok_u4 a, tok_u4 b, int part) {
     if constexpr (std::is_same<T, __bf16>::value) {
         acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(tok_b8, a), __builtin_bit_cast(tok_b8, b), acc, 0, 0, 0);
     } else if constexpr (std::is_same<T, _Float16>::value) {
         acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(tok_h8, a), __builtin_bit_cast(tok_h8, b), acc, 0, 0, 0);
     } else {
         const sel_f4 x = __builtin_bit_cast(sel_f4, a), y = __builtin_bit_cast(sel_f4, b);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[e], y[e], acc, 0, 0, 0);
+        acc = __builtin_amdgcn_mfma_f32_16x16x4f32(x[part], y[part], acc, 0, 0, 0);
     }
 }
 
@@ -59,8 +58,10 @@ template <int BM_, int BN_, int WM_, int WN_> struct TokShape {
     static constexpr int kWaveM = BM / WM, kWaveN = BN / WN, MI = kWaveM / 16, NI = kWaveN / 16;
     static constexpr int kStage = (BM + BN) * TOK_KB;
     static constexpr int kEpilogue = 8 * WM * BN, kLds = 2 * kStage + kEpilogue;  // an epilogue has 8 bytes per column and wave of m
-    // work-groups to a compute unit, by the LDS and the registers of eight waves
-    static constexpr int kAtOnce = (160 << 10) / kLds < 8 / kWaves ? (160 << 10) / kLds : 8 / kWaves;
+    // work-groups to a compute unit, by the LDS and by the registers: a wave that holds more than 32 tiles has a SIMD for itself
+    static constexpr int kByRegisters = MI * NI > 32 ? 1 : 8 / kWaves;
+    static constexpr bool kPinned = MI * NI > 32, kPair = kWaves == 8;
+    static constexpr int kAtOnce = (160 << 10) / kLds < kByRegisters ? (160 << 10) / kLds : kByRegisters;
     static_assert(kWaveM % 16 == 0 && kWaveN % 16 == 0, "waves hold whole tiles");
 };
 
@@ -80,56 +81,75 @@ static __device__ __forceinline__ void tok_load_lds(const char* from, char* to) 
 }
 
 // One operand's part of a stage: instruction i of a wave brings rows 8 i ... 8 i + 7.  Row r's 16 bytes c lie at c ^ (r % 8),
-// so that 8 rows' same bytes lie in different banks.
+// so that 8 rows' same bytes lie in different banks.  Every wave has as many instructions (where there are fewer rows several
+// bring the same ones), so that it knows by their number which have arrived.
 template <int ROWS, int WAVES, int HALF> struct TokLoader {
     static constexpr int kAll = ROWS / 8, kMine = (kAll + WAVES - 1) / WAVES;
     const char* at[kMine];
 
-    __device__ __forceinline__ void begin(const TokRows& t, long long row0, int wave, int lane, long long k0) {
+    static __device__ __forceinline__ int part(int lane) { return 16 * ((lane % 8) ^ (lane / 8)); }
+    static __device__ __forceinline__ int instruction(int wave, int q) {
+        const int i = wave + q * WAVES;
+        return kAll % WAVES == 0 ? i : min(i, kAll - 1);
+    }
+    static __device__ __forceinline__ const char* row_at(const TokRows& t, long long row0, int row, long long k0) {
         const long long first = HALF ? row0 / 2 : row0;
         const int last = (int)min((long long)ROWS, t.rows - first) - 1;
-        const unsigned c = 16 * ((lane % 8) ^ (lane / 8));
-#pragma unroll
-        for (int q = 0; q < kMine; ++q) {
-            int row = 8 * (wave + q * WAVES) + lane / 8;
-            const char* p = t.p;
-            if constexpr (HALF > 0) {
-                p = row / HALF % 2 ? t.p2 : t.p;
-                row = row / (2 * HALF) * HALF + row % HALF;
-            }
-            at[q] = p + first * t.ld + k0 + (unsigned)min(row, last) * (unsigned)t.ld + c;
+        const char* p = t.p;
+        if constexpr (HALF > 0) {
+            p = row / HALF % 2 ? t.p2 : t.p;
+            row = row / (2 * HALF) * HALF + row % HALF;
         }
+        return p + first * t.ld + k0 + (unsigned)min(row, last) * (unsigned)t.ld;
     }
-    // `left`: bytes of k from here on
-    __device__ __forceinline__ void load(char* to, int wave, int lane, int left) {
-        const int c = 16 * ((lane % 8) ^ (lane / 8));
+    __device__ __forceinline__ void begin(const TokRows& t, long long row0, int wave, int lane, long long k0) {
 #pragma unroll
-        for (int q = 0; q < kMine; ++q) {
-            const int i = wave + q * WAVES;
-            if (kAll % WAVES == 0 || i < kAll) {
-                tok_load_lds(c < left ? at[q] : reinterpret_cast<const char*>(&tok_zeros), to + i * 1024);
-                at[q] += TOK_KB;
+        for (int q = 0; q < kMine; ++q) at[q] = row_at(t, row0, 8 * instruction(wave, q) + lane / 8, k0) + part(lane);
+    }
+    // The last `left` bytes of k: what lies behind the end of a row is read from elsewhere
+    __device__ __forceinline__ void cut(int lane, int left) {
+#pragma unroll
+        for (int q = 0; q < kMine; ++q) at[q] = part(lane) < left ? at[q] : reinterpret_cast<const char*>(&tok_zeros);
+    }
+    __device__ __forceinline__ void load(char* to, int wave, int q) {
+        tok_load_lds(at[q], to + instruction(wave, q) * 1024);
+        at[q] += TOK_KB;
+    }
+};
+
+// A wave's part of half a stage, 64 bytes of k
+template <class S> struct TokPart {
+    static constexpr int kReads = S::MI + S::NI;
+    tok_u4 a[S::MI], b[S::NI];
+    // its q-th 16 rows: those of B, which all of A's meet, come first
+    __device__ __forceinline__ void read_one(int q, const char* from_a, const char* from_b, int c) {
+        if (q < S::NI) b[q] = *reinterpret_cast<const tok_u4*>(from_b + c + q * 16 * TOK_KB);
+        else a[q - S::NI] = *reinterpret_cast<const tok_u4*>(from_a + c + (q - S::NI) * 16 * TOK_KB);
+    }
+    __device__ __forceinline__ void read(const char* from_a, const char* from_b, int c) {
+#pragma unroll
+        for (int q = 0; q < kReads; ++q) read_one(q, from_a, from_b, c);
+    }
+    // Products q of n, in steps: the results of a wave that has a SIMD for itself stay in their registers.  (The compiler's own
+    // form of these products has another register for the result than for the addend, and moved results about.  That a
+    // result is not read too early is seen to here: as an addend 63 products later, otherwise behind tok_settle.)
+    template <class T> __device__ __forceinline__ void multiply(sel_f4 (&acc)[S::MI][S::NI], int q, int n) const {
+        constexpr int kProducts = S::MI * S::NI * (sizeof(T) == 2 ? 1 : 4);
+#pragma unroll
+        for (int e = q * kProducts / n; e < (q + 1) * kProducts / n; ++e) {
+            const int part = e / (S::MI * S::NI), i = e / S::NI % S::MI, j = e % S::NI;
+            if constexpr (!S::kPinned) {
+                tok_mma<T>(acc[i][j], a[i], b[j], part);
+            } else if constexpr (std::is_same<T, __bf16>::value) {
+                asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(a[i]), "v"(b[j]));
+            } else if constexpr (std::is_same<T, _Float16>::value) {
+                asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(a[i]), "v"(b[j]));
+            } else {
+                asm volatile("v_mfma_f32_16x16x4_f32 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(a[i][part]), "v"(b[j][part]));
             }
         }
     }
 };
-
-template <class T, class S>
-__device__ __forceinline__ void tok_stage(sel_f4 (&acc)[S::MI][S::NI], const char* a, const char* b, int l, int g) {
-#pragma unroll
-    for (int sub = 0; sub < 2; ++sub) {
-        const int c = ((4 * sub + g) ^ (l & 7)) * 16 + l * TOK_KB;
-        tok_u4 fa[S::MI], fb[S::NI];
-#pragma unroll
-        for (int i = 0; i < S::MI; ++i) fa[i] = *reinterpret_cast<const tok_u4*>(a + c + i * 16 * TOK_KB);
-#pragma unroll
-        for (int j = 0; j < S::NI; ++j) fb[j] = *reinterpret_cast<const tok_u4*>(b + c + j * 16 * TOK_KB);
-#pragma unroll
-        for (int i = 0; i < S::MI; ++i)
-#pragma unroll
-            for (int j = 0; j < S::NI; ++j) tok_mma<T>(acc[i][j], fa[i], fb[j]);
-    }
-}
 
 // Tile `id` of m_tiles x n_tiles: bands of 8 tiles of m, so that the tiles under way at once on a die share rows in its L2
 static __device__ __forceinline__ void tok_tile(int id, int m_tiles, int n_tiles, int& m, int& n) {
@@ -140,10 +160,35 @@ static __device__ __forceinline__ void tok_tile(int id, int m_tiles, int n_tiles
     n = at / wide;
 }
 
-// As many work-groups as run at once go over the tiles, those of a die over neighbouring ones.  The first stage of the next
-// tile is on its way during the last one of a tile and its epilogue.  Tiles of rows that do not count are no tiles.
+// Waits until the products before it are done: a result that is read behind the loop's branch needs it (see sel_settle).
+// Waves that have a SIMD for themselves hold results in accumulation registers, others among the vector registers.
+template <class S> __device__ __forceinline__ void tok_settle(sel_f4 (&acc)[S::MI][S::NI]) {
+    auto touch = [&] {
+#pragma unroll
+        for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+            for (int j = 0; j < S::NI; ++j) {
+                if constexpr (S::kPinned) asm volatile("" : "+a"(acc[i][j]));
+                else asm volatile("" : "+v"(acc[i][j]));
+            }
+    };
+    touch();
+    asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
+    touch();
+}
+
+template <int N> __device__ __forceinline__ void tok_wait() {  // until all but the last N loads have come, and all is read
+    static_assert(N < 64, "what the counter holds");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// As many work-groups as run at once go over the tiles, those of a die over neighbouring ones; tiles of rows that do not count
+// are no tiles.  The stages of all its tiles are one stream to a work-group: what is on its way does not stop at a
+// tile's end.
 template <class T, class S, int HALF, class Epilogue>
-__global__ __launch_bounds__(S::kThreads) void tok_product_kernel(TokProduct p, Epilogue epilogue) {
+__global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_product_kernel(TokProduct p, Epilogue epilogue) {
     extern __shared__ __attribute__((aligned(16))) char tok_lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NHIP_WAVE), lane = threadIdx.x % NHIP_WAVE;
     TokPlace at;
@@ -171,66 +216,179 @@ __global__ __launch_bounds__(S::kThreads) void tok_product_kernel(TokProduct p, 
         t.stages = min(all, t.k0 + per) - t.k0;
         return t;
     };
-    TokLoader<S::BM, S::kWaves, HALF> la;
-    TokLoader<S::BN, S::kWaves, 0> lb;
-    long long left = 0;
-    auto begin = [&](const Tile& t) {
-        const long long k0 = (long long)t.k0 * TOK_KB;
-        left = bytes - k0;
-        la.begin(p.a, (long long)t.m * S::BM, wave, lane, k0);
-        lb.begin(p.b, (long long)t.n * S::BN, wave, lane, k0);
+    // the stream: what is sent for next
+    using LoaderA = TokLoader<S::BM, S::kWaves, HALF>;
+    using LoaderB = TokLoader<S::BN, S::kWaves, 0>;
+    constexpr int kLoads = LoaderA::kMine + LoaderB::kMine;
+    LoaderA la;
+    LoaderB lb;
+    int coming = id - step, coming_left = 0;  // its tile, the stages of it that are left
+    long long left = 0;                       // bytes of k
+    auto load = [&](int q, int place) {
+        char* const to = tok_lds + place * S::kStage;
+        if (q < LoaderA::kMine) la.load(to, wave, q);
+        else lb.load(to + S::BM * TOK_KB, wave, q - LoaderA::kMine);
     };
-    auto fetch = [&](int stage) {
-        char* const to = tok_lds + stage * S::kStage;
-        const int some = (int)min(left, (long long)TOK_KB);
-        la.load(to, wave, lane, some);
-        lb.load(to + S::BM * TOK_KB, wave, lane, some);
+    auto sent = [&] {
         left -= TOK_KB;
+        --coming_left;
+    };
+    auto prepare = [&] {  // where a stage's rows are; behind the last stage there are zeros to send for
+        if (coming_left == 0) {
+            while (coming < end && coming_left == 0) {
+                coming += step;
+                if (coming < end) coming_left = tile(coming).stages;
+            }
+            if (coming >= end) {
+                left = 0;
+                coming_left = 1;
+            } else {
+                const Tile t = tile(coming);
+                const long long k0 = (long long)t.k0 * TOK_KB;
+                left = bytes - k0;
+                la.begin(p.a, (long long)t.m * S::BM, wave, lane, k0);
+                lb.begin(p.b, (long long)t.n * S::BN, wave, lane, k0);
+            }
+        }
+        if (left < TOK_KB) {  // (a stage of zeros is `left` below zero for the next one: that is cut, too)
+            la.cut(lane, (int)left);
+            lb.cut(lane, (int)left);
+        }
     };
 
-    int stage = 0;
-    bool ready = false;  // the tile's first stage is on its way
-    Tile next = tile(id);
-    while (id < end) {
-        const Tile now = next;
+    if (id >= end) return;
+#pragma unroll 1
+    for (int s = 0; s < 2; ++s) {
+        prepare();
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q)
+            if (!S::kPair || s == 0 || q < kLoads / 2) load(q, s);  // (pairs of groups: half of the second one, as always)
+        if (!S::kPair || s == 0) sent();
+    }
+    tok_wait<0>();
+    constexpr int kSteps = TokPart<S>::kReads;
+    const int c0 = (at.g ^ (at.l & 7)) * 16 + at.l * TOK_KB, c1 = c0 ^ 64;
+    int place = 0;  // of the stage that is multiplied next
+    for (; id < end; id += step) {
+        const Tile now = tile(id);
         at.m_tile = now.m;
         at.n_tile = now.n;
         at.split = now.split;
-        id += step;
-        next = tile(id);
-        const bool more = id < end && next.stages > 0;
         sel_f4 acc[S::MI][S::NI];
 #pragma unroll
         for (int i = 0; i < S::MI; ++i)
 #pragma unroll
             for (int j = 0; j < S::NI; ++j) acc[i][j] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        if (!ready && now.stages > 0) {
-            __syncthreads();  // (both stages are read)
-            begin(now);
-            fetch(stage);
+        const char* const a0 = tok_lds + at.wave_m * S::kWaveM * TOK_KB;
+        const char* const b0 = tok_lds + (S::BM + at.wave_n * S::kWaveN) * TOK_KB;
+        if constexpr (S::kPair) {
+            // Two groups of four waves, one of each to a SIMD, take turns: while one multiplies a quarter of its tile by a stage,
+            // the other reads its next quarter's operands and sends for more.  The second group is half a turn behind, which
+            // the barriers before and behind the tile bring about and undo.
+            constexpr int HM = S::MI / 2, HN = S::NI / 2;
+            tok_u4 a[2][HM], b[2][2][HN];
+            auto read_a = [&](int h) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int i = 0; i < HM; ++i)
+                        a[s][i] = *reinterpret_cast<const tok_u4*>(a0 + place * S::kStage + (s ? c1 : c0) + (h * HM + i) * 16 * TOK_KB);
+            };
+            auto read_b = [&](int h) {
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int j = 0; j < HN; ++j)
+                        b[h][s][j] = *reinterpret_cast<const tok_u4*>(b0 + place * S::kStage + (s ? c1 : c0) + (h * HN + j) * 16 * TOK_KB);
+            };
+            auto turn = [&] {
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_s_barrier();
+                asm volatile("" ::: "memory");
+                __builtin_amdgcn_sched_barrier(0);
+            };
+            auto multiply = [&](int hm, int hn) {
+                turn();
+                __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                    for (int e = 0; e < (sizeof(T) == 2 ? 1 : 4); ++e)
+#pragma unroll
+                        for (int i = 0; i < HM; ++i)
+#pragma unroll
+                            for (int j = 0; j < HN; ++j) tok_mma<T>(acc[hm * HM + i][hn * HN + j], a[s][i], b[hn][s][j], e);
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+                turn();
+            };
+            auto loads = [&](int from, int to, int where) {
+#pragma unroll
+                for (int q = 0; q < kLoads; ++q)
+                    if (q >= from && q < to) load(q, where);
+            };
+            const bool behind = wave >= S::kWaves / 2;
+            if (behind) turn();
+            for (int k = 0; k < now.stages; ++k) {
+                read_a(0);
+                read_b(0);
+                loads(kLoads / 2, kLoads * 3 / 4, place ^ 1);
+                multiply(0, 0);
+                read_b(1);
+                loads(kLoads * 3 / 4, kLoads, place ^ 1);
+                sent();
+                multiply(0, 1);
+                read_a(1);
+                asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (all of this stage's place is read)
+                multiply(1, 1);
+                prepare();
+                loads(0, kLoads / 2, place);
+                asm volatile("s_waitcnt vmcnt(%0)" ::"n"(kLoads / 2) : "memory");  // the next stage has come
+                multiply(1, 0);
+                place ^= 1;
+            }
+            if (!behind) turn();
+        } else {
+            TokPart<S> first, second;
+            tok_settle<S>(acc);  // (zeros, too, are written before they are an addend)
+            if (now.stages > 0) first.read(a0 + place * S::kStage, b0 + place * S::kStage, c0);
+            // Half a stage: `next` is read, and `loads` are sent for, between the products.  (Products first: the compiler waits for
+            // all reads before the first one, which have come then; and no read among the last quarter, whose time a read takes.)
+            auto half = [&](const TokPart<S>& mine, TokPart<S>& next, int from, int c, auto&& loads) {
+#pragma unroll
+                for (int q = 0; q < kSteps; ++q) {
+                    mine.template multiply<T>(acc, q, kSteps);
+#pragma unroll
+                    for (int o = 4 * q / 3; o < 4 * (q + 1) / 3 && o < kSteps; ++o)
+                        next.read_one(o, a0 + from * S::kStage, b0 + from * S::kStage, c);
+                    loads(q);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            };
+            auto stage = [&] {
+                half(first, second, place, c1, [](int) {});
+                tok_wait<0>();  // the other stage has come, this one is read
+                half(second, first, place ^ 1, c0, [&](int q) {  // (behind the tile's last stage `first` is read for nothing)
+#pragma unroll
+                    for (int o = 2 * q * kLoads / kSteps; o < 2 * (q + 1) * kLoads / kSteps && o < kLoads; ++o) load(o, place);
+                });
+                place ^= 1;
+                sent();
+            };
+            // whole stages of this tile are sent for without a branch; its last one, and those of the next tiles, in a loop of their own
+            int k = 0;
+            for (; k + 3 < now.stages; ++k) stage();
+            for (; k < now.stages; ++k) {
+                prepare();
+                stage();
+            }
         }
-        ready = now.stages > 0 && more;
-        for (int k = 0; k < now.stages; ++k) {
-            __syncthreads();  // this stage has come, the other one is read
-            const bool last = k + 1 == now.stages;
-            if (last && more) begin(next);
-            if (!last || more) fetch(stage ^ 1);
-            const char* const a = tok_lds + stage * S::kStage;
-            tok_stage<T, S>(acc, a + at.wave_m * S::kWaveM * TOK_KB, a + (S::BM + at.wave_n * S::kWaveN) * TOK_KB, at.l, at.g);
-            stage ^= 1;
-        }
-        // (a result that is read behind the loop's branch: see sel_settle)
-#pragma unroll
-        for (int i = 0; i < S::MI; ++i)
-#pragma unroll
-            for (int j = 0; j < S::NI; ++j) asm volatile("" : "+v"(acc[i][j]));
-        asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
-#pragma unroll
-        for (int i = 0; i < S::MI; ++i)
-#pragma unroll
-            for (int j = 0; j < S::NI; ++j) asm volatile("" : "+v"(acc[i][j]));
-        epilogue.template run<T, S>(at, acc);
+        tok_settle<S>(acc);
+        TokPlace here = at;
+        asm volatile("" : "+v"(here.l), "+v"(here.g));  // (or what an epilogue forms of them is kept over all tiles, and spilled)
+        epilogue.template run<T, S>(here, acc);
     }
+    tok_wait<0>();  // (nothing arrives in the LDS of a work-group that has ended)
 }
 
 // Four values of column n in rows m ... m + 3 (a lane's part of a tile), stored along m at g[n, m] and along n at gt[m, n].
