@@ -75,9 +75,12 @@ struct TokPlace {
 
 static __device__ const tok_u4 tok_zeros = {0, 0, 0, 0};  // what lies behind the end of a row
 
+// 16 bytes to a lane, straight into the LDS: lane i's to `to` + 16 i.  (The builtin of this has the compiler wait for all such
+// loads before reads of the LDS that it cannot tell apart from them: half of what was under way had to arrive a turn early.  The
+// kernel waits by their number instead, tok_wait and the turns; no register is written.)
 static __device__ __forceinline__ void tok_load_lds(const char* from, char* to) {
-    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)from,
-                                     (__attribute__((address_space(3))) void*)to, 16, 0, 0);
+    const unsigned at = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char*)to;
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(at), "v"(from) : "memory", "m0");
 }
 
 // One operand's part of a stage: instruction i of a wave brings rows 8 i ... 8 i + 7.  Row r's 16 bytes c lie at c ^ (r % 8),
