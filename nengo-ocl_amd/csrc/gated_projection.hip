@@ -5,6 +5,9 @@
 //
 // A wave's tile holds equal features of both weights, so that activation and product happen in its registers.  The
 // backward pass forms g and u again and keeps dg and du, in the type of x, for the two products that read them.
+#include <algorithm>
+#include <optional>
+
 #include "token_layout.h"
 
 namespace {
@@ -107,20 +110,19 @@ int check(const nhip_gated_args* a) {
 }
 
 struct Space : TokSpace {
-    long long padded, x_ld, piece, g_ld, gt_ld, dx_ld;
-    long long x = 0, gate = 0, up = 0, xt, wt, g, gt, dx;
+    long long x_ld, piece;
+    long long x = 0, gate = 0, up = 0;
     bool pad_x, pad_w;
-    TokCut cut;
+    std::optional<TokGradient> gradient;
     Space(const nhip_gated_args& a, bool grad) {
         const long long size = sel_size(a.type), d = a.channels, rows = a.rows > 0 ? a.rows : 1;
-        padded = tok_round(rows, TOK_MOST_TILE);
         x_ld = tok_round(d, 64);
-        cut = tok_cut(a.rows, d, 2 * tok_round(a.features, 128), (int)size);  // rows of both weights, whole tiles of each
-        piece = cut.piece / 2;
-        if (!grad) {
-            // as many features as a launch's grid holds
-            const long long most = (1LL << 21) / (padded / 256) * 128;
-            piece = tok_round(a.features, 128) < most ? tok_round(a.features, 128) : most;
+        if (grad) {
+            gradient.emplace(*this, a.rows, d, 2 * tok_round(a.features, 128), size);
+            piece = gradient->piece / 2;
+        } else {
+            // as many features as a launch's tiles reach
+            piece = std::min(tok_round(a.features, 128), (1LL << 21) / (tok_round(rows, 256) / 256) * 64);
         }
         pad_x = !tok_rows_wide(a.x, a.x_stride * size, d * size);
         pad_w = !tok_rows_wide(a.gate, a.gate_stride * size, d * size) || !tok_rows_wide(a.up, a.up_stride * size, d * size) ||
@@ -129,16 +131,6 @@ struct Space : TokSpace {
         if (pad_w) {
             gate = take(piece * x_ld * size);
             up = take(piece * x_ld * size);
-        }
-        if (grad) {
-            g_ld = tok_ld(2 * piece);
-            gt_ld = tok_ld(padded);
-            dx_ld = tok_round(d, TOK_MOST_TILE);
-            xt = take(d * gt_ld * size);
-            wt = take(d * g_ld * size);
-            g = take(padded * g_ld * size);
-            gt = take(2 * piece * gt_ld * size);
-            dx = take(cut.splits * padded * dx_ld * 4);
         }
     }
 };
@@ -180,7 +172,7 @@ template <class T> int forward(hipStream_t st, const nhip_gated_args& a, const S
     for (long long f0 = 0; f0 < a.features; f0 += s.piece) {
         const long long n = a.features - f0 < s.piece ? a.features - f0 : s.piece;
         TOK_TRY(weight_rows<T>(st, a, s, w, f0, n, rows));
-        TOK_TRY(tok_with_shape(2 * n, a.rows, [&](auto shape) {
+        TOK_TRY(tok_with_shape(2 * n, a.rows, sizeof(T), 1, [&](auto shape) {
             using S = decltype(shape);
             TokProduct p{rows, x, nullptr, nullptr, a.channels * (long long)sizeof(T), (int)((2 * n + S::BM - 1) / S::BM),
                          (int)((a.rows + S::BN - 1) / S::BN), 1};
@@ -196,44 +188,27 @@ template <class T> int backward(hipStream_t st, const nhip_gated_args& a, const 
     const long long d = a.channels;
     TokRows x, rows;
     TOK_TRY(x_rows<T>(st, a, s, w, x));
-    TOK_TRY(tok_transpose<T>(st, TokTranspose{a.x, a.x_stride, w + s.xt, s.gt_ld, a.rows, d, s.padded, nullptr, 0}));
+    const TokGradient& gr = *s.gradient;
+    TOK_TRY(gr.lay_out_x<T>(st, w, a.x, a.x_stride, nullptr));
     for (long long f0 = 0; f0 < a.features; f0 += s.piece) {
         const long long n = a.features - f0 < s.piece ? a.features - f0 : s.piece;
         // the second weights' part begins behind the last tile of the first one's, whose zeros lie between
-        const long long second = tok_round(n, tok_with_shape(2 * n, a.rows, [](auto shape) { return decltype(shape)::BM / 2; }));
+        const long long second = tok_round(n, tok_with_shape(2 * n, a.rows, sizeof(T), 1, [](auto shape) { return decltype(shape)::BM / 2; }));
         const long long both = second + tok_round(n, 64);
         TOK_TRY(weight_rows<T>(st, a, s, w, f0, n, rows));
         if (a.rows)
-            TOK_TRY(tok_with_shape(2 * n, a.rows, [&](auto shape) {
+            TOK_TRY(tok_with_shape(2 * n, a.rows, sizeof(T), 1, [&](auto shape) {
                 using S = decltype(shape);
                 TokProduct p{rows, x, nullptr, nullptr, d * size, (int)((2 * n + S::BM - 1) / S::BM),
                              (int)((a.rows + S::BN - 1) / S::BN), 1};
-                return tok_product<T, S, S::kWaveM / 2>(st, p, Backward{a.dy, a.dy_stride, f0, n, second, w + s.g, w + s.gt, s.g_ld,
-                                                                        s.gt_ld, a.activation});
+                return tok_product<T, S, S::kWaveM / 2>(st, p, Backward{a.dy, a.dy_stride, f0, n, second, w + gr.g,
+                                                                        gr.gt_of<T>(w), gr.g_ld, gr.gt_ld, a.activation});
             }));
-        TOK_TRY(tok_with_shape(d, 2 * n, [&](auto shape) {
-            using S = decltype(shape);
-            TokProduct p{TokRows{w + s.xt, nullptr, s.gt_ld * size, d}, TokRows{w + s.gt, nullptr, s.gt_ld * size, second + n},
-                         nullptr, nullptr, a.rows * size, (int)((d + S::BM - 1) / S::BM), (int)((second + n + S::BN - 1) / S::BN), 1};
-            return tok_product<T, S, 0>(st, p, TokStoreRows{static_cast<T*>(a.dgate) + f0 * d, static_cast<T*>(a.dup) + f0 * d, d, n,
-                                                            second, nullptr});
-        }));
-        if (!a.rows) continue;
-        for (int k = 0; k < 2; ++k) {
-            const long long ld = k ? a.up_stride : a.gate_stride;
-            const T* const from = static_cast<const T*>(k ? a.up : a.gate) + f0 * ld;
-            TOK_TRY(tok_transpose<T>(st, TokTranspose{from, ld, static_cast<T*>(static_cast<void*>(w + s.wt)) + k * second, s.g_ld, n, d,
-                                                      k ? tok_round(n, 64) : second, nullptr, 0}));
-        }
-        TOK_TRY(tok_with_shape(d, a.rows, [&](auto shape) {
-            using S = decltype(shape);
-            TokProduct p{TokRows{w + s.wt, nullptr, s.g_ld * size, d}, TokRows{w + s.g, nullptr, s.g_ld * size, a.rows}, nullptr, nullptr,
-                         both * size, (int)((d + S::BM - 1) / S::BM), (int)((a.rows + S::BN - 1) / S::BN), s.cut.splits};
-            return tok_product<T, S, 0>(st, p, TokAddParts{reinterpret_cast<float*>(w + s.dx), s.dx_ld, s.padded * s.dx_ld, f0 > 0});
-        }));
+        TOK_TRY(gr.weights<T>(st, w, x, nullptr, second + n, n, second, static_cast<T*>(a.dgate) + f0 * d,
+                              static_cast<T*>(a.dup) + f0 * d, nullptr));
+        if (a.rows) TOK_TRY(gr.inputs<T>(st, w, rows, nullptr, both, n, second, f0 > 0));
     }
-    return tok_join<T>(st, TokJoin{reinterpret_cast<float*>(w + s.dx), s.dx_ld, s.padded * s.dx_ld, s.cut.splits, nullptr, nullptr,
-                                   a.dx, a.rows, d});
+    return gr.finish<T>(st, w, nullptr, nullptr, a.dx);
 }
 
 int run(void* stream, const nhip_gated_args* args, bool grad) {

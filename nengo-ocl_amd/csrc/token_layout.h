@@ -219,21 +219,109 @@ template <class T> static inline int tok_join(hipStream_t stream, const TokJoin&
     return 0;
 }
 
-// How the gradient's work is cut: pieces of `piece` weights' rows (a multiple of 256), the dx product in `splits` parts of k
-struct TokCut {
-    long long piece;
-    int splits;
+// The two products behind G: dW = G' x and dx = G W, for the rows of a piece of W.  16-bit elements in large tiles are read as
+// they lie, G and x by columns for dW, W for dx; others go through transposed copies, which for small products cost less than
+// they are.  (8192 tokens, 65536 words, 2048 channels: the copies took 7 % of the gradient's time.)
+struct TokGradient {
+    long long rows, d, size;
+    long long padded, piece, g_ld, gt_ld, dx_ld;
+    long long g = 0, gt = 0, xt = 0, wt = 0, dx = 0, dw = 0;  // in the workspace
+    int dx_splits, dw_splits;
+    bool across;
+
+    // `weights`: rows of W (of both, whole tiles of each); they are gone through in equal pieces whose G takes 512 MB at most
+    TokGradient(TokSpace& space, long long rows_, long long d_, long long weights, long long size_)
+        : rows(rows_), d(d_), size(size_) {
+        padded = tok_round(rows > 0 ? rows : 1, TOK_MOST_TILE);
+        long long most = (512LL << 20) / (padded * size) / 256 * 256;
+        most = most < 256 ? 256 : most;
+        const long long pieces = (weights + most - 1) / most;
+        piece = tok_round((weights + pieces - 1) / pieces, 256);
+        g_ld = tok_ld(piece);
+        gt_ld = tok_ld(padded);
+        dx_ld = tok_round(d, TOK_MOST_TILE);
+        const long long dw_bytes = piece * dx_ld * 4, dx_bytes = padded * dx_ld * 4, room = 256LL << 20;
+        dx_splits = tok_splits(d, rows, (int)size, piece * size);
+        dw_splits = tok_splits(d, piece, (int)size, rows * size);
+        if (dx_splits > 1 && dx_splits * dx_bytes > room) dx_splits = room / dx_bytes > 1 ? (int)(room / dx_bytes) : 1;
+        if (dw_splits > 1 && dw_splits * dw_bytes > room) dw_splits = room / dw_bytes > 1 ? (int)(room / dw_bytes) : 1;
+        across = size == 2 && tok_is_large(d, rows, 2, dx_splits) && tok_is_large(d, piece, 2, dw_splits);
+        g = space.take(padded * g_ld * size);
+        if (!across) {
+            gt = space.take(piece * gt_ld * size);
+            xt = space.take(d * gt_ld * size);
+            wt = space.take(d * g_ld * size);
+        }
+        dx = space.take(dx_splits * dx_bytes);
+        if (dw_splits > 1) dw = space.take(dw_splits * dw_bytes);
+    }
+    template <class T> T* gt_of(char* w) const { return across ? nullptr : reinterpret_cast<T*>(w + gt); }
+
+    // x (its rows that count) by channels, once for all pieces
+    template <class T> int lay_out_x(hipStream_t st, char* w, const void* x, long long ld, const int* live) const {
+        return across ? 0 : tok_transpose<T>(st, TokTranspose{x, ld, w + xt, gt_ld, rows, d, padded, live, 0});
+    }
+
+    // dW: `n` rows of G's columns, of which those below `first` go to out and `first` from `second` on to out2 (if there is one)
+    template <class T>
+    int weights(hipStream_t st, char* w, const TokRows& x, const int* live, long long n, long long first, long long second,
+                T* out, T* out2, const float* scale) const {
+        TokRows a{w + xt, nullptr, gt_ld * size, d}, b{w + gt, nullptr, gt_ld * size, n};
+        if (across) {
+            a = x;
+            a.across = tok_round(d * size, 16);
+            b = TokRows{w + g, nullptr, g_ld * size, n};
+            b.across = g_ld * size;
+        }
+        auto go = [&](const auto& epilogue) {
+            // (large in every piece if in a whole one: G's layout goes by that)
+            auto run = [&](auto shape) {
+                using S = decltype(shape);
+                constexpr int kAcross = std::is_same<S, TokLarge>::value && sizeof(T) == 2 ? 3 : 0;
+                TokProduct p{a, b, nullptr, live, rows * size, (int)((d + S::BM - 1) / S::BM), (int)((n + S::BN - 1) / S::BN), dw_splits};
+                if (kAcross && !across) return tok_product<T, S, 0>(st, p, epilogue);
+                return tok_product<T, S, 0, kAcross>(st, p, epilogue);
+            };
+            return across ? run(TokLarge()) : tok_with_shape(d, n, (int)size, dw_splits, run);
+        };
+        if (dw_splits == 1) return go(TokStoreRows{out, out2, d, first, out2 ? second : 0, scale});
+        float* const parts = reinterpret_cast<float*>(w + dw);
+        const long long part = piece * dx_ld;
+        if (int e = go(TokAddParts{parts, dx_ld, part, 0})) return e;
+        if (int e = tok_join<T>(st, TokJoin{parts, dx_ld, part, dw_splits, nullptr, scale, out, first, d})) return e;
+        return out2 ? tok_join<T>(st, TokJoin{parts + second * dx_ld, dx_ld, part, dw_splits, nullptr, scale, out2, first, d}) : 0;
+    }
+
+    // dx += G W over `k` columns of G; W's rows (p2: from `second` on, `first` of each matrix) lie at the places that `rows_of` has
+    template <class T>
+    int inputs(hipStream_t st, char* w, const TokRows& rows_of, const int* live, long long k, long long first, long long second,
+               bool add) const {
+        TokRows a{w + wt, nullptr, g_ld * size, d};
+        if (across) {
+            a = rows_of;
+            a.across = tok_round(d * size, 16);
+            a.second = second;
+            a.k_rows = first;
+        } else {
+            for (int part = 0; part < (rows_of.p2 ? 2 : 1); ++part)
+                if (int e = tok_transpose<T>(st, TokTranspose{part ? rows_of.p2 : rows_of.p, rows_of.ld / size,
+                                                              reinterpret_cast<T*>(w + wt) + part * second, g_ld, first, d,
+                                                              rows_of.p2 && !part ? second : tok_round(first, 64), nullptr, 0}))
+                    return e;
+        }
+        const TokRows b{w + g, nullptr, g_ld * size, rows};
+        const TokAddParts epilogue{reinterpret_cast<float*>(w + dx), dx_ld, padded * dx_ld, add};
+        auto run = [&](auto shape) {
+            using S = decltype(shape);
+            constexpr int kAcross = std::is_same<S, TokLarge>::value && sizeof(T) == 2 ? 1 : 0;
+            TokProduct p{a, b, live, nullptr, k * size, (int)((d + S::BM - 1) / S::BM), (int)((rows + S::BN - 1) / S::BN), dx_splits};
+            if (kAcross && !across) return tok_product<T, S, 0>(st, p, epilogue);
+            return tok_product<T, S, 0, kAcross>(st, p, epilogue);
+        };
+        return across ? run(TokLarge()) : tok_with_shape(d, rows, (int)size, dx_splits, run);
+    }
+
+    template <class T> int finish(hipStream_t st, char* w, const int* where, const float* scale, void* out) const {
+        return tok_join<T>(st, TokJoin{reinterpret_cast<float*>(w + dx), dx_ld, padded * dx_ld, dx_splits, where, scale, out, rows, d});
+    }
 };
-static inline TokCut tok_cut(long long rows, long long channels, long long weights, int size) {
-    TokCut c;
-    const long long padded = tok_round(rows > 0 ? rows : 1, 256);
-    long long most = (512LL << 20) / (padded * size) / 256 * 256;
-    most = most < 256 ? 256 : most;
-    const long long pieces = (weights + most - 1) / most;
-    c.piece = tok_round((weights + pieces - 1) / pieces, 256);
-    const long long tiles = ((channels + 127) / 128) * ((rows + 127) / 128), stages = c.piece * size / TOK_KB;
-    long long s = 1;
-    while (s < 64 && tiles * s * 2 <= 512 && stages / (s * 2) >= 16 && s * 2 * padded * tok_round(channels, 256) * 4 <= (256LL << 20)) s *= 2;
-    c.splits = (int)s;
-    return c;
-}

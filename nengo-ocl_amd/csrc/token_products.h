@@ -18,6 +18,7 @@
 typedef unsigned tok_u4 __attribute__((ext_vector_type(4)));
 typedef __bf16 tok_b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 tok_h8 __attribute__((ext_vector_type(8)));
+typedef __bf16 sel_b4 __attribute__((ext_vector_type(4)));
 
 #define TOK_MOST_LD (1 << 23)  // 256 rows lie within 2^31 bytes
 #define TOK_KB 128  // bytes of k in a stage: 64 elements of 16 bits, 32 of 32
@@ -41,6 +42,9 @@ struct TokRows {
     const char *p, *p2;
     long long ld;
     long long rows;  // that there are (of each): those beyond are read as the last one
+    // An operand that lies across (16 bits, tiles of 256): rows along m (n), one to a k, of `across` bytes; what lies beyond them
+    // is read as their last 16.  p2: the rows from k = `second` on (a multiple of 64) are those at p2, k_rows of each matrix.
+    long long across = 0, second = 0, k_rows = 0;
 };
 
 struct TokProduct {
@@ -120,6 +124,46 @@ template <int ROWS, int WAVES, int HALF> struct TokLoader {
     }
 };
 
+// The same for an operand that lies across: a stage is 64 rows of 512 bytes, one to a k.  Instruction i of a wave brings rows 2 i
+// and 2 i + 1.  Reads of 4 k by 16 columns (ds_read_b64_tr_b16) take rows 8 g + 4 h + 0 ... 3 of all four lane groups g at
+// once: these lie next to each other in the LDS, 32 bytes between two instructions' rows, and meet no bank more often than
+// their 512 bytes have to.
+#define TOK_ACROSS 1056  // bytes of two rows in the LDS
+template <int WAVES> struct TokAcross {
+    static constexpr int kMine = 32 / WAVES;
+    static_assert(WAVES == 8, "");
+    const char* at[kMine];
+    static __device__ __forceinline__ int place(int wave, int q) {
+        return (8 * (wave / 2 % 2) + 2 * (wave / 4) + wave % 2 + 16 * (q / 2) + 4 * (q % 2)) * TOK_ACROSS;
+    }
+    __device__ __forceinline__ void begin(const TokRows& t, long long col0, int wave, int lane, long long k0) {
+        const long long c = min(2 * col0 + 16 * (lane % 32), t.across - 16);
+        const bool other = t.p2 && k0 >= t.second;
+#pragma unroll
+        for (int q = 0; q < kMine; ++q)
+            at[q] = (other ? t.p2 : t.p) + (k0 - (other ? t.second : 0) + 2 * (wave + q * WAVES) + lane / 32) * t.ld + c;
+    }
+    __device__ __forceinline__ void cut(int wave, int lane, long long left) {  // rows of k that are left
+#pragma unroll
+        for (int q = 0; q < kMine; ++q)
+            at[q] = 2 * (wave + q * WAVES) + lane / 32 < left ? at[q] : reinterpret_cast<const char*>(&tok_zeros);
+    }
+    __device__ __forceinline__ void load(char* to, int wave, int q, long long ld) {
+        tok_load_lds(at[q], to + place(wave, q));
+        at[q] += 64 * ld;
+    }
+};
+
+// 8 k (from half a stage, s) of column l of a unit of 16 columns: `from` is the lane's place in the unit
+static __device__ __forceinline__ tok_u4 tok_read_across(const char* from, int s, int unit) {
+    typedef __attribute__((address_space(3))) sel_b4* lds;
+    typedef unsigned pair __attribute__((ext_vector_type(2)));
+    const char* const p = from + s * 16 * TOK_ACROSS + unit * 32;
+    const pair lo = __builtin_bit_cast(pair, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds)p));
+    const pair hi = __builtin_bit_cast(pair, __builtin_amdgcn_ds_read_tr16_b64_v4bf16((lds)(p + 8 * TOK_ACROSS)));
+    return tok_u4{lo.x, lo.y, hi.x, hi.y};
+}
+
 // A wave's part of half a stage, 64 bytes of k
 template <class S> struct TokPart {
     static constexpr int kReads = S::MI + S::NI;
@@ -190,17 +234,21 @@ template <int N> __device__ __forceinline__ void tok_wait() {  // until all but 
 // As many work-groups as run at once go over the tiles, those of a die over neighbouring ones; tiles of rows that do not count
 // are no tiles.  The stages of all its tiles are one stream to a work-group: what is on its way does not stop at a
 // tile's end.
-template <class T, class S, int HALF, class Epilogue>
+// ACROSS: bit 0: A lies across, bit 1: B does
+template <class T, class S, int HALF, int ACROSS, class Epilogue>
 __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_product_kernel(TokProduct p, Epilogue epilogue) {
     extern __shared__ __attribute__((aligned(16))) char tok_lds[];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NHIP_WAVE), lane = threadIdx.x % NHIP_WAVE;
+    static_assert(ACROSS == 0 || (S::kPair && sizeof(T) == 2 && HALF == 0), "");
+    constexpr bool kAX = ACROSS & 1, kBX = ACROSS & 2;
+    constexpr int kBytesA = kAX ? 32 * TOK_ACROSS : S::BM * TOK_KB, kStage = kBytesA + (kBX ? 32 * TOK_ACROSS : S::BN * TOK_KB);
     TokPlace at;
     at.live = (int)(p.live ? min((long long)*p.live, p.b.rows) : p.b.rows);
     at.wave_m = wave % S::WM;
     at.wave_n = wave / S::WM;
     at.l = lane % 16;
     at.g = lane / 16;
-    at.lds = tok_lds + 2 * S::kStage;
+    at.lds = tok_lds + 2 * kStage;
     const int n_tiles = (at.live + S::BN - 1) / S::BN, tiles = p.m_tiles * n_tiles, total = tiles * p.splits;
     const long long bytes = p.k_live ? (long long)*p.k_live * (int)sizeof(T) : p.k_bytes;
     const int all = (int)((bytes + TOK_KB - 1) / TOK_KB), per = (all + p.splits - 1) / p.splits;
@@ -220,17 +268,23 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
         return t;
     };
     // the stream: what is sent for next
-    using LoaderA = TokLoader<S::BM, S::kWaves, HALF>;
-    using LoaderB = TokLoader<S::BN, S::kWaves, 0>;
+    using LoaderA = typename std::conditional<kAX, TokAcross<8>, TokLoader<S::BM, S::kWaves, HALF>>::type;
+    using LoaderB = typename std::conditional<kBX, TokAcross<8>, TokLoader<S::BN, S::kWaves, 0>>::type;
     constexpr int kLoads = LoaderA::kMine + LoaderB::kMine;
     LoaderA la;
     LoaderB lb;
     int coming = id - step, coming_left = 0;  // its tile, the stages of it that are left
+    int coming_m = 0;
     long long left = 0;                       // bytes of k
     auto load = [&](int q, int place) {
-        char* const to = tok_lds + place * S::kStage;
-        if (q < LoaderA::kMine) la.load(to, wave, q);
-        else lb.load(to + S::BM * TOK_KB, wave, q - LoaderA::kMine);
+        char* const to = tok_lds + place * kStage;
+        if (q < LoaderA::kMine) {
+            if constexpr (kAX) la.load(to, wave, q, p.a.ld);
+            else la.load(to, wave, q);
+        } else {
+            if constexpr (kBX) lb.load(to + kBytesA, wave, q - LoaderA::kMine, p.b.ld);
+            else lb.load(to + kBytesA, wave, q - LoaderA::kMine);
+        }
     };
     auto sent = [&] {
         left -= TOK_KB;
@@ -249,13 +303,23 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
                 const Tile t = tile(coming);
                 const long long k0 = (long long)t.k0 * TOK_KB;
                 left = bytes - k0;
-                la.begin(p.a, (long long)t.m * S::BM, wave, lane, k0);
-                lb.begin(p.b, (long long)t.n * S::BN, wave, lane, k0);
+                la.begin(p.a, (long long)t.m * S::BM, wave, lane, kAX ? k0 / (int)sizeof(T) : k0);
+                lb.begin(p.b, (long long)t.n * S::BN, wave, lane, kBX ? k0 / (int)sizeof(T) : k0);
+                coming_m = t.m;
             }
         }
+        if constexpr (kAX)
+            if (p.a.p2 && left > 0) {  // two matrices: the second one's rows begin, the rows of one end
+                const long long k = (bytes - left) / (int)sizeof(T);
+                if (k == p.a.second) la.begin(p.a, (long long)coming_m * S::BM, wave, lane, k);
+                const long long rest = p.a.k_rows - (k < p.a.second ? k : k - p.a.second);
+                if (rest < 64) la.cut(wave, lane, rest);
+            }
         if (left < TOK_KB) {  // (a stage of zeros is `left` below zero for the next one: that is cut, too)
-            la.cut(lane, (int)left);
-            lb.cut(lane, (int)left);
+            if constexpr (kAX) la.cut(wave, lane, left / (int)sizeof(T));
+            else la.cut(lane, (int)left);
+            if constexpr (kBX) lb.cut(wave, lane, left / (int)sizeof(T));
+            else lb.cut(lane, (int)left);
         }
     };
 
@@ -271,6 +335,7 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
     tok_wait<0>();
     constexpr int kSteps = TokPart<S>::kReads;
     const int c0 = (at.g ^ (at.l & 7)) * 16 + at.l * TOK_KB, c1 = c0 ^ 64;
+    const int cx = (2 * at.g + at.l / 8) * TOK_ACROSS + at.l / 4 % 2 * 512 + at.l % 4 * 8;  // across
     int place = 0;  // of the stage that is multiplied next
     for (; id < end; id += step) {
         const Tile now = tile(id);
@@ -282,8 +347,8 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
         for (int i = 0; i < S::MI; ++i)
 #pragma unroll
             for (int j = 0; j < S::NI; ++j) acc[i][j] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
-        const char* const a0 = tok_lds + at.wave_m * S::kWaveM * TOK_KB;
-        const char* const b0 = tok_lds + (S::BM + at.wave_n * S::kWaveN) * TOK_KB;
+        const char* const a0 = tok_lds + (kAX ? at.wave_m * S::kWaveM * 2 + cx : at.wave_m * S::kWaveM * TOK_KB);
+        const char* const b0 = tok_lds + kBytesA + (kBX ? at.wave_n * S::kWaveN * 2 + cx : at.wave_n * S::kWaveN * TOK_KB);
         if constexpr (S::kPair) {
             // Two groups of four waves, one of each to a SIMD, take turns: while one multiplies a quarter of its tile by a stage,
             // the other reads its next quarter's operands and sends for more.  The second group is half a turn behind, which
@@ -294,15 +359,19 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int i = 0; i < HM; ++i)
-                        a[s][i] = *reinterpret_cast<const tok_u4*>(a0 + place * S::kStage + (s ? c1 : c0) + (h * HM + i) * 16 * TOK_KB);
+                    for (int i = 0; i < HM; ++i) {
+                        if constexpr (kAX) a[s][i] = tok_read_across(a0 + place * kStage, s, h * HM + i);
+                        else a[s][i] = *reinterpret_cast<const tok_u4*>(a0 + place * kStage + (s ? c1 : c0) + (h * HM + i) * 16 * TOK_KB);
+                    }
             };
             auto read_b = [&](int h) {
 #pragma unroll
                 for (int s = 0; s < 2; ++s)
 #pragma unroll
-                    for (int j = 0; j < HN; ++j)
-                        b[h][s][j] = *reinterpret_cast<const tok_u4*>(b0 + place * S::kStage + (s ? c1 : c0) + (h * HN + j) * 16 * TOK_KB);
+                    for (int j = 0; j < HN; ++j) {
+                        if constexpr (kBX) b[h][s][j] = tok_read_across(b0 + place * kStage, s, h * HN + j);
+                        else b[h][s][j] = *reinterpret_cast<const tok_u4*>(b0 + place * kStage + (s ? c1 : c0) + (h * HN + j) * 16 * TOK_KB);
+                    }
             };
             auto turn = [&] {
                 asm volatile("" ::: "memory");
@@ -354,7 +423,7 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
         } else {
             TokPart<S> first, second;
             tok_settle<S>(acc);  // (zeros, too, are written before they are an addend)
-            if (now.stages > 0) first.read(a0 + place * S::kStage, b0 + place * S::kStage, c0);
+            if (now.stages > 0) first.read(a0 + place * kStage, b0 + place * kStage, c0);
             // Half a stage: `next` is read, and `loads` are sent for, between the products.  (Products first: the compiler waits for
             // all reads before the first one, which have come then; and no read among the last quarter, whose time a read takes.)
             auto half = [&](const TokPart<S>& mine, TokPart<S>& next, int from, int c, auto&& loads) {
@@ -363,7 +432,7 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
                     mine.template multiply<T>(acc, q, kSteps);
 #pragma unroll
                     for (int o = 4 * q / 3; o < 4 * (q + 1) / 3 && o < kSteps; ++o)
-                        next.read_one(o, a0 + from * S::kStage, b0 + from * S::kStage, c);
+                        next.read_one(o, a0 + from * kStage, b0 + from * kStage, c);
                     loads(q);
                     __builtin_amdgcn_sched_barrier(0);
                 }
@@ -394,13 +463,16 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
     tok_wait<0>();  // (nothing arrives in the LDS of a work-group that has ended)
 }
 
-// Four values of column n in rows m ... m + 3 (a lane's part of a tile), stored along m at g[n, m] and along n at gt[m, n].
+// Four values of column n in rows m ... m + 3 (a lane's part of a tile), stored along m at g[n, m] and (unless it is NULL) along n
+// at gt[m, n].
 // 16 bits: the four lanes of neighbouring columns exchange theirs, so that each stores four neighbours along n, too.
 template <class T>
 __device__ __forceinline__ void tok_store_both(T* g, long long g_ld, T* gt, long long gt_ld, long long n, long long m,
                                                const float (&v)[4]) {
     T* const to = g + n * g_ld + m;
-    if constexpr (sizeof(T) == 2) {
+    if (!gt) {
+        sel_store<T, 4>(to, v);
+    } else if constexpr (sizeof(T) == 2) {
         typedef unsigned pair __attribute__((ext_vector_type(2)));
         SelPack<T, 4> q;
 #pragma unroll
@@ -428,25 +500,43 @@ __device__ __forceinline__ void tok_store_both(T* g, long long g_ld, T* gt, long
     }
 }
 
-template <class T, class S, int HALF, class E>
+template <class T, class S, int HALF, int ACROSS = 0, class E>
 static inline int tok_product(hipStream_t stream, const TokProduct& p, const E& epilogue) {
     const long long tiles = (long long)p.m_tiles * p.n_tiles * p.splits, groups = 256 * S::kAtOnce;
     if (tiles == 0) return 0;
     if (tiles > 0x3fffffff) return NHIP_E_BADARG;
-    auto kernel = tok_product_kernel<T, S, HALF, E>;
-    if (int e = sel_allow_lds(stream, kernel, S::kLds)) return e;
-    NHIP_LAUNCH(kernel, dim3((unsigned)(tiles < groups ? tiles : groups)), dim3(S::kThreads), S::kLds, stream, p, epilogue);
+    auto kernel = tok_product_kernel<T, S, HALF, ACROSS, E>;
+    constexpr int kLds = S::kLds + (ACROSS ? 2 * 64 * (TOK_ACROSS - 1024) : 0);
+    if (int e = sel_allow_lds(stream, kernel, kLds)) return e;
+    NHIP_LAUNCH(kernel, dim3((unsigned)(tiles < groups ? tiles : groups)), dim3(S::kThreads), kLds, stream, p, epilogue);
     NHIP_LAUNCH_CHECK();
     return 0;
 }
 
-// Calls f(tile shape) for a product of m x n
-template <class F> static inline int tok_with_shape(long long m, long long n, F&& f) {
-    const long long large = ((m + 255) / 256) * ((n + 255) / 256);
-    if (n > 128 && large >= 128) return f(TokShape<256, 256, 2, 4>());
+using TokLarge = TokShape<256, 256, 2, 4>;
+#define TOK_LEAST_BM 128  // of all shapes
+#define TOK_MOST_TILE 256
+
+// The shape of a product of m x n in elements of `size` bytes: tiles of 256 x 256 where they are enough to go round, of fewer
+// columns where there are few.  (8192 x 11008 x 2048 in bfloat16: 1320 TFLOP/s by tiles of 256, 800 by tiles of 128; in 32 bits,
+// where the matrix instructions take as long either way, the smaller ones share 256 compute units more evenly.)
+static inline bool tok_is_large(long long m, long long n, int size, int splits) {
+    const long long large = ((m + 255) / 256) * ((n + 255) / 256) * splits;
+    return n > 128 && m > 128 && large >= (size == 2 ? 96 : 512);
+}
+template <class F> static inline int tok_with_shape(long long m, long long n, int size, int splits, F&& f) {
+    if (tok_is_large(m, n, size, splits)) return f(TokLarge());
     if (n > 64) return f(TokShape<128, 128, 2, 2>());
     if (n > 16) return f(TokShape<128, 64, 4, 1>());
     return f(TokShape<128, 16, 4, 1>());
 }
-#define TOK_LEAST_BM 128  // of the shapes above
-#define TOK_MOST_TILE 256
+
+// Into how many parts k (of k_bytes) is cut so that a product of m x n goes round 256 compute units, parts of eight stages at least.
+static inline int tok_splits(long long m, long long n, int size, long long k_bytes) {
+    const long long stages = k_bytes / TOK_KB, most = stages / 8 < 64 ? stages / 8 : 64;
+    long long s = 1;
+    if (size == 2 && n > 128 && m > 128) s = 256 / (((m + 255) / 256) * ((n + 255) / 256));
+    else s = 512 / (((m + 127) / 128) * ((n + 127) / 128));
+    s = s < most ? s : most;
+    return (int)(s < 1 ? 1 : s);
+}

@@ -7,6 +7,9 @@
 // The forward pass forms tiles of z and leaves of each the maximum and the sum of a token's exponentials and the
 // logits of its targets.  The backward pass goes over the vocabulary in pieces: a piece's part of G is formed from z again and kept,
 // in the type of x, for the two products that read it.
+#include <algorithm>
+#include <optional>
+
 #include "token_layout.h"
 
 namespace {
@@ -403,11 +406,11 @@ __global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
     }
 }
 
-// Backward: G of the tile, in both layouts
+// Backward: G of the tile
 template <bool TOP> struct Gradient {
     Targets targets;
     const float *dloss, *lse, *scale;
-    void *g, *gt;             // [live, g_ld], [words, gt_ld]
+    void *g, *gt;             // [live, g_ld], [words, gt_ld] (or NULL)
     long long g_ld, gt_ld;
     int words, word0;
     float per_temperature;
@@ -442,7 +445,7 @@ template <bool TOP> struct Gradient {
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
                 const T v = (T)(d * (__builtin_amdgcn_exp2f(fmaf(z, c, -lse2)) - share));
                 static_cast<T*>(g)[n * g_ld + m0 + rel] = v;
-                static_cast<T*>(gt)[(m0 + rel) * gt_ld + n] = v;
+                if (gt) static_cast<T*>(gt)[(m0 + rel) * gt_ld + n] = v;
             };
             if (counts) {
                 if constexpr (TOP) {
@@ -474,15 +477,13 @@ bool wide_weight(const nhip_loss_args& a) {
 }
 
 struct Space : TokSpace {
-    long long padded, x_ld, piece, g_ld, gt_ld, dx_ld;
-    long long row, where, label, count, flag, word, share, self, first, blocks, x, weight, part, logits, xt, wt, g, gt, dx;
-    TokCut cut;
+    long long padded, x_ld, piece;
+    long long row, where, label, count, flag, word, share, self, first, blocks, x, weight, part, logits;
+    std::optional<TokGradient> gradient;
     Space(const nhip_loss_args& a, bool grad) {
         const long long size = sel_size(a.type), rows = a.rows > 0 ? a.rows : 1, top = a.top;
         padded = tok_round(rows, TOK_MOST_TILE);
         x_ld = tok_round(a.channels, 64);
-        cut = tok_cut(a.rows, a.channels, a.words, (int)size);
-        piece = cut.piece;
         row = take(padded * 4);
         where = take(rows * 4);
         label = take(padded * 4);
@@ -497,20 +498,18 @@ struct Space : TokSpace {
             first = take(rows * blocks * 2);
         }
         x = take(padded * x_ld * size);
-        weight = wide_weight(a) ? 0 : take(piece * x_ld * size);
-        if (!grad) {
+        if (grad) {
+            gradient.emplace(*this, a.rows, a.channels, a.words, size);
+            piece = gradient->piece;
+        } else {
+            // as many words as a launch's tiles reach, and where they are copied as fit 512 MB
+            piece = (1LL << 22) / (padded / 256) * 128;
+            if (!wide_weight(a)) piece = std::min(piece, std::max(256LL, (512LL << 20) / (x_ld * size) / 256 * 256));
+            piece = std::min(piece, tok_round(a.words, 256));
             part = take((tok_round(a.words, piece) / TOK_LEAST_BM) * padded * 8);
             logits = take(padded * (top ? top : 1) * 4);
-        } else {
-            g_ld = tok_ld(piece);
-            gt_ld = tok_ld(padded);
-            dx_ld = tok_round(a.channels, TOK_MOST_TILE);
-            xt = take((long long)a.channels * gt_ld * size);
-            wt = take((long long)a.channels * g_ld * size);
-            g = take(padded * g_ld * size);
-            gt = take(piece * gt_ld * size);
-            dx = take(cut.splits * padded * dx_ld * 4);
         }
+        weight = wide_weight(a) ? 0 : take(piece * x_ld * size);
     }
 };
 
@@ -565,7 +564,7 @@ template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Sp
         const long long words = a.words - v0 < s.piece ? a.words - v0 : s.piece;
         TokRows rows;
         TOK_TRY(piece_rows<T>(st, a, s, w, v0, words, rows));
-        TOK_TRY(tok_with_shape(words, a.rows, [&](auto shape) {
+        TOK_TRY(tok_with_shape(words, a.rows, sizeof(T), 1, [&](auto shape) {
             using S = decltype(shape);
             TokProduct p{rows, TokRows{w + s.x, nullptr, s.x_ld * (long long)sizeof(T), a.rows}, count, nullptr,
                          a.channels * (long long)sizeof(T), (int)((words + S::BM - 1) / S::BM),
@@ -594,7 +593,8 @@ template <class T> int backward(hipStream_t st, const nhip_loss_args& a, const S
     Targets t;
     TOK_TRY(prepare<T>(st, a, s, w, true, t));
     const int* const count = reinterpret_cast<int*>(w + s.count);
-    TOK_TRY(tok_transpose<T>(st, TokTranspose{w + s.x, s.x_ld, w + s.xt, s.gt_ld, a.rows, a.channels, s.padded, count, 0}));
+    const TokGradient& gr = *s.gradient;
+    TOK_TRY(gr.lay_out_x<T>(st, w, w + s.x, s.x_ld, count));
     float* scale = nullptr;
     if constexpr (std::is_same<T, _Float16>::value) {
         scale = reinterpret_cast<float*>(w + s.count) + 16;
@@ -606,36 +606,23 @@ template <class T> int backward(hipStream_t st, const nhip_loss_args& a, const S
         const long long words = a.words - v0 < s.piece ? a.words - v0 : s.piece;
         TokRows rows;
         TOK_TRY(piece_rows<T>(st, a, s, w, v0, words, rows));
-        const TokRows g{w + s.g, nullptr, s.g_ld * size, a.rows};
-        TOK_TRY(tok_with_shape(words, a.rows, [&](auto shape) {
+        const TokRows x{w + s.x, nullptr, s.x_ld * size, a.rows};
+        TOK_TRY(tok_with_shape(words, a.rows, sizeof(T), 1, [&](auto shape) {
             using S = decltype(shape);
-            TokProduct p{rows, TokRows{w + s.x, nullptr, s.x_ld * size, a.rows}, count, nullptr, d * size,
+            TokProduct p{rows, x, count, nullptr, d * size,
                          (int)((words + S::BM - 1) / S::BM), (int)((a.rows + S::BN - 1) / S::BN), 1};
             auto go = [&](auto top) {
-                Gradient<decltype(top)::value> e{t, a.dloss, a.lse, scale, w + s.g, w + s.gt, s.g_ld, s.gt_ld, (int)words, (int)v0,
+                Gradient<decltype(top)::value> e{t, a.dloss, a.lse, scale, w + gr.g, gr.gt_of<T>(w), gr.g_ld, gr.gt_ld, (int)words, (int)v0,
                                                  1.0f / a.temperature};
                 return tok_product<T, S, 0>(st, p, e);
             };
             return a.top ? go(std::true_type()) : go(std::false_type());
         }));
-        TOK_TRY(tok_with_shape(d, words, [&](auto shape) {
-            using S = decltype(shape);
-            TokProduct p{TokRows{w + s.xt, nullptr, s.gt_ld * size, d}, TokRows{w + s.gt, nullptr, s.gt_ld * size, words}, nullptr,
-                         count, 0, (int)((d + S::BM - 1) / S::BM), (int)((words + S::BN - 1) / S::BN), 1};
-            return tok_product<T, S, 0>(st, p, TokStoreRows{static_cast<T*>(a.dweight) + v0 * d, nullptr, d, words, 0,
-                                                            scale ? scale + 1 : nullptr});
-        }));
-        const T* const from = static_cast<const T*>(a.weight) + v0 * a.weight_stride;
-        TOK_TRY(tok_transpose<T>(st, TokTranspose{from, a.weight_stride, w + s.wt, s.g_ld, words, d, tok_round(words, 64), nullptr, 0}));
-        TOK_TRY(tok_with_shape(d, a.rows, [&](auto shape) {
-            using S = decltype(shape);
-            TokProduct p{TokRows{w + s.wt, nullptr, s.g_ld * size, d}, g, count, nullptr, words * size,
-                         (int)((d + S::BM - 1) / S::BM), (int)((a.rows + S::BN - 1) / S::BN), s.cut.splits};
-            return tok_product<T, S, 0>(st, p, TokAddParts{reinterpret_cast<float*>(w + s.dx), s.dx_ld, s.padded * s.dx_ld, v0 > 0});
-        }));
+        TOK_TRY(gr.weights<T>(st, w, x, count, words, words, 0, static_cast<T*>(a.dweight) + v0 * d, static_cast<T*>(nullptr),
+                              scale ? scale + 1 : nullptr));
+        TOK_TRY(gr.inputs<T>(st, w, rows, count, words, words, 0, v0 > 0));
     }
-    return tok_join<T>(st, TokJoin{reinterpret_cast<float*>(w + s.dx), s.dx_ld, s.padded * s.dx_ld, s.cut.splits,
-                                   reinterpret_cast<int*>(w + s.where), scale ? scale + 1 : nullptr, a.dx, a.rows, d});
+    return gr.finish<T>(st, w, reinterpret_cast<int*>(w + s.where), scale ? scale + 1 : nullptr, a.dx);
 }
 
 int run(void* stream, const nhip_loss_args* args, bool grad) {
