@@ -172,11 +172,17 @@ template <class T> int forward(hipStream_t st, const nhip_gated_args& a, const S
     for (long long f0 = 0; f0 < a.features; f0 += s.piece) {
         const long long n = a.features - f0 < s.piece ? a.features - f0 : s.piece;
         TOK_TRY(weight_rows<T>(st, a, s, w, f0, n, rows));
+        TokProduct p{rows, x, nullptr, nullptr, a.channels * (long long)sizeof(T), 0, 0, 1};
+        const Forward e{a.y, a.features, f0, n, a.activation};
+        if (a.rows <= TOK_FEW) {
+            TOK_TRY((tok_few<T, 2, 1>(st, p, e)));
+            continue;
+        }
         TOK_TRY(tok_with_shape(2 * n, a.rows, sizeof(T), 1, [&](auto shape) {
             using S = decltype(shape);
-            TokProduct p{rows, x, nullptr, nullptr, a.channels * (long long)sizeof(T), (int)((2 * n + S::BM - 1) / S::BM),
-                         (int)((a.rows + S::BN - 1) / S::BN), 1};
-            return tok_product<T, S, S::kWaveM / 2>(st, p, Forward{a.y, a.features, f0, n, a.activation});
+            p.m_tiles = (int)((2 * n + S::BM - 1) / S::BM);
+            p.n_tiles = (int)((a.rows + S::BN - 1) / S::BN);
+            return tok_product<T, S, S::kWaveM / 2>(st, p, e);
         }));
     }
     return 0;

@@ -209,13 +209,13 @@ static __device__ __forceinline__ void tok_tile(int id, int m_tiles, int n_tiles
 
 // Waits until the products before it are done: a result that is read behind the loop's branch needs it (see sel_settle).
 // Waves that have a SIMD for themselves hold results in accumulation registers, others among the vector registers.
-template <class S> __device__ __forceinline__ void tok_settle(sel_f4 (&acc)[S::MI][S::NI]) {
+template <bool PINNED, int MI, int NI> __device__ __forceinline__ void tok_settle(sel_f4 (&acc)[MI][NI]) {
     auto touch = [&] {
 #pragma unroll
-        for (int i = 0; i < S::MI; ++i)
+        for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < S::NI; ++j) {
-                if constexpr (S::kPinned) asm volatile("" : "+a"(acc[i][j]));
+            for (int j = 0; j < NI; ++j) {
+                if constexpr (PINNED) asm volatile("" : "+a"(acc[i][j]));
                 else asm volatile("" : "+v"(acc[i][j]));
             }
     };
@@ -422,7 +422,7 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
             if (!behind) turn();
         } else {
             TokPart<S> first, second;
-            tok_settle<S>(acc);  // (zeros, too, are written before they are an addend)
+            tok_settle<S::kPinned>(acc);  // (zeros, too, are written before they are an addend)
             if (now.stages > 0) first.read(a0 + place * kStage, b0 + place * kStage, c0);
             // Half a stage: `next` is read, and `loads` are sent for, between the products.  (Products first: the compiler waits for
             // all reads before the first one, which have come then; and no read among the last quarter, whose time a read takes.)
@@ -455,12 +455,122 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
                 stage();
             }
         }
-        tok_settle<S>(acc);
+        tok_settle<S::kPinned>(acc);
         TokPlace here = at;
         asm volatile("" : "+v"(here.l), "+v"(here.g));  // (or what an epilogue forms of them is kept over all tiles, and spilled)
         epilogue.template run<T, S>(here, acc);
     }
     tok_wait<0>();  // (nothing arrives in the LDS of a work-group that has ended)
+}
+
+// Few columns (16 NI): nothing is read twice, so that all is the time that A takes to arrive.  A work-group has MT tiles of 16 rows;
+// its four waves have a quarter of k each, straight from memory into registers, U steps of 64 bytes of k under way while as
+// many are multiplied, and add up their sums in the LDS.  (One row, 2048 channels, 2 x 5504 features in bfloat16: 45 MB in 10 us;
+// tiles of 128 rows through the LDS, 86 work-groups, took 18.)
+template <int MT_, int NI_> struct TokFew {
+    static constexpr int MT = MT_, NI = NI_, kWaves = 4, U = 8 / MT_;
+    using Shape = TokShape<16 * MT_, 16, 1, 1>;  // what an epilogue sees: a wave has a tile of 16 columns
+};
+
+template <class T, class F, int HALF, class Epilogue>
+__global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_few_kernel(TokProduct p, Epilogue epilogue) {
+    constexpr int MT = F::MT, NI = F::NI, U = F::U;
+    __shared__ sel_f4 s_sum[F::kWaves][MT][NI][NHIP_WAVE];
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NHIP_WAVE), lane = threadIdx.x % NHIP_WAVE;
+    TokPlace at;
+    at.m_tile = nhip_xcd_remap(blockIdx.x, gridDim.x);
+    at.split = at.wave_m = at.wave_n = 0;
+    at.l = lane % 16;
+    at.g = lane / 16;
+    at.live = (int)(p.live ? min((long long)*p.live, p.b.rows) : p.b.rows);
+    at.lds = nullptr;
+    if (at.live <= 0) return;
+    const int bytes = (int)p.k_bytes, steps = (bytes + 63) / 64, per = (steps + F::kWaves - 1) / F::kWaves;
+    const int first = min(steps, wave * per), n = min(steps, first + per) - first;
+    const char *a[MT], *b[NI];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const bool other = HALF && i >= MT / 2;  // (equal rows of both matrices, as an epilogue wants them)
+        const long long r = (long long)at.m_tile * (HALF ? 8 * MT : 16 * MT) + 16 * (other ? i - MT / 2 : i) + at.l;
+        a[i] = (other ? p.a.p2 : p.a.p) + min(r, p.a.rows - 1) * p.a.ld + 16 * at.g;
+    }
+#pragma unroll
+    for (int j = 0; j < NI; ++j) b[j] = p.b.p + min(16LL * j + at.l, (long long)at.live - 1) * p.b.ld + 16 * at.g;
+    struct Batch {
+        tok_u4 a[U][MT], b[U][NI];
+    };
+    // (unconditional: what lies behind the end of k, or of the wave's part, is read from elsewhere)
+    auto load = [&](Batch& v, int step) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (first + step + u) * 64;
+            const bool is = step + u < n && k + 16 * at.g < bytes;
+            const char* const zeros = reinterpret_cast<const char*>(&tok_zeros);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) v.a[u][i] = *reinterpret_cast<const tok_u4*>(is ? a[i] + k : zeros);
+#pragma unroll
+            for (int j = 0; j < NI; ++j) v.b[u][j] = *reinterpret_cast<const tok_u4*>(is ? b[j] + k : zeros);
+        }
+    };
+    sel_f4 acc[MT][NI];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](const Batch& v) {
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int e = 0; e < (sizeof(T) == 2 ? 1 : 4); ++e)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) tok_mma<T>(acc[i][j], v.a[u][i], v.b[u][j], e);
+    };
+    Batch even, odd;
+    load(even, 0);
+    for (int step = 0; step < n; step += 2 * U) {
+        load(odd, step + U);
+        multiply(even);
+        load(even, step + 2 * U);
+        multiply(odd);
+    }
+    tok_settle<false>(acc);
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) s_sum[wave][i][j][lane] = acc[i][j];
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+        if (j % F::kWaves != wave || 16 * j >= at.live) continue;
+        sel_f4 sum[MT][1];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+            sum[i][0] = s_sum[0][i][j][lane];
+#pragma unroll
+            for (int w = 1; w < F::kWaves; ++w) sum[i][0] += s_sum[w][i][j][lane];
+        }
+        at.n_tile = j;
+        epilogue.template run<T, typename F::Shape>(at, sum);
+    }
+}
+
+#define TOK_FEW 64  // rows of B that the kernel for few columns takes
+template <class T, int MT, int HALF, class E>
+static inline int tok_few(hipStream_t stream, TokProduct p, const E& epilogue) {
+    const long long rows = HALF ? 8 * MT : 16 * MT, tiles = (p.a.rows + rows - 1) / rows;
+    if (tiles == 0 || p.b.rows == 0) return 0;
+    if (p.b.rows > TOK_FEW || tiles > 0xffffff) return NHIP_E_BADARG;
+    auto go = [&](auto few) {
+        using F = decltype(few);
+        NHIP_LAUNCH((tok_few_kernel<T, F, HALF, E>), dim3((unsigned)tiles), dim3(F::kWaves * NHIP_WAVE), 0, stream, p, epilogue);
+        return (int)hipGetLastError();
+    };
+    if (p.b.rows <= 16) return go(TokFew<MT, 1>());
+    if (p.b.rows <= 32) return go(TokFew<MT, 2>());
+    if (p.b.rows <= 48) return go(TokFew<MT, 3>());
+    return go(TokFew<MT, 4>());
 }
 
 // Four values of column n in rows m ... m + 3 (a lane's part of a tile), stored along m at g[n, m] and (unless it is NULL) along n
@@ -514,7 +624,7 @@ static inline int tok_product(hipStream_t stream, const TokProduct& p, const E& 
 }
 
 using TokLarge = TokShape<256, 256, 2, 4>;
-#define TOK_LEAST_BM 128  // of all shapes
+#define TOK_LEAST_BM 64  // of all shapes, and of the kernel for few columns
 #define TOK_MOST_TILE 256
 
 // The shape of a product of m x n in elements of `size` bytes: tiles of 256 x 256 where they are enough to go round, of fewer

@@ -287,7 +287,7 @@ template <bool TOP> struct Statistics {
         const long long n0 = (long long)at.n_tile * S::BN;
         const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g;  // within the piece
         const int w0 = word0 + at.m_tile * S::BM;
-        __syncthreads();  // (the tile before is done with the LDS)
+        if (S::WM > 1) __syncthreads();  // (the tile before is done with the LDS)
         const float c = kLog2e * per_temperature;
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
@@ -311,7 +311,11 @@ template <bool TOP> struct Statistics {
                     if (m0 + 16 * i + r < words) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -top2));
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
-            if (at.g == 0) s_part[at.wave_m * S::BN + local] = float2{top2, sum};
+            if constexpr (S::WM > 1) {
+                if (at.g == 0) s_part[at.wave_m * S::BN + local] = float2{top2, sum};
+            } else {
+                if (at.g == 0 && n < at.live) part[(long long)(tile0 + at.m_tile) * ld + n] = float2{top2, sum};
+            }
             auto pick = [&](int word, float* to) {
                 const int rel = word - word0 - m0;
                 if (rel < 0 || rel >= S::kWaveM || (rel & 15) >= 4) return;
@@ -332,12 +336,14 @@ template <bool TOP> struct Statistics {
                 }
             }
         }
-        __syncthreads();
-        for (int k = threadIdx.x; k < S::BN; k += S::kThreads) {
-            float2 a = s_part[k];
+        if constexpr (S::WM > 1) {
+            __syncthreads();
+            for (int k = threadIdx.x; k < S::BN; k += S::kThreads) {
+                float2 a = s_part[k];
 #pragma unroll
-            for (int w = 1; w < S::WM; ++w) a = joined(a, s_part[w * S::BN + k]);
-            if (n0 + k < at.live) part[(long long)(tile0 + at.m_tile) * ld + n0 + k] = a;
+                for (int w = 1; w < S::WM; ++w) a = joined(a, s_part[w * S::BN + k]);
+                if (n0 + k < at.live) part[(long long)(tile0 + at.m_tile) * ld + n0 + k] = a;
+            }
         }
     }
     // of two parts, neither of which is more than infinite
@@ -564,20 +570,24 @@ template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Sp
         const long long words = a.words - v0 < s.piece ? a.words - v0 : s.piece;
         TokRows rows;
         TOK_TRY(piece_rows<T>(st, a, s, w, v0, words, rows));
-        TOK_TRY(tok_with_shape(words, a.rows, sizeof(T), 1, [&](auto shape) {
-            using S = decltype(shape);
-            TokProduct p{rows, TokRows{w + s.x, nullptr, s.x_ld * (long long)sizeof(T), a.rows}, count, nullptr,
-                         a.channels * (long long)sizeof(T), (int)((words + S::BM - 1) / S::BM),
-                         (int)((a.rows + S::BN - 1) / S::BN), 1};
-            auto go = [&](auto top) {
-                Statistics<decltype(top)::value> e{t, reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits),
-                                                   s.padded, (int)words, (int)v0, tiles, 1.0f / a.temperature};
+        TokProduct p{rows, TokRows{w + s.x, nullptr, s.x_ld * (long long)sizeof(T), a.rows}, count, nullptr,
+                     a.channels * (long long)sizeof(T), 0, 0, 1};
+        auto go = [&](auto top) {
+            Statistics<decltype(top)::value> e{t, reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits),
+                                               s.padded, (int)words, (int)v0, tiles, 1.0f / a.temperature};
+            if (a.rows <= TOK_FEW) {
+                tiles += (int)((words + TOK_LEAST_BM - 1) / TOK_LEAST_BM);
+                return tok_few<T, TOK_LEAST_BM / 16, 0>(st, p, e);
+            }
+            return tok_with_shape(words, a.rows, sizeof(T), 1, [&](auto shape) {
+                using S = decltype(shape);
+                p.m_tiles = (int)((words + S::BM - 1) / S::BM);
+                p.n_tiles = (int)((a.rows + S::BN - 1) / S::BN);
+                tiles += p.m_tiles;
                 return tok_product<T, S, 0>(st, p, e);
-            };
-            const int rc = a.top ? go(std::true_type()) : go(std::false_type());
-            tiles += p.m_tiles;
-            return rc;
-        }));
+            });
+        };
+        TOK_TRY(a.top ? go(std::true_type()) : go(std::false_type()));
     }
     if (!a.rows) return 0;
     Finish f{reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits), t, reinterpret_cast<float*>(w + s.self),
