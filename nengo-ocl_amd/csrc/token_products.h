@@ -463,12 +463,12 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
     tok_wait<0>();  // (nothing arrives in the LDS of a work-group that has ended)
 }
 
-// Few columns (16 NI): nothing is read twice, so that all is the time that A takes to arrive.  A work-group has MT tiles of 16 rows;
+// Up to 16 columns: nothing is read twice, so that all is the time that A takes to arrive.  A work-group has MT tiles of 16 rows;
 // its four waves have a quarter of k each, straight from memory into registers, U steps of 64 bytes of k under way while as
-// many are multiplied, and add up their sums in the LDS.  (One row, 2048 channels, 2 x 5504 features in bfloat16: 45 MB in 10 us;
-// tiles of 128 rows through the LDS, 86 work-groups, took 18.)
-template <int MT_, int NI_> struct TokFew {
-    static constexpr int MT = MT_, NI = NI_, kWaves = 4, U = 8 / MT_;
+// many are multiplied, and add up their sums in the LDS.  (One row, 2048 channels, 2 x 5504 features in bfloat16: 45 MB in 13 us,
+// 205 MB of a vocabulary in 43, 4.8 TB/s; tiles of 128 rows through the LDS, 86 work-groups, took 18.)
+template <int MT_> struct TokFew {
+    static constexpr int MT = MT_, NI = 1, kWaves = 4, U = 8 / MT_;
     using Shape = TokShape<16 * MT_, 16, 1, 1>;  // what an epilogue sees: a wave has a tile of 16 columns
 };
 
@@ -556,21 +556,140 @@ __global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_few_kernel(TokPr
     }
 }
 
-#define TOK_FEW 64  // rows of B that the kernel for few columns takes
+// 17 to 64 columns (16 NI): B, which all waves of a work-group read, goes through the LDS, 256 bytes of k at a time; A still goes
+// straight into registers.  Two waves share rows and have half of k each.  (48 rows, 2304 channels, 2 x 6144 features in
+// float16: B from the L2 into every wave's registers took 24 us, as much again as A.)
+template <int MT_, int NI_> struct TokSome {
+    static constexpr int MT = MT_, NI = NI_, kWaves = 4, kRows = 32 * MT_;  // of A, to a work-group
+    static constexpr int kChunk = 256, kSteps = kChunk / 64, kPart = 16 * NI * kChunk, kLds = 4 * kPart;
+    using Shape = TokShape<16 * MT_, 16, 1, 1>;
+};
+
+template <class T, class F, int HALF, class Epilogue>
+__global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_some_kernel(TokProduct p, Epilogue epilogue) {
+    constexpr int MT = F::MT, NI = F::NI;
+    extern __shared__ __attribute__((aligned(16))) char tok_lds[];  // [2 in turn][2 halves of k][16 NI rows][256]
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NHIP_WAVE), lane = threadIdx.x % NHIP_WAVE;
+    const int mine = wave % 2, half = wave / 2;
+    TokPlace at;
+    at.m_tile = 2 * nhip_xcd_remap(blockIdx.x, gridDim.x) + mine;
+    at.split = at.wave_m = at.wave_n = 0;
+    at.l = lane % 16;
+    at.g = lane / 16;
+    at.live = (int)(p.live ? min((long long)*p.live, p.b.rows) : p.b.rows);
+    at.lds = nullptr;
+    if (at.live <= 0) return;
+    const int bytes = (int)p.k_bytes, chunks = (bytes + F::kChunk - 1) / F::kChunk, per = (chunks + 1) / 2;  // the same of both halves
+    const int k0 = half * per * F::kChunk;
+    const char* a[MT];
+#pragma unroll
+    for (int i = 0; i < MT; ++i) {
+        const bool other = HALF && i >= MT / 2;
+        const long long r = (long long)at.m_tile * (HALF ? 8 * MT : 16 * MT) + 16 * (other ? i - MT / 2 : i) + at.l;
+        a[i] = (other ? p.a.p2 : p.a.p) + min(r, p.a.rows - 1) * p.a.ld + 16 * at.g;
+    }
+    const char* const zeros = reinterpret_cast<const char*>(&tok_zeros);
+    // Instruction i of the two waves of a half brings rows 4 i ... 4 i + 3; row r's 16 bytes c lie at c ^ (r % 8).
+    constexpr int kLoads = 16 * NI / 8;
+    auto send = [&](int chunk) {
+        char* const to = tok_lds + ((chunk & 1) * 2 + half) * F::kPart;
+#pragma unroll
+        for (int q = 0; q < kLoads; ++q) {
+            const int i = mine + 2 * q, row = 4 * i + lane / 16, k = k0 + chunk * F::kChunk + 16 * ((lane % 16) ^ (row & 7));
+            const char* const from = p.b.p + (long long)min(row, at.live - 1) * p.b.ld + k;
+            tok_load_lds(k < bytes ? from : zeros, to + i * 1024);
+        }
+    };
+    tok_u4 even[F::kSteps][MT], odd[F::kSteps][MT];
+    auto load = [&](tok_u4 (&v)[F::kSteps][MT], int chunk) {  // (unconditional: what lies behind the end is read from elsewhere)
+#pragma unroll
+        for (int s = 0; s < F::kSteps; ++s) {
+            const int k = k0 + chunk * F::kChunk + 64 * s;
+            const bool is = chunk < per && k + 16 * at.g < bytes;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) v[s][i] = *reinterpret_cast<const tok_u4*>(is ? a[i] + k : zeros);
+        }
+    };
+    sel_f4 acc[MT][NI];
+#pragma unroll
+    for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) acc[i][j] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    // a chunk: the next one's rows are sent for and loaded first
+    auto go = [&](int chunk, const tok_u4 (&v)[F::kSteps][MT], tok_u4 (&next)[F::kSteps][MT]) {
+        tok_wait<F::kSteps * MT>();  // B's part has come, A's may still be under way; the part before it is read
+        send(chunk + 1);             // (behind the last one: zeros)
+        __builtin_amdgcn_sched_barrier(0);
+        load(next, chunk + 1);
+        __builtin_amdgcn_sched_barrier(0);
+        const char* const from = tok_lds + ((chunk & 1) * 2 + half) * F::kPart + at.l * F::kChunk;
+#pragma unroll
+        for (int s = 0; s < F::kSteps; ++s) {
+            tok_u4 b[NI];
+#pragma unroll
+            for (int j = 0; j < NI; ++j)
+                b[j] = *reinterpret_cast<const tok_u4*>(from + j * 16 * F::kChunk + (((4 * s + at.g) ^ (at.l & 7)) << 4));
+#pragma unroll
+            for (int e = 0; e < (sizeof(T) == 2 ? 1 : 4); ++e)
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j) tok_mma<T>(acc[i][j], v[s][i], b[j], e);
+        }
+    };
+    send(0);
+    __builtin_amdgcn_sched_barrier(0);
+    load(even, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    for (int chunk = 0; chunk < per; chunk += 2) {
+        go(chunk, even, odd);
+        if (chunk + 1 < per) go(chunk + 1, odd, even);
+    }
+    tok_settle<false>(acc);
+    tok_wait<0>();  // (all is read, and nothing comes any more)
+    sel_f4* const s_sum = reinterpret_cast<sel_f4*>(tok_lds) + (mine * MT * NI) * NHIP_WAVE + lane;
+    if (half) {
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int j = 0; j < NI; ++j) s_sum[(i * NI + j) * NHIP_WAVE] = acc[i][j];
+    }
+    __syncthreads();
+    if (half) return;
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+        if (16 * j >= at.live) continue;
+        sel_f4 sum[MT][1];
+#pragma unroll
+        for (int i = 0; i < MT; ++i) sum[i][0] = acc[i][j] + s_sum[(i * NI + j) * NHIP_WAVE];
+        at.n_tile = j;
+        epilogue.template run<T, typename F::Shape>(at, sum);
+    }
+}
+
+#define TOK_FEW 64  // rows of B that the kernels for few columns take
+// MT: tiles of 16 rows to a wave (of both matrices, where there are two)
 template <class T, int MT, int HALF, class E>
 static inline int tok_few(hipStream_t stream, TokProduct p, const E& epilogue) {
     const long long rows = HALF ? 8 * MT : 16 * MT, tiles = (p.a.rows + rows - 1) / rows;
     if (tiles == 0 || p.b.rows == 0) return 0;
-    if (p.b.rows > TOK_FEW || tiles > 0xffffff) return NHIP_E_BADARG;
-    auto go = [&](auto few) {
-        using F = decltype(few);
+    if (p.b.rows > TOK_FEW || tiles > 0xffffff || p.k_bytes > 0x3fffffff) return NHIP_E_BADARG;
+    if (p.b.rows <= 16) {
+        using F = TokFew<MT>;
         NHIP_LAUNCH((tok_few_kernel<T, F, HALF, E>), dim3((unsigned)tiles), dim3(F::kWaves * NHIP_WAVE), 0, stream, p, epilogue);
+        NHIP_LAUNCH_CHECK();
+        return 0;
+    }
+    auto go = [&](auto some) {
+        using F = decltype(some);
+        auto kernel = tok_some_kernel<T, F, HALF, E>;
+        if (int e = sel_allow_lds(stream, kernel, F::kLds)) return e;
+        NHIP_LAUNCH(kernel, dim3((unsigned)((tiles + 1) / 2)), dim3(F::kWaves * NHIP_WAVE), F::kLds, stream, p, epilogue);
         return (int)hipGetLastError();
     };
-    if (p.b.rows <= 16) return go(TokFew<MT, 1>());
-    if (p.b.rows <= 32) return go(TokFew<MT, 2>());
-    if (p.b.rows <= 48) return go(TokFew<MT, 3>());
-    return go(TokFew<MT, 4>());
+    if (p.b.rows <= 32) return go(TokSome<MT, 2>());
+    if (p.b.rows <= 48) return go(TokSome<MT, 3>());
+    return go(TokSome<MT, 4>());
 }
 
 // Four values of column n in rows m ... m + 3 (a lane's part of a tile), stored along m at g[n, m] and (unless it is NULL) along n
@@ -624,7 +743,7 @@ static inline int tok_product(hipStream_t stream, const TokProduct& p, const E& 
 }
 
 using TokLarge = TokShape<256, 256, 2, 4>;
-#define TOK_LEAST_BM 64  // of all shapes, and of the kernel for few columns
+#define TOK_LEAST_BM 32  // of all shapes, and of the kernels for few columns
 #define TOK_MOST_TILE 256
 
 // The shape of a product of m x n in elements of `size` bytes: tiles of 256 x 256 where they are enough to go round, of fewer

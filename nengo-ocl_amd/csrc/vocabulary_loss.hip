@@ -371,8 +371,7 @@ struct Finish {
 };
 
 __global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
-    __shared__ float2 s[kFinishLanes][16];
-    __shared__ float s_loss[kFinishLanes][16];
+    __shared__ float3 s[16][16];
     const int k = threadIdx.x % 16, q = threadIdx.x / 16, live = *a.count;
     if ((long long)blockIdx.x * 16 >= live) return;
     const int n = min((int)blockIdx.x * 16 + k, live - 1), row = a.targets.row[n];
@@ -385,7 +384,6 @@ __global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
         for (int o = 0; o < 4; ++o)
             if (t + o * kFinishLanes < a.tiles) v = Statistics<false>::joined(v, some[o]);
     }
-    s[q][k] = v;
     float loss = 0.0f;
     if (a.targets.top) {  // sum q (lse - z), whose sum of q times lse follows
         for (int e = q; e < a.targets.top; e += kFinishLanes) {
@@ -393,23 +391,30 @@ __global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
             const float share = a.targets.share[at];
             if (a.targets.word[at] != kNoWord && share != 0.0f) loss = fmaf(share, a.logits[(long long)n * a.targets.top + e], loss);
         }
-        s_loss[q][k] = loss;
     }
+    // four lanes of a wave have one token, then 16 waves; always in the same order
+    auto join = [&](int d) {
+        v = Statistics<false>::joined(v, float2{__shfl_xor(v.x, d), __shfl_xor(v.y, d)});
+        loss += __shfl_xor(loss, d);
+    };
+    join(16);
+    join(32);
+    if (q % 4 == 0) s[q / 4][k] = float3{v.x, v.y, loss};
     __syncthreads();
-    if (q) return;
-#pragma unroll 8
-    for (int o = 1; o < kFinishLanes; ++o) v = Statistics<false>::joined(v, s[o][k]);
+    if (threadIdx.x >= NHIP_WAVE) return;
+    v = float2{s[q][k].x, s[q][k].y};
+    loss = s[q][k].z;
+#pragma unroll
+    for (int o = 4; o < 16; o += 4) {
+        v = Statistics<false>::joined(v, float2{s[q + o][k].x, s[q + o][k].y});
+        loss += s[q + o][k].z;
+    }
+    join(16);
+    join(32);
+    if (q || (int)blockIdx.x * 16 + k >= live) return;
     const float lse = (v.x + __builtin_amdgcn_logf(v.y)) * kLn2;
-    if (a.targets.top) {
-        for (int o = 1; o < kFinishLanes; ++o) loss += s_loss[o][k];
-        loss = a.self[row] + (lse - loss);  // (the shares' sum is one)
-    } else {
-        loss = lse - a.logits[n];
-    }
-    if ((int)blockIdx.x * 16 + k < live) {
-        a.loss[row] = loss;
-        a.lse[row] = lse;
-    }
+    a.loss[row] = a.targets.top ? a.self[row] + (lse - loss) : lse - a.logits[n];  // (the shares' sum is one)
+    a.lse[row] = lse;
 }
 
 // Backward: G of the tile
