@@ -142,11 +142,37 @@ __global__ __launch_bounds__(NHIP_WG, 2) void layer_norm_grad_kernel(nhip_layer_
         }
     };
     const float per = 1.0f / (float)width;
-    // the sums of a row (the second ones share no words of `s` with the first, nor with each other)
+    // A row's sums, between waves through words of `s` that the sums before them do not use: one barrier each, since whoever
+    // writes there again has passed the other one in between.  (The norm of 8192 x 2048 in bfloat16 with four barriers to
+    // a sum, 46 us; with one to all three, 41.)
+    auto first_sum = [&](float v) {
+        v = sel_wave_sum(v);
+        if constexpr (L > NHIP_WAVE) {
+            if (lane % NHIP_WAVE == 0) s[threadIdx.x / NHIP_WAVE] = v;
+            __syncthreads();
+            v = (s[0] + s[1]) + (s[2] + s[3]);
+        }
+        return v;
+    };
     auto finish = [&](float& squares, float& e, float& eu) {
-        const float inv = 1.0f / sqrtf(norm_sum<L>(squares, s + 4) / (float)width + a.eps);
-        e = norm_sum<L>(e, s + 8) * per;
-        eu = norm_sum<L>(eu, s + 12) * inv * per;
+        squares = sel_wave_sum(squares);
+        e = sel_wave_sum(e);
+        eu = sel_wave_sum(eu);
+        if constexpr (L > NHIP_WAVE) {
+            const int w = threadIdx.x / NHIP_WAVE;
+            if (lane % NHIP_WAVE == 0) {
+                s[4 + w] = squares;
+                s[8 + w] = e;
+                s[12 + w] = eu;
+            }
+            __syncthreads();
+            squares = (s[4] + s[5]) + (s[6] + s[7]);
+            e = (s[8] + s[9]) + (s[10] + s[11]);
+            eu = (s[12] + s[13]) + (s[14] + s[15]);
+        }
+        const float inv = 1.0f / sqrtf(squares / (float)width + a.eps);
+        e *= per;
+        eu *= inv * per;
         return inv;
     };
 
@@ -175,7 +201,7 @@ __global__ __launch_bounds__(NHIP_WG, 2) void layer_norm_grad_kernel(nhip_layer_
                 if (kAhead) fetch(next[r], row + step, channel(r));
 #pragma unroll
             for (int r = 0; r < R; ++r) sum_v(channel(r), u[r], sum);
-            const float mean = norm_sum<L>(sum, s) / (float)width;
+            const float mean = first_sum(sum) / (float)width;
 #pragma unroll
             for (int r = 0; r < R; ++r) sum_rest(channel(r), u[r], w[r], mean, squares, e, eu);
             const float inv = finish(squares, e, eu);
@@ -219,7 +245,7 @@ __global__ __launch_bounds__(NHIP_WG, 2) void layer_norm_grad_kernel(nhip_layer_
                 open(raw, u);
                 sum_v(c, u, sum);
             }
-            const float mean = norm_sum<L>(sum, s) / (float)width;
+            const float mean = first_sum(sum) / (float)width;
             for (int c = lane * V; c < width; c += L * V) {
                 weights(c, w);
                 fetch(raw, row, c);
