@@ -34,21 +34,34 @@ struct Forward {
     template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
         constexpr int H = S::MI / 2;
         const bool wide = tok_fours(y, features, sizeof(T));
+        const bool lines = features % 8 == 0 && ((uintptr_t)y & 15) == 0;
+        static_assert(sizeof(T) == 4 || H % 4 || H == 4, "tok_put has four tiles");
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
             const long long n = (long long)at.n_tile * S::BN + at.wave_n * S::kWaveN + 16 * j + at.l;
-            if (n >= at.live) continue;
-            T* const to = static_cast<T*>(y) + n * features + f0;
-#pragma unroll
-            for (int i = 0; i < H; ++i) {
-                const long long f = ((long long)at.m_tile * S::BM + at.wave_m * S::kWaveM) / 2 + 16 * i + 4 * at.g;
-                float v[4];
+            auto value = [&](int i, float(&v)[4]) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float act, slope;
                     activate(activation, acc[i][j][r], act, slope);
                     v[r] = act * acc[i + H][j][r];
                 }
+            };
+            if constexpr (sizeof(T) == 2 && H % 4 == 0) {
+                if (lines) {
+                    const long long c = ((long long)at.m_tile * S::BM + at.wave_m * S::kWaveM) / 2;
+                    tok_put<T>(at, static_cast<T*>(y) + (n - at.l) * features + f0 + c, features,
+                               (int)max(0LL, min(16LL, at.live - (n - at.l))), (int)max(0LL, min(64LL, n_features - c)), value);
+                    continue;
+                }
+            }
+            if (n >= at.live) continue;
+            T* const to = static_cast<T*>(y) + n * features + f0;
+#pragma unroll
+            for (int i = 0; i < H; ++i) {
+                const long long f = ((long long)at.m_tile * S::BM + at.wave_m * S::kWaveM) / 2 + 16 * i + 4 * at.g;
+                float v[4];
+                value(i, v);
                 if (wide && f + 4 <= n_features) {
                     sel_store<T, 4>(to + f, v);
                 } else {
@@ -71,31 +84,50 @@ struct Backward {
     template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
         constexpr int H = S::MI / 2;
         const bool wide = tok_fours(dy, dy_ld, sizeof(T));
+        const long long c = ((long long)at.m_tile * S::BM + at.wave_m * S::kWaveM) / 2;  // of the piece's features
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
             const long long n = (long long)at.n_tile * S::BN + at.wave_n * S::kWaveN + 16 * j + at.l;
             const bool counts = n < at.live;
             const T* const from = static_cast<const T*>(dy) + (counts ? n : 0) * dy_ld + f0;
+            float d[H][4];
+            if (wide && c + 16 * H <= n_features) {
 #pragma unroll
-            for (int i = 0; i < H; ++i) {
-                const long long f = ((long long)at.m_tile * S::BM + at.wave_m * S::kWaveM) / 2 + 16 * i + 4 * at.g;
-                float d[4], dg[4], du[4];
-                if (wide && f + 4 <= n_features) {
-                    sel_load<T, 4>(from + f, d);
-                } else {
+                for (int i = 0; i < H; ++i) sel_load<T, 4>(from + c + 16 * i + 4 * at.g, d[i]);
+            } else {
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) d[r] = f + r < n_features ? (float)from[f + r] : 0.0f;
-                }
+                for (int i = 0; i < H; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) d[i][r] = (float)from[min(c + 16 * i + 4 * at.g + r, n_features - 1)];
+            }
+            // g and u become dg and du in their places
+#pragma unroll
+            for (int i = 0; i < H; ++i)
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     float act, slope;
                     activate(activation, acc[i][j][r], act, slope);
-                    const bool is = counts && f + r < n_features;
-                    dg[r] = is ? d[r] * acc[i + H][j][r] * slope : 0.0f;
-                    du[r] = is ? d[r] * act : 0.0f;
+                    const bool is = counts && c + 16 * i + 4 * at.g + r < n_features;
+                    acc[i][j][r] = is ? d[i][r] * acc[i + H][j][r] * slope : 0.0f;
+                    acc[i + H][j][r] = is ? d[i][r] * act : 0.0f;
                 }
-                tok_store_both<T>(static_cast<T*>(g), g_ld, static_cast<T*>(gt), gt_ld, n, f, dg);
-                tok_store_both<T>(static_cast<T*>(g), g_ld, static_cast<T*>(gt), gt_ld, n, second + f, du);
+            if constexpr (sizeof(T) == 2 && H % 4 == 0) {
+                if (!gt) {
+#pragma unroll
+                    for (int which = 0; which < 2; ++which)
+                        tok_put<T>(at, static_cast<T*>(g) + (n - at.l) * g_ld + which * second + c, g_ld, 16, 64,
+                                   [&](int i, float(&v)[4]) {
+#pragma unroll
+                                       for (int r = 0; r < 4; ++r) v[r] = acc[i + which * H][j][r];
+                                   });
+                    continue;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < S::MI; ++i) {
+                const float v[4] = {acc[i][j][0], acc[i][j][1], acc[i][j][2], acc[i][j][3]};
+                tok_store_both<T>(static_cast<T*>(g), g_ld, static_cast<T*>(gt), gt_ld, n,
+                                  (i < H ? 0 : second) + c + 16 * (i % H) + 4 * at.g, v);
             }
         }
     }

@@ -125,6 +125,7 @@ struct TokStoreRows {
     const float* scale;          // 1 / that of G, or NULL
     template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
         const float k = scale ? *scale : 1.0f;
+        const bool lines = ld % 8 == 0 && (((uintptr_t)out | (uintptr_t)out2) & 15) == 0;
         const bool wide = tok_fours(out, ld, sizeof(T)) && (!out2 || tok_fours(out2, ld, sizeof(T)));
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
@@ -133,6 +134,20 @@ struct TokStoreRows {
             if (second && w >= second) {
                 w -= second;
                 to = static_cast<T*>(out2);
+            }
+            if constexpr (sizeof(T) == 2 && S::MI % 4 == 0) {
+                if (lines) {  // (all lanes' columns are of the same matrix: `second` is a multiple of 16)
+                    const long long w0 = w - at.l, d0 = (long long)at.m_tile * S::BM + at.wave_m * S::kWaveM;
+                    const int some = (int)max(0LL, min(16LL, rows - w0));
+#pragma unroll
+                    for (int i = 0; i < S::MI; i += 4)
+                        tok_put<T>(at, to + w0 * ld + d0 + 16 * i, ld, some, (int)max(0LL, min(64LL, ld - d0 - 16 * i)),
+                                   [&](int e, float(&v)[4]) {
+#pragma unroll
+                                       for (int r = 0; r < 4; ++r) v[r] = acc[i + e][j][r] * k;
+                                   });
+                    continue;
+                }
             }
             if (w >= rows) continue;
             to += w * ld;

@@ -36,6 +36,8 @@ template <class T> __device__ __forceinline__ void tok_mma(sel_f4& acc, tok_u4 a
     }
 }
 
+#define TOK_PUT 2048  // bytes of the LDS that tok_put has to a wave
+
 // An operand: rows of `ld` bytes at p (multiples of 16 both; TOK_MOST_LD at most).  HALF != 0: two matrices side by side, the
 // second at p2; of every 2 HALF rows of a tile the first half are the first one's, so that a wave holds equal rows of both.
 struct TokRows {
@@ -61,7 +63,8 @@ template <int BM_, int BN_, int WM_, int WN_> struct TokShape {
     static constexpr int kWaves = WM * WN, kThreads = kWaves * NHIP_WAVE;
     static constexpr int kWaveM = BM / WM, kWaveN = BN / WN, MI = kWaveM / 16, NI = kWaveN / 16;
     static constexpr int kStage = (BM + BN) * TOK_KB;
-    static constexpr int kEpilogue = 8 * WM * BN, kLds = 2 * kStage + kEpilogue;  // an epilogue has 8 bytes per column and wave of m
+    // an epilogue has 8 bytes per column and wave of m, or TOK_PUT to a wave
+    static constexpr int kEpilogue = 8 * WM * BN > TOK_PUT * kWaves ? 8 * WM * BN : TOK_PUT * kWaves, kLds = 2 * kStage + kEpilogue;
     // work-groups to a compute unit, by the LDS and by the registers: a wave that holds more than 32 tiles has a SIMD for itself
     static constexpr int kByRegisters = MI * NI > 32 ? 1 : 8 / kWaves;
     static constexpr bool kPinned = MI * NI > 32, kPair = kWaves == 8;
@@ -75,6 +78,7 @@ struct TokPlace {
     int wave_m, wave_n, l, g;   // lane % 16, lane / 16
     int live;                   // rows of B that count
     char* lds;                  // S::kEpilogue bytes, the epilogue's own
+    int wave;
 };
 
 static __device__ const tok_u4 tok_zeros = {0, 0, 0, 0};  // what lies behind the end of a row
@@ -126,8 +130,9 @@ template <int ROWS, int WAVES, int HALF> struct TokLoader {
 
 // The same for an operand that lies across: a stage is 64 rows of 512 bytes, one to a k.  Instruction i of a wave brings rows 2 i
 // and 2 i + 1.  Reads of 4 k by 16 columns (ds_read_b64_tr_b16) take rows 8 g + 4 h + 0 ... 3 of all four lane groups g at
-// once: these lie next to each other in the LDS, 32 bytes between two instructions' rows, and meet no bank more often than
-// their 512 bytes have to.
+// once: these lie next to each other in the LDS, 32 bytes between two instructions' rows.  (Rows 2 i and 2 i + 1 meet in the same
+// banks.  With the odd rows' units exchanged they do not, and the gradient of 8192 x 65536 logits took 4110 us, not 4080: the
+// LDS is not what it waits for.)
 #define TOK_ACROSS 1056  // bytes of two rows in the LDS
 template <int WAVES> struct TokAcross {
     static constexpr int kMine = 32 / WAVES;
@@ -154,7 +159,7 @@ template <int WAVES> struct TokAcross {
     }
 };
 
-// 8 k (from half a stage, s) of column l of a unit of 16 columns: `from` is the lane's place in the unit
+// 8 k (from half a stage, s) of column l of a unit of 16 columns: `from` is the lane's place in unit 0
 static __device__ __forceinline__ tok_u4 tok_read_across(const char* from, int s, int unit) {
     typedef __attribute__((address_space(3))) sel_b4* lds;
     typedef unsigned pair __attribute__((ext_vector_type(2)));
@@ -244,6 +249,7 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
     constexpr int kBytesA = kAX ? 32 * TOK_ACROSS : S::BM * TOK_KB, kStage = kBytesA + (kBX ? 32 * TOK_ACROSS : S::BN * TOK_KB);
     TokPlace at;
     at.live = (int)(p.live ? min((long long)*p.live, p.b.rows) : p.b.rows);
+    at.wave = wave;
     at.wave_m = wave % S::WM;
     at.wave_n = wave / S::WM;
     at.l = lane % 16;
@@ -479,7 +485,7 @@ __global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_few_kernel(TokPr
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NHIP_WAVE), lane = threadIdx.x % NHIP_WAVE;
     TokPlace at;
     at.m_tile = nhip_xcd_remap(blockIdx.x, gridDim.x);
-    at.split = at.wave_m = at.wave_n = 0;
+    at.split = at.wave_m = at.wave_n = at.wave = 0;
     at.l = lane % 16;
     at.g = lane / 16;
     at.live = (int)(p.live ? min((long long)*p.live, p.b.rows) : p.b.rows);
@@ -573,7 +579,7 @@ __global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_some_kernel(TokP
     const int mine = wave % 2, half = wave / 2;
     TokPlace at;
     at.m_tile = 2 * nhip_xcd_remap(blockIdx.x, gridDim.x) + mine;
-    at.split = at.wave_m = at.wave_n = 0;
+    at.split = at.wave_m = at.wave_n = at.wave = 0;
     at.l = lane % 16;
     at.g = lane / 16;
     at.live = (int)(p.live ? min((long long)*p.live, p.b.rows) : p.b.rows);
@@ -690,6 +696,39 @@ static inline int tok_few(hipStream_t stream, TokProduct p, const E& epilogue) {
     if (p.b.rows <= 32) return go(TokSome<MT, 2>());
     if (p.b.rows <= 48) return go(TokSome<MT, 3>());
     return go(TokSome<MT, 4>());
+}
+
+// 64 values along m of 16 columns, value(i, v) being a lane's four of tile i of four, to rows of `ld` elements of 16 bits at `to`
+// (16-byte aligned): through the wave's part of the LDS, so that a lane stores 16 bytes and a row gets whole lines.
+// (Stored as they lie, 8 bytes to a lane in rows of 32: the gradient of 8192 x 65536 logits, 20 % masked, 718 us to a half, 680 so.)
+template <class T, class F>
+__device__ __forceinline__ void tok_put(const TokPlace& at, T* to, long long ld, int rows, int cols, F&& value) {
+    static_assert(sizeof(T) == 2, "");
+    char* const lds = at.lds + at.wave * TOK_PUT;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float v[4];
+        value(i, v);
+        sel_store<T, 4>(reinterpret_cast<T*>(lds + at.l * 128 + ((2 * i + at.g / 2) ^ (at.l & 7)) * 16 + at.g % 2 * 8), v);
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int lane = at.l + 16 * at.g, c = lane % 8;
+#pragma unroll
+    for (int q = 0; q < 2; ++q) {
+        const int row = 8 * q + lane / 8;
+        const tok_u4 v = *reinterpret_cast<const tok_u4*>(lds + row * 128 + ((c ^ (row & 7)) * 16));
+        if (row >= rows) continue;
+        T* const p = to + row * ld + 8 * c;
+        if (8 * c + 8 <= cols) {
+            *reinterpret_cast<tok_u4*>(p) = v;
+        } else {
+            const SelPack<T, 8> e = __builtin_bit_cast(SelPack<T, 8>, v);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                if (8 * c + k < cols) p[k] = e.v[k];
+        }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
 }
 
 // Four values of column n in rows m ... m + 3 (a lane's part of a tile), stored along m at g[n, m] and (unless it is NULL) along n

@@ -289,50 +289,68 @@ template <bool TOP> struct Statistics {
         const int w0 = word0 + at.m_tile * S::BM;
         if (S::WM > 1) __syncthreads();  // (the tile before is done with the LDS)
         const float c = kLog2e * per_temperature;
+        // what the tokens have, before it is needed: loads under a condition are waited for one by one
+        int lo[S::NI], hi[S::NI], row[S::NI];
+        auto token = [&](int j) { return n0 + at.wave_n * S::kWaveN + 16 * j + at.l; };
 #pragma unroll
-        for (int j = 0; j < S::NI; ++j) {
-            const int local = at.wave_n * S::kWaveN + 16 * j + at.l;
-            const long long n = n0 + local;
-            float most = -INFINITY;
+        for (int j = 0; j < S::NI; ++j) row[j] = (TOP ? targets.row : targets.label)[min(token(j), at.live - 1LL)];
+        if constexpr (TOP) {
 #pragma unroll
-            for (int i = 0; i < S::MI; ++i)
+            for (int j = 0; j < S::NI; ++j) targets.range(row[j], w0, w0 + S::BM, lo[j], hi[j]);
+        }
+        auto go = [&](auto whole) {
+            auto is = [&](int i, int r) { return decltype(whole)::value || m0 + 16 * i + r < words; };
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (m0 + 16 * i + r < words) most = fmaxf(most, acc[i][j][r]);
-            most = fmaxf(most, __shfl_xor(most, 16));
-            most = fmaxf(most, __shfl_xor(most, 32));
-            float top2 = most * c;
-            if (!(fabsf(top2) < INFINITY)) top2 = 0.0f;  // (infinities then reach the sum as they are)
-            float sum = 0.0f;
-#pragma unroll
-            for (int i = 0; i < S::MI; ++i)
-#pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    if (m0 + 16 * i + r < words) sum += __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -top2));
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if constexpr (S::WM > 1) {
-                if (at.g == 0) s_part[at.wave_m * S::BN + local] = float2{top2, sum};
-            } else {
-                if (at.g == 0 && n < at.live) part[(long long)(tile0 + at.m_tile) * ld + n] = float2{top2, sum};
-            }
-            auto pick = [&](int word, float* to) {
-                const int rel = word - word0 - m0;
-                if (rel < 0 || rel >= S::kWaveM || (rel & 15) >= 4) return;
+            for (int j = 0; j < S::NI; ++j) {
+                const int local = at.wave_n * S::kWaveN + 16 * j + at.l;
+                const long long n = n0 + local;
+                float most = -INFINITY;
 #pragma unroll
                 for (int i = 0; i < S::MI; ++i)
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
-                        if (rel == 16 * i + r) *to = acc[i][j][r] * per_temperature;
+                    for (int r = 0; r < 4; ++r) most = is(i, r) ? fmaxf(most, acc[i][j][r]) : most;
+                most = fmaxf(most, __shfl_xor(most, 16));
+                most = fmaxf(most, __shfl_xor(most, 32));
+                float top2 = most * c;
+                if (!(fabsf(top2) < INFINITY)) top2 = 0.0f;  // (infinities then reach the sum as they are)
+                float sum = 0.0f;
+#pragma unroll
+                for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float e = __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -top2));
+                        sum += is(i, r) ? e : 0.0f;
+                    }
+                sum += __shfl_xor(sum, 16);
+                sum += __shfl_xor(sum, 32);
+                if constexpr (S::WM > 1) {
+                    if (at.g == 0) s_part[at.wave_m * S::BN + local] = float2{top2, sum};
+                } else {
+                    if (at.g == 0 && n < at.live) part[(long long)(tile0 + at.m_tile) * ld + n] = float2{top2, sum};
+                }
+            }
+        };
+        if ((at.m_tile + 1) * S::BM <= words) go(std::true_type());
+        else go(std::false_type());
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+            const long long n = token(j);
+            auto pick = [&](int word, float* to) {
+                const int rel = word - word0 - m0;
+                if (rel < 0 || rel >= S::kWaveM || (rel & 15) >= 4) return;
+                float z = 0.0f;
+#pragma unroll
+                for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) z = rel == 16 * i + r ? acc[i][j][r] : z;
+                *to = z * per_temperature;
             };
             if (n < at.live) {
                 if constexpr (TOP) {
-                    const long long from = (long long)targets.row[n] * targets.top;
-                    int lo, hi;
-                    targets.range(targets.row[n], w0, w0 + S::BM, lo, hi);
-                    for (int k = lo; k < hi; ++k) pick(targets.word[from + k], logits + n * targets.top + k);
+                    const int* const word = targets.word + (long long)row[j] * targets.top;
+                    for (int k = lo[j]; k < hi[j]; ++k) pick(word[k], logits + n * targets.top + k);
                 } else {
-                    pick(targets.label[n], logits + n);
+                    pick(row[j], logits + n);
                 }
             }
         }
@@ -430,19 +448,50 @@ template <bool TOP> struct Gradient {
         const long long n0 = (long long)at.n_tile * S::BN;
         const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g, w0 = word0 + at.m_tile * S::BM;
         const float c = kLog2e * per_temperature, k = scale ? *scale * per_temperature : per_temperature;
+        // what the tokens have, before it is needed: loads under a condition are waited for one by one
+        int row[S::NI], label[S::NI], lo[S::NI], hi[S::NI];
+        float d[S::NI], lse2[S::NI];
+        auto token = [&](int j) { return n0 + at.wave_n * S::kWaveN + 16 * j + at.l; };
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
-            const long long n = n0 + at.wave_n * S::kWaveN + 16 * j + at.l;
+            row[j] = targets.row[min(token(j), at.live - 1LL)];
+            if constexpr (!TOP) label[j] = targets.label[min(token(j), at.live - 1LL)];
+        }
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+            d[j] = dloss[row[j]] * k;
+            lse2[j] = lse[row[j]] * kLog2e;
+            if constexpr (TOP) targets.range(row[j], w0, w0 + S::BM, lo[j], hi[j]);
+        }
+        const bool whole = (at.m_tile + 1) * S::BM <= words;
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j) {
+            const long long n = token(j);
             const bool counts = n < at.live;
-            const int row = counts ? targets.row[n] : 0;
-            const float d = counts ? dloss[row] * k : 0.0f, lse2 = counts ? lse[row] * kLog2e : 0.0f;
+            auto value = [&](int i, float(&v)[4]) {
 #pragma unroll
-            for (int i = 0; i < S::MI; ++i) {
-                float v[4];
+                for (int r = 0; r < 4; ++r) {
+                    const float p = d[j] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -lse2[j]));
+                    v[r] = counts && (whole || m0 + 16 * i + r < words) ? p : 0.0f;
+                }
+            };
+            bool stored = false;
+            if constexpr (sizeof(T) == 2 && S::MI % 4 == 0) {
+                if (!gt) {
+                    stored = true;
 #pragma unroll
-                for (int r = 0; r < 4; ++r)
-                    v[r] = counts && m0 + 16 * i + r < words ? d * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -lse2)) : 0.0f;
-                tok_store_both<T>(static_cast<T*>(g), g_ld, static_cast<T*>(gt), gt_ld, n, m0 + 16 * i, v);
+                    for (int i = 0; i < S::MI; i += 4)
+                        tok_put<T>(at, static_cast<T*>(g) + (n - at.l) * g_ld + m0 - 4 * at.g + 16 * i, g_ld, 16, 64,
+                                   [&](int e, float(&v)[4]) { value(i + e, v); });
+                }
+            }
+            if (!stored) {
+#pragma unroll
+                for (int i = 0; i < S::MI; ++i) {
+                    float v[4];
+                    value(i, v);
+                    tok_store_both<T>(static_cast<T*>(g), g_ld, static_cast<T*>(gt), gt_ld, n, m0 + 16 * i, v);
+                }
             }
             // the targets' elements once more, when what the wave has stored there has arrived
             auto take = [&](int word, float share) {
@@ -454,18 +503,16 @@ template <bool TOP> struct Gradient {
 #pragma unroll
                     for (int r = 0; r < 4; ++r) z = rel == 16 * i + r ? acc[i][j][r] : z;
                 asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-                const T v = (T)(d * (__builtin_amdgcn_exp2f(fmaf(z, c, -lse2)) - share));
+                const T v = (T)(d[j] * (__builtin_amdgcn_exp2f(fmaf(z, c, -lse2[j])) - share));
                 static_cast<T*>(g)[n * g_ld + m0 + rel] = v;
                 if (gt) static_cast<T*>(gt)[(m0 + rel) * gt_ld + n] = v;
             };
             if (counts) {
                 if constexpr (TOP) {
-                    const long long from = (long long)row * targets.top;
-                    int lo, hi;
-                    targets.range(row, w0, w0 + S::BM, lo, hi);
-                    for (int e = lo; e < hi; ++e) take(targets.word[from + e], targets.share[from + e]);
+                    const long long from = (long long)row[j] * targets.top;
+                    for (int e = lo[j]; e < hi[j]; ++e) take(targets.word[from + e], targets.share[from + e]);
                 } else {
-                    take(targets.label[n], 1.0f);
+                    take(label[j], 1.0f);
                 }
             }
         }
