@@ -240,7 +240,7 @@ template <class T> static inline int tok_join(hipStream_t stream, const TokJoin&
 struct TokGradient {
     long long rows, d, size;
     long long padded, piece, g_ld, gt_ld, dx_ld;
-    long long g = 0, gt = 0, xt = 0, wt = 0, dx = 0, dw = 0;  // in the workspace
+    long long g = 0, gt = 0, xt = 0, wt = 0, dx = 0, dw = 0, dw_parts;  // in the workspace
     int dx_splits, dw_splits;
     bool across;
 
@@ -268,7 +268,23 @@ struct TokGradient {
             wt = space.take(d * g_ld * size);
         }
         dx = space.take(dx_splits * dx_bytes);
-        if (dw_splits > 1) dw = space.take(dw_splits * dw_bytes);
+        dw_parts = dw_splits > 1 ? dw_splits * dw_bytes : 0;
+        long long n0;
+        if (const int s = tail(weights < piece ? tok_round(weights, 64) : piece, n0, room)) dw_parts = s * tok_round(piece - n0, 256) * dx_ld * 4;
+        if (dw_parts) dw = space.take(dw_parts);
+    }
+
+    // Tiles go round 256 compute units whole times and then some: the last columns of G, from n0 on, whose tiles are the rest of the
+    // last round, are cut along k into parts that fill it.  0 where that gives nothing: no whole round, or a rest that fills it, or
+    // too short a k for what the parts' sums take.  (8192 tokens, 2 x 5504 features, 2048 channels, 344 tiles: 405 us; 256, and 88 in
+    // two parts, 330.)
+    int tail(long long n, long long& n0, long long room) const {
+        if (!across || dw_splits > 1) return 0;
+        const long long m_tiles = (d + 255) / 256, n_tiles = (n + 255) / 256, whole = m_tiles * n_tiles / 256 * 256 / m_tiles;
+        const long long rest = m_tiles * (n_tiles - whole), parts = rest > 0 ? (256 / rest < 8 ? 256 / rest : 8) : 0;
+        n0 = whole * 256;
+        if (whole < 1 || parts < 2 || rows * size / TOK_KB < 48 || parts * tok_round(n - n0, 256) * dx_ld * 4 > room) return 0;
+        return (int)parts;
     }
     template <class T> T* gt_of(char* w) const { return across ? nullptr : reinterpret_cast<T*>(w + gt); }
 
@@ -281,30 +297,49 @@ struct TokGradient {
     template <class T>
     int weights(hipStream_t st, char* w, const TokRows& x, const int* live, long long n, long long first, long long second,
                 T* out, T* out2, const float* scale) const {
-        TokRows a{w + xt, nullptr, gt_ld * size, d}, b{w + gt, nullptr, gt_ld * size, n};
+        TokRows a{w + xt, nullptr, gt_ld * size, d};
         if (across) {
             a = x;
             a.across = tok_round(d * size, 16);
-            b = TokRows{w + g, nullptr, g_ld * size, n};
-            b.across = g_ld * size;
         }
-        auto go = [&](const auto& epilogue) {
+        // columns from ... to - 1 of G
+        auto go = [&](long long from, long long to, int splits, const auto& epilogue) {
+            TokRows b{w + gt + from * gt_ld * size, nullptr, gt_ld * size, to - from};
+            if (across) {
+                b = TokRows{w + g + from * size, nullptr, g_ld * size, to - from};
+                b.across = (g_ld - from) * size;
+            }
             // (large in every piece if in a whole one: G's layout goes by that)
             auto run = [&](auto shape) {
                 using S = decltype(shape);
                 constexpr int kAcross = std::is_same<S, TokLarge>::value && sizeof(T) == 2 ? 3 : 0;
-                TokProduct p{a, b, nullptr, live, rows * size, (int)((d + S::BM - 1) / S::BM), (int)((n + S::BN - 1) / S::BN), dw_splits};
+                TokProduct p{a, b, nullptr, live, rows * size, (int)((d + S::BM - 1) / S::BM),
+                             (int)((to - from + S::BN - 1) / S::BN), splits};
                 if (kAcross && !across) return tok_product<T, S, 0>(st, p, epilogue);
                 return tok_product<T, S, 0, kAcross>(st, p, epilogue);
             };
-            return across ? run(TokLarge()) : tok_with_shape(d, n, (int)size, dw_splits, run);
+            return across ? run(TokLarge()) : tok_with_shape(d, to - from, (int)size, splits, run);
         };
-        if (dw_splits == 1) return go(TokStoreRows{out, out2, d, first, out2 ? second : 0, scale});
+        const TokStoreRows store{out, out2, d, first, out2 ? second : 0, scale};
+        long long n0 = 0;
+        int splits = dw_splits;
+        if (splits == 1) {
+            splits = tail(n, n0, dw_parts);
+            if (!splits) return go(0, n, 1, store);
+            if (int e = go(0, n0, 1, store)) return e;
+        }
         float* const parts = reinterpret_cast<float*>(w + dw);
-        const long long part = piece * dx_ld;
-        if (int e = go(TokAddParts{parts, dx_ld, part, 0})) return e;
-        if (int e = tok_join<T>(st, TokJoin{parts, dx_ld, part, dw_splits, nullptr, scale, out, first, d})) return e;
-        return out2 ? tok_join<T>(st, TokJoin{parts + second * dx_ld, dx_ld, part, dw_splits, nullptr, scale, out2, first, d}) : 0;
+        const long long part = tok_round(n - n0, 256) * dx_ld;
+        if (int e = go(n0, n, splits, TokAddParts{parts, dx_ld, part, 0})) return e;
+        // the sums of columns from ... to - 1, which are rows of `to_rows` from its first on
+        auto join = [&](long long from, long long to, long long base, T* to_rows) {
+            from = from > n0 ? from : n0;
+            if (from >= to) return 0;
+            return tok_join<T>(st, TokJoin{parts + (from - n0) * dx_ld, dx_ld, part, splits, nullptr, scale,
+                                           to_rows + (from - base) * d, to - from, d});
+        };
+        if (int e = join(0, first, 0, out)) return e;
+        return out2 ? join(second, second + first, second, out2) : 0;
     }
 
     // dx += G W over `k` columns of G; W's rows (p2: from `second` on, `first` of each matrix) lie at the places that `rows_of` has
