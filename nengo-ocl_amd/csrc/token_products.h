@@ -802,6 +802,7 @@ template <class F> static inline int tok_with_shape(long long m, long long n, in
 // Into how many parts k (of k_bytes) is cut so that a product of m x n goes round 256 compute units, parts of eight stages at least.
 static inline int tok_splits(long long m, long long n, int size, long long k_bytes) {
     const long long stages = k_bytes / TOK_KB, most = stages / 8 < 64 ? stages / 8 : 64;
+    if (m < 1 || n < 1) return 1;
     long long s = 1;
     if (size == 2 && n > 128 && m > 128) s = 256 / (((m + 255) / 256) * ((n + 255) / 256));
     else s = 512 / (((m + 127) / 128) * ((n + 127) / 128));

@@ -33,14 +33,17 @@ def host(monkeypatch):
     return host_queue(monkeypatch)
 
 
+PLACE = "cpu"  # where the definitions are computed
+
+
 def wide(t):
-    return None if t is None else t.detach().cpu().double()
+    return None if t is None else t.detach().to(PLACE).double()
 
 
 def within(got, want, bound, name="", apart=0.0):
     """|got - want| <= bound + the rounding of the result, element by element; in 32 bits the norm, too: 128 u of the result's,
     and `apart` where the result is a difference of what is larger."""
-    got64, want = wide(got), want.detach().cpu().double()
+    got64, want = wide(got), wide(want)
     assert got64.shape == want.shape, (name, got64.shape, want.shape)
     if not want.numel():
         return
@@ -156,7 +159,8 @@ def test_layer_norm_of_a_mean_far_from_zero(queue, ops, dtype):
 
 # -------------------------------------------------------------------------- gated projection
 def act(name, g):
-    return g * torch.sigmoid(g) if name == "silu" else 0.5 * g * (1 + torch.erf(g / math.sqrt(2.0)))
+    # (erfc(-t) for 1 + erf(t), the same value: the sum loses its digits where g is far below zero, 2**-53 of 1e-12 at -7)
+    return g * torch.sigmoid(g) if name == "silu" else 0.5 * g * torch.special.erfc(g * -math.sqrt(0.5))
 
 
 GATED = [(1, 64, 64, "silu"), (3, 40, 33, "gelu"), (17, 130, 70, "silu"), (64, 256, 200, "gelu"), (65, 128, 300, "silu"),
@@ -239,20 +243,17 @@ def teacher_inputs(seed, dtype, n, d, v, masked, top):
 def shares(given, temperature):
     """[n, words] shares of the targets, sum q log q, which rows count."""
     n, v = given["x"].shape[0], given["weight"].shape[0]
-    q, self = torch.zeros(n, v, dtype=torch.float64), torch.zeros(n, dtype=torch.float64)
-    for r in range(n):
-        if "labels" in given:
-            w = int(given["labels"][r])
-            if 0 <= w < v:
-                q[r, w] = 1.0
-            continue
-        words, t = given["indices"][r].cpu().long(), wide(given["logits"][r]) / temperature
-        ok = (words >= 0) & (words < v) & (t > -math.inf)
-        if ok.any():
-            p = torch.softmax(t[ok], 0)
-            q[r].index_add_(0, words[ok], p)
-            self[r] = torch.special.xlogy(p, p).sum()
-    return q, self, q.sum(1) > 0
+    q = torch.zeros(n, v, dtype=torch.float64, device=PLACE)
+    if "labels" in given:
+        words, logits = given["labels"].to(PLACE).long()[:, None], torch.zeros(n, 1, dtype=torch.float64, device=PLACE)
+    else:
+        words, logits = given["indices"].to(PLACE).long(), wide(given["logits"]) / temperature
+    ok = (words >= 0) & (words < v) & (logits > -math.inf)
+    counts = ok.any(1)
+    p = torch.softmax(torch.where(ok, logits, -math.inf), 1)
+    p = torch.where(ok, p, 0.0)  # (of a row without any, too)
+    q.scatter_add_(1, words.clamp(0, v - 1), p)
+    return q, torch.special.xlogy(p, p).sum(1), counts
 
 
 def loss_definition(given, temperature):
@@ -294,8 +295,9 @@ def check_loss_gradients(got, given, temperature, dloss, lse):
     size = G.abs() + off
     n, v = G.shape
     # p and q are each off by some roundings of themselves, 8 E, also where their difference is smaller (a vocabulary of one
-    # word: p = q = 1, G = 0 and off by 8 E scale); the products carry that on
-    both = 8 * E * scale.abs() * (p + q)
+    # word: p = q = 1, G = 0 and off by 8 E scale); and exp(z - lse) by those of z and lse, numbers of 32 bits whose
+    # own steps are E of them (2000: 1e-4, and p as much of itself).  The products carry that on.
+    both = 8 * E * scale.abs() * (p * (1 + z.abs() + lse64.abs()[:, None]) + q)
     within(got.x, G @ w, off @ w.abs() + (v + 8) * E * (size @ w.abs()), "x", (both @ w.abs()).norm())
     within(got.weight, G.t() @ x, off.t() @ x.abs() + (n + 8) * E * (size.t() @ x.abs()), "weight", (both.t() @ x.abs()).norm())
     return G
