@@ -246,7 +246,7 @@ template <class T> int backward(hipStream_t st, const nhip_gated_args& a, const 
                               static_cast<T*>(a.dup) + f0 * d, nullptr));
         if (a.rows) TOK_TRY(gr.inputs<T>(st, w, rows, nullptr, both, n, second, f0 > 0));
     }
-    return gr.finish<T>(st, w, nullptr, nullptr, a.dx);
+    return gr.finish<T>(st, w, nullptr, nullptr, nullptr, a.dx);
 }
 
 int run(void* stream, const nhip_gated_args* args, bool grad) {

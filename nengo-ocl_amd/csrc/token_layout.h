@@ -199,10 +199,13 @@ struct TokJoin {
     const float* scale;
     void* out;
     long long rows, cols;
+    const int* live = nullptr;  // not NULL: as many parts as the product had by its tiles of live rows (tok_parts), n_parts at most
+    int slots = 0, m_tiles = 0, bn = 1;
 };
 
 template <class T, int V> __global__ __launch_bounds__(NHIP_WG) void tok_join_kernel(TokJoin a) {
     const float k = a.scale ? *a.scale : 1.0f;
+    const int n_parts = a.live ? tok_parts(a.slots, a.m_tiles * ((*a.live + a.bn - 1) / a.bn), a.n_parts) : a.n_parts;
     const long long packs = (a.cols + V - 1) / V, all = a.rows * packs;
     for (long long q = (long long)blockIdx.x * NHIP_WG + threadIdx.x; q < all; q += (long long)gridDim.x * NHIP_WG) {
         const long long r = q / packs, c = q % packs * V, from = a.where ? a.where[r] : r;
@@ -211,7 +214,7 @@ template <class T, int V> __global__ __launch_bounds__(NHIP_WG) void tok_join_ke
         for (int e = 0; e < V; ++e) sum[e] = 0.0f;
         if (from >= 0) {
             const float* p = a.parts + from * a.ld + c;
-            for (int s = 0; s < a.n_parts; ++s) {
+            for (int s = 0; s < n_parts; ++s) {
                 sel_load<float, V>(p + s * a.part, v);
 #pragma unroll
                 for (int e = 0; e < V; ++e) sum[e] += v[e];
@@ -241,7 +244,7 @@ struct TokGradient {
     long long rows, d, size;
     long long padded, piece, g_ld, gt_ld, dx_ld;
     long long g = 0, gt = 0, xt = 0, wt = 0, dx = 0, dw = 0, dw_parts;  // in the workspace
-    int dx_splits, dw_splits;
+    int dx_splits, dx_most, dw_splits;
     bool across;
 
     // `weights`: rows of W (of both, whole tiles of each); they are gone through in equal pieces whose G takes 512 MB at most
@@ -256,9 +259,12 @@ struct TokGradient {
         gt_ld = tok_ld(padded);
         dx_ld = tok_round(d, TOK_MOST_TILE);
         const long long dw_bytes = piece * dx_ld * 4, dx_bytes = padded * dx_ld * 4, room = 256LL << 20;
+        // (rows that do not count leave work-groups to the others' parts: room for more parts than all rows need)
         dx_splits = tok_splits(d, rows, (int)size, piece * size);
+        dx_most = (int)tok_most_splits(piece * size);
         dw_splits = tok_splits(d, piece, (int)size, rows * size);
-        if (dx_splits > 1 && dx_splits * dx_bytes > room) dx_splits = room / dx_bytes > 1 ? (int)(room / dx_bytes) : 1;
+        if (dx_most > 1 && dx_most * dx_bytes > room) dx_most = room / dx_bytes > 1 ? (int)(room / dx_bytes) : 1;
+        if (dx_splits > dx_most) dx_splits = dx_most;
         if (dw_splits > 1 && dw_splits * dw_bytes > room) dw_splits = room / dw_bytes > 1 ? (int)(room / dw_bytes) : 1;
         across = size == 2 && tok_is_large(d, rows, 2, dx_splits) && tok_is_large(d, piece, 2, dw_splits);
         g = space.take(padded * g_ld * size);
@@ -267,7 +273,7 @@ struct TokGradient {
             xt = space.take(d * gt_ld * size);
             wt = space.take(d * g_ld * size);
         }
-        dx = space.take(dx_splits * dx_bytes);
+        dx = space.take(dx_most * dx_bytes);
         dw_parts = dw_splits > 1 ? dw_splits * dw_bytes : 0;
         long long n0;
         if (const int s = tail(weights < piece ? tok_round(weights, 64) : piece, n0, room)) dw_parts = s * tok_round(piece - n0, 256) * dx_ld * 4;
@@ -364,14 +370,25 @@ struct TokGradient {
         auto run = [&](auto shape) {
             using S = decltype(shape);
             constexpr int kAcross = std::is_same<S, TokLarge>::value && sizeof(T) == 2 ? 1 : 0;
-            TokProduct p{a, b, live, nullptr, k * size, (int)((d + S::BM - 1) / S::BM), (int)((rows + S::BN - 1) / S::BN), dx_splits};
+            TokProduct p{a, b, live, nullptr, k * size, (int)((d + S::BM - 1) / S::BM), (int)((rows + S::BN - 1) / S::BN),
+                         live ? dx_most : dx_splits, live ? 256 * S::kAtOnce : 0};
             if (kAcross && !across) return tok_product<T, S, 0>(st, p, epilogue);
             return tok_product<T, S, 0, kAcross>(st, p, epilogue);
         };
         return across ? run(TokLarge()) : tok_with_shape(d, rows, (int)size, dx_splits, run);
     }
 
-    template <class T> int finish(hipStream_t st, char* w, const int* where, const float* scale, void* out) const {
-        return tok_join<T>(st, TokJoin{reinterpret_cast<float*>(w + dx), dx_ld, padded * dx_ld, dx_splits, where, scale, out, rows, d});
+    template <class T> int finish(hipStream_t st, char* w, const int* where, const int* live, const float* scale, void* out) const {
+        TokJoin join{reinterpret_cast<float*>(w + dx), dx_ld, padded * dx_ld, live ? dx_most : dx_splits, where, scale, out, rows, d};
+        auto shape_of = [&](auto shape) {
+            using S = decltype(shape);
+            join.live = live;
+            join.slots = 256 * S::kAtOnce;
+            join.m_tiles = (int)((d + S::BM - 1) / S::BM);
+            join.bn = S::BN;
+            return 0;
+        };
+        if (live) across ? shape_of(TokLarge()) : tok_with_shape(d, rows, (int)size, dx_splits, shape_of);
+        return tok_join<T>(st, join);
     }
 };

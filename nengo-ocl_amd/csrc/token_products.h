@@ -55,8 +55,15 @@ struct TokProduct {
     const int* k_live; // how many elements of k count (device), or NULL
     long long k_bytes; // of a row
     int m_tiles, n_tiles;
-    int splits;        // parts that k is cut into
+    int splits;        // parts that k is cut into: so many, or
+    int slots = 0;     // (not zero) as many as let the tiles of rows that count take so many work-groups, up to `splits`
 };
+
+// How many parts k has: where rows do not count, whose number the host does not know, tiles are fewer and parts more
+static __host__ __device__ __forceinline__ int tok_parts(int slots, int tiles, int most) {
+    const int n = slots / (tiles > 0 ? tiles : 1);
+    return n < 1 ? 1 : n < most ? n : most;
+}
 
 template <int BM_, int BN_, int WM_, int WN_> struct TokShape {
     static constexpr int BM = BM_, BN = BN_, WM = WM_, WN = WN_;     // tile, waves along m and n
@@ -255,9 +262,10 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
     at.l = lane % 16;
     at.g = lane / 16;
     at.lds = tok_lds + 2 * kStage;
-    const int n_tiles = (at.live + S::BN - 1) / S::BN, tiles = p.m_tiles * n_tiles, total = tiles * p.splits;
+    const int n_tiles = (at.live + S::BN - 1) / S::BN, tiles = p.m_tiles * n_tiles;
+    const int splits = p.slots ? tok_parts(p.slots, tiles, p.splits) : p.splits, total = tiles * splits;
     const long long bytes = p.k_live ? (long long)*p.k_live * (int)sizeof(T) : p.k_bytes;
-    const int all = (int)((bytes + TOK_KB - 1) / TOK_KB), per = (all + p.splits - 1) / p.splits;
+    const int all = (int)((bytes + TOK_KB - 1) / TOK_KB), per = (all + splits - 1) / splits;
     const int dies = min(NHIP_NXCD, (int)gridDim.x), die = blockIdx.x % dies, step = ((int)gridDim.x - die + dies - 1) / dies;
     const int end = (int)((long long)total * (die + 1) / dies);
     int id = (int)((long long)total * die / dies) + blockIdx.x / dies;
@@ -799,13 +807,17 @@ template <class F> static inline int tok_with_shape(long long m, long long n, in
     return f(TokShape<128, 16, 4, 1>());
 }
 
-// Into how many parts k (of k_bytes) is cut so that a product of m x n goes round 256 compute units, parts of eight stages at least.
+// Into how many parts k (of k_bytes) is cut so that a product of m x n goes round 256 compute units, parts of eight stages at
+// least; and the most parts that there may be.
+static inline long long tok_most_splits(long long k_bytes) {
+    const long long n = k_bytes / TOK_KB / 8;
+    return n < 1 ? 1 : n < 64 ? n : 64;
+}
 static inline int tok_splits(long long m, long long n, int size, long long k_bytes) {
-    const long long stages = k_bytes / TOK_KB, most = stages / 8 < 64 ? stages / 8 : 64;
     if (m < 1 || n < 1) return 1;
+    const long long most = tok_most_splits(k_bytes);
     long long s = 1;
     if (size == 2 && n > 128 && m > 128) s = 256 / (((m + 255) / 256) * ((n + 255) / 256));
     else s = 512 / (((m + 127) / 128) * ((n + 127) / 128));
-    s = s < most ? s : most;
-    return (int)(s < 1 ? 1 : s);
+    return (int)(s < 1 ? 1 : s < most ? s : most);
 }

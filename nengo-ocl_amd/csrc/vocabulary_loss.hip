@@ -232,27 +232,36 @@ template <class T> __global__ __launch_bounds__(NHIP_WG) void gather_kernel(Gath
     }
 }
 
-// What G is scaled by in float16, whose range does not hold the gradient of a mean over many tokens: a power of two that
-// brings its largest magnitude to 2^13 ... 2^14; and the reverse.
-__global__ __launch_bounds__(1024) void scale_kernel(const float* dloss, const int* row, const int* count, float per_temperature,
-                                                     float* scale) {
+// What G is scaled by in 16 bits, and the reverse: `most` over the largest magnitude of the tokens' dloss.  Where all tokens have
+// the same one (a mean), the targets' elements, p - 1 times one, lose next to nothing when they are rounded; and
+// in float16 (2^14) the gradient of a mean over many tokens stays in the type's range.
+__global__ __launch_bounds__(1024) void scale_kernel(const float* dloss, const int* where, long long rows, float per_temperature,
+                                                     float most, float* scale) {
     __shared__ float s[16];
-    float most = 0.0f;
-    for (int n = threadIdx.x; n < *count; n += 1024) {
-        const float v = fabsf(dloss[row[n]] * per_temperature);
-        if (v < INFINITY) most = fmaxf(most, v);
+    float top = 0.0f;
+    for (long long r = threadIdx.x; r < rows; r += 4 * 1024) {
+        float v[4];
+        int at[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            v[e] = dloss[min(r + e * 1024, rows - 1)];
+            at[e] = where[min(r + e * 1024, rows - 1)];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float m = fabsf(v[e] * per_temperature);
+            if (at[e] >= 0 && m < INFINITY) top = fmaxf(top, m);
+        }
     }
 #pragma unroll
-    for (int d = 1; d < NHIP_WAVE; d *= 2) most = fmaxf(most, __shfl_xor(most, d));
-    if (threadIdx.x % NHIP_WAVE == 0) s[threadIdx.x / NHIP_WAVE] = most;
+    for (int d = 1; d < NHIP_WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    if (threadIdx.x % NHIP_WAVE == 0) s[threadIdx.x / NHIP_WAVE] = top;
     __syncthreads();
     if (threadIdx.x == 0) {
-        for (int w = 1; w < 16; ++w) most = fmaxf(most, s[w]);
-        int e = 14;
-        if (most > 0.0f) frexpf(most, &e);
-        e = e < -100 ? -100 : e > 100 ? 100 : e;
-        scale[0] = ldexpf(1.0f, 14 - e);
-        scale[1] = ldexpf(1.0f, e - 14);
+        for (int w = 1; w < 16; ++w) top = fmaxf(top, s[w]);
+        top = top > 0.0f ? fminf(fmaxf(top, 0x1p-100f), 0x1p100f) : most;
+        scale[0] = most / top;
+        scale[1] = top / most;
     }
 }
 
@@ -658,9 +667,10 @@ template <class T> int backward(hipStream_t st, const nhip_loss_args& a, const S
     const TokGradient& gr = *s.gradient;
     TOK_TRY(gr.lay_out_x<T>(st, w, w + s.x, s.x_ld, count));
     float* scale = nullptr;
-    if constexpr (std::is_same<T, _Float16>::value) {
+    if (sizeof(T) == 2 && a.rows) {
         scale = reinterpret_cast<float*>(w + s.count) + 16;
-        NHIP_LAUNCH(scale_kernel, dim3(1), dim3(1024), 0, st, a.dloss, t.row, count, 1.0f / a.temperature, scale);
+        NHIP_LAUNCH(scale_kernel, dim3(1), dim3(1024), 0, st, a.dloss, reinterpret_cast<int*>(w + s.where), a.rows,
+                    1.0f / a.temperature, std::is_same<T, _Float16>::value ? 0x1p14f : 1.0f, scale);
         NHIP_LAUNCH_CHECK();
     }
     const long long d = a.channels;
@@ -684,7 +694,7 @@ template <class T> int backward(hipStream_t st, const nhip_loss_args& a, const S
                               scale ? scale + 1 : nullptr));
         TOK_TRY(gr.inputs<T>(st, w, rows, count, words, words, 0, v0 > 0));
     }
-    return gr.finish<T>(st, w, reinterpret_cast<int*>(w + s.where), scale ? scale + 1 : nullptr, a.dx);
+    return gr.finish<T>(st, w, reinterpret_cast<int*>(w + s.where), count, scale ? scale + 1 : nullptr, a.dx);
 }
 
 int run(void* stream, const nhip_loss_args* args, bool grad) {
