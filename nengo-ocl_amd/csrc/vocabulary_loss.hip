@@ -16,7 +16,7 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 constexpr int kNoWord = 0x7fffffff;
-constexpr int kMostTop = 256, kBlock = TOK_LEAST_BM;
+constexpr int kMostTop = 256;
 constexpr long long kMostRows = 1 << 20, kMostChannels = 1 << 20;
 
 __device__ __forceinline__ long long word_at(const void* p, int wide, long long i) {
@@ -35,8 +35,8 @@ struct Shares {
     float* share;
     float* self;    // sum q log q
     int* flag;      // 0: the row counts, -1: it has no entries
-    unsigned short* first;  // [rows, blocks]: entries below the first word of each block of kBlock words
-    int blocks;
+    unsigned short* first;  // [rows, blocks]: entries below the first word of each block of `block` words
+    int blocks, block;
 };
 
 template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares a) {
@@ -134,10 +134,10 @@ template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares
     }
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     for (int b = lane; b < a.blocks; b += NHIP_WAVE) {
-        int lo = 0, hi = before;  // (b kBlock stays below 2^31: so do the words)
+        int lo = 0, hi = before;  // (b times block stays below 2^31: so do the words)
         while (lo < hi) {
             const int mid = (lo + hi) / 2;
-            if (s_merged[wave][mid] < b * kBlock) lo = mid + 1;
+            if (s_merged[wave][mid] < b * a.block) lo = mid + 1;
             else hi = mid;
         }
         a.first[row * a.blocks + b] = (unsigned short)lo;
@@ -272,12 +272,12 @@ struct Targets {
     const float* share;
     const int* row;     // of a live token
     const unsigned short* first;
-    int top, blocks;
-    // where the entries of words w0 ... w1 - 1 (multiples of kBlock) begin and end among a row's
+    int top, blocks, block;
+    // where the entries of words w0 ... w1 - 1 (multiples of `block`) begin and end among a row's
     __device__ __forceinline__ void range(long long r, int w0, int w1, int& lo, int& hi) const {
         const unsigned short* const of = first + r * blocks;
-        lo = of[min(w0 / kBlock, blocks - 1)];
-        hi = of[min(w1 / kBlock, blocks - 1)];
+        lo = of[min(w0 / block, blocks - 1)];
+        hi = of[min(w1 / block, blocks - 1)];
     }
 };
 
@@ -545,7 +545,7 @@ bool wide_weight(const nhip_loss_args& a) {
 
 struct Space : TokSpace {
     long long padded, x_ld, piece;
-    long long row, where, label, count, flag, word, share, self, first, blocks, x, weight, part, logits;
+    long long row, where, label, count, flag, word, share, self, first, blocks, block, x, weight, part, logits;
     std::optional<TokGradient> gradient;
     Space(const nhip_loss_args& a, bool grad) {
         const long long size = sel_size(a.type), rows = a.rows > 0 ? a.rows : 1, top = a.top;
@@ -555,13 +555,15 @@ struct Space : TokSpace {
         where = take(rows * 4);
         label = take(padded * 4);
         count = take(256);
-        flag = word = share = self = first = blocks = 0;
+        flag = word = share = self = first = blocks = block = 0;
         if (top) {
             flag = take(rows * 4);
             word = take(rows * top * 4);
             share = take(rows * top * 4);
             self = take(rows * 4);
-            blocks = (a.words + kBlock - 1) / kBlock + 1;  // (the last one: all entries)
+            // as fine as the tiles: those of the kernels for few columns, or of the others
+            block = !grad && a.rows <= TOK_FEW ? TOK_LEAST_BM : 128;
+            blocks = (a.words + block - 1) / block + 1;  // (the last one: all entries)
             first = take(rows * blocks * 2);
         }
         x = take(padded * x_ld * size);
@@ -585,7 +587,7 @@ struct Space : TokSpace {
 // The rows that count, and the targets of all rows
 template <class T> int prepare(hipStream_t st, const nhip_loss_args& a, const Space& s, char* w, bool grad, Targets& t) {
     t = Targets{reinterpret_cast<int*>(w + s.label), reinterpret_cast<int*>(w + s.word), reinterpret_cast<float*>(w + s.share),
-                reinterpret_cast<int*>(w + s.row), reinterpret_cast<unsigned short*>(w + s.first), a.top, (int)s.blocks};
+                reinterpret_cast<int*>(w + s.row), reinterpret_cast<unsigned short*>(w + s.first), a.top, (int)s.blocks, (int)s.block};
     Gather gather{a.x, a.targets, a.wide_targets, a.words, a.type, 0, a.x_stride, a.rows, a.channels, (int)s.x_ld, w + s.x,
                   reinterpret_cast<int*>(w + s.row), reinterpret_cast<int*>(w + s.where), reinterpret_cast<int*>(w + s.label),
                   reinterpret_cast<int*>(w + s.count), grad ? nullptr : a.loss, grad ? nullptr : a.lse, gather_rows(a.rows)};
@@ -593,7 +595,7 @@ template <class T> int prepare(hipStream_t st, const nhip_loss_args& a, const Sp
     if (a.top && a.rows) {
         Shares sh{a.targets, a.target_logits, a.wide_targets, a.logits_type, a.top, a.words, a.rows, 1.0f / a.temperature,
                   reinterpret_cast<int*>(w + s.word), reinterpret_cast<float*>(w + s.share), reinterpret_cast<float*>(w + s.self),
-                  reinterpret_cast<int*>(w + s.flag), reinterpret_cast<unsigned short*>(w + s.first), (int)s.blocks};
+                  reinterpret_cast<int*>(w + s.flag), reinterpret_cast<unsigned short*>(w + s.first), (int)s.blocks, (int)s.block};
         const dim3 grid((unsigned)((a.rows + 3) / 4));
         if (a.top <= 64) NHIP_LAUNCH((shares_kernel<1>), grid, dim3(NHIP_WG), 0, st, sh);
         else if (a.top <= 128) NHIP_LAUNCH((shares_kernel<2>), grid, dim3(NHIP_WG), 0, st, sh);
