@@ -267,12 +267,18 @@ __global__ __launch_bounds__(1024) void scale_kernel(const float* dloss, const i
 
 // ----------------------------------------------------------------------------------- tiles of z
 struct Targets {
-    const int* label;   // [live], or
+    const void* label;  // [live], or
     const int* word;    // [rows, top], sorted, with
     const float* share;
-    const int* row;     // of a live token
+    const int* row;     // of a live token; NULL: tokens are rows, of which not all count
     const unsigned short* first;
-    int top, blocks, block;
+    int top, blocks, block, wide_label, n_words;
+    const int* flag;    // [rows] with `row` NULL and a teacher: below zero where a row does not count
+    __device__ __forceinline__ int row_of(long long n) const { return row ? row[n] : (int)n; }
+    __device__ __forceinline__ int label_of(long long n) const {  // -1: the token does not count
+        const long long w = word_at(label, wide_label, n);
+        return w >= 0 && w < n_words ? (int)w : -1;
+    }
     // where the entries of words w0 ... w1 - 1 (multiples of `block`) begin and end among a row's
     __device__ __forceinline__ void range(long long r, int w0, int w1, int& lo, int& hi) const {
         const unsigned short* const of = first + r * blocks;
@@ -302,7 +308,10 @@ template <bool TOP> struct Statistics {
         int lo[S::NI], hi[S::NI], row[S::NI];
         auto token = [&](int j) { return n0 + at.wave_n * S::kWaveN + 16 * j + at.l; };
 #pragma unroll
-        for (int j = 0; j < S::NI; ++j) row[j] = (TOP ? targets.row : targets.label)[min(token(j), at.live - 1LL)];
+        for (int j = 0; j < S::NI; ++j) {
+            const long long n = min(token(j), at.live - 1LL);
+            row[j] = TOP ? targets.row_of(n) : targets.label_of(n);
+        }
         if constexpr (TOP) {
 #pragma unroll
             for (int j = 0; j < S::NI; ++j) targets.range(row[j], w0, w0 + S::BM, lo[j], hi[j]);
@@ -391,24 +400,25 @@ struct Finish {
     const float* logits;
     Targets targets;
     const float* self;
-    const int* count;
+    const int* count;  // NULL: `rows`
     long long ld;
-    int tiles;
+    int tiles, rows;
     float *loss, *lse;
 };
 
 __global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
     __shared__ float3 s[16][16];
-    const int k = threadIdx.x % 16, q = threadIdx.x / 16, live = *a.count;
+    const int k = threadIdx.x % 16, q = threadIdx.x / 16, live = a.count ? *a.count : a.rows;
     if ((long long)blockIdx.x * 16 >= live) return;
-    const int n = min((int)blockIdx.x * 16 + k, live - 1), row = a.targets.row[n];
+    const int n = min((int)blockIdx.x * 16 + k, live - 1), row = a.targets.row_of(n);
+    const bool is = a.targets.row || (a.targets.top ? a.targets.flag[n] : a.targets.label_of(n)) >= 0;
     float2 v = {0.0f, 0.0f};
-    for (int t = q; t < a.tiles; t += 4 * kFinishLanes) {
-        float2 some[4];
+    for (int t = q; t < a.tiles; t += 8 * kFinishLanes) {
+        float2 some[8];
 #pragma unroll
-        for (int o = 0; o < 4; ++o) some[o] = a.part[(long long)min(t + o * kFinishLanes, a.tiles - 1) * a.ld + n];
+        for (int o = 0; o < 8; ++o) some[o] = a.part[(long long)min(t + o * kFinishLanes, a.tiles - 1) * a.ld + n];
 #pragma unroll
-        for (int o = 0; o < 4; ++o)
+        for (int o = 0; o < 8; ++o)
             if (t + o * kFinishLanes < a.tiles) v = Statistics<false>::joined(v, some[o]);
     }
     float loss = 0.0f;
@@ -440,8 +450,8 @@ __global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
     join(32);
     if (q || (int)blockIdx.x * 16 + k >= live) return;
     const float lse = (v.x + __builtin_amdgcn_logf(v.y)) * kLn2;
-    a.loss[row] = a.targets.top ? a.self[row] + (lse - loss) : lse - a.logits[n];  // (the shares' sum is one)
-    a.lse[row] = lse;
+    a.loss[row] = !is ? 0.0f : a.targets.top ? a.self[row] + (lse - loss) : lse - a.logits[n];  // (the shares' sum is one)
+    a.lse[row] = is ? lse : 0.0f;
 }
 
 // Backward: G of the tile
@@ -463,8 +473,8 @@ template <bool TOP> struct Gradient {
         auto token = [&](int j) { return n0 + at.wave_n * S::kWaveN + 16 * j + at.l; };
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
-            row[j] = targets.row[min(token(j), at.live - 1LL)];
-            if constexpr (!TOP) label[j] = targets.label[min(token(j), at.live - 1LL)];
+            row[j] = targets.row_of(min(token(j), at.live - 1LL));
+            if constexpr (!TOP) label[j] = targets.label_of(min(token(j), at.live - 1LL));
         }
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
@@ -584,10 +594,12 @@ struct Space : TokSpace {
 
 #define TOK_TRY(call) do { if (int e_ = (call)) return e_; } while (0)
 
-// The rows that count, and the targets of all rows
-template <class T> int prepare(hipStream_t st, const nhip_loss_args& a, const Space& s, char* w, bool grad, Targets& t) {
-    t = Targets{reinterpret_cast<int*>(w + s.label), reinterpret_cast<int*>(w + s.word), reinterpret_cast<float*>(w + s.share),
-                reinterpret_cast<int*>(w + s.row), reinterpret_cast<unsigned short*>(w + s.first), a.top, (int)s.blocks, (int)s.block};
+// The rows that count (or all, as they are), and the targets of all rows
+template <class T>
+int prepare(hipStream_t st, const nhip_loss_args& a, const Space& s, char* w, bool grad, bool as_they_are, Targets& t) {
+    t = Targets{w + s.label, reinterpret_cast<int*>(w + s.word), reinterpret_cast<float*>(w + s.share),
+                reinterpret_cast<int*>(w + s.row), reinterpret_cast<unsigned short*>(w + s.first), a.top, (int)s.blocks, (int)s.block,
+                0, a.words, reinterpret_cast<int*>(w + s.flag)};
     Gather gather{a.x, a.targets, a.wide_targets, a.words, a.type, 0, a.x_stride, a.rows, a.channels, (int)s.x_ld, w + s.x,
                   reinterpret_cast<int*>(w + s.row), reinterpret_cast<int*>(w + s.where), reinterpret_cast<int*>(w + s.label),
                   reinterpret_cast<int*>(w + s.count), grad ? nullptr : a.loss, grad ? nullptr : a.lse, gather_rows(a.rows)};
@@ -603,6 +615,12 @@ template <class T> int prepare(hipStream_t st, const nhip_loss_args& a, const Sp
         NHIP_LAUNCH_CHECK();
         gather.labels = w + s.flag;  // 0 or -1
         gather.wide_labels = 0;
+    }
+    if (as_they_are) {
+        t.row = nullptr;
+        t.label = a.targets;
+        t.wide_label = a.wide_targets;
+        return 0;
     }
     const long long groups = (a.rows + gather.per - 1) / gather.per;
     NHIP_LAUNCH((gather_kernel<T>), dim3((unsigned)(groups ? groups : 1)), dim3(NHIP_WG), 0, st, gather);
@@ -626,15 +644,18 @@ template <class T> int piece_rows(hipStream_t st, const nhip_loss_args& a, const
 template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Space& s) {
     char* const w = static_cast<char*>(a.workspace);
     Targets t;
-    TOK_TRY(prepare<T>(st, a, s, w, false, t));
-    const int* const count = reinterpret_cast<int*>(w + s.count);
+    // few rows are computed all, where they lie: to bring together those that count would take a launch
+    const bool all = a.rows <= TOK_FEW && tok_rows_wide(a.x, a.x_stride * (long long)sizeof(T), a.channels * (long long)sizeof(T));
+    TOK_TRY(prepare<T>(st, a, s, w, false, all, t));
+    const int* const count = all ? nullptr : reinterpret_cast<int*>(w + s.count);
+    const TokRows x = all ? TokRows{static_cast<const char*>(a.x), nullptr, a.x_stride * (long long)sizeof(T), a.rows}
+                          : TokRows{w + s.x, nullptr, s.x_ld * (long long)sizeof(T), a.rows};
     int tiles = 0;
     for (long long v0 = 0; v0 < a.words; v0 += s.piece) {
         const long long words = a.words - v0 < s.piece ? a.words - v0 : s.piece;
         TokRows rows;
         TOK_TRY(piece_rows<T>(st, a, s, w, v0, words, rows));
-        TokProduct p{rows, TokRows{w + s.x, nullptr, s.x_ld * (long long)sizeof(T), a.rows}, count, nullptr,
-                     a.channels * (long long)sizeof(T), 0, 0, 1};
+        TokProduct p{rows, x, count, nullptr, a.channels * (long long)sizeof(T), 0, 0, 1};
         auto go = [&](auto top) {
             Statistics<decltype(top)::value> e{t, reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits),
                                                s.padded, (int)words, (int)v0, tiles, 1.0f / a.temperature};
@@ -654,7 +675,7 @@ template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Sp
     }
     if (!a.rows) return 0;
     Finish f{reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits), t, reinterpret_cast<float*>(w + s.self),
-             count, s.padded, tiles, a.loss, a.lse};
+             count, s.padded, tiles, (int)a.rows, a.loss, a.lse};
     NHIP_LAUNCH(finish_kernel, dim3((unsigned)((a.rows + 15) / 16)), dim3(16 * kFinishLanes), 0, st, f);
     NHIP_LAUNCH_CHECK();
     return 0;
@@ -664,7 +685,7 @@ template <class T> int backward(hipStream_t st, const nhip_loss_args& a, const S
     constexpr long long size = sizeof(T);
     char* const w = static_cast<char*>(a.workspace);
     Targets t;
-    TOK_TRY(prepare<T>(st, a, s, w, true, t));
+    TOK_TRY(prepare<T>(st, a, s, w, true, false, t));
     const int* const count = reinterpret_cast<int*>(w + s.count);
     const TokGradient& gr = *s.gradient;
     TOK_TRY(gr.lay_out_x<T>(st, w, w + s.x, s.x_ld, count));

@@ -462,3 +462,24 @@ def test_the_library_refuses_what_python_does_not_see(ops):  # noqa: F811
     for more in (dict(dout=0), dict(dx=0), dict(dweight=0), dict(dv=one), dict(bias=one, dbias=0), dict(workspace=0)):
         assert lib.nhip_layer_norm_grad(None, ref(norm(**more))) == bad, more
     assert lib.nhip_layer_norm_grad(None, ref(norm(workspace_bytes=1))) == too_big
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 16, 17, 64, 65])
+@pytest.mark.parametrize("bad", [NAN, INF])
+def test_few_rows_of_which_not_all_count(queue, ops, n, bad):  # noqa: F811
+    """Few rows are computed all, also those that do not count: none, all, and some of them, whatever they hold."""
+    for given, entry in ((loss_inputs(71, BF16, n, 72, 257, 0.5)[0], ops.plan_vocabulary_loss),
+                         (teacher_inputs(72, BF16, n, 72, 257, 0.5, 9)[0], ops.plan_teacher_loss)):
+        key = "labels" if "labels" in given else "indices"
+        for left in (torch.arange(n) % 2 == 0, torch.ones(n, dtype=torch.bool), torch.zeros(n, dtype=torch.bool)):
+            words = given[key].clone()
+            words[words < 0] = 3
+            words[words >= 257] = 4
+            clean = run(entry(queue, **dict(given, **{key: words})))
+            words[left.cuda()] = 257 if n % 2 else -1
+            x = given["x"].clone()
+            x[left.cuda()] = bad
+            got = run(entry(queue, **dict(given, **{key: words, "x": x})))
+            for a, b in zip(clean, got):
+                assert torch.isfinite(a).all() and not b[left].any() and same(a[~left], b[~left])
