@@ -72,11 +72,10 @@ template <int BM_, int BN_, int WM_, int WN_> struct TokShape {
     static constexpr int kStage = (BM + BN) * TOK_KB;
     // an epilogue has 8 bytes per column and wave of m, or TOK_PUT to a wave
     static constexpr int kEpilogue = 8 * WM * BN > TOK_PUT * kWaves ? 8 * WM * BN : TOK_PUT * kWaves, kLds = 2 * kStage + kEpilogue;
-    // work-groups to a compute unit, by the LDS and by the registers: a wave that holds more than 32 tiles has a SIMD for itself
-    static constexpr int kByRegisters = MI * NI > 32 ? 1 : 8 / kWaves;
-    static constexpr bool kPinned = MI * NI > 32, kPair = kWaves == 8;
-    static constexpr int kAtOnce = (160 << 10) / kLds < kByRegisters ? (160 << 10) / kLds : kByRegisters;
-    static_assert(kWaveM % 16 == 0 && kWaveN % 16 == 0, "waves hold whole tiles");
+    static constexpr bool kPair = kWaves == 8;
+    // work-groups to a compute unit, by the LDS and by the registers: two waves to a SIMD
+    static constexpr int kAtOnce = (160 << 10) / kLds < 8 / kWaves ? (160 << 10) / kLds : 8 / kWaves;
+    static_assert(kWaveM % 16 == 0 && kWaveN % 16 == 0 && MI * NI <= 32, "waves hold whole tiles, in half of a SIMD's registers");
 };
 
 // Where a work-group's wave is
@@ -189,23 +188,13 @@ template <class S> struct TokPart {
 #pragma unroll
         for (int q = 0; q < kReads; ++q) read_one(q, from_a, from_b, c);
     }
-    // Products q of n, in steps: the results of a wave that has a SIMD for itself stay in their registers.  (The compiler's own
-    // form of these products has another register for the result than for the addend, and moved results about.  That a
-    // result is not read too early is seen to here: as an addend 63 products later, otherwise behind tok_settle.)
+    // products q of n, in steps
     template <class T> __device__ __forceinline__ void multiply(sel_f4 (&acc)[S::MI][S::NI], int q, int n) const {
         constexpr int kProducts = S::MI * S::NI * (sizeof(T) == 2 ? 1 : 4);
 #pragma unroll
         for (int e = q * kProducts / n; e < (q + 1) * kProducts / n; ++e) {
             const int part = e / (S::MI * S::NI), i = e / S::NI % S::MI, j = e % S::NI;
-            if constexpr (!S::kPinned) {
-                tok_mma<T>(acc[i][j], a[i], b[j], part);
-            } else if constexpr (std::is_same<T, __bf16>::value) {
-                asm volatile("v_mfma_f32_16x16x32_bf16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(a[i]), "v"(b[j]));
-            } else if constexpr (std::is_same<T, _Float16>::value) {
-                asm volatile("v_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(a[i]), "v"(b[j]));
-            } else {
-                asm volatile("v_mfma_f32_16x16x4_f32 %0, %1, %2, %0" : "+a"(acc[i][j]) : "v"(a[i][part]), "v"(b[j][part]));
-            }
+            tok_mma<T>(acc[i][j], a[i], b[j], part);
         }
     }
 };
@@ -220,16 +209,12 @@ static __device__ __forceinline__ void tok_tile(int id, int m_tiles, int n_tiles
 }
 
 // Waits until the products before it are done: a result that is read behind the loop's branch needs it (see sel_settle).
-// Waves that have a SIMD for themselves hold results in accumulation registers, others among the vector registers.
-template <bool PINNED, int MI, int NI> __device__ __forceinline__ void tok_settle(sel_f4 (&acc)[MI][NI]) {
+template <int MI, int NI> __device__ __forceinline__ void tok_settle(sel_f4 (&acc)[MI][NI]) {
     auto touch = [&] {
 #pragma unroll
         for (int i = 0; i < MI; ++i)
 #pragma unroll
-            for (int j = 0; j < NI; ++j) {
-                if constexpr (PINNED) asm volatile("" : "+a"(acc[i][j]));
-                else asm volatile("" : "+v"(acc[i][j]));
-            }
+            for (int j = 0; j < NI; ++j) asm volatile("" : "+v"(acc[i][j]));
     };
     touch();
     asm volatile("s_nop 15\n\ts_nop 3" ::: "memory");
@@ -436,7 +421,6 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
             if (!behind) turn();
         } else {
             TokPart<S> first, second;
-            tok_settle<S::kPinned>(acc);  // (zeros, too, are written before they are an addend)
             if (now.stages > 0) first.read(a0 + place * kStage, b0 + place * kStage, c0);
             // Half a stage: `next` is read, and `loads` are sent for, between the products.  (Products first: the compiler waits for
             // all reads before the first one, which have come then; and no read among the last quarter, whose time a read takes.)
@@ -469,7 +453,7 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
                 stage();
             }
         }
-        tok_settle<S::kPinned>(acc);
+        tok_settle(acc);
         TokPlace here = at;
         asm volatile("" : "+v"(here.l), "+v"(here.g));  // (or what an epilogue forms of them is kept over all tiles, and spilled)
         epilogue.template run<T, S>(here, acc);
@@ -549,7 +533,7 @@ __global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_few_kernel(TokPr
         load(even, step + 2 * U);
         multiply(odd);
     }
-    tok_settle<false>(acc);
+    tok_settle(acc);
 #pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
@@ -659,7 +643,7 @@ __global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_some_kernel(TokP
         go(chunk, even, odd);
         if (chunk + 1 < per) go(chunk + 1, odd, even);
     }
-    tok_settle<false>(acc);
+    tok_settle(acc);
     tok_wait<0>();  // (all is read, and nothing comes any more)
     sel_f4* const s_sum = reinterpret_cast<sel_f4*>(tok_lds) + (mine * MT * NI) * NHIP_WAVE + lane;
     if (half) {
