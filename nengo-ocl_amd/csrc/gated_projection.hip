@@ -205,6 +205,7 @@ template <class T> int forward(hipStream_t st, const nhip_gated_args& a, const S
         const long long n = a.features - f0 < s.piece ? a.features - f0 : s.piece;
         TOK_TRY(weight_rows<T>(st, a, s, w, f0, n, rows));
         TokProduct p{rows, x, nullptr, nullptr, a.channels * (long long)sizeof(T), 0, 0, 1};
+        p.last = f0 + n == a.features;
         const Forward e{a.y, a.features, f0, n, a.activation};
         if (a.rows <= TOK_FEW) {
             TOK_TRY((tok_few<T, 2, 1>(st, p, e)));
@@ -262,7 +263,7 @@ int run(void* stream, const nhip_gated_args* args, bool grad) {
         using T = decltype(t);
         rc = grad ? backward<T>(static_cast<hipStream_t>(stream), a, s) : forward<T>(static_cast<hipStream_t>(stream), a, s);
     });
-    return rc;
+    return tok_end(static_cast<hipStream_t>(stream), rc);
 }
 
 }  // namespace

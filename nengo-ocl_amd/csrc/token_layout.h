@@ -81,7 +81,7 @@ template <class T> static inline int tok_transpose(hipStream_t stream, TokTransp
     const long long x = a.out_rows / 64, y = (a.cols + 63) / 64;
     if (x > 0xffffff || y > SEL_MAX_GRID_Y) return NHIP_E_BADARG;
     a.wide = tok_rows_wide(a.in, a.ld * (long long)sizeof(T), 16);
-    NHIP_LAUNCH((tok_transpose_kernel<T>), dim3((unsigned)x, (unsigned)y), dim3(NHIP_WG), 0, stream, a);
+    TOK_LAUNCH(false, (tok_transpose_kernel<T>), dim3((unsigned)x, (unsigned)y), dim3(NHIP_WG), 0, stream, a);
     NHIP_LAUNCH_CHECK();
     return 0;
 }
@@ -111,7 +111,7 @@ template <class T> __global__ __launch_bounds__(NHIP_WG) void tok_pad_kernel(Tok
 template <class T> static inline int tok_pad(hipStream_t stream, const TokPad& a) {
     if (a.rows <= 0) return 0;
     const long long groups = (a.rows * (a.out_ld * (long long)sizeof(T) / 16) + NHIP_WG - 1) / NHIP_WG;
-    NHIP_LAUNCH((tok_pad_kernel<T>), dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(NHIP_WG), 0, stream, a);
+    TOK_LAUNCH(false, (tok_pad_kernel<T>), dim3((unsigned)(groups < 16384 ? groups : 16384)), dim3(NHIP_WG), 0, stream, a);
     NHIP_LAUNCH_CHECK();
     return 0;
 }
@@ -201,6 +201,7 @@ struct TokJoin {
     long long rows, cols;
     const int* live = nullptr;  // not NULL: as many parts as the product had by its tiles of live rows (tok_parts), n_parts at most
     int slots = 0, m_tiles = 0, bn = 1;
+    bool last = false;  // the entry point's last launch
 };
 
 template <class T, int V> __global__ __launch_bounds__(NHIP_WG) void tok_join_kernel(TokJoin a) {
@@ -231,8 +232,8 @@ template <class T> static inline int tok_join(hipStream_t stream, const TokJoin&
     const int v = tok_fours(a.out, a.cols, sizeof(T)) ? 4 : 1;
     const long long groups = (a.rows * (a.cols / v) + NHIP_WG - 1) / NHIP_WG;
     const dim3 grid((unsigned)(groups < 16384 ? groups : 16384));
-    if (v == 4) NHIP_LAUNCH((tok_join_kernel<T, 4>), grid, dim3(NHIP_WG), 0, stream, a);
-    else NHIP_LAUNCH((tok_join_kernel<T, 1>), grid, dim3(NHIP_WG), 0, stream, a);
+    if (v == 4) TOK_LAUNCH(a.last, (tok_join_kernel<T, 4>), grid, dim3(NHIP_WG), 0, stream, a);
+    else TOK_LAUNCH(a.last, (tok_join_kernel<T, 1>), grid, dim3(NHIP_WG), 0, stream, a);
     NHIP_LAUNCH_CHECK();
     return 0;
 }
@@ -371,7 +372,7 @@ struct TokGradient {
             using S = decltype(shape);
             constexpr int kAcross = std::is_same<S, TokLarge>::value && sizeof(T) == 2 ? 1 : 0;
             TokProduct p{a, b, live, nullptr, k * size, (int)((d + S::BM - 1) / S::BM), (int)((rows + S::BN - 1) / S::BN),
-                         live ? dx_most : dx_splits, live ? 256 * S::kAtOnce : 0};
+                         live ? dx_most : dx_splits, false, live ? 256 * S::kAtOnce : 0};
             if (kAcross && !across) return tok_product<T, S, 0>(st, p, epilogue);
             return tok_product<T, S, 0, kAcross>(st, p, epilogue);
         };
@@ -389,6 +390,7 @@ struct TokGradient {
             return 0;
         };
         if (live) across ? shape_of(TokLarge()) : tok_with_shape(d, rows, (int)size, dx_splits, shape_of);
+        join.last = true;
         return tok_join<T>(st, join);
     }
 };

@@ -20,6 +20,27 @@ typedef __bf16 tok_b8 __attribute__((ext_vector_type(8)));
 typedef _Float16 tok_h8 __attribute__((ext_vector_type(8)));
 typedef __bf16 sel_b4 __attribute__((ext_vector_type(4)));
 
+// An entry point's first launch carries the start event, the one that is known to be its last (`last`) the stop event; where that
+// is not launched (no rows) the stop event is recorded behind the others.
+#define TOK_LAUNCH(last, kernel, grid, block, lds, stream, ...)                              \
+    do {                                                                                     \
+        const hipEvent_t start_ = nhip_launch_events.start;                                  \
+        const hipEvent_t stop_ = (last) ? nhip_launch_events.stop : nullptr;                 \
+        if (start_ || stop_) {                                                               \
+            nhip_launch_events = NhipLaunchEvents{nullptr, stop_ ? nullptr : nhip_launch_events.stop}; \
+            hipExtLaunchKernelGGL(kernel, grid, block, lds, stream, start_, stop_, 0, __VA_ARGS__);    \
+        } else {                                                                             \
+            hipLaunchKernelGGL(kernel, grid, block, lds, stream, __VA_ARGS__);               \
+        }                                                                                    \
+    } while (0)
+static inline int tok_end(hipStream_t stream, int rc) {
+    const NhipLaunchEvents left = nhip_launch_events;
+    if (left.start || !left.stop) return rc;
+    nhip_launch_events = NhipLaunchEvents{nullptr, nullptr};
+    const int e = (int)hipEventRecord(left.stop, stream);
+    return rc ? rc : e;
+}
+
 #define TOK_MOST_LD (1 << 23)  // 256 rows lie within 2^31 bytes
 #define TOK_KB 128  // bytes of k in a stage: 64 elements of 16 bits, 32 of 32
 
@@ -56,6 +77,7 @@ struct TokProduct {
     long long k_bytes; // of a row
     int m_tiles, n_tiles;
     int splits;        // parts that k is cut into: so many, or
+    bool last = false; // the entry point's last launch
     int slots = 0;     // (not zero) as many as let the tiles of rows that count take so many work-groups, up to `splits`
 };
 
@@ -674,7 +696,7 @@ static inline int tok_few(hipStream_t stream, TokProduct p, const E& epilogue) {
     if (p.b.rows > TOK_FEW || tiles > 0xffffff || p.k_bytes > 0x3fffffff) return NHIP_E_BADARG;
     if (p.b.rows <= 16) {
         using F = TokFew<MT>;
-        NHIP_LAUNCH((tok_few_kernel<T, F, HALF, E>), dim3((unsigned)tiles), dim3(F::kWaves * NHIP_WAVE), 0, stream, p, epilogue);
+        TOK_LAUNCH(p.last, (tok_few_kernel<T, F, HALF, E>), dim3((unsigned)tiles), dim3(F::kWaves * NHIP_WAVE), 0, stream, p, epilogue);
         NHIP_LAUNCH_CHECK();
         return 0;
     }
@@ -682,7 +704,7 @@ static inline int tok_few(hipStream_t stream, TokProduct p, const E& epilogue) {
         using F = decltype(some);
         auto kernel = tok_some_kernel<T, F, HALF, E>;
         if (int e = sel_allow_lds(stream, kernel, F::kLds)) return e;
-        NHIP_LAUNCH(kernel, dim3((unsigned)((tiles + 1) / 2)), dim3(F::kWaves * NHIP_WAVE), F::kLds, stream, p, epilogue);
+        TOK_LAUNCH(p.last, kernel, dim3((unsigned)((tiles + 1) / 2)), dim3(F::kWaves * NHIP_WAVE), F::kLds, stream, p, epilogue);
         return (int)hipGetLastError();
     };
     if (p.b.rows <= 32) return go(TokSome<MT, 2>());
@@ -768,7 +790,7 @@ static inline int tok_product(hipStream_t stream, const TokProduct& p, const E& 
     auto kernel = tok_product_kernel<T, S, HALF, ACROSS, E>;
     constexpr int kLds = S::kLds + (ACROSS ? 2 * 64 * (TOK_ACROSS - 1024) : 0);
     if (int e = sel_allow_lds(stream, kernel, kLds)) return e;
-    NHIP_LAUNCH(kernel, dim3((unsigned)(tiles < groups ? tiles : groups)), dim3(S::kThreads), kLds, stream, p, epilogue);
+    TOK_LAUNCH(p.last, kernel, dim3((unsigned)(tiles < groups ? tiles : groups)), dim3(S::kThreads), kLds, stream, p, epilogue);
     NHIP_LAUNCH_CHECK();
     return 0;
 }

@@ -609,9 +609,9 @@ int prepare(hipStream_t st, const nhip_loss_args& a, const Space& s, char* w, bo
                   reinterpret_cast<int*>(w + s.word), reinterpret_cast<float*>(w + s.share), reinterpret_cast<float*>(w + s.self),
                   reinterpret_cast<int*>(w + s.flag), reinterpret_cast<unsigned short*>(w + s.first), (int)s.blocks, (int)s.block};
         const dim3 grid((unsigned)((a.rows + 3) / 4));
-        if (a.top <= 64) NHIP_LAUNCH((shares_kernel<1>), grid, dim3(NHIP_WG), 0, st, sh);
-        else if (a.top <= 128) NHIP_LAUNCH((shares_kernel<2>), grid, dim3(NHIP_WG), 0, st, sh);
-        else NHIP_LAUNCH((shares_kernel<4>), grid, dim3(NHIP_WG), 0, st, sh);
+        if (a.top <= 64) TOK_LAUNCH(false, (shares_kernel<1>), grid, dim3(NHIP_WG), 0, st, sh);
+        else if (a.top <= 128) TOK_LAUNCH(false, (shares_kernel<2>), grid, dim3(NHIP_WG), 0, st, sh);
+        else TOK_LAUNCH(false, (shares_kernel<4>), grid, dim3(NHIP_WG), 0, st, sh);
         NHIP_LAUNCH_CHECK();
         gather.labels = w + s.flag;  // 0 or -1
         gather.wide_labels = 0;
@@ -623,7 +623,7 @@ int prepare(hipStream_t st, const nhip_loss_args& a, const Space& s, char* w, bo
         return 0;
     }
     const long long groups = (a.rows + gather.per - 1) / gather.per;
-    NHIP_LAUNCH((gather_kernel<T>), dim3((unsigned)(groups ? groups : 1)), dim3(NHIP_WG), 0, st, gather);
+    TOK_LAUNCH(false, (gather_kernel<T>), dim3((unsigned)(groups ? groups : 1)), dim3(NHIP_WG), 0, st, gather);
     NHIP_LAUNCH_CHECK();
     return 0;
 }
@@ -676,7 +676,7 @@ template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Sp
     if (!a.rows) return 0;
     Finish f{reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits), t, reinterpret_cast<float*>(w + s.self),
              count, s.padded, tiles, (int)a.rows, a.loss, a.lse};
-    NHIP_LAUNCH(finish_kernel, dim3((unsigned)((a.rows + 15) / 16)), dim3(16 * kFinishLanes), 0, st, f);
+    TOK_LAUNCH(true, finish_kernel, dim3((unsigned)((a.rows + 15) / 16)), dim3(16 * kFinishLanes), 0, st, f);
     NHIP_LAUNCH_CHECK();
     return 0;
 }
@@ -692,7 +692,7 @@ template <class T> int backward(hipStream_t st, const nhip_loss_args& a, const S
     float* scale = nullptr;
     if (sizeof(T) == 2 && a.rows) {
         scale = reinterpret_cast<float*>(w + s.count) + 16;
-        NHIP_LAUNCH(scale_kernel, dim3(1), dim3(1024), 0, st, a.dloss, reinterpret_cast<int*>(w + s.where), a.rows,
+        TOK_LAUNCH(false, scale_kernel, dim3(1), dim3(1024), 0, st, a.dloss, reinterpret_cast<int*>(w + s.where), a.rows,
                     1.0f / a.temperature, std::is_same<T, _Float16>::value ? 0x1p14f : 1.0f, scale);
         NHIP_LAUNCH_CHECK();
     }
@@ -733,7 +733,7 @@ int run(void* stream, const nhip_loss_args* args, bool grad) {
         using T = decltype(t);
         rc = grad ? backward<T>(static_cast<hipStream_t>(stream), a, s) : forward<T>(static_cast<hipStream_t>(stream), a, s);
     });
-    return rc;
+    return tok_end(static_cast<hipStream_t>(stream), rc);
 }
 
 }  // namespace

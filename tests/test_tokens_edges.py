@@ -483,3 +483,21 @@ def test_few_rows_of_which_not_all_count(queue, ops, n, bad):  # noqa: F811
             got = run(entry(queue, **dict(given, **{key: words, "x": x})))
             for a, b in zip(clean, got):
                 assert torch.isfinite(a).all() and not b[left].any() and same(a[~left], b[~left])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [0, 3, 70, 300])
+def test_events_span_all_launches(queue, ops, n):  # noqa: F811
+    """A timed plan's events enclose all that its entry point launches; none are left for the next one."""
+    for name, (given, make) in calls(ops, queue, 73, BF16, max(n, 1), 520, 9001).items():
+        given = {k: t[:n] if t is not None and t.dim() and t.shape[0] == max(n, 1) and k not in ("weight", "bias", "gate", "up")
+                 else t for k, t in given.items()}
+        plan = make(**given)
+        for _ in range(2):
+            plan(profiling=True)
+        plan.update_profiling()
+        assert not queue.lib.nhip_launch_events_pending(), name
+        assert plan.n_calls in (0, 2) if n == 0 else plan.n_calls == 2, name
+        assert all(t >= 0.0 for t in plan.ctimes), name
+        if n == 300 and name == "loss_grad":  # at least its 6 M N K operations at the highest rate there is
+            assert min(plan.ctimes) > 6 * 0.6 * n * 520 * 9001 / 2.6e15, plan.ctimes
