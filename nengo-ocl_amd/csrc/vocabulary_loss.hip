@@ -5,7 +5,7 @@
 //     G[n, v] = dloss[n] / temperature (exp(z[n, v] - lse[n]) - q[n, v]),   dx = G weight,   dweight = G' x
 //
 // The forward pass forms tiles of z and leaves of each the maximum and the sum of a token's exponentials and the
-// logits of its targets.  The backward pass goes over the vocabulary in pieces: a piece's part of G is formed from z again and kept,
+// logit of its label, or the sum of its targets' q z.  The backward pass goes over the vocabulary in pieces: a piece's part of G is formed from z again and kept,
 // in the type of x, for the two products that read it.
 #include <algorithm>
 #include <optional>
@@ -279,33 +279,38 @@ struct Targets {
         const long long w = word_at(label, wide_label, n);
         return w >= 0 && w < n_words ? (int)w : -1;
     }
-    // where the entries of words w0 ... w1 - 1 (multiples of `block`) begin and end among a row's
+    // where the entries of words w0 ... w1 - 1 (and some around them, to whole blocks) begin and end among a row's
     __device__ __forceinline__ void range(long long r, int w0, int w1, int& lo, int& hi) const {
         const unsigned short* const of = first + r * blocks;
         lo = of[min(w0 / block, blocks - 1)];
-        hi = of[min(w1 / block, blocks - 1)];
+        hi = of[min((w1 + block - 1) / block, blocks - 1)];
     }
 };
 
-// Forward: of each token in the tile the maximum of z and the sum of exp(z - maximum), in powers of two, and the logits of
-// its targets.
+// Forward: of each token in the tile the maximum of z and the sum of exp(z - maximum), in powers of two, and the logit of
+// its label, or the sum of its targets' q z.  (4096 tokens, 32000 words, 64 of them targets, 1024 channels: without targets the
+// kernel would take 45 us less of 250.  A wave waits for row, range and first target, one after the other; loaded while
+// the tile is multiplied they need registers that there are not: 13 spilled, 60 us more.)
 template <bool TOP> struct Statistics {
     Targets targets;
     float2* part;      // [tiles of the whole vocabulary, ld]
-    float* logits;     // [live, top]
+    float* picked;     // [live]: the label's logit; of each tile the sum of shares and logits of a teacher's targets, as `part`
     long long ld;
     int words, word0, tile0;  // words of the piece, its first word, its first tile
     float per_temperature;
 
     template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
-        float2* const s_part = reinterpret_cast<float2*>(at.lds);              // [WM][BN]
+        float2* const s_part = reinterpret_cast<float2*>(at.lds);  // [WM][BN]
+        float* const s_picked = reinterpret_cast<float*>(s_part + S::WM * S::BN);
+        static_assert(12 * S::WM * S::BN <= S::kEpilogue, "");
         const long long n0 = (long long)at.n_tile * S::BN;
         const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g;  // within the piece
-        const int w0 = word0 + at.m_tile * S::BM;
+        const int w0 = word0 + at.m_tile * S::BM + at.wave_m * S::kWaveM;
         if (S::WM > 1) __syncthreads();  // (the tile before is done with the LDS)
         const float c = kLog2e * per_temperature;
         // what the tokens have, before it is needed: loads under a condition are waited for one by one
-        int lo[S::NI], hi[S::NI], row[S::NI];
+        int lo[S::NI], hi[S::NI], row[S::NI], word[S::NI];
+        float share[S::NI];
         auto token = [&](int j) { return n0 + at.wave_n * S::kWaveN + 16 * j + at.l; };
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
@@ -314,7 +319,13 @@ template <bool TOP> struct Statistics {
         }
         if constexpr (TOP) {
 #pragma unroll
-            for (int j = 0; j < S::NI; ++j) targets.range(row[j], w0, w0 + S::BM, lo[j], hi[j]);
+            for (int j = 0; j < S::NI; ++j) targets.range(row[j], w0, w0 + S::kWaveM, lo[j], hi[j]);
+#pragma unroll
+            for (int j = 0; j < S::NI; ++j) {
+                const long long e = (long long)row[j] * targets.top + min(lo[j], targets.top - 1);
+                word[j] = targets.word[e];
+                share[j] = targets.share[e];
+            }
         }
         auto go = [&](auto whole) {
             auto is = [&](int i, int r) { return decltype(whole)::value || m0 + 16 * i + r < words; };
@@ -353,32 +364,53 @@ template <bool TOP> struct Statistics {
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
             const long long n = token(j);
-            auto pick = [&](int word, float* to) {
-                const int rel = word - word0 - m0;
-                if (rel < 0 || rel >= S::kWaveM || (rel & 15) >= 4) return;
+            auto is_mine = [&](int rel) { return rel >= 0 && rel < S::kWaveM && (rel & 15) < 4; };
+            auto logit = [&](int rel) {
                 float z = 0.0f;
 #pragma unroll
                 for (int i = 0; i < S::MI; ++i)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) z = rel == 16 * i + r ? acc[i][j][r] : z;
-                *to = z * per_temperature;
+                return z * per_temperature;
             };
-            if (n < at.live) {
-                if constexpr (TOP) {
-                    const int* const word = targets.word + (long long)row[j] * targets.top;
-                    for (int k = lo[j]; k < hi[j]; ++k) pick(word[k], logits + n * targets.top + k);
-                } else {
-                    pick(row[j], logits + n);
+            if constexpr (TOP) {
+                float sum = 0.0f;
+                // (the first target's loads are under no condition: the compiler would wait for each of them)
+                asm volatile("" : "+v"(word[j]), "+v"(share[j]));
+                const long long from = (long long)row[j] * targets.top;
+                float q = n < at.live && lo[j] < hi[j] ? share[j] : 0.0f;
+                int rel = word[j] - word0 - m0;
+                for (int k = lo[j];;) {
+                    if (!is_mine(rel)) q = 0.0f;
+                    if (__any(q != 0.0f)) sum = q != 0.0f ? fmaf(q, logit(rel), sum) : sum;
+                    const bool more = n < at.live && ++k < hi[j];
+                    if (!__any(more)) break;
+                    q = more ? targets.share[from + k] : 0.0f;
+                    rel = more ? targets.word[from + k] - word0 - m0 : -1;
                 }
+                sum += __shfl_xor(sum, 16);
+                sum += __shfl_xor(sum, 32);
+                if (at.g == 0) {
+                    if (S::WM > 1) s_picked[at.wave_m * S::BN + (int)(n - n0)] = sum;
+                    else if (n < at.live) picked[(long long)(tile0 + at.m_tile) * ld + n] = sum;
+                }
+            } else if (n < at.live && is_mine(row[j] - word0 - m0)) {
+                picked[n] = logit(row[j] - word0 - m0);
             }
         }
         if constexpr (S::WM > 1) {
             __syncthreads();
             for (int k = threadIdx.x; k < S::BN; k += S::kThreads) {
                 float2 a = s_part[k];
+                float sum = TOP ? s_picked[k] : 0.0f;
 #pragma unroll
-                for (int w = 1; w < S::WM; ++w) a = joined(a, s_part[w * S::BN + k]);
-                if (n0 + k < at.live) part[(long long)(tile0 + at.m_tile) * ld + n0 + k] = a;
+                for (int w = 1; w < S::WM; ++w) {
+                    a = joined(a, s_part[w * S::BN + k]);
+                    if (TOP) sum += s_picked[w * S::BN + k];
+                }
+                if (n0 + k >= at.live) continue;
+                part[(long long)(tile0 + at.m_tile) * ld + n0 + k] = a;
+                if (TOP) picked[(long long)(tile0 + at.m_tile) * ld + n0 + k] = sum;
             }
         }
     }
@@ -397,7 +429,7 @@ template <bool TOP> struct Statistics {
 constexpr int kFinishLanes = 64;
 struct Finish {
     const float2* part;
-    const float* logits;
+    const float* picked;
     Targets targets;
     const float* self;
     const int* count;  // NULL: `rows`
@@ -421,14 +453,9 @@ __global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
         for (int o = 0; o < 8; ++o)
             if (t + o * kFinishLanes < a.tiles) v = Statistics<false>::joined(v, some[o]);
     }
-    float loss = 0.0f;
-    if (a.targets.top) {  // sum q (lse - z), whose sum of q times lse follows
-        for (int e = q; e < a.targets.top; e += kFinishLanes) {
-            const long long at = (long long)row * a.targets.top + e;
-            const float share = a.targets.share[at];
-            if (a.targets.word[at] != kNoWord && share != 0.0f) loss = fmaf(share, a.logits[(long long)n * a.targets.top + e], loss);
-        }
-    }
+    float loss = 0.0f;  // sum q z
+    if (a.targets.top)
+        for (int t = q; t < a.tiles; t += kFinishLanes) loss += a.picked[(long long)t * a.ld + n];
     // four lanes of a wave have one token, then 16 waves; always in the same order
     auto join = [&](int d) {
         v = Statistics<false>::joined(v, float2{__shfl_xor(v.x, d), __shfl_xor(v.y, d)});
@@ -450,7 +477,7 @@ __global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
     join(32);
     if (q || (int)blockIdx.x * 16 + k >= live) return;
     const float lse = (v.x + __builtin_amdgcn_logf(v.y)) * kLn2;
-    a.loss[row] = !is ? 0.0f : a.targets.top ? a.self[row] + (lse - loss) : lse - a.logits[n];  // (the shares' sum is one)
+    a.loss[row] = !is ? 0.0f : a.targets.top ? a.self[row] + (lse - loss) : lse - a.picked[n];  // (the shares' sum is one)
     a.lse[row] = is ? lse : 0.0f;
 }
 
@@ -465,7 +492,7 @@ template <bool TOP> struct Gradient {
 
     template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
         const long long n0 = (long long)at.n_tile * S::BN;
-        const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g, w0 = word0 + at.m_tile * S::BM;
+        const int m0 = at.m_tile * S::BM + at.wave_m * S::kWaveM + 4 * at.g, w0 = word0 + at.m_tile * S::BM + at.wave_m * S::kWaveM;
         const float c = kLog2e * per_temperature, k = scale ? *scale * per_temperature : per_temperature;
         // what the tokens have, before it is needed: loads under a condition are waited for one by one
         int row[S::NI], label[S::NI], lo[S::NI], hi[S::NI];
@@ -480,19 +507,44 @@ template <bool TOP> struct Gradient {
         for (int j = 0; j < S::NI; ++j) {
             d[j] = dloss[row[j]] * k;
             lse2[j] = lse[row[j]] * kLog2e;
-            if constexpr (TOP) targets.range(row[j], w0, w0 + S::BM, lo[j], hi[j]);
+            if constexpr (TOP) targets.range(row[j], w0, w0 + S::kWaveM, lo[j], hi[j]);
         }
+        // of a teacher's targets in the tile the first is taken before the element is stored: most tiles have no second of a token
+        // (4096 tokens, 32000 words, 64 of them targets, 1024 channels: 697 us; 680 so, 687 with two)
+        constexpr int kTaken = TOP ? 1 : 0;
+        int place[S::NI][kTaken + 1];
+        float share[S::NI][kTaken + 1];
+#pragma unroll
+        for (int j = 0; j < S::NI; ++j)
+#pragma unroll
+            for (int t = 0; t < kTaken; ++t) {
+                const long long e = (long long)row[j] * targets.top + min(lo[j] + t, targets.top - 1);
+                place[j][t] = lo[j] + t < hi[j] ? targets.word[e] - word0 - m0 : -1;
+                share[j][t] = targets.share[e] * d[j];
+            }
         const bool whole = (at.m_tile + 1) * S::BM <= words;
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
             const long long n = token(j);
             const bool counts = n < at.live;
+            int taken = 0;  // of the wave: so many targets at most has a token of the column
+#pragma unroll
+            for (int t = 0; t < kTaken; ++t) {
+                if (!counts) place[j][t] = -1;
+                if (__any(place[j][t] >= 0 && place[j][t] < S::kWaveM)) taken = t + 1;
+            }
             auto value = [&](int i, float(&v)[4]) {
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const float p = d[j] * __builtin_amdgcn_exp2f(fmaf(acc[i][j][r], c, -lse2[j]));
                     v[r] = counts && (whole || m0 + 16 * i + r < words) ? p : 0.0f;
                 }
+#pragma unroll
+                for (int t = 0; t < kTaken; ++t)
+                    if (t < taken) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] -= place[j][t] == 16 * i + r ? share[j][t] : 0.0f;
+                    }
             };
             bool stored = false;
             if constexpr (sizeof(T) == 2 && S::MI % 4 == 0) {
@@ -529,7 +581,7 @@ template <bool TOP> struct Gradient {
             if (counts) {
                 if constexpr (TOP) {
                     const long long from = (long long)row[j] * targets.top;
-                    for (int e = lo[j]; e < hi[j]; ++e) take(targets.word[from + e], targets.share[from + e]);
+                    for (int e = lo[j] + kTaken; e < hi[j]; ++e) take(targets.word[from + e], targets.share[from + e]);
                 } else {
                     take(label[j], 1.0f);
                 }
@@ -555,7 +607,7 @@ bool wide_weight(const nhip_loss_args& a) {
 
 struct Space : TokSpace {
     long long padded, x_ld, piece;
-    long long row, where, label, count, flag, word, share, self, first, blocks, block, x, weight, part, logits;
+    long long row, where, label, count, flag, word, share, self, first, blocks, block, x, weight, part, picked;
     std::optional<TokGradient> gradient;
     Space(const nhip_loss_args& a, bool grad) {
         const long long size = sel_size(a.type), rows = a.rows > 0 ? a.rows : 1, top = a.top;
@@ -585,8 +637,9 @@ struct Space : TokSpace {
             piece = (1LL << 22) / (padded / 256) * 128;
             if (!wide_weight(a)) piece = std::min(piece, std::max(256LL, (512LL << 20) / (x_ld * size) / 256 * 256));
             piece = std::min(piece, tok_round(a.words, 256));
-            part = take((tok_round(a.words, piece) / TOK_LEAST_BM) * padded * 8);
-            logits = take(padded * (top ? top : 1) * 4);
+            const long long tiles = tok_round(a.words, piece) / TOK_LEAST_BM;
+            part = take(tiles * padded * 8);
+            picked = take((top ? tiles : 1) * padded * 4);
         }
         weight = wide_weight(a) ? 0 : take(piece * x_ld * size);
     }
@@ -657,7 +710,7 @@ template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Sp
         TOK_TRY(piece_rows<T>(st, a, s, w, v0, words, rows));
         TokProduct p{rows, x, count, nullptr, a.channels * (long long)sizeof(T), 0, 0, 1};
         auto go = [&](auto top) {
-            Statistics<decltype(top)::value> e{t, reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits),
+            Statistics<decltype(top)::value> e{t, reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.picked),
                                                s.padded, (int)words, (int)v0, tiles, 1.0f / a.temperature};
             if (a.rows <= TOK_FEW) {
                 tiles += (int)((words + TOK_LEAST_BM - 1) / TOK_LEAST_BM);
@@ -674,7 +727,7 @@ template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Sp
         TOK_TRY(a.top ? go(std::true_type()) : go(std::false_type()));
     }
     if (!a.rows) return 0;
-    Finish f{reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.logits), t, reinterpret_cast<float*>(w + s.self),
+    Finish f{reinterpret_cast<float2*>(w + s.part), reinterpret_cast<float*>(w + s.picked), t, reinterpret_cast<float*>(w + s.self),
              count, s.padded, tiles, (int)a.rows, a.loss, a.lse};
     TOK_LAUNCH(true, finish_kernel, dim3((unsigned)((a.rows + 15) / 16)), dim3(16 * kFinishLanes), 0, st, f);
     NHIP_LAUNCH_CHECK();
