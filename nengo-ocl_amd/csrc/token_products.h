@@ -799,7 +799,7 @@ static inline int tok_product(hipStream_t stream, const TokProduct& p, const E& 
 }
 
 using TokLarge = TokShape<256, 256, 2, 4>;
-#define TOK_LEAST_BM 32  // of all shapes, and of the kernels for few columns
+#define TOK_LEAST_BM 32  // of the kernels for few columns (without HALF); other shapes' tiles have 128 rows at least
 #define TOK_MOST_TILE 256
 
 // The shape of a product of m x n in elements of `size` bytes: tiles of 256 x 256 where they are enough to go round, of fewer

@@ -445,17 +445,23 @@ __global__ __launch_bounds__(16 * kFinishLanes) void finish_kernel(Finish a) {
     const int n = min((int)blockIdx.x * 16 + k, live - 1), row = a.targets.row_of(n);
     const bool is = a.targets.row || (a.targets.top ? a.targets.flag[n] : a.targets.label_of(n)) >= 0;
     float2 v = {0.0f, 0.0f};
+    float loss = 0.0f;  // sum q z
     for (int t = q; t < a.tiles; t += 8 * kFinishLanes) {
         float2 some[8];
+        float z[8];
 #pragma unroll
-        for (int o = 0; o < 8; ++o) some[o] = a.part[(long long)min(t + o * kFinishLanes, a.tiles - 1) * a.ld + n];
+        for (int o = 0; o < 8; ++o) {
+            const long long at = (long long)min(t + o * kFinishLanes, a.tiles - 1) * a.ld + n;
+            some[o] = a.part[at];
+            z[o] = a.targets.top ? a.picked[at] : 0.0f;
+        }
 #pragma unroll
         for (int o = 0; o < 8; ++o)
-            if (t + o * kFinishLanes < a.tiles) v = Statistics<false>::joined(v, some[o]);
+            if (t + o * kFinishLanes < a.tiles) {
+                v = Statistics<false>::joined(v, some[o]);
+                loss += z[o];
+            }
     }
-    float loss = 0.0f;  // sum q z
-    if (a.targets.top)
-        for (int t = q; t < a.tiles; t += kFinishLanes) loss += a.picked[(long long)t * a.ld + n];
     // four lanes of a wave have one token, then 16 waves; always in the same order
     auto join = [&](int d) {
         v = Statistics<false>::joined(v, float2{__shfl_xor(v.x, d), __shfl_xor(v.y, d)});
@@ -633,11 +639,11 @@ struct Space : TokSpace {
             gradient.emplace(*this, a.rows, a.channels, a.words, size);
             piece = gradient->piece;
         } else {
-            // as many words as a launch's tiles reach, and where they are copied as fit 512 MB
-            piece = (1LL << 22) / (padded / 256) * 128;
+            // as many words as a launch's tiles reach (256 tokens: 2^28), and where they are copied as fit 512 MB
+            piece = (1LL << 21) / (padded / 256) * 128;
             if (!wide_weight(a)) piece = std::min(piece, std::max(256LL, (512LL << 20) / (x_ld * size) / 256 * 256));
             piece = std::min(piece, tok_round(a.words, 256));
-            const long long tiles = tok_round(a.words, piece) / TOK_LEAST_BM;
+            const long long tiles = tok_round(a.words, piece) / (a.rows <= TOK_FEW ? TOK_LEAST_BM : 128);
             part = take(tiles * padded * 8);
             picked = take((top ? tiles : 1) * padded * 4);
         }

@@ -73,3 +73,42 @@ def test_gated_projection(queue, ops, dtype, n, d, f, name):  # noqa: F811
            og @ gate.abs() + ou @ up.abs() + (2 * f + 8) * E * (sg @ gate.abs() + su @ up.abs()), "x")
     within(got.gate, dg.t() @ x, og.t() @ x.abs() + (n + 8) * E * (sg.t() @ x.abs()), "gate")
     within(got.up, du.t() @ x, ou.t() @ x.abs() + (n + 8) * E * (su.t() @ x.abs()), "up")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [8193, 65537, 70001])
+def test_many_tokens_of_which_some_count(queue, ops, n):  # noqa: F811
+    """Tokens are brought together in groups of 64 and of 1024."""
+    given, m = loss_inputs(24, BF16, n, 8, 40, 0.4)
+    loss, lse = ops.vocabulary_loss(queue, **given)
+    check_losses(loss, lse, given, 1.0)
+    dloss = (torch.rand(n, generator=m.gen) / n).cuda()
+    check_loss_gradients(ops.vocabulary_loss_grad(queue, dloss, lse=lse, **given), given, 1.0, dloss, lse)
+    given, m = teacher_inputs(25, BF16, n, 8, 40, 0.4, 3)
+    loss, lse = ops.teacher_loss(queue, **given)
+    check_losses(loss, lse, given, 1.0)
+    check_loss_gradients(ops.teacher_loss_grad(queue, dloss, lse=lse, **given), given, 1.0, dloss, lse)
+
+
+@pytest.mark.gpu
+def test_offsets_behind_32_bits(queue, ops):  # noqa: F811
+    """Rows of x and of weights that lie more than 2**31 elements behind the first: the same as where they are near."""
+    n, d, v = 5, 64, 300
+    room = torch.empty(n, 1 << 30, device="cuda", dtype=BF16)  # the last row 2**32 elements behind the first
+    given, m = loss_inputs(26, BF16, n, d, v, 0.0)
+    x, weight = room[:, :d], room[:, d:2 * d]
+    x.copy_(given["x"])
+    want = ops.vocabulary_loss(queue, **given)
+    got = ops.vocabulary_loss(queue, x, given["weight"], given["labels"])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    dloss = torch.rand(n, generator=m.gen).cuda()
+    a, b = (ops.vocabulary_loss_grad(queue, dloss, t, given["weight"], given["labels"], want[1]) for t in (x, given["x"]))
+    assert torch.equal(a.x, b.x) and torch.equal(a.weight, b.weight)
+    near, words = given["weight"][:n].contiguous(), given["labels"] % n
+    weight.copy_(near)
+    for t in (given["x"], x):
+        got, want = (ops.vocabulary_loss(queue, t, w, words) for w in (weight, near))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+        assert torch.equal(ops.gated_projection(queue, t, weight, weight), ops.gated_projection(queue, t, near, near))
+        gain = torch.ones(d, device="cuda")
+        assert torch.equal(ops.layer_norm(queue, t, gain)[0], ops.layer_norm(queue, given["x"], gain)[0])
