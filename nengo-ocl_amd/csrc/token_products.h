@@ -803,11 +803,13 @@ using TokLarge = TokShape<256, 256, 2, 4>;
 #define TOK_MOST_TILE 256
 
 // The shape of a product of m x n in elements of `size` bytes: tiles of 256 x 256 where they are enough to go round, of fewer
-// columns where there are few.  (8192 x 11008 x 2048 in bfloat16: 1320 TFLOP/s by tiles of 256, 800 by tiles of 128; in 32 bits,
-// where the matrix instructions take as long either way, the smaller ones share 256 compute units more evenly.)
-static inline bool tok_is_large(long long m, long long n, int size, int splits) {
+// columns where there are few.  (8192 x 11008 x 2048 in bfloat16: 1320 TFLOP/s by tiles of 256, 800 by tiles of 128.  These are all
+// under way at once up to 512, which are 128 large ones: 25000 x 250 x 2048 in 31 us, by large tiles 44; 19200 x 500 x 2048 in
+// 54, by large tiles 47.  In 32 bits, where the matrix instructions take as long either way, the smaller ones share 256
+// compute units more evenly.)
+static inline bool tok_is_large(long long m, long long n, int size, int splits, int least = 129) {
     const long long large = ((m + 255) / 256) * ((n + 255) / 256) * splits;
-    return n > 128 && m > 128 && large >= (size == 2 ? 96 : 512);
+    return n > 128 && m > 128 && large >= (size == 2 ? least : 512);
 }
 template <class F> static inline int tok_with_shape(long long m, long long n, int size, int splits, F&& f) {
     if (tok_is_large(m, n, size, splits)) return f(TokLarge());
