@@ -501,3 +501,60 @@ def test_events_span_all_launches(queue, ops, n):  # noqa: F811
         assert all(t >= 0.0 for t in plan.ctimes), name
         if n == 300 and name == "loss_grad":  # at least its 6 M N K operations at the highest rate there is
             assert min(plan.ctimes) > 6 * 0.6 * n * 520 * 9001 / 2.6e15, plan.ctimes
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype, n, d, v", [(BF16, 40, 72, 257), (BF16, 300, 520, 9001), (F32, 300, 130, 310)])
+def test_rows_that_are_one(queue, ops, dtype, n, d, v):  # noqa: F811
+    """Inputs whose rows all lie at the same place (a stride of zero): the same as their copies, bit for bit."""
+    for name, (given, make) in calls(ops, queue, 74, dtype, n, d, v).items():
+        one = {k: given[k][:1].expand(n, -1) if k in ("x", "residual", "dy", "dout", "dv") and given.get(k) is not None else given[k]
+               for k in given}
+        if "labels" in one:
+            one["labels"] = one["labels"].clone()
+            one["labels"][0] = 1
+        copies = {k: t.contiguous() if t is not None else None for k, t in one.items()}
+        assert all(same(a, b) for a, b in zip(run(make(**one)), run(make(**copies)))), name
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_one_row_without_leading_axes(queue, ops, dtype):  # noqa: F811
+    m = Maker(75)
+    x, w = m.normal(72, dtype=dtype), m.normal(257, 72, dtype=dtype, scale=0.1)
+    label = torch.tensor(5, device="cuda")
+    for a, b in ((ops.vocabulary_loss(queue, x, w, label), ops.vocabulary_loss(queue, x[None], w, label[None])),
+                 ((ops.gated_projection(queue, x, w, w),), (ops.gated_projection(queue, x[None], w, w),)),
+                 (ops.layer_norm(queue, x, torch.ones(72, device="cuda"))[:1],
+                  ops.layer_norm(queue, x[None], torch.ones(72, device="cuda"))[:1])):
+        for s, t in zip(a, b):
+            assert s.shape == t.shape[1:] and same(s, t[0])
+
+
+@pytest.mark.gpu
+def test_two_streams_at_once(ops):  # noqa: F811
+    """Plans on two streams, under way together, give what they give alone."""
+    from nengo_ocl_amd.hipraggedarray import Queue
+
+    queues = [Queue(0), Queue(0)]
+    plans = []
+    for k, q in enumerate(queues):
+        made = calls(ops, q, 76 + k, BF16, 300, 520, 9001)
+        q.finish()
+        torch.cuda.synchronize()
+        plans.append([make(**given) for given, make in made.values()])
+    alone = [[run(p) for p in of] for of in plans]
+    for _ in range(3):
+        for of in plans:
+            for p in of:
+                for t in outputs(p):
+                    t.fill_(NAN)
+        torch.cuda.synchronize()
+        for a, b in zip(*plans):
+            a.enqueue()
+            b.enqueue()
+        for q in queues:
+            q.finish()
+        for of, want in zip(plans, alone):
+            for p, w in zip(of, want):
+                assert all(same(s, t) for s, t in zip(outputs(p), w))
