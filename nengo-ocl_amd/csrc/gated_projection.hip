@@ -74,15 +74,30 @@ struct Forward {
     }
 };
 
-// dg and du of the tile, in both layouts: columns (rows) of du come `second` behind those of dg
-struct Backward {
+// dg and du of the tile, in both layouts: columns (rows) of du come `second` behind those of dg.  They are rounded to the
+// type of x, the type in which the matrix cores multiply them with x and the weights: once, to half a step.  (A gradient in
+// bfloat16 is off by 0.0023 of its norm, 0.0017 of it the rounding of the result; two parts to each of them would
+// save that and double two of the three products.)
+//
+// Float16 holds less than their range: 2000 times an activation of 40 is beyond it.  A wave leaves the largest of its tile, and where
+// the largest of all is beyond the type, or so small that what matters is among its subnormal numbers, the product is formed
+// once more, and they are stored by a power of two that brings the largest to 2^14 ... 2^15 (Range).  Others are stored as they are:
+// the launches that look for the largest and that then do nothing take 28 us of 1056 (8192 rows, 2048 channels, 5504 features;
+// 6 of 63 with 700, 512, 1376), the product once more 370.  (A kernel of its own for each: one that does both spills ten registers.)
+enum class Kept { plain, measured, scaled };
+template <Kept KEPT> struct Backward {
     const void* dy;
     long long dy_ld, f0, n_features, second;
     void *g, *gt;
     long long g_ld, gt_ld;
     int activation;
+    int m_tiles;
+    float* most;         // measured: [tiles, waves], the largest finite magnitude
+    const float* scale;  // scaled
     template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
         constexpr int H = S::MI / 2;
+        float top = 0.0f;
+        const float k = KEPT == Kept::scaled ? *scale : 1.0f;
         const bool wide = tok_fours(dy, dy_ld, sizeof(T));
         const long long c = ((long long)at.m_tile * S::BM + at.wave_m * S::kWaveM) / 2;  // of the piece's features
 #pragma unroll
@@ -111,6 +126,17 @@ struct Backward {
                     acc[i][j][r] = is ? d[i][r] * acc[i + H][j][r] * slope : 0.0f;
                     acc[i + H][j][r] = is ? d[i][r] * act : 0.0f;
                 }
+            if constexpr (KEPT != Kept::plain) {
+#pragma unroll
+                for (int i = 0; i < S::MI; ++i)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float v = acc[i][j][r];
+                        if (KEPT == Kept::measured) top = fabsf(v) < INFINITY ? fmaxf(top, fabsf(v)) : top;
+                        else acc[i][j][r] = v * k;
+                    }
+                asm volatile("" : "+v"(top));  // (a column at a time: with all of them at once registers are spilled)
+            }
             if constexpr (sizeof(T) == 2 && H % 4 == 0) {
                 if (!gt) {
 #pragma unroll
@@ -130,8 +156,42 @@ struct Backward {
                                   (i < H ? 0 : second) + c + 16 * (i % H) + 4 * at.g, v);
             }
         }
+        if constexpr (KEPT == Kept::measured) {
+#pragma unroll
+            for (int e = 1; e < NHIP_WAVE; e *= 2) top = fmaxf(top, __shfl_xor(top, e));
+            if (at.l + at.g == 0) most[((long long)at.n_tile * m_tiles + at.m_tile) * S::kWaves + at.wave_n * S::WM + at.wave_m] = top;
+        }
     }
 };
+
+// Float16: from the tiles' largest magnitudes what dg and du are scaled by (and the reverse), and the rows that are formed once
+// more: none where the type holds the largest, and nothing above 2^-6 of it is subnormal (elements of a normal distribution's
+// product, a thirtieth of the largest, are rounded to as much as their results are).
+struct Range {
+    const float* most;
+    long long n;
+    int rows;
+    float* scale;  // [2]
+    int* live;
+};
+constexpr float kLeastRange = 0x1p-8f, kMostRange = 65504.0f;
+
+__global__ __launch_bounds__(1024) void range_kernel(Range a) {
+    __shared__ float s[16];
+    float top = 0.0f;
+    for (long long i = threadIdx.x; i < a.n; i += 1024) top = fmaxf(top, a.most[i]);
+#pragma unroll
+    for (int d = 1; d < NHIP_WAVE; d *= 2) top = fmaxf(top, __shfl_xor(top, d));
+    if (threadIdx.x % NHIP_WAVE == 0) s[threadIdx.x / NHIP_WAVE] = top;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 16; ++w) top = fmaxf(top, s[w]);
+    const bool fits = top == 0.0f || (top >= kLeastRange && top <= kMostRange);
+    const int e = fits ? 0 : 14 - max(ilogbf(top), -100);
+    a.scale[0] = ldexpf(1.0f, e);
+    a.scale[1] = ldexpf(1.0f, -e);
+    *a.live = fits ? 0 : a.rows;
+}
 
 int check(const nhip_gated_args* a) {
     if (!a || a->channels <= 0 || a->features <= 0 || a->rows < 0) return NHIP_E_BADARG;
@@ -143,7 +203,7 @@ int check(const nhip_gated_args* a) {
 
 struct Space : TokSpace {
     long long x_ld, piece;
-    long long x = 0, gate = 0, up = 0;
+    long long x = 0, gate = 0, up = 0, most = 0, scale = 0;
     bool pad_x, pad_w;
     std::optional<TokGradient> gradient;
     Space(const nhip_gated_args& a, bool grad) {
@@ -152,6 +212,11 @@ struct Space : TokSpace {
         if (grad) {
             gradient.emplace(*this, a.rows, d, 2 * tok_round(a.features, 128), size);
             piece = gradient->piece / 2;
+            if (a.type == NHIP_F16 && a.rows) {
+                const long long last = a.features % piece;  // (of the last piece, whose shape may be another one)
+                most = take(std::max(waves(a, std::min<long long>(a.features, piece)), last ? waves(a, last) : 0) * 4);
+                scale = take(256);
+            }
         } else {
             // as many features as a launch's tiles reach
             piece = std::min(tok_round(a.features, 128), (1LL << 21) / (tok_round(rows, 256) / 256) * 64);
@@ -164,6 +229,13 @@ struct Space : TokSpace {
             gate = take(piece * x_ld * size);
             up = take(piece * x_ld * size);
         }
+    }
+    // of all tiles that form dg and du for n features
+    static long long waves(const nhip_gated_args& a, long long n) {
+        return tok_with_shape(2 * n, a.rows, sel_size(a.type), 1, [&](auto shape) {
+            using S = decltype(shape);
+            return (2 * n + S::BM - 1) / S::BM * ((a.rows + S::BN - 1) / S::BN) * S::kWaves;
+        });
     }
 };
 
@@ -235,17 +307,33 @@ template <class T> int backward(hipStream_t st, const nhip_gated_args& a, const 
         const long long second = tok_round(n, tok_with_shape(2 * n, a.rows, sizeof(T), 1, [](auto shape) { return decltype(shape)::BM / 2; }));
         const long long both = second + tok_round(n, 64);
         TOK_TRY(weight_rows<T>(st, a, s, w, f0, n, rows));
-        if (a.rows)
-            TOK_TRY(tok_with_shape(2 * n, a.rows, sizeof(T), 1, [&](auto shape) {
+        constexpr bool kRange = std::is_same<T, _Float16>::value;
+        float* const most = reinterpret_cast<float*>(w + s.most);
+        float* const scale = reinterpret_cast<float*>(w + s.scale);
+        int* const live = reinterpret_cast<int*>(scale + 2);
+        auto form = [&](auto kept) {
+            return tok_with_shape(2 * n, a.rows, sizeof(T), 1, [&](auto shape) {
                 using S = decltype(shape);
-                TokProduct p{rows, x, nullptr, nullptr, d * size, (int)((2 * n + S::BM - 1) / S::BM),
+                constexpr Kept k = decltype(kept)::value;
+                TokProduct p{rows, x, k == Kept::scaled ? live : nullptr, nullptr, d * size, (int)((2 * n + S::BM - 1) / S::BM),
                              (int)((a.rows + S::BN - 1) / S::BN), 1};
-                return tok_product<T, S, S::kWaveM / 2>(st, p, Backward{a.dy, a.dy_stride, f0, n, second, w + gr.g,
-                                                                        gr.gt_of<T>(w), gr.g_ld, gr.gt_ld, a.activation});
-            }));
+                return tok_product<T, S, S::kWaveM / 2>(st, p, Backward<k>{a.dy, a.dy_stride, f0, n, second, w + gr.g, gr.gt_of<T>(w),
+                                                                           gr.g_ld, gr.gt_ld, a.activation, p.m_tiles, most, scale});
+            });
+        };
+        if (a.rows) {
+            TOK_TRY(form(std::integral_constant<Kept, kRange ? Kept::measured : Kept::plain>()));
+            if constexpr (kRange) {
+                const Range r{most, Space::waves(a, n), (int)a.rows, scale, live};
+                TOK_LAUNCH(false, range_kernel, dim3(1), dim3(1024), 0, st, r);
+                NHIP_LAUNCH_CHECK();
+                TOK_TRY(form(std::integral_constant<Kept, Kept::scaled>()));
+            }
+        }
+        const float* const back = kRange && a.rows ? scale + 1 : nullptr;
         TOK_TRY(gr.weights<T>(st, w, x, nullptr, second + n, n, second, static_cast<T*>(a.dgate) + f0 * d,
-                              static_cast<T*>(a.dup) + f0 * d, nullptr));
-        if (a.rows) TOK_TRY(gr.inputs<T>(st, w, rows, nullptr, both, n, second, f0 > 0));
+                              static_cast<T*>(a.dup) + f0 * d, back));
+        if (a.rows) TOK_TRY(gr.inputs<T>(st, w, rows, nullptr, both, n, second, f0 > 0, back));
     }
     return gr.finish<T>(st, w, nullptr, nullptr, nullptr, a.dx);
 }

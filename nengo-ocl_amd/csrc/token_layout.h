@@ -169,11 +169,14 @@ struct TokStoreRows {
 };
 
 // dx[n, d] = sum_w G[n, w] W[w, d], added up over pieces of the weights in 32 bits, in parts (splits of k)
-struct TokAddParts {
+// (SCALED: pieces of G have a scale each.  A kernel of its own: the others take 3 % more of a gradient's time with it.)
+template <bool SCALED> struct TokAddParts {
     float* parts;
     long long ld, part;  // elements of a row, of a part
     int add;
+    const float* scale;  // 1 / that of G
     template <class T, class S> __device__ __forceinline__ void run(const TokPlace& at, sel_f4 (&acc)[S::MI][S::NI]) const {
+        const float k = SCALED ? *scale : 1.0f;
         float* const mine = parts + at.split * part;
 #pragma unroll
         for (int j = 0; j < S::NI; ++j) {
@@ -183,7 +186,8 @@ struct TokAddParts {
             for (int i = 0; i < S::MI; ++i) {
                 const long long d = (long long)at.m_tile * S::BM + at.wave_m * S::kWaveM + 16 * i + 4 * at.g;
                 sel_f4* const to = reinterpret_cast<sel_f4*>(mine + n * ld + d);
-                *to = add ? *to + acc[i][j] : acc[i][j];
+                const sel_f4 v = SCALED ? acc[i][j] * k : acc[i][j];
+                *to = add ? *to + v : v;
             }
             asm volatile("" ::: "memory");  // (a column's sums at a time: all of them at once are more than the registers hold)
         }
@@ -341,7 +345,7 @@ struct TokGradient {
         }
         float* const parts = reinterpret_cast<float*>(w + dw);
         const long long part = tok_round(n - n0, 256) * dx_ld;
-        if (int e = go(n0, n, splits, TokAddParts{parts, dx_ld, part, 0})) return e;
+        if (int e = go(n0, n, splits, TokAddParts<false>{parts, dx_ld, part, 0, nullptr})) return e;
         // the sums of columns from ... to - 1, which are rows of `to_rows` from its first on
         auto join = [&](long long from, long long to, long long base, T* to_rows) {
             from = from > n0 ? from : n0;
@@ -356,7 +360,7 @@ struct TokGradient {
     // dx += G W over `k` columns of G; W's rows (p2: from `second` on, `first` of each matrix) lie at the places that `rows_of` has
     template <class T>
     int inputs(hipStream_t st, char* w, const TokRows& rows_of, const int* live, long long k, long long first, long long second,
-               bool add) const {
+               bool add, const float* scale = nullptr) const {
         TokRows a{w + wt, nullptr, g_ld * size, d};
         if (across) {
             a = rows_of;
@@ -371,16 +375,21 @@ struct TokGradient {
                     return e;
         }
         const TokRows b{w + g, nullptr, g_ld * size, rows};
-        const TokAddParts epilogue{reinterpret_cast<float*>(w + dx), dx_ld, padded * dx_ld, add};
-        auto run = [&](auto shape) {
-            using S = decltype(shape);
-            constexpr int kAcross = std::is_same<S, TokLarge>::value && sizeof(T) == 2 ? 1 : 0;
-            TokProduct p{a, b, live, nullptr, k * size, (int)((d + S::BM - 1) / S::BM), (int)((rows + S::BN - 1) / S::BN),
-                         live ? dx_most : dx_splits, false, live ? 256 * S::kAtOnce : 0};
-            if (kAcross && !across) return tok_product<T, S, 0>(st, p, epilogue);
-            return tok_product<T, S, 0, kAcross>(st, p, epilogue);
+        auto add_to = [&](auto scaled) {
+            const TokAddParts<decltype(scaled)::value> epilogue{reinterpret_cast<float*>(w + dx), dx_ld, padded * dx_ld, add, scale};
+            auto run = [&](auto shape) {
+                using S = decltype(shape);
+                constexpr int kAcross = std::is_same<S, TokLarge>::value && sizeof(T) == 2 ? 1 : 0;
+                TokProduct p{a, b, live, nullptr, k * size, (int)((d + S::BM - 1) / S::BM), (int)((rows + S::BN - 1) / S::BN),
+                             live ? dx_most : dx_splits, false, live ? 256 * S::kAtOnce : 0};
+                if (kAcross && !across) return tok_product<T, S, 0>(st, p, epilogue);
+                return tok_product<T, S, 0, kAcross>(st, p, epilogue);
+            };
+            return across ? run(TokLarge()) : tok_with_shape(d, rows, (int)size, dx_splits, run);
         };
-        return across ? run(TokLarge()) : tok_with_shape(d, rows, (int)size, dx_splits, run);
+        if constexpr (std::is_same<T, _Float16>::value)
+            if (scale) return add_to(std::true_type());
+        return add_to(std::false_type());
     }
 
     template <class T> int finish(hipStream_t st, char* w, const int* where, const int* live, const float* scale, void* out) const {

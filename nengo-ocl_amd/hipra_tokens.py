@@ -28,7 +28,8 @@ Sums, statistics, losses and the gradients of the norm's parameters are float32,
 every call.  A result of 16 bits is rounded once; the gradients of products go through one more rounding, that of
 what stands between the two products (the gradient of the logits, of both projections) to the type of the
 inputs.  In 16 bits the gradient of the logits is scaled by the largest magnitude of `dloss` first (in float16 to the
-type's range) and the products' results back again; that of the projections is not, and has the range of the type.
+type's range) and the products' results back again; that of the projections is in float16, by a power of two, where
+its largest magnitude is beyond the type or below 2**-8 (which takes their product once more).
 
 Rows of the losses that do not count (a label outside the vocabulary, no target of a teacher) have a loss and a
 logarithm of zero, no gradient, and take no part in any sum, whatever they hold; they cost nothing in the products.
