@@ -51,7 +51,7 @@ typedef struct nhip_gated_args {
  * top > 0:   targets[n, top] are words and target_logits[n, top] a teacher's logits there: with
  *            q = softmax(target_logits[n] / temperature),
  *            loss[n] = sum_k q[k] (log q[k] - z[n, targets[n, k]] + lse[n]).
- *            Entries whose word is outside the vocabulary, or whose logit / temperature is -inf, are left out.
+ *            Entries whose word is outside the vocabulary, or whose logit is -inf, are left out.
  * Rows whose word is outside the vocabulary, or without entries, count nothing: loss and lse are zero there,
  * whatever x holds.  Gradients (the *_grad entries): dloss, and lse as the forward pass wrote it -> dx,
  * dweight (contiguous, of the type of x). */

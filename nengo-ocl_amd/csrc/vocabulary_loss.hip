@@ -25,7 +25,8 @@ __device__ __forceinline__ long long word_at(const void* p, int wide, long long 
 
 // ------------------------------------------------------------------------- a teacher's shares
 // A wave takes a row: shares of its entries, sorted by word, equal words added up, so that a tile finds its targets in one
-// range and no element of G has two.
+// range and no element of G has two.  A logit is taken off the row's largest before the temperature divides it: the lowest
+// value of 32 bits over a temperature below one would be -inf, which is no entry.
 struct Shares {
     const void *words, *logits;
     int wide, logits_type, top, n_words;
@@ -57,7 +58,7 @@ template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares
         t[q] = -INFINITY;
         if (e < a.top) {
             const long long w = word_at(a.words, a.wide, r * a.top + e);
-            const float v = sel_element(a.logits, a.logits_type, r * a.top + e) * a.per_temperature;
+            const float v = sel_element(a.logits, a.logits_type, r * a.top + e);
             if (w >= 0 && w < a.n_words && !(v == -INFINITY)) {
                 id[q] = (int)w;
                 t[q] = v;
@@ -74,7 +75,8 @@ template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares
     float sum = 0.0f, x[Q];
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-        x[q] = id[q] == kNoWord ? 0.0f : sel_exp(t[q] - most);
+        t[q] = (t[q] - most) * a.per_temperature;
+        x[q] = id[q] == kNoWord ? 0.0f : sel_exp(t[q]);
         sum += x[q];
     }
     sum = sel_wave_sum(sum);
@@ -85,7 +87,7 @@ template <int Q> __global__ __launch_bounds__(NHIP_WG) void shares_kernel(Shares
     for (int q = 0; q < Q; ++q) {
         const int e = lane + q * NHIP_WAVE;
         const float share = id[q] == kNoWord ? 0.0f : x[q] / sum;
-        self += share == 0.0f ? 0.0f : share * (t[q] - most - log_sum);
+        self += share == 0.0f ? 0.0f : share * (t[q] - log_sum);
         s_word[wave][e] = id[q];
         s_share[wave][e] = x[q] = share;
     }

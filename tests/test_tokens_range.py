@@ -1,5 +1,5 @@
 """Float16: gradients of the gated projection whose parts between the products the type does not hold, although it holds the
-result.  Definitions and tolerances are those of test_tokens.py.
+result; a teacher's logits that a temperature takes beyond 32 bits.  Definitions and tolerances are those of test_tokens.py.
 
 What stands between the products, dg and du, is stored by a power of two where its largest magnitude is beyond the type or below
 2**-8: then the largest is 2**14 at least, half of the type's smallest step 2**-25 is 2**-39 of it.  Where it is stored as it
@@ -10,7 +10,8 @@ import pytest
 import torch
 
 import test_tokens
-from test_tokens import E, F16, U, gated_bounds, gated_inputs, ops, wide, within  # noqa: F401
+from test_tokens import (E, F16, F32, U, check_loss_gradients, check_losses, gated_bounds, gated_inputs, ops,  # noqa: F401
+                         teacher_inputs, wide, within)
 
 
 @pytest.fixture(autouse=True)
@@ -108,3 +109,26 @@ def test_gated_gradient_recorded(queue, ops):  # noqa: F811
         assert all(torch.equal(a, b) for a, b in zip(got, want))
         if scale <= 1.0:
             check_gated_gradients(plan.gradients, dy, given, "silu")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n, top", [(6, 9), (70, 40), (300, 200)])
+@pytest.mark.parametrize("dtype", [F32, torch.bfloat16])
+@pytest.mark.parametrize("temperature", [0.1, 0.5, 1.0, 4.0])
+def test_teacher_logits_beyond_32_bits_over_a_temperature(queue, ops, n, top, dtype, temperature):  # noqa: F811
+    """A type's lowest value is a value at any temperature: in a row of them, and beside others; only -inf is left out."""
+    given, m = teacher_inputs(85, F32, n, 40, 500, 0.0, top)
+    low = torch.finfo(dtype).min
+    logits = given["logits"].to(dtype)
+    logits[0] = low
+    logits[1, ::2] = low
+    logits[2] = -2e38
+    logits[3, 0], logits[3, 1:] = low, float("-inf")
+    logits[4] = 2e38
+    logits[5] = float("-inf")
+    given["logits"] = logits
+    loss, lse = ops.teacher_loss(queue, temperature=temperature, **given)
+    check_losses(loss, lse, given, temperature)
+    assert loss[:5].all() and not loss[5]
+    dloss = (torch.rand(n, generator=m.gen) / n).cuda()
+    check_loss_gradients(ops.teacher_loss_grad(queue, dloss, lse=lse, temperature=temperature, **given), given, temperature, dloss, lse)
