@@ -46,7 +46,7 @@ typedef struct nhip_gated_args {
     long long workspace_bytes;
 } nhip_gated_args;
 
-/* z[n, v] = (x[n] . weight[v]) / temperature,  lse[n] = log sum_v exp(z[n, v]).
+/* z[n, v] = (x[n] . weight[v]) / temperature,  lse[n] = log sum_v exp(z[n, v]);  temperature: 2^-126 to 2^126.
  * top == 0:  targets[n] is a word, loss[n] = lse[n] - z[n, targets[n]].
  * top > 0:   targets[n, top] are words and target_logits[n, top] a teacher's logits there: with
  *            q = softmax(target_logits[n] / temperature),

@@ -603,7 +603,7 @@ int check(const nhip_loss_args* a) {
     if (!a || a->channels <= 0 || a->words <= 0 || a->rows < 0 || a->top < 0) return NHIP_E_BADARG;
     if (a->type < NHIP_F32 || a->type > NHIP_F16 || a->rows > kMostRows || a->top > kMostTop) return NHIP_E_BADARG;
     if (a->top && (a->logits_type < NHIP_F32 || a->logits_type > NHIP_F16)) return NHIP_E_BADARG;
-    if (!(a->temperature > 0.0f) || !(a->temperature < INFINITY)) return NHIP_E_BADARG;
+    if (!(a->temperature >= 0x1p-126f) || !(a->temperature <= 0x1p126f)) return NHIP_E_BADARG;  // (its reciprocal is one of 32 bits)
     if (a->words > kNoWord - 4096 || a->channels > kMostChannels) return NHIP_E_BADARG;
     return 0;
 }

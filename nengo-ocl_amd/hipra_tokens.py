@@ -265,8 +265,8 @@ def _loss(queue, x, weight, targets, logits=None, temperature=1.0):
     if logits is None:
         targets, wide = _words(queue, "labels", targets, lead)
     else:
-        if not 0.0 < temperature < float("inf"):
-            raise ValueError("temperature is %r" % (temperature,))
+        if not 2.0 ** -126 <= temperature <= 2.0 ** 126:
+            raise ValueError("temperature is %r: 2**-126 to 2**126, numbers of float32 and their reciprocals" % (temperature,))
         targets = _plain(targets)
         if targets.dim() != len(lead) + 1 or not 1 <= targets.shape[-1] <= MAX_TOP:
             raise ValueError("indices has shape %s: %s with 1 to %d targets is wanted"
