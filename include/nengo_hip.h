@@ -879,8 +879,8 @@ int nhip_block_norm_grad(void *stream, const nhip_norm_args *args);
 int nhip_block_norm_grad_workspace(const nhip_norm_args *args, long long *bytes_out);
 
 /* ---- operators over tokens ---------------------------------------------------
- * The arguments are described in nengo_hip_tokens.h.  Sizes: the norm takes 1 to 2^27 - 1 channels and 0 to
- * 2^31 - 1 rows; products 0 to 2^20 rows, 1 to 2^20 channels and features; losses any words from 1 up to
+ * The arguments are described in nengo_hip_tokens.h.  Sizes: the norm takes 1 to 2^27 - 1 channels (its
+ * gradient to 2^27 - 32) and 0 to 2^31 - 1 rows; products 0 to 2^20 rows, 1 to 2^20 channels and features; losses any words from 1 up to
  * 2^31 - 4097, top up to 256.  Others are refused with NHIP_E_BADARG before any launch.  The `*_workspace` functions
  * give the bytes of workspace that a call with these arguments needs (a smaller one is refused with NHIP_E_TOOBIG);
  * its contents need not be kept between calls. */

@@ -381,7 +381,7 @@ extern "C" int nhip_block_norm_grad(void* stream, const nhip_norm_args* args) {
     if (int e = nhip_block_norm_grad_workspace(args, &need)) return e;
     const nhip_norm_args& a = *args;
     if (!a.dweight || (a.scale && !a.dscale)) return NHIP_E_BADARG;
-    if (a.channels >= 1 << 27) return NHIP_E_BADARG;  // (columns of the sums' launch: 16 threads each, two to a channel)
+    if (2LL * a.channels > SEL_MAX_SUMS) return NHIP_E_BADARG;
     if (a.rows && (!a.dout || !a.dx || (a.gate && !a.dgate))) return NHIP_E_BADARG;
     if (need > a.workspace_bytes) return NHIP_E_TOOBIG;
     if (!a.workspace) return NHIP_E_BADARG;

@@ -329,7 +329,7 @@ extern "C" int nhip_layer_norm(void* stream, const nhip_layer_norm_args* args) {
 
 extern "C" int nhip_layer_norm_grad_workspace(const nhip_layer_norm_args* args, long long* bytes_out) {
     if (int e = check(args)) return e;
-    if (!bytes_out) return NHIP_E_BADARG;
+    if (!bytes_out || 2LL * args->channels > SEL_MAX_SUMS) return NHIP_E_BADARG;
     *bytes_out = (long long)sum_rows(args->rows, kMostGroups) * 2 * args->channels * 4;
     return 0;
 }

@@ -240,6 +240,7 @@ struct SelReduce {
     float *out2, *out3;
 };
 #define SEL_REDUCE_WAVES 16
+#define SEL_MAX_SUMS (((1LL << 32) / (SEL_REDUCE_WAVES * NHIP_WAVE) - 1) * NHIP_WAVE)  // columns: an axis has fewer than 2^32 threads
 
 static __global__ __launch_bounds__(SEL_REDUCE_WAVES * NHIP_WAVE) void sel_reduce_kernel(SelReduce a) {
     __shared__ float s[SEL_REDUCE_WAVES][NHIP_WAVE];

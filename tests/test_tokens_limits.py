@@ -36,3 +36,28 @@ def test_temperatures(host, ops):  # noqa: F811
             assert entry(None, loss_arguments(ops, temperature=t)) == bad, t
         for t in (2.0 ** -126, 2.0 ** 126):
             assert entry(None, loss_arguments(ops, temperature=t)) == too_big, t  # (of the workspace)
+
+
+def test_channels_of_the_norms_gradients(ops):  # noqa: F811
+    """The launch that adds up the sums for weight and bias takes 2**28 - 64 columns, two to a channel: more are refused before
+    the first launch (the workspace of one byte, checked behind them, tells that they were not)."""
+    from nengo_ocl_amd import _lib, hipra_selective
+
+    lib, bad, too_big, need = _lib.lib(), -1, -4, ctypes.c_longlong()
+
+    def layer(channels):
+        return ctypes.byref(ops._LayerNormArgs(channels=channels, rows=1, eps=1e-5, x=ONE, x_stride=channels, weight=ONE, out=ONE,
+                                               dout=ONE, dout_stride=channels, dx=ONE, dweight=ONE, workspace=ONE, workspace_bytes=1))
+
+    def block(channels):
+        return ctypes.byref(hipra_selective._NormArgs(channels=channels, groups=1, rows=1, eps=1e-5, x=ONE, x_stride=channels,
+                                                      weight=ONE, out=ONE, dout=ONE, dout_stride=channels, dx=ONE, dweight=ONE,
+                                                      workspace=ONE, workspace_bytes=1))
+
+    most = 2 ** 27 - 32
+    for entry, given in ((lib.nhip_layer_norm_grad, layer), (lib.nhip_block_norm_grad, block)):
+        assert entry(None, given(most)) == too_big
+        for channels in (most + 1, 2 ** 27 - 1):
+            assert entry(None, given(channels)) == bad, channels
+    assert lib.nhip_layer_norm_grad_workspace(layer(most), ctypes.byref(need)) == 0 and need.value == 2 * 4 * most
+    assert lib.nhip_layer_norm_grad_workspace(layer(most + 1), ctypes.byref(need)) == bad
