@@ -283,7 +283,7 @@ template <class T> int forward(hipStream_t st, const nhip_gated_args& a, const S
             TOK_TRY((tok_few<T, 2, 1>(st, p, e)));
             continue;
         }
-        TOK_TRY(tok_with_shape(2 * n, a.rows, sizeof(T), 1, [&](auto shape) {
+        TOK_TRY(tok_with_many(2 * n, a.rows, sizeof(T), 1, [&](auto shape) {
             using S = decltype(shape);
             p.m_tiles = (int)((2 * n + S::BM - 1) / S::BM);
             p.n_tiles = (int)((a.rows + S::BN - 1) / S::BN);
@@ -333,7 +333,7 @@ template <class T> int backward(hipStream_t st, const nhip_gated_args& a, const 
         const float* const back = kRange && a.rows ? scale + 1 : nullptr;
         TOK_TRY(gr.weights<T>(st, w, x, nullptr, second + n, n, second, static_cast<T*>(a.dgate) + f0 * d,
                               static_cast<T*>(a.dup) + f0 * d, back));
-        if (a.rows) TOK_TRY(gr.inputs<T>(st, w, rows, nullptr, both, n, second, f0 > 0, back));
+        if (a.rows) TOK_TRY((gr.inputs<T, kRange>(st, w, rows, nullptr, both, n, second, f0 > 0, back)));
     }
     return gr.finish<T>(st, w, nullptr, nullptr, nullptr, a.dx);
 }

@@ -358,7 +358,7 @@ struct TokGradient {
     }
 
     // dx += G W over `k` columns of G; W's rows (p2: from `second` on, `first` of each matrix) lie at the places that `rows_of` has
-    template <class T>
+    template <class T, bool SCALED = false>
     int inputs(hipStream_t st, char* w, const TokRows& rows_of, const int* live, long long k, long long first, long long second,
                bool add, const float* scale = nullptr) const {
         TokRows a{w + wt, nullptr, g_ld * size, d};
@@ -375,21 +375,16 @@ struct TokGradient {
                     return e;
         }
         const TokRows b{w + g, nullptr, g_ld * size, rows};
-        auto add_to = [&](auto scaled) {
-            const TokAddParts<decltype(scaled)::value> epilogue{reinterpret_cast<float*>(w + dx), dx_ld, padded * dx_ld, add, scale};
-            auto run = [&](auto shape) {
-                using S = decltype(shape);
-                constexpr int kAcross = std::is_same<S, TokLarge>::value && sizeof(T) == 2 ? 1 : 0;
-                TokProduct p{a, b, live, nullptr, k * size, (int)((d + S::BM - 1) / S::BM), (int)((rows + S::BN - 1) / S::BN),
-                             live ? dx_most : dx_splits, false, live ? 256 * S::kAtOnce : 0};
-                if (kAcross && !across) return tok_product<T, S, 0>(st, p, epilogue);
-                return tok_product<T, S, 0, kAcross>(st, p, epilogue);
-            };
-            return across ? run(TokLarge()) : tok_with_shape(d, rows, (int)size, dx_splits, run);
+        const TokAddParts<SCALED> epilogue{reinterpret_cast<float*>(w + dx), dx_ld, padded * dx_ld, add, scale};
+        auto run = [&](auto shape) {
+            using S = decltype(shape);
+            constexpr int kAcross = std::is_same<S, TokLarge>::value && sizeof(T) == 2 ? 1 : 0;
+            TokProduct p{a, b, live, nullptr, k * size, (int)((d + S::BM - 1) / S::BM), (int)((rows + S::BN - 1) / S::BN),
+                         live ? dx_most : dx_splits, false, live ? 256 * S::kAtOnce : 0};
+            if (kAcross && !across) return tok_product<T, S, 0>(st, p, epilogue);
+            return tok_product<T, S, 0, kAcross>(st, p, epilogue);
         };
-        if constexpr (std::is_same<T, _Float16>::value)
-            if (scale) return add_to(std::true_type());
-        return add_to(std::false_type());
+        return across ? run(TokLarge()) : tok_with_shape(d, rows, (int)size, dx_splits, run);
     }
 
     template <class T> int finish(hipStream_t st, char* w, const int* where, const int* live, const float* scale, void* out) const {

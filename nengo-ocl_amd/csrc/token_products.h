@@ -488,18 +488,18 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
 // many are multiplied, and add up their sums in the LDS.  (One row, 2048 channels, 2 x 5504 features in bfloat16: 45 MB in 13 us,
 // 205 MB of a vocabulary in 43, 4.8 TB/s; tiles of 128 rows through the LDS, 86 work-groups, took 18.)
 template <int MT_> struct TokFew {
-    static constexpr int MT = MT_, NI = 1, kWaves = 4, U = 8 / MT_;
+    static constexpr int MT = MT_, kWaves = 4, U = 8 / MT_;
     using Shape = TokShape<16 * MT_, 16, 1, 1>;  // what an epilogue sees: a wave has a tile of 16 columns
 };
 
 template <class T, class F, int HALF, class Epilogue>
 __global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_few_kernel(TokProduct p, Epilogue epilogue) {
-    constexpr int MT = F::MT, NI = F::NI, U = F::U;
-    __shared__ sel_f4 s_sum[F::kWaves][MT][NI][NHIP_WAVE];
+    constexpr int MT = F::MT, U = F::U;
+    __shared__ sel_f4 s_sum[F::kWaves][MT][NHIP_WAVE];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / NHIP_WAVE), lane = threadIdx.x % NHIP_WAVE;
     TokPlace at;
     at.m_tile = nhip_xcd_remap(blockIdx.x, gridDim.x);
-    at.split = at.wave_m = at.wave_n = at.wave = 0;
+    at.n_tile = at.split = at.wave_m = at.wave_n = at.wave = 0;
     at.l = lane % 16;
     at.g = lane / 16;
     at.live = (int)(p.live ? min((long long)*p.live, p.b.rows) : p.b.rows);
@@ -507,17 +507,16 @@ __global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_few_kernel(TokPr
     if (at.live <= 0) return;
     const int bytes = (int)p.k_bytes, steps = (bytes + 63) / 64, per = (steps + F::kWaves - 1) / F::kWaves;
     const int first = min(steps, wave * per), n = min(steps, first + per) - first;
-    const char *a[MT], *b[NI];
+    const char* a[MT];
 #pragma unroll
     for (int i = 0; i < MT; ++i) {
         const bool other = HALF && i >= MT / 2;  // (equal rows of both matrices, as an epilogue wants them)
         const long long r = (long long)at.m_tile * (HALF ? 8 * MT : 16 * MT) + 16 * (other ? i - MT / 2 : i) + at.l;
         a[i] = (other ? p.a.p2 : p.a.p) + min(r, p.a.rows - 1) * p.a.ld + 16 * at.g;
     }
-#pragma unroll
-    for (int j = 0; j < NI; ++j) b[j] = p.b.p + min(16LL * j + at.l, (long long)at.live - 1) * p.b.ld + 16 * at.g;
+    const char* const b = p.b.p + min((long long)at.l, (long long)at.live - 1) * p.b.ld + 16 * at.g;
     struct Batch {
-        tok_u4 a[U][MT], b[U][NI];
+        tok_u4 a[U][MT], b[U];
     };
     // (unconditional: what lies behind the end of k, or of the wave's part, is read from elsewhere)
     auto load = [&](Batch& v, int step) {
@@ -528,24 +527,19 @@ __global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_few_kernel(TokPr
             const char* const zeros = reinterpret_cast<const char*>(&tok_zeros);
 #pragma unroll
             for (int i = 0; i < MT; ++i) v.a[u][i] = *reinterpret_cast<const tok_u4*>(is ? a[i] + k : zeros);
-#pragma unroll
-            for (int j = 0; j < NI; ++j) v.b[u][j] = *reinterpret_cast<const tok_u4*>(is ? b[j] + k : zeros);
+            v.b[u] = *reinterpret_cast<const tok_u4*>(is ? b + k : zeros);
         }
     };
-    sel_f4 acc[MT][NI];
+    sel_f4 acc[MT][1];
 #pragma unroll
-    for (int i = 0; i < MT; ++i)
-#pragma unroll
-        for (int j = 0; j < NI; ++j) acc[i][j] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (int i = 0; i < MT; ++i) acc[i][0] = sel_f4{0.0f, 0.0f, 0.0f, 0.0f};
     auto multiply = [&](const Batch& v) {
 #pragma unroll
         for (int u = 0; u < U; ++u)
 #pragma unroll
             for (int e = 0; e < (sizeof(T) == 2 ? 1 : 4); ++e)
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NI; ++j) tok_mma<T>(acc[i][j], v.a[u][i], v.b[u][j], e);
+                for (int i = 0; i < MT; ++i) tok_mma<T>(acc[i][0], v.a[u][i], v.b[u], e);
     };
     Batch even, odd;
     load(even, 0);
@@ -557,23 +551,14 @@ __global__ __launch_bounds__(F::kWaves * NHIP_WAVE, 2) void tok_few_kernel(TokPr
     }
     tok_settle(acc);
 #pragma unroll
+    for (int i = 0; i < MT; ++i) s_sum[wave][i][lane] = acc[i][0];
+    __syncthreads();
+    if (wave) return;
+#pragma unroll
     for (int i = 0; i < MT; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) s_sum[wave][i][j][lane] = acc[i][j];
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < NI; ++j) {
-        if (j % F::kWaves != wave || 16 * j >= at.live) continue;
-        sel_f4 sum[MT][1];
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            sum[i][0] = s_sum[0][i][j][lane];
-#pragma unroll
-            for (int w = 1; w < F::kWaves; ++w) sum[i][0] += s_sum[w][i][j][lane];
-        }
-        at.n_tile = j;
-        epilogue.template run<T, typename F::Shape>(at, sum);
-    }
+        for (int w = 1; w < F::kWaves; ++w) acc[i][0] += s_sum[w][i][lane];
+    epilogue.template run<T, typename F::Shape>(at, acc);
 }
 
 // 17 to 64 columns (16 NI): B, which all waves of a work-group read, goes through the LDS, 256 bytes of k at a time; A still goes
@@ -811,9 +796,13 @@ static inline bool tok_is_large(long long m, long long n, int size, int splits, 
     const long long large = ((m + 255) / 256) * ((n + 255) / 256) * splits;
     return n > 128 && m > 128 && large >= (size == 2 ? least : 512);
 }
-template <class F> static inline int tok_with_shape(long long m, long long n, int size, int splits, F&& f) {
+// (of more than TOK_FEW columns: fewer go to tok_few, or may be any)
+template <class F> static inline int tok_with_many(long long m, long long n, int size, int splits, F&& f) {
     if (tok_is_large(m, n, size, splits)) return f(TokLarge());
-    if (n > 64) return f(TokShape<128, 128, 2, 2>());
+    return f(TokShape<128, 128, 2, 2>());
+}
+template <class F> static inline int tok_with_shape(long long m, long long n, int size, int splits, F&& f) {
+    if (n > 64) return tok_with_many(m, n, size, splits, f);
     if (n > 16) return f(TokShape<128, 64, 4, 1>());
     return f(TokShape<128, 16, 4, 1>());
 }

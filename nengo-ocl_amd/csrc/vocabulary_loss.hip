@@ -724,7 +724,7 @@ template <class T> int forward(hipStream_t st, const nhip_loss_args& a, const Sp
                 tiles += (int)((words + TOK_LEAST_BM - 1) / TOK_LEAST_BM);
                 return tok_few<T, TOK_LEAST_BM / 16, 0>(st, p, e);
             }
-            return tok_with_shape(words, a.rows, sizeof(T), 1, [&](auto shape) {
+            return tok_with_many(words, a.rows, sizeof(T), 1, [&](auto shape) {
                 using S = decltype(shape);
                 p.m_tiles = (int)((words + S::BM - 1) / S::BM);
                 p.n_tiles = (int)((a.rows + S::BN - 1) / S::BN);
