@@ -5,6 +5,11 @@
 //
 // All of it moves memory: every array is read or written once, a row stays in registers between its sums and their
 // use.  The mean is taken away before squares are summed, so that a mean far from zero costs no digits.
+//
+// Rows that registers do not hold are read three times: forward above 1024 packs of 16 bytes (8192 channels of 16 bits; 1024 where rows
+// are no whole packs), backward above 4096 channels (1024), where the sums for weight and bias go through memory for each
+// row, too.  bfloat16 with a residual, 8192 rows: forward 1504 channels 17 us, 1500 48, 8192 111; gradient 1504 channels 52 us,
+// 1500 111, 4096 125, 8192 495 (134 for its bytes).
 #include "norm_rows.h"
 
 namespace {

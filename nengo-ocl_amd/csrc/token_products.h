@@ -486,7 +486,7 @@ __global__ __launch_bounds__(S::kThreads, S::kAtOnce * S::kWaves / 4) void tok_p
 // Up to 16 columns: nothing is read twice, so that all is the time that A takes to arrive.  A work-group has MT tiles of 16 rows;
 // its four waves have a quarter of k each, straight from memory into registers, U steps of 64 bytes of k under way while as
 // many are multiplied, and add up their sums in the LDS.  (One row, 2048 channels, 2 x 5504 features in bfloat16: 45 MB in 13 us,
-// 205 MB of a vocabulary in 43, 4.8 TB/s; tiles of 128 rows through the LDS, 86 work-groups, took 18.)
+// 205 MB of a vocabulary in 36, part of it from the last cache; tiles of 128 rows through the LDS, 86 work-groups, took 18.)
 template <int MT_> struct TokFew {
     static constexpr int MT = MT_, kWaves = 4, U = 8 / MT_;
     using Shape = TokShape<16 * MT_, 16, 1, 1>;  // what an epilogue sees: a wave has a tile of 16 columns

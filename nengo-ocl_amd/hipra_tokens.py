@@ -21,8 +21,8 @@ Plans, queues, streams and arrays are as in `hipra_selective`: a ``plan_*`` func
 and returns a `Plan` bound to them, the function without the prefix enqueues it once, in order with torch's
 current stream.  Arrays are torch tensors or `DeviceArray`, float32, bfloat16 or float16, ``[..., channels]`` with
 leading axes whose rows lie at one distance.  The norm's parameters are float32; the weights of products have
-the type of what they multiply, ``[rows, channels]``.  Every plan has a workspace of its own.  Outputs may not
-overlap inputs.  At most 2**20 rows go into a product, and 256 targets of a teacher to a row.
+the type of what they multiply, ``[rows, channels]``.  Every plan has a workspace of its own, of the bytes that the
+C library's ``*_workspace`` function names.  Outputs may not overlap inputs.  At most 2**20 rows go into a product, and 256 targets of a teacher to a row.
 
 Sums, statistics, losses and the gradients of the norm's parameters are float32, added up in the same order on
 every call.  A result of 16 bits is rounded once; the gradients of products go through one more rounding, that of
@@ -337,7 +337,7 @@ def plan_teacher_loss(queue, x, weight, indices, logits, temperature=1.0, loss=N
     """How far ``p = softmax(x weight' / temperature)`` is from a teacher of whom the largest logits are known:
     ``sum_k q[k] (log q[k] - log p[indices[k]])`` with ``q = softmax(logits / temperature)`` over these alone.
     `indices` ``[..., k]`` (int32 or int64) are their words, `logits` ``[..., k]`` (float32, bfloat16 or float16) their
-    values.  An index outside the vocabulary, or a value of -inf, is left out; a token without any does not
+    values; `temperature` is 2**-126 to 2**126.  An index outside the vocabulary, or a value of -inf, is left out; a token without any does not
     count, and has zeros; an index named twice is two targets, whose shares of p's gradient add up.  ``plan.loss``,
     ``plan.lse`` as for `plan_vocabulary_loss`, the latter of the logits over the temperature."""
     given = _teacher(queue, x, weight, indices, logits, temperature)
