@@ -58,6 +58,8 @@ def around(queue, plan):
             start, stop = plan._events_to_profile[-1]
             rows.append((events.between(a, start), events.between(start, stop), events.between(stop, b)))
         plan.update_profiling()
+        with torch.cuda.stream(queue.stream):
+            load.zero_()
         a = events.record(queue.handle)
         for _ in range(10):
             plan.enqueue()
